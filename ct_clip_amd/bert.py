@@ -6,6 +6,11 @@ The reference calls ``self.text_transformer(input_ids, attention_mask=...)[0]`` 
 with biased dense projections, softmax attention with key-padding mask, erf-GELU FFN (HF modeling_bert.py: BertEmbeddings,
 BertSelfAttention, BertSelfOutput, BertIntermediate, BertOutput) -- runs through ``ct_clip_amd.functional``.
 The pooler is skipped: CT-CLIP discards it (ct_clip.py:686,762).
+
+Reports longer than the position table (512 rows), all as attributes of the HF config (``BertConfig(..., position_embedding_type="rotary", attention_window=256)``):
+  position_embedding_type = "rotary"   rotary positions on q and k instead of the absolute table (which is then neither read nor trained); rotary_dim (default: the whole
+                                       head), rope_theta (10000), rotary_layout ("half" | "interleaved"), rope_scaling (dict, ``functional.RotaryPositions``);
+  attention_window = n or (l, r)       every token attends within its window, cost linear in the length; attention_sinks first tokens (default 1: [CLS]) stay visible.
 """
 import math
 
@@ -16,6 +21,28 @@ from . import functional as Fn
 def is_hf_bert(module):
     return hasattr(module, "embeddings") and hasattr(module, "encoder") and hasattr(module.encoder, "layer") \
         and hasattr(module.embeddings, "word_embeddings")
+
+
+def _long_report_options(bert, dh):
+    """-> (RotaryPositions or None, (left, right) or None, sinks) from the config."""
+    cfg = bert.config
+    kind = getattr(cfg, "position_embedding_type", "absolute") or "absolute"
+    if kind not in ("absolute", "rotary"):
+        raise NotImplementedError("only absolute and rotary position embeddings are implemented")
+    rope = None
+    if kind == "rotary":
+        scaling = getattr(cfg, "rope_scaling", None)
+        key = (getattr(cfg, "rotary_dim", None) or dh, float(getattr(cfg, "rope_theta", None) or 10000.0), getattr(cfg, "rotary_layout", None) or "half",
+               tuple(sorted(scaling.items())) if scaling else None)
+        held = bert.__dict__.get("_ctclip_rope")
+        if held is None or held[0] != key:
+            held = bert.__dict__["_ctclip_rope"] = (key, Fn.RotaryPositions(key[0], base=key[1], layout=key[2], scaling=scaling))
+        rope = held[1]
+    window = getattr(cfg, "attention_window", None)
+    if window is not None:
+        window = (int(window), int(window)) if not isinstance(window, (tuple, list)) else (int(window[0]), int(window[1]))
+    sinks = getattr(cfg, "attention_sinks", None)
+    return rope, window, 1 if sinks is None else int(sinks)
 
 
 def bert_last_hidden_state(bert, input_ids, attention_mask, dtype, operand_dtype=None, cls_only=False):
@@ -34,8 +61,7 @@ def bert_last_hidden_state(bert, input_ids, attention_mask, dtype, operand_dtype
     cfg = bert.config
     if getattr(cfg, "hidden_act", "gelu") != "gelu":
         raise NotImplementedError(f"hidden_act={cfg.hidden_act!r}: only erf-GELU BERT is implemented")
-    if getattr(cfg, "position_embedding_type", "absolute") != "absolute":
-        raise NotImplementedError("only absolute position embeddings are implemented")
+    rope, window, sinks = _long_report_options(bert, cfg.hidden_size // cfg.num_attention_heads)
     # train-mode dropout (HF modeling_bert.py: BertEmbeddings, BertSelfAttention, BertSelfOutput, BertOutput).  Masks are
     # counter-based (Philox, ct_clip_amd/csrc/common.h): one 62-bit seed per forward drawn from torch's CPU generator (so that
     # torch.manual_seed reproduces a run), call sites separated by stream ids / seed offsets, regenerated in backward.
@@ -54,7 +80,9 @@ def bert_last_hidden_state(bert, input_ids, attention_mask, dtype, operand_dtype
     dh = hidden // nh
     eps = cfg.layer_norm_eps
 
-    x = Fn.BertEmbedFn.apply(ids, emb.word_embeddings.weight, emb.position_embeddings.weight,
+    if rope is None and T > emb.position_embeddings.weight.shape[0]:
+        raise ValueError(f"{T} tokens, and {emb.position_embeddings.weight.shape[0]} rows in the position table (config.position_embedding_type = \"rotary\" has none)")
+    x = Fn.BertEmbedFn.apply(ids, emb.word_embeddings.weight, emb.position_embeddings.weight if rope is None else None,
                              emb.token_type_embeddings.weight, dtype)
     x = Fn.layer_norm(x, emb.LayerNorm.weight, emb.LayerNorm.bias, eps)
     x = drop(x, None, 0)
@@ -69,11 +97,17 @@ def bert_last_hidden_state(bert, input_ids, attention_mask, dtype, operand_dtype
         sa, so = layer.attention.self, layer.attention.output
         # (x feeds the attention AND the residual connection: the node hands back a view of x for the latter, so that in backward the residual
         # path's gradient is added inside the grad-input GEMM's epilogue instead of by an elementwise accumulation kernel)
-        c, x_res = Fn.QkvSdpaFn.apply(x, sa.query.weight, sa.key.weight, sa.value.weight, sa.query.bias, sa.key.bias, sa.value.bias, keymask,
-                                      Bsz, T, nh, dh, scale, (p_att, seed + 1 + li) if p_att > 0 else None, od, True)
-        if cls_only and li == nlayers - 1 and T > 1:
+        drop_att = (p_att, seed + 1 + li) if p_att > 0 else None
+        last_cls = cls_only and li == nlayers - 1 and T > 1
+        qkv_args = (x, sa.query.weight, sa.key.weight, sa.value.weight, sa.query.bias, sa.key.bias, sa.value.bias, keymask, Bsz, T, nh, dh, scale, drop_att)
+        if rope is None and window is None:
+            c, x_res = Fn.QkvSdpaFn.apply(*qkv_args, od, True)
+        else:
+            c, x_res = Fn.QkvWindowFn.apply(*qkv_args, rope, window or (-1, -1), sinks if window else 0, last_cls, od, True)
+        if last_cls:
             # rows b * T of the attention output and of the layer input: everything behind them in this layer is row-wise
-            c = c.view(Bsz, T * c.shape[1])[:, :c.shape[1]].contiguous()
+            if c.shape[0] != Bsz:
+                c = c.view(Bsz, T * c.shape[1])[:, :c.shape[1]].contiguous()
             x_res = x_res.view(Bsz, T * hidden)[:, :hidden].contiguous()
         if p_hid > 0:    # dense -> dropout -> + input -> LayerNorm
             h1 = drop(Fn.linear(c, so.dense.weight, so.dense.bias, out_dtype=dtype, operand_dtype=od), x_res, 1 + 2 * li)

@@ -1,0 +1,334 @@
+// Shared pieces of the windowed attention kernels (win_attn.hip: forward, win_attn_bwd.hip: backward).
+//
+// Position i of a query sees key j when j <= i + right, and j >= i - left or j < sinks, and the key mask does not hide j.  O = softmax(scale q k^T + mask) v.
+// Both products of a pass run on mfma 32x32 (bf16: x16, f32: x2) in the orientation S^T = K Q^T: a lane owns ONE query (column lane & 31) and 16 keys of a
+// 32 x 32 block in registers, register r of half h = lane >> 5 being key 8 (r >> 2) + 4 h + (r & 3).  Row maximum and sum are therefore in-lane plus one
+// exchange between the halves, and P^T feeds the second product as it stands: slot e of half h of the k-step G is key 16 G + 8 (e >> 2) + 4 h + (e & 3), and the
+// matching V^T operand is two transposing LDS reads (ds_read_b64_tr_b16: four keys of one column per lane) of the row-major tile.  No transposed copies exist.
+//
+// LDS tiles are row-major without padding; the 16-byte chunks of row r are XOR-permuted with swz(r) so that the 16 rows of a ds_read_b128 group and the four
+// rows x 64 bytes of a transposing read fall into distinct 16-byte slots of the 256-byte bank row.
+#pragma once
+#include "common.h"
+
+namespace win {
+
+constexpr float LOG2E_ = 1.4426950408889634f, LN2_ = 0.6931471805599453f;
+constexpr float HIDDEN = -1e30f;          // an additive key mask value at or below this (or NaN) hides the key: HF's finfo.min, -inf
+constexpr int QB = 128;                   // rows (queries, or keys in the dK / dV kernel) of a workgroup: 4 waves x 32
+
+struct Params {
+  const void *q, *k, *v, *o, *dout;
+  const float* keymask;                   // additive, (key rows) f32, or null
+  const int32_t* offsets;                 // packed sequences: first row of each (nseq + 1), or null: sequence b = rows b * Lq / b * Lk
+  const int32_t* tiles;                   // packed sequences: (sequence, 128-row tile) of every tile
+  int ntiles;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta;                     // [H][query rows]: log2-domain log-sum-exp (+inf for a row that sees nothing), rowsum(dO o O)
+  float* part;                            // workspace of split passes
+  int nseq, Lq, Lk, H, Hk, G;
+  int left, right, sinks, q_start;
+  int64_t Mq, Mk;
+  int64_t ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
+  float scale, scale2;                    // scale2 = scale * log2 e
+  uint64_t seed; const unsigned long long* seed_state; float drop_p, inv_keep;
+  int nsplit;
+  int s32, nchunk;                        // backward: keys of sink blocks (multiple of 32), chunks of the rows beyond their window
+};
+
+template <typename T, int D> struct Geo {
+  static constexpr int ESZ = (int)sizeof(T);
+  static constexpr int ROWB = D * ESZ;                     // bytes of a tile row
+  static constexpr int NCH = ROWB / 16;                    // 16-byte chunks of a row
+  static constexpr int KT = ESZ == 2 ? 64 : 32;            // keys of a forward / dQ step
+  static constexpr int NB = D / 32;                        // 32-column blocks of a head
+};
+// chunk permutation of row r (see the header comment); NCH = 4, 8, 16 or 32 chunks per row
+template <int NCH> __device__ __forceinline__ int swz(int r) {
+  if (NCH == 4) return (r >> 2) & 3;
+  if (NCH == 8) { const int m = (r >> 1) & 7; return ((m & 1) << 2) | (m >> 1); }
+  return ((r & 3) << 2) | ((r >> 2) & 3);
+}
+template <typename T, int D> __device__ __forceinline__ int lds_at(int row, int chunk) { return row * Geo<T, D>::ROWB + ((chunk ^ swz<Geo<T, D>::NCH>(row)) << 4); }
+
+// operand whose rows are the matrix product's rows / columns and whose contraction runs along D: bf16 slot (g, e) of half h = column 16 g + 8 h + e,
+// f32 instruction 4 g + e = column 8 g + 4 h + e
+template <typename T, int D> struct RowFrag;
+template <int D> struct RowFrag<bf16_t, D> { bf16x8 v[D / 16]; };
+template <int D> struct RowFrag<float, D> { f32x4 v[D / 8]; };
+template <typename T, int D> __device__ __forceinline__ void row_frag_zero(RowFrag<T, D>& f) {
+#pragma unroll
+  for (int g = 0; g < Geo<T, D>::NCH / 2; ++g) { const u32x4 z = {0, 0, 0, 0}; f.v[g] = __builtin_bit_cast(decltype(f.v[0] + f.v[0]), z); }
+}
+template <typename T, int D> __device__ __forceinline__ void row_frag_global(RowFrag<T, D>& f, const T* row, int half) {
+#pragma unroll
+  for (int g = 0; g < Geo<T, D>::NCH / 2; ++g) {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(row) + (2 * g + half) * 16);
+    f.v[g] = __builtin_bit_cast(decltype(f.v[0] + f.v[0]), w);
+  }
+}
+template <typename T, int D> __device__ __forceinline__ void row_frag_lds(RowFrag<T, D>& f, const char* tile, int row, int half) {
+#pragma unroll
+  for (int g = 0; g < Geo<T, D>::NCH / 2; ++g) {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(tile + lds_at<T, D>(row, 2 * g + half));
+    f.v[g] = __builtin_bit_cast(decltype(f.v[0] + f.v[0]), w);
+  }
+}
+template <int D> __device__ __forceinline__ f32x16 mma_rows(const RowFrag<bf16_t, D>& a, const RowFrag<bf16_t, D>& b, f32x16 c) {
+#pragma unroll
+  for (int g = 0; g < D / 16; ++g) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v[g], b.v[g], c, 0, 0, 0);
+  return c;
+}
+template <int D> __device__ __forceinline__ f32x16 mma_rows(const RowFrag<float, D>& a, const RowFrag<float, D>& b, f32x16 c) {
+#pragma unroll
+  for (int g = 0; g < D / 8; ++g)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[g][e], b.v[g][e], c, 0, 0, 0);
+  return c;
+}
+// a lane's half of a row's dot product
+template <int D> __device__ __forceinline__ float row_dot(const RowFrag<bf16_t, D>& a, const RowFrag<bf16_t, D>& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int g = 0; g < D / 16; ++g) {
+    const u32x4 x = __builtin_bit_cast(u32x4, a.v[g]), y = __builtin_bit_cast(u32x4, b.v[g]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16), s);
+      s = fmaf(__uint_as_float(x[e] & 0xffff0000u), __uint_as_float(y[e] & 0xffff0000u), s);
+    }
+  }
+  return s;
+}
+template <int D> __device__ __forceinline__ float row_dot(const RowFrag<float, D>& a, const RowFrag<float, D>& b) {
+  float s = 0.f;
+#pragma unroll
+  for (int g = 0; g < D / 8; ++g)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s = fmaf(a.v[g][e], b.v[g][e], s);
+  return s;
+}
+// 32 probabilities (or dS) of a lane's query / key, 16 registers, as the second product's operand
+template <typename T> struct PFrag;
+template <> struct PFrag<bf16_t> { bf16x8 v[2]; };
+template <> struct PFrag<float> { float v[16]; };
+__device__ __forceinline__ void p_frag(PFrag<bf16_t>& f, const float (&p)[16]) {
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack2bf(p[8 * g + 2 * e], p[8 * g + 2 * e + 1]);
+    f.v[g] = __builtin_bit_cast(bf16x8, w);
+  }
+}
+__device__ __forceinline__ void p_frag(PFrag<float>& f, const float (&p)[16]) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) f.v[r] = p[r];
+}
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+// acc[i] += (32-column block i of the tile rows row0 ... row0 + 31)^T x P: the second product, operand read transposed from the row-major tile
+template <int D> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[D / 32], const char* tile, int row0, const PFrag<bf16_t>& p, int lane) {
+  const int half = lane >> 5, t = lane & 15, g1 = (lane >> 4) & 1;
+#pragma unroll
+  for (int G = 0; G < 2; ++G)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const int chunk = 4 * i + 2 * g1 + ((t & 3) >> 1);
+      const int r = 16 * G + 4 * half + (t >> 2);          // (row0 is a multiple of 32: the chunk permutation does not see it)
+      const char* lo = tile + row0 * Geo<bf16_t, D>::ROWB + lds_at<bf16_t, D>(r, chunk) + (t & 1) * 8;
+      const char* hi = tile + row0 * Geo<bf16_t, D>::ROWB + lds_at<bf16_t, D>(r + 8, chunk) + (t & 1) * 8;
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lo));
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(hi));
+      const bf16x8 op = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op, p.v[G], acc[i], 0, 0, 0);
+    }
+}
+template <int D> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[D / 32], const char* tile, int row0, const PFrag<float>& p, int lane) {
+  const int half = lane >> 5, c = lane & 31;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int row = 8 * (r >> 2) + 4 * half + (r & 3);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const float a = *reinterpret_cast<const float*>(tile + row0 * Geo<float, D>::ROWB + lds_at<float, D>(row, 8 * i + (c >> 2)) + (c & 3) * 4);
+      acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p.v[r], acc[i], 0, 0, 0);
+    }
+  }
+}
+
+// ---- a tile's journey from memory through registers to LDS: ROWS rows of D elements by NT threads
+template <typename T, int D, int ROWS, int NT> struct Stage {
+  static constexpr int N = ROWS * Geo<T, D>::NCH / NT;     // 16-byte chunks per thread
+  static_assert(N >= 1 && ROWS * Geo<T, D>::NCH % NT == 0, "whole chunks per thread");
+  u32x4 w[N];
+  __device__ static __forceinline__ int row(int tid, int i) { return (tid + i * NT) / Geo<T, D>::NCH; }
+  __device__ static __forceinline__ int chunk(int tid, int i) { return (tid + i * NT) % Geo<T, D>::NCH; }
+  // rows first ... of a sequence that has `n` of them (n >= 1), base = its row 0; rows outside are read from the nearest one inside, and zeroed by put()
+  __device__ __forceinline__ void get(const T* base, int64_t ld, int first, int n, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      int j = first + row(tid, i);
+      j = j < 0 ? 0 : (j < n ? j : n - 1);
+      w[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base + (int64_t)j * ld) + chunk(tid, i) * 16);
+    }
+  }
+  // keep: bit i = chunk i belongs to a row that may be seen (a hidden row is stored as zeros: whatever it holds, NaN included, never meets a product)
+  __device__ __forceinline__ void put(char* tile, uint32_t keep, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const u32x4 z = {0, 0, 0, 0};
+      *reinterpret_cast<u32x4*>(tile + lds_at<T, D>(row(tid, i), chunk(tid, i))) = (keep >> i) & 1 ? w[i] : z;
+    }
+  }
+};
+
+// visibility of the 32 x 32 block (query positions lo ... hi, keys j0 ... j0 + 31) by position: 0 nothing, 1 some, 2 everything
+__device__ __forceinline__ int block_sight(int lo, int hi, int j0, int left, int right, int sinks, int Lk) {
+  if (j0 > hi + right || j0 >= Lk || (j0 + 31 < lo - left && j0 >= sinks)) return 0;
+  return (j0 + 31 <= lo + right && j0 + 31 < Lk && (j0 >= hi - left || j0 + 31 < sinks)) ? 2 : 1;
+}
+
+// dropout multipliers of a lane's query row qi and the 16 keys j0 + 8 (r >> 2) + 4 h + (r & 3): common.h attn_drop_block (one Philox call per 2 rows x 4 keys).
+// PAIRED: lanes c, c ^ 1 hold rows 2 n, 2 n + 1 of one sequence and head, so each draws two of the four blocks and they swap
+template <bool PAIRED> __device__ __forceinline__ void drop_of_query(float (&m)[16], const Params& p, int64_t sh, int qi, int j0, int half) {
+  const uint64_t seed = p.seed + (p.seed_state ? p.seed_state[0] : 0ull);
+  const uint32_t thr = attn_drop_threshold(p.drop_p);
+  u32x4 w[4];
+  if (PAIRED) {
+    const int par = (int)(threadIdx.x & 1);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const u32x4 own = attn_drop_block(seed, sh, p.Lk, qi, j0 + 8 * (2 * s + par) + 4 * half);
+      u32x4 oth;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) oth[e] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own[e], 0xB1, 0xF, 0xF, true);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { w[2 * s][e] = par ? oth[e] : own[e]; w[2 * s + 1][e] = par ? own[e] : oth[e]; }
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) w[s] = attn_drop_block(seed, sh, p.Lk, qi, j0 + 8 * s + 4 * half);
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) m[r] = attn_drop_pick(w[r >> 2], qi, r & 3, thr, p.inv_keep);
+}
+
+// which unit of work a workgroup has.  Units of one (sequence, k|v head) are neighbours and one XCD (workgroup index mod 8) gets a contiguous run of them, so
+// that a key tile read by the query tiles around it comes from that XCD's L2.  Packed sequences: heads outermost, so that a run holds every sequence.
+struct Unit { int b, hk, g, tile; bool real; };
+__device__ __forceinline__ Unit unit_of(const Params& p, int id, int n, int per_seq_tiles, int G) {
+  const int per = (n + 7) >> 3;
+  const int v = (id & 7) * per + (id >> 3);
+  Unit u{0, 0, 0, 0, v < n};
+  if (!u.real) return u;
+  u.g = v % G;
+  int w = v / G;
+  if (p.offsets) {
+    const int i = w % p.ntiles;
+    u.hk = w / p.ntiles;
+    u.b = p.tiles[2 * i];
+    u.tile = p.tiles[2 * i + 1];
+    u.real = u.b >= 0 && u.b < p.nseq && u.tile >= 0 && u.tile < (1 << 22);
+  } else {
+    u.tile = w % per_seq_tiles;
+    w /= per_seq_tiles;
+    u.hk = w % p.Hk;
+    u.b = w / p.Hk;
+  }
+  return u;
+}
+// rows of sequence b; packed offsets are clamped to the tensors, whatever they hold
+struct Rows { int64_t q0, k0; int lq, lk; };
+__device__ __forceinline__ Rows rows_of(const Params& p, int b) {
+  Rows r;
+  if (p.offsets) {
+    int64_t a = p.offsets[b], e = p.offsets[b + 1];
+    a = a < 0 ? 0 : (a > p.Mq ? p.Mq : a);
+    e = e < a ? a : (e > p.Mq ? p.Mq : e);
+    r.q0 = r.k0 = a;
+    r.lq = r.lk = (int)(e - a < p.Lk ? e - a : p.Lk);
+  } else {
+    r.q0 = (int64_t)b * p.Lq; r.k0 = (int64_t)b * p.Lk;
+    r.lq = p.Lq; r.lk = p.Lk;
+  }
+  return r;
+}
+// key tiles (of KT keys) that positions lo ... hi can see: nsink tiles from 0, then first ... first + n - nsink - 1
+struct TileList { int nsink, first, n; };
+template <int KT> __device__ __host__ __forceinline__ TileList tile_list(int lo, int hi, int left, int right, int sinks, int Lk) {
+  TileList t;
+  const int jhi = hi + right < Lk - 1 ? hi + right : Lk - 1;
+  int jlo = lo - left; if (jlo < 0) jlo = 0;
+  const int s = sinks < jhi + 1 ? sinks : jhi + 1;
+  t.nsink = s > 0 ? (s + KT - 1) / KT : 0;
+  t.first = jlo / KT; if (t.first < t.nsink) t.first = t.nsink;
+  const int last = jhi >= jlo ? jhi / KT : -1;
+  t.n = t.nsink + (last >= t.first ? last - t.first + 1 : 0);
+  return t;
+}
+__device__ __forceinline__ int tile_at(const TileList& t, int i) { return i < t.nsink ? i : t.first + i - t.nsink; }
+
+// what the keys of a tile look like through the key mask: 0 every value 0, 1 some not, 2 all hidden
+__device__ __forceinline__ int mask_state(float kb, bool on) {
+  const uint64_t any = __builtin_amdgcn_ballot_w64(on && kb != 0.f), seen = __builtin_amdgcn_ballot_w64(on && kb > -INFINITY);
+  return seen == 0 ? 2 : (any != 0 ? 1 : 0);
+}
+__device__ __forceinline__ float mask_value(float km) { return km > HIDDEN ? km * LOG2E_ : -INFINITY; }      // (NaN hides)
+
+// a lane's row of O: columns 32 i + 8 g + 4 h + e; four consecutive columns per store
+template <typename T, int D> __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[D / 32], float mul, int half) {
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = acc[i][4 * g + e] * mul;
+      store4(row + 32 * i + 8 * g + 4 * half, o);
+    }
+}
+
+// lanes of a wave exchange through LDS: its operations retire in order, so only the compiler has to keep them in place
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+
+// ---- host side
+inline int check_shape(int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, int Hk, int D, int left, int right, int sinks, int q_start, bool packed, int dtype) {
+  if (nseq < 0 || Lq < 0 || Lk < 0 || H < 1 || Hk < 1 || H % Hk || sinks < 0 || q_start < 0 || left < -1 || right < -1) { ctclip_set_error("win_attn: bad sizes (H a multiple of the k|v heads, window >= -1, sinks, q_start >= 0)"); return CTCLIP_EBADARG; }
+  if ((D != 32 && D != 64 && D != 128) || (dtype != DT_F32 && dtype != DT_BF16)) { ctclip_set_error("win_attn: heads of 32, 64 or 128, f32 or bf16"); return CTCLIP_EUNSUPPORTED; }
+  if (Lk > (1 << 29) || H > 65535 || (int64_t)Mq > ((int64_t)1 << 31) - 256 || (int64_t)Mk > ((int64_t)1 << 31) - 256) { ctclip_set_error("win_attn: too many rows or heads"); return CTCLIP_EUNSUPPORTED; }
+  if (packed ? (Lq != Lk || Mq != Mk || q_start) : ((int64_t)q_start + Lq > Lk || Mq != (int64_t)nseq * Lq || Mk != (int64_t)nseq * Lk)) { ctclip_set_error("win_attn: query rows must be positions of the key axis (q_start + Lq <= Lk); packed sequences: q and k|v share their rows"); return CTCLIP_EBADARG; }
+  return CTCLIP_OK;
+}
+inline int check_rows(const void* x, int64_t ld, int heads, int D, int dtype, bool written, const char* what) {
+  const int e = dtype == DT_F32 ? 4 : 2;
+  if (!x) { ctclip_set_error("win_attn: null tensor"); return CTCLIP_EBADARG; }
+  if ((reinterpret_cast<uintptr_t>(x) % 16) || (ld * e) % 16 || ld < 0 || (written && ld < (int64_t)heads * D)) { ctclip_set_error(what); return CTCLIP_EBADARG; }
+  return CTCLIP_OK;
+}
+inline void fill(Params& p, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, int Hk, int left, int right, int sinks, int q_start, float scale, float dropout_p,
+          uint64_t seed, const int32_t* offsets, const int32_t* tiles, int ntiles, const float* keymask) {
+  p.nseq = nseq; p.Lq = Lq; p.Lk = Lk; p.Mq = Mq; p.Mk = Mk; p.H = H; p.Hk = Hk; p.G = H / Hk;
+  p.left = left < 0 || left > Lk ? Lk : left; p.right = right < 0 || right > Lk ? Lk : right; p.sinks = sinks < Lk ? sinks : Lk; p.q_start = q_start;
+  p.scale = scale; p.scale2 = scale * LOG2E_;
+  p.seed = seed; p.seed_state = ctclip_step_state(); p.drop_p = dropout_p; p.inv_keep = dropout_p > 0.f ? 1.f / (1.f - dropout_p) : 1.f;
+  p.offsets = offsets; p.tiles = tiles; p.ntiles = ntiles; p.keymask = keymask;
+}
+
+template <auto KERNEL> int raise_lds(int bytes) {       // more than 64 KB of LDS is opted into, once per kernel and device
+  static bool done[64] = {};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) { ctclip_set_error("win_attn: no device"); return CTCLIP_EBADARG; }
+  if (!done[dev]) {
+    const hipError_t e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) { ctclip_set_error("win_attn: LDS size refused"); return -(1000 + (int)e); }
+    done[dev] = true;
+  }
+  return CTCLIP_OK;
+}
+
+}  // namespace win

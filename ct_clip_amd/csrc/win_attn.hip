@@ -1,0 +1,412 @@
+// Attention in a sliding window with sinks on gfx950, forward (definitions, operand layouts and LDS image: win_attn.h).
+//
+//   fwd_kernel   a workgroup owns 128 query rows of one (sequence, head), a wave 32 of them; the key tiles that the rows' windows and the sinks cover
+//                pass through a double-buffered LDS ring (one barrier per tile, the next tile's loads in flight under the current one's products).
+//   rows_kernel  few query rows against many keys (one token, the [CLS] row): the rows of all heads that share a k|v head are ONE 32-row block, the four
+//                waves take different key tiles and the axis is split over workgroups until the chip is full.  Bound by reading k and v once.
+//   join_kernel  folds the split passes of either.
+// One pass over the keys with the running maximum and sum of the softmax in f32, log2 domain.  P is rounded to the operand type (bf16: 2^-9 relative, one
+// rounding per probability) because the matrix cores read it; sums are taken of the unrounded values.
+#include "win_attn.h"
+
+namespace win {
+
+template <int D> struct SoftRow {          // the running softmax of a lane's query
+  f32x16 acc[D / 32];
+  float m, l;
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY; l = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+  }
+};
+
+// one 32-key block: scores -> running softmax -> acc.  pos = the lane's query position, kb = additive mask of the block's keys in LDS (or null)
+template <typename T, int D, bool DROP, bool PAIRED>
+__device__ __forceinline__ void key_block(SoftRow<D>& st, const RowFrag<T, D>& qf, const char* ktile, const char* vtile, int row0, const float* kb, const Params& p,
+                                          int j0, int pos, int lk, bool partial, int lane, int64_t sh, int qi) {
+  const int half = lane >> 5, c = lane & 31;
+  RowFrag<T, D> kf;
+  row_frag_lds<T, D>(kf, ktile, row0 + c, half);
+  f32x16 s;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = 0.f;
+  s = mma_rows<D>(kf, qf, s);
+  float v[16];
+  float sc = p.scale2;                                     // (scale > 0: the maximum may be taken of the unscaled scores; one rounding in the fma below)
+  if (kb) {
+    sc = 1.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(kb + 8 * g + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * g + e] = fmaf(s[4 * g + e], p.scale2, a[e]);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v[r] = s[r];
+  }
+  if (partial) {
+    const int b = j0 + 4 * half;
+    const int hi = (pos + p.right < lk - 1 ? pos + p.right : lk - 1) - b, lo = pos - p.left - b, sk = p.sinks - b;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int j = 8 * (r >> 2) + (r & 3);
+      v[r] = (j <= hi && (j >= lo || j < sk)) ? v[r] : -INFINITY;
+    }
+  }
+  float mx = v[0];
+#pragma unroll
+  for (int r = 1; r < 16; ++r) mx = fmaxf(mx, v[r]);
+  mx = half_max(mx);
+  const float mn = fmaxf(st.m, mx * sc);
+  const float ms = mn == -INFINITY ? 0.f : mn;             // nothing seen so far: every exp2 below is exp2(-inf) = 0
+  const float alpha = __builtin_amdgcn_exp2f(st.m - ms);
+  float pr[16], ps = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) { pr[r] = __builtin_amdgcn_exp2f(fmaf(v[r], sc, -ms)); ps += pr[r]; }
+  st.l = st.l * alpha + ps;
+  if (DROP) {                                              // on the normalised probabilities: the sum above stays undropped
+    float dm[16];
+    drop_of_query<PAIRED>(dm, p, sh, qi, j0, half);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) pr[r] *= dm[r];
+  }
+  PFrag<T> pf;
+  p_frag(pf, pr);
+  if (__builtin_amdgcn_ballot_w64(mn != st.m) != 0) {      // wave-uniform: no rescale while no maximum moved
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st.acc[i][r] *= alpha;
+  }
+  st.m = mn;
+  mma_cols<D>(st.acc, vtile, row0, pf, lane);
+}
+
+template <typename T, int D, bool DROP>
+__global__ __launch_bounds__(256, 2) void fwd_kernel(Params p, int nunits, int nqt) {
+  typedef Geo<T, D> G;
+  constexpr int KT = G::KT, TILE = KT * G::ROWB;
+  extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K | V], additive mask [2][KT], mask state [2]
+  float* kb = reinterpret_cast<float*>(lds + 4 * TILE);
+  int* state = reinterpret_cast<int*>(kb + 2 * KT);
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Unit u = unit_of(p, blockIdx.x, nunits, nqt, p.G);
+  if (!u.real) return;
+  const Rows rw = rows_of(p, u.b);
+  const int q0 = u.tile * QB;
+  if (q0 >= rw.lq) return;
+  const int h = u.hk * p.G + u.g, nq = rw.lq - q0 < QB ? rw.lq - q0 : QB;
+  const int lo = p.q_start + q0, hi = lo + nq - 1;                 // positions of the workgroup's rows
+  const TileList tl = tile_list<KT>(lo, hi, p.left, p.right, p.sinks, rw.lk);
+  const int i0 = (int)((int64_t)tl.n * blockIdx.y / p.nsplit), i1 = (int)((int64_t)tl.n * (blockIdx.y + 1) / p.nsplit);
+  const int jhi = hi + p.right, jlo = lo - p.left;                 // keys outside [jlo, jhi] and the sinks are seen by no row of the workgroup
+
+  int row = q0 + 32 * wave + c;
+  const bool real = row < rw.lq;
+  row = real ? row : rw.lq - 1;
+  const int wlo = lo + 32 * wave, whi = wlo + 31 < hi ? wlo + 31 : hi;      // the wave's positions (whi < wlo: it has none)
+  const int pos = p.q_start + row;
+  RowFrag<T, D> qf;
+  row_frag_global<T, D>(qf, reinterpret_cast<const T*>(p.q) + (rw.q0 + row) * p.ldq + (int64_t)h * D, half);
+  const T* kbase = reinterpret_cast<const T*>(p.k) + rw.k0 * p.ldk + (int64_t)u.hk * D;
+  const T* vbase = reinterpret_cast<const T*>(p.v) + rw.k0 * p.ldv + (int64_t)u.hk * D;
+  const float* mbase = p.keymask ? p.keymask + rw.k0 : nullptr;
+
+  typedef Stage<T, D, KT, 256> St;
+  St sk, sv;
+  uint32_t keep = 0;
+  float km = 0.f;
+  auto fetch = [&](int j0) {
+    sk.get(kbase, p.ldk, j0, rw.lk, tid);
+    sv.get(vbase, p.ldv, j0, rw.lk, tid);
+    keep = 0;
+#pragma unroll
+    for (int i = 0; i < St::N; ++i) {
+      const int j = j0 + St::row(tid, i);
+      bool on = j < rw.lk && j <= jhi && (j >= jlo || j < p.sinks);
+      if (mbase) on = on && mbase[j < rw.lk ? j : rw.lk - 1] > HIDDEN;
+      keep |= (uint32_t)on << i;
+    }
+    if (mbase) { const int j = j0 + (tid & (KT - 1)); km = mask_value(mbase[j < rw.lk ? j : rw.lk - 1]); }
+  };
+  auto deposit = [&](int buf) {
+    sk.put(lds + buf * 2 * TILE, keep, tid);
+    sv.put(lds + buf * 2 * TILE + TILE, keep, tid);
+    if (mbase && wave == 0) {
+      if (tid < KT) kb[buf * KT + tid] = km;
+      const int s = mask_state(km, tid < KT);
+      if (tid == 0) state[buf] = s;
+    }
+  };
+
+  SoftRow<D> st;
+  st.clear();
+  const int64_t sh = (int64_t)u.b * p.H + h;
+  if (i0 < i1) {
+    fetch(tile_at(tl, i0) * KT);
+    deposit(0);
+  }
+  __syncthreads();
+  for (int it = i0; it < i1; ++it) {
+    const int buf = (it - i0) & 1, j0 = tile_at(tl, it) * KT;
+    if (it + 1 < i1) fetch(tile_at(tl, it + 1) * KT);
+    const int ms = mbase ? __builtin_amdgcn_readfirstlane(state[buf]) : 0;
+    if (ms != 2) {
+#pragma unroll
+      for (int b = 0; b < KT / 32; ++b) {
+        const int sight = whi < wlo ? 0 : block_sight(wlo, whi, j0 + 32 * b, p.left, p.right, p.sinks, rw.lk);
+        if (sight)
+          key_block<T, D, DROP, true>(st, qf, lds + buf * 2 * TILE, lds + buf * 2 * TILE + TILE, 32 * b, ms ? kb + buf * KT + 32 * b : nullptr, p, j0 + 32 * b, pos,
+                                      rw.lk, sight == 1, lane, sh, row);
+      }
+    }
+    if (it + 1 < i1) deposit(buf ^ 1);
+    __syncthreads();
+  }
+  const float l = half_sum(st.l);
+  if (!real) return;
+  if (p.nsplit > 1) {
+    const int64_t r = ((int64_t)blockIdx.y * p.H + h) * p.Mq + rw.q0 + row;
+    const int64_t rows = (int64_t)p.nsplit * p.H * p.Mq;
+    store_row<float, D>(p.part + 2 * rows + r * D, st.acc, 1.f, half);
+    if (half == 0) { p.part[r] = st.m; p.part[rows + r] = l; }
+    return;
+  }
+  store_row<T, D>(reinterpret_cast<T*>(p.out) + (rw.q0 + row) * p.ldo + (int64_t)h * D, st.acc, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), half);
+  if (half == 0 && p.lse) p.lse[(int64_t)h * p.Mq + rw.q0 + row] = l == 0.f ? INFINITY : st.m + __builtin_amdgcn_logf(l);
+}
+
+// ---- few query rows: R = Lq * G <= 32 rows (row c = head g = c / Lq of the group, query c % Lq)
+template <typename T, int D, bool DROP>
+__global__ __launch_bounds__(256, 2) void rows_kernel(Params p, int nunits) {
+  typedef Geo<T, D> G;
+  constexpr int TILE = 32 * G::ROWB;
+  extern __shared__ __attribute__((aligned(16))) char lds[];       // four waves x [K | V] of 32 keys; reused to fold the waves
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Unit u = unit_of(p, blockIdx.x, nunits, 1, 1);
+  if (!u.real) return;
+  const Rows rw = rows_of(p, u.b);
+  const int R = rw.lq * p.G;
+  const int lo = p.q_start, hi = p.q_start + rw.lq - 1;
+  const TileList tl = tile_list<32>(lo, hi, p.left, p.right, p.sinks, rw.lk);
+  const int i0 = (int)((int64_t)tl.n * blockIdx.y / p.nsplit), i1 = (int)((int64_t)tl.n * (blockIdx.y + 1) / p.nsplit);
+  const int jhi = hi + p.right, jlo = lo - p.left;
+  const int rc = c < R ? c : R - 1;
+  const int g = rc / rw.lq, row = rc - g * rw.lq, h = u.hk * p.G + g, pos = p.q_start + row;
+  RowFrag<T, D> qf;
+  row_frag_global<T, D>(qf, reinterpret_cast<const T*>(p.q) + (rw.q0 + row) * p.ldq + (int64_t)h * D, half);
+  const T* kbase = reinterpret_cast<const T*>(p.k) + rw.k0 * p.ldk + (int64_t)u.hk * D;
+  const T* vbase = reinterpret_cast<const T*>(p.v) + rw.k0 * p.ldv + (int64_t)u.hk * D;
+  const float* mbase = p.keymask ? p.keymask + rw.k0 : nullptr;
+  char* ktile = lds + wave * (2 * TILE + 128);
+  char* vtile = ktile + TILE;
+  float* kb = reinterpret_cast<float*>(vtile + TILE);
+
+  typedef Stage<T, D, 32, 64> St;
+  St sk, sv;
+  uint32_t keep = 0;
+  float km = 0.f;
+  auto fetch = [&](int j0) {
+    sk.get(kbase, p.ldk, j0, rw.lk, lane);
+    sv.get(vbase, p.ldv, j0, rw.lk, lane);
+    keep = 0;
+#pragma unroll
+    for (int i = 0; i < St::N; ++i) {
+      const int j = j0 + St::row(lane, i);
+      bool on = j < rw.lk && j <= jhi && (j >= jlo || j < p.sinks);
+      if (mbase) on = on && mbase[j < rw.lk ? j : rw.lk - 1] > HIDDEN;
+      keep |= (uint32_t)on << i;
+    }
+    if (mbase) { const int j = j0 + c; km = mask_value(mbase[j < rw.lk ? j : rw.lk - 1]); }
+  };
+  SoftRow<D> st;
+  st.clear();
+  const int64_t sh = (int64_t)u.b * p.H + h;
+  int it = i0 + wave;
+  if (it < i1) fetch(tile_at(tl, it) * 32);
+  for (; it < i1; it += 4) {                                       // (no barrier: a wave's tiles are its own, and its LDS operations keep their order)
+    const int j0 = tile_at(tl, it) * 32;
+    sk.put(ktile, keep, lane);
+    sv.put(vtile, keep, lane);
+    int ms = 0;
+    if (mbase) { if (half == 0) kb[c] = km; ms = __builtin_amdgcn_readfirstlane(mask_state(km, true)); }
+    if (it + 4 < i1) fetch(tile_at(tl, it + 4) * 32);
+    wave_sync();
+    const int sight = block_sight(lo, hi, j0, p.left, p.right, p.sinks, rw.lk);
+    if (sight && ms != 2) key_block<T, D, DROP, false>(st, qf, ktile, vtile, 0, ms ? kb : nullptr, p, j0, pos, rw.lk, sight == 1, lane, sh, row);
+    wave_sync();
+  }
+  // fold the four waves: row maxima first, then sums and accumulators under the common maximum
+  float* fm = reinterpret_cast<float*>(lds);                       // [4][32] maxima, [4][32] sums, [4][32][D + 4] accumulators (+ 4: two lanes' rows a bank apart)
+  float* fl = fm + 128;
+  float* fa = fl + 128;
+  const float l = half_sum(st.l);
+  __syncthreads();
+  if (half == 0) { fm[wave * 32 + c] = st.m; fl[wave * 32 + c] = l; }
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 a = {st.acc[i][4 * q], st.acc[i][4 * q + 1], st.acc[i][4 * q + 2], st.acc[i][4 * q + 3]};
+      *reinterpret_cast<f32x4*>(fa + (wave * 32 + c) * (D + 4) + 32 * i + 8 * q + 4 * half) = a;
+    }
+  __syncthreads();
+  constexpr int PER = D / 8;                                       // eight threads per row, D / 8 columns each
+  const int fr = tid >> 3, fc = (tid & 7) * PER;
+  if (fr >= R) return;
+  float m = fm[fr];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) m = fmaxf(m, fm[w * 32 + fr]);
+  const float ms = m == -INFINITY ? 0.f : m;
+  float lsum = 0.f, o[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) o[e] = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = __builtin_amdgcn_exp2f(fm[w * 32 + fr] - ms);
+    lsum = fmaf(fl[w * 32 + fr], f, lsum);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] = fmaf(fa[(w * 32 + fr) * (D + 4) + fc + e], f, o[e]);
+  }
+  const int og = fr / rw.lq, orow = fr - og * rw.lq, oh = u.hk * p.G + og;
+  if (p.nsplit > 1) {
+    const int64_t r = ((int64_t)blockIdx.y * p.H + oh) * p.Mq + rw.q0 + orow, rows = (int64_t)p.nsplit * p.H * p.Mq;
+#pragma unroll
+    for (int e = 0; e < PER; e += 4) { const float t[4] = {o[e], o[e + 1], o[e + 2], o[e + 3]}; store4(p.part + 2 * rows + r * D + fc + e, t); }
+    if ((tid & 7) == 0) { p.part[r] = m; p.part[rows + r] = lsum; }
+    return;
+  }
+  const float mul = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
+  T* dst = reinterpret_cast<T*>(p.out) + (rw.q0 + orow) * p.ldo + (int64_t)oh * D + fc;
+#pragma unroll
+  for (int e = 0; e < PER; e += 4) { const float t[4] = {o[e] * mul, o[e + 1] * mul, o[e + 2] * mul, o[e + 3] * mul}; store4(dst + e, t); }
+  if ((tid & 7) == 0 && p.lse) p.lse[(int64_t)oh * p.Mq + rw.q0 + orow] = lsum == 0.f ? INFINITY : m + __builtin_amdgcn_logf(lsum);
+}
+
+// out = sum_s exp2(m_s - M) acc_s / sum_s exp2(m_s - M) l_s over the split passes; D / 4 threads per (head, row)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void join_kernel(Params p) {
+  const int64_t n = (int64_t)p.H * p.Mq, rows = (int64_t)p.nsplit * n;
+  const int64_t i = (int64_t)blockIdx.x * (256 / (D / 4)) + threadIdx.x / (D / 4);
+  const int col = (threadIdx.x % (D / 4)) * 4;
+  if (i >= n) return;
+  float m = -INFINITY;
+  for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, p.part[s * n + i]);
+  const float ms = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float f = __builtin_amdgcn_exp2f(p.part[s * n + i] - ms);
+    l = fmaf(p.part[rows + s * n + i], f, l);
+    float a[4];
+    load4(p.part + 2 * rows + (s * n + i) * D + col, a);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(a[e], f, o[e]);
+  }
+  const int64_t h = i / p.Mq, row = i - h * p.Mq;
+  const float mul = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= mul;
+  store4(reinterpret_cast<T*>(p.out) + row * p.ldo + h * D + col, o);
+  if (col == 0 && p.lse) p.lse[i] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// ---- host side
+struct Plan { bool rows; int nsplit; };
+// Which kernel, and over how many workgroups a key axis is split: see the figures at each rule.
+inline Plan plan(int nseq, int Lq, int Lk, int H, int Hk, int left, int right, int sinks, int q_start, bool packed) {
+  Plan pl{false, 1};
+  const int G = H / Hk;
+  if (packed) return pl;
+  if ((int64_t)Lq * G <= 32) {
+    pl.rows = true;
+    const TileList tl = tile_list<32>(q_start, q_start + Lq - 1, left, right, sinks, Lk);
+    const int64_t units = (int64_t)nseq * Hk;
+    int64_t s = cdiv(512, units);
+    if (s > tl.n / 8) s = tl.n / 8;
+    pl.nsplit = (int)(s < 1 ? 1 : s);
+    return pl;
+  }
+  const int64_t units = (int64_t)nseq * H * cdiv(Lq, QB);
+  if (units < 256) {
+    const int last = (int)((Lq - 1) / QB) * QB;
+    const TileList tl = tile_list<64>(q_start + last, q_start + Lq - 1, left, right, sinks, Lk);
+    int64_t s = cdiv(512, units);
+    if (s > tl.n / 4) s = tl.n / 4;
+    pl.nsplit = (int)(s < 1 ? 1 : s);
+  }
+  return pl;
+}
+
+template <typename T, int D, bool DROP> int launch_fwd(Params& p, const Plan& pl, hipStream_t s) {
+  typedef Geo<T, D> G;
+  if (pl.rows) {
+    const int64_t nu = (int64_t)p.nseq * p.Hk;
+    if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many sequences"); return CTCLIP_EUNSUPPORTED; }
+    int lds = 4 * (2 * 32 * G::ROWB + 128);
+    const int fold = 1024 + 4 * 32 * (D + 4) * 4;
+    if (fold > lds) lds = fold;
+    const int rc = raise_lds<rows_kernel<T, D, DROP>>(lds);
+    if (rc) return rc;
+    hipLaunchKernelGGL((rows_kernel<T, D, DROP>), dim3((unsigned)(8 * cdiv(nu, 8)), p.nsplit), dim3(256), lds, s, p, (int)nu);
+  } else {
+    const int nqt = (int)cdiv(p.Lq, QB);
+    const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.H : (int64_t)p.nseq * p.H * nqt;
+    if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
+    const int lds = 4 * G::KT * G::ROWB + 2 * G::KT * 4 + 16;
+    const int rc = raise_lds<fwd_kernel<T, D, DROP>>(lds);
+    if (rc) return rc;
+    hipLaunchKernelGGL((fwd_kernel<T, D, DROP>), dim3((unsigned)(8 * cdiv(nu, 8)), p.nsplit), dim3(256), lds, s, p, (int)nu, nqt);
+  }
+  int rc = ctclip_check_launch("win_attn_fwd");
+  if (rc || p.nsplit == 1) return rc;
+  hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)cdiv((int64_t)p.H * p.Mq, 256 / (D / 4))), dim3(256), 0, s, p);
+  return ctclip_check_launch("win_attn_fwd join");
+}
+template <typename T, int D> int launch_fwd_d(Params& p, const Plan& pl, hipStream_t s) {
+  return p.drop_p > 0.f ? launch_fwd<T, D, true>(p, pl, s) : launch_fwd<T, D, false>(p, pl, s);
+}
+template <typename T> int launch_fwd_t(Params& p, const Plan& pl, int D, hipStream_t s) {
+  return D == 32 ? launch_fwd_d<T, 32>(p, pl, s) : (D == 64 ? launch_fwd_d<T, 64>(p, pl, s) : launch_fwd_d<T, 128>(p, pl, s));
+}
+}  // namespace win
+
+// bytes of workspace of ctclip_win_attn_fwd (split passes; 0: none)
+extern "C" int64_t ctclip_win_attn_fwd_workspace(int nseq, int Lq, int Lk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int packed) {
+  if (nseq < 1 || Lq < 1 || Lk < 1 || H < 1 || Hk < 1 || H % Hk || packed) return 0;
+  const int l = left < 0 || left > Lk ? Lk : left, r = right < 0 || right > Lk ? Lk : right, s = sinks < Lk ? sinks : Lk;
+  const win::Plan pl = win::plan(nseq, Lq, Lk, H, Hk, l, r, s, q_start, false);
+  return pl.nsplit > 1 ? (int64_t)pl.nsplit * H * nseq * Lq * (D + 2) * 4 : 0;
+}
+
+// q (Mq, H D), k | v (Mk, Hk D) -> out (Mq, H D), lse [H][Mq] f32 (log2 domain; optional: backward needs it).  Sequence b = rows b Lq ... of q and b Lk ... of
+// k | v; with offsets (nseq + 1, int32) the rows offsets[b] ... offsets[b + 1] - 1 of all three (Lq = Lk = the longest), tiles = (sequence, 128-row tile) pairs.
+// keymask: additive f32 per key row; a value <= -1e30 or NaN hides the key, whatever k and v hold there.
+extern "C" int ctclip_win_attn_fwd(const void* q, const void* k, const void* v, const float* keymask, const int32_t* offsets, const int32_t* tiles, int ntiles, void* out,
+                                   float* lse, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, int Hk, int D, int left, int right, int sinks, int q_start,
+                                   int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, float dropout_p, uint64_t dropout_seed, int dtype, void* workspace,
+                                   int64_t workspace_bytes, hipStream_t stream) {
+  using namespace win;
+  int rc = check_shape(nseq, Lq, Lk, Mq, Mk, H, Hk, D, left, right, sinks, q_start, offsets != nullptr, dtype);
+  if (rc) return rc;
+  if (!(scale > 0.f) || !(scale < 1e30f) || !(dropout_p >= 0.f) || !(dropout_p < 1.f)) { ctclip_set_error("win_attn_fwd: scale > 0, 0 <= dropout < 1"); return CTCLIP_EBADARG; }
+  if (nseq == 0 || Lq == 0 || (offsets && ntiles == 0)) return CTCLIP_OK;
+  if (offsets && (!tiles || ntiles < 0)) { ctclip_set_error("win_attn_fwd: packed sequences need their tiles"); return CTCLIP_EBADARG; }
+  if ((rc = check_rows(q, ldq, H, D, dtype, false, "win_attn_fwd: q rows 16-byte aligned")) || (rc = check_rows(k, ldk, Hk, D, dtype, false, "win_attn_fwd: k rows 16-byte aligned")) ||
+      (rc = check_rows(v, ldv, Hk, D, dtype, false, "win_attn_fwd: v rows 16-byte aligned")) || (rc = check_rows(out, ldo, H, D, dtype, true, "win_attn_fwd: out rows 16-byte aligned, apart"))) return rc;
+  Params p{};
+  fill(p, nseq, Lq, Lk, Mq, Mk, H, Hk, left, right, sinks, q_start, scale, dropout_p, dropout_seed, offsets, tiles, ntiles, keymask);
+  p.q = q; p.k = k; p.v = v; p.out = out; p.lse = lse; p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo;
+  const Plan pl = plan(nseq, Lq, Lk, H, Hk, p.left, p.right, p.sinks, q_start, offsets != nullptr);
+  p.nsplit = pl.nsplit;
+  if (p.nsplit > 1) {
+    if (!workspace || workspace_bytes < (int64_t)p.nsplit * H * Mq * (D + 2) * 4 || reinterpret_cast<uintptr_t>(workspace) % 16) { ctclip_set_error("win_attn_fwd: workspace"); return CTCLIP_EWORKSPACE; }
+    p.part = (float*)workspace;
+  }
+  return dtype == DT_F32 ? launch_fwd_t<float>(p, pl, D, stream) : launch_fwd_t<bf16_t>(p, pl, D, stream);
+}

@@ -1,0 +1,548 @@
+// Attention in a sliding window with sinks on gfx950, backward (definitions, operand layouts and LDS image: win_attn.h).
+//
+// With P from the forward pass's log-sum-exp and Delta = rowsum(dO o O):  dV = P^T dO,  dS = P o (dO V^T - Delta),  dQ = scale dS K,  dK = scale dS^T Q.
+//   dq_kernel     query rows as in the forward kernel: S^T, dP^T with a query per lane, dQ^T += K^T dS^T.  Also writes Delta.
+//   dkv_kernel    128 keys of one (sequence, k|v head), 32 per wave: k, v and both gradients stay in registers while the query rows whose windows hold the keys pass
+//                 through a double-buffered LDS ring, for every query head that shares the keys: their gradients are summed here, no atomics.
+//   dkv_sink_kernel  the sinks meet EVERY later row: one key block would walk the whole sequence while all others walk a window.  The pairs (sink, row beyond its
+//                 window) are a pass of their own, split over the rows, a wave per 32-row tile; f32 partial sums.
+//   dkv_reduce_kernel  adds the partial sums of split keys in a fixed order.  Every result is bit-reproducible.
+// Seven products per visible block (five are needed at least; the other two are S and dP again, because dQ across key tiles would need float atomics).
+#include "win_attn.h"
+
+namespace win {
+
+template <typename T, int D, bool DROP>
+__global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nqt) {
+  typedef Geo<T, D> G;
+  constexpr int KT = G::KT, TILE = KT * G::ROWB;
+  extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K | V], additive mask [2][KT], mask state [2]
+  float* kb = reinterpret_cast<float*>(lds + 4 * TILE);
+  int* state = reinterpret_cast<int*>(kb + 2 * KT);
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Unit u = unit_of(p, blockIdx.x, nunits, nqt, p.G);
+  if (!u.real) return;
+  const Rows rw = rows_of(p, u.b);
+  const int q0 = u.tile * QB;
+  if (q0 >= rw.lq) return;
+  const int h = u.hk * p.G + u.g, nq = rw.lq - q0 < QB ? rw.lq - q0 : QB;
+  const int lo = p.q_start + q0, hi = lo + nq - 1;
+  const TileList tl = tile_list<KT>(lo, hi, p.left, p.right, p.sinks, rw.lk);
+  const int jhi = hi + p.right, jlo = lo - p.left;
+
+  int row = q0 + 32 * wave + c;
+  const bool real = row < rw.lq;
+  row = real ? row : rw.lq - 1;
+  const int wlo = lo + 32 * wave, whi = wlo + 31 < hi ? wlo + 31 : hi;
+  const int pos = p.q_start + row;
+  RowFrag<T, D> qf, df;
+  row_frag_global<T, D>(qf, reinterpret_cast<const T*>(p.q) + (rw.q0 + row) * p.ldq + (int64_t)h * D, half);
+  row_frag_global<T, D>(df, reinterpret_cast<const T*>(p.dout) + (rw.q0 + row) * p.lddo + (int64_t)h * D, half);
+  float delta;
+  {
+    RowFrag<T, D> of;
+    row_frag_global<T, D>(of, reinterpret_cast<const T*>(p.o) + (rw.q0 + row) * p.ldo + (int64_t)h * D, half);
+    delta = half_sum(row_dot<D>(of, df));
+  }
+  const float lse = p.lse[(int64_t)h * p.Mq + rw.q0 + row];
+  if (real && half == 0) p.delta[(int64_t)h * p.Mq + rw.q0 + row] = delta;
+  const T* kbase = reinterpret_cast<const T*>(p.k) + rw.k0 * p.ldk + (int64_t)u.hk * D;
+  const T* vbase = reinterpret_cast<const T*>(p.v) + rw.k0 * p.ldv + (int64_t)u.hk * D;
+  const float* mbase = p.keymask ? p.keymask + rw.k0 : nullptr;
+
+  typedef Stage<T, D, KT, 256> St;
+  St sk, sv;
+  uint32_t keep = 0;
+  float km = 0.f;
+  auto fetch = [&](int j0) {
+    sk.get(kbase, p.ldk, j0, rw.lk, tid);
+    sv.get(vbase, p.ldv, j0, rw.lk, tid);
+    keep = 0;
+#pragma unroll
+    for (int i = 0; i < St::N; ++i) {
+      const int j = j0 + St::row(tid, i);
+      bool on = j < rw.lk && j <= jhi && (j >= jlo || j < p.sinks);
+      if (mbase) on = on && mbase[j < rw.lk ? j : rw.lk - 1] > HIDDEN;
+      keep |= (uint32_t)on << i;
+    }
+    if (mbase) { const int j = j0 + (tid & (KT - 1)); km = mask_value(mbase[j < rw.lk ? j : rw.lk - 1]); }
+  };
+  auto deposit = [&](int buf) {
+    sk.put(lds + buf * 2 * TILE, keep, tid);
+    sv.put(lds + buf * 2 * TILE + TILE, keep, tid);
+    if (mbase && wave == 0) {
+      if (tid < KT) kb[buf * KT + tid] = km;
+      const int s = mask_state(km, tid < KT);
+      if (tid == 0) state[buf] = s;
+    }
+  };
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+  const int64_t sh = (int64_t)u.b * p.H + h;
+  if (tl.n > 0) {
+    fetch(tile_at(tl, 0) * KT);
+    deposit(0);
+  }
+  __syncthreads();
+  for (int it = 0; it < tl.n; ++it) {
+    const int buf = it & 1, j0 = tile_at(tl, it) * KT;
+    if (it + 1 < tl.n) fetch(tile_at(tl, it + 1) * KT);
+    const int ms = mbase ? __builtin_amdgcn_readfirstlane(state[buf]) : 0;
+    if (ms != 2) {
+      const char* ktile = lds + buf * 2 * TILE;
+#pragma unroll
+      for (int b = 0; b < KT / 32; ++b) {
+        const int jb = j0 + 32 * b;
+        const int sight = whi < wlo ? 0 : block_sight(wlo, whi, jb, p.left, p.right, p.sinks, rw.lk);
+        if (!sight) continue;
+        RowFrag<T, D> kf;
+        row_frag_lds<T, D>(kf, ktile, 32 * b + c, half);
+        f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+        s = mma_rows<D>(kf, qf, s);
+        row_frag_lds<T, D>(kf, ktile + TILE, 32 * b + c, half);
+        dp = mma_rows<D>(kf, df, dp);
+        float pr[16];
+        if (ms) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(kb + buf * KT + 32 * b + 8 * g + 4 * half);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pr[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], p.scale2, a[e] - lse));
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, -lse));
+        }
+        if (sight == 1) {
+          const int bb = jb + 4 * half;
+          const int jh = (pos + p.right < rw.lk - 1 ? pos + p.right : rw.lk - 1) - bb, jl = pos - p.left - bb, sk_ = p.sinks - bb;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = 8 * (r >> 2) + (r & 3);
+            pr[r] = (j <= jh && (j >= jl || j < sk_)) ? pr[r] : 0.f;
+          }
+        }
+        if (DROP) {
+          float dm[16];
+          drop_of_query<true>(dm, p, sh, row, jb, half);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] *= dm[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) pr[r] *= dp[r] - delta;
+        PFrag<T> pf;
+        p_frag(pf, pr);
+        mma_cols<D>(acc, ktile, 32 * b, pf, lane);
+      }
+    }
+    if (it + 1 < tl.n) deposit(buf ^ 1);
+    __syncthreads();
+  }
+  if (real) store_row<T, D>(reinterpret_cast<T*>(p.dq) + (rw.q0 + row) * p.lddq + (int64_t)h * D, acc, p.scale, half);
+}
+
+// the 32 queries of a staged tile (rows row0 ... of it) against the 32 keys of a wave
+template <typename T, int D> struct KeyState {
+  RowFrag<T, D> kf, vf;
+  f32x16 dk[D / 32], dv[D / 32];
+};
+// dropout multipliers of a lane's key and the 16 queries row + 8 (r >> 2) + 4 h + (r & 3).  The four lanes of a key quad need the same eight blocks (2 rows x 4 keys
+// each): every lane draws two and the words travel by DPP quad broadcasts.
+template <int LANE> __device__ __forceinline__ uint32_t quad_bcast(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, LANE * 0x55, 0xF, 0xF, true); }
+__device__ __forceinline__ void drop_of_key(float (&m)[16], const Params& p, int64_t sh, int row, int j, int half) {
+  const uint64_t seed = p.seed + (p.seed_state ? p.seed_state[0] : 0ull);
+  const uint32_t thr = attn_drop_threshold(p.drop_p);
+  const int ln = (int)(threadIdx.x & 3);
+  u32x4 own[2];                            // blocks 2 ln, 2 ln + 1: rows row + 8 ln + 4 h + {0, 1}, {2, 3}
+#pragma unroll
+  for (int s = 0; s < 2; ++s) own[s] = attn_drop_block(seed, sh, p.Lk, row + 8 * ln + 4 * half + 2 * s, j);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    u32x4 w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[0][e] = quad_bcast<0>(own[s][e]); w[1][e] = quad_bcast<1>(own[s][e]); w[2][e] = quad_bcast<2>(own[s][e]); w[3][e] = quad_bcast<3>(own[s][e]);
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) m[4 * g + 2 * s + e] = attn_drop_pick(w[g], e, j, thr, p.inv_keep);
+  }
+}
+// FAR: the sink pass (keys seen because they are sinks, j < i - left); otherwise the window (i - left <= j <= i + right)
+template <typename T, int D, bool DROP, bool FAR>
+__device__ __forceinline__ void query_block(KeyState<T, D>& st, const char* qtile, const char* dtile, const float* lse, const float* delta, int row0, const Params& p, int row,
+                                            int j, float kbias, bool partial, int lane, int64_t sh) {
+  const int half = lane >> 5, c = lane & 31;
+  RowFrag<T, D> f;
+  row_frag_lds<T, D>(f, qtile, row0 + c, half);
+  f32x16 s, dp;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+  s = mma_rows<D>(f, st.kf, s);
+  row_frag_lds<T, D>(f, dtile, row0 + c, half);
+  dp = mma_rows<D>(f, st.vf, dp);
+  float pr[16], ds[16];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(lse + row0 + 8 * g + 4 * half);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pr[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], p.scale2, kbias - a[e]));
+  }
+  if (partial) {                           // row >= j - right, row <= j + left (positions), or beyond: row > j + left and j a sink
+    const int b = p.q_start + row + 4 * half;
+    const int rl = j - p.right - b, rh = j + p.left - b;
+    const bool sink = j < p.sinks;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int i = 8 * (r >> 2) + (r & 3);
+      pr[r] = (FAR ? (sink && i > rh) : (i >= rl && i <= rh)) ? pr[r] : 0.f;
+    }
+  }
+  float dm[16];
+  if (DROP) drop_of_key(dm, p, sh, row, j, half);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 d = *reinterpret_cast<const f32x4*>(delta + row0 + 8 * g + 4 * half);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = 4 * g + e;
+      ds[r] = pr[r] * ((DROP ? dp[r] * dm[r] : dp[r]) - d[e]);
+      if (DROP) pr[r] *= dm[r];
+    }
+  }
+  PFrag<T> pf;
+  p_frag(pf, pr);
+  mma_cols<D>(st.dv, dtile, row0, pf, lane);
+  p_frag(pf, ds);
+  mma_cols<D>(st.dk, qtile, row0, pf, lane);
+}
+
+// a wave's 32 keys into registers; hidden keys and keys past the end are zeros and carry a bias of -inf
+template <typename T, int D> __device__ __forceinline__ float load_keys(KeyState<T, D>& st, const Params& p, const Rows& rw, int hk, int j, int half) {
+  const int jr = j < rw.lk ? j : rw.lk - 1;
+  const float km = p.keymask ? p.keymask[rw.k0 + jr] : 0.f;
+  const bool on = j < rw.lk && km > HIDDEN;
+  row_frag_global<T, D>(st.kf, reinterpret_cast<const T*>(p.k) + (rw.k0 + jr) * p.ldk + (int64_t)hk * D, half);
+  row_frag_global<T, D>(st.vf, reinterpret_cast<const T*>(p.v) + (rw.k0 + jr) * p.ldv + (int64_t)hk * D, half);
+  if (!on) { row_frag_zero<T, D>(st.kf); row_frag_zero<T, D>(st.vf); }
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) { st.dk[i][r] = 0.f; st.dv[i][r] = 0.f; }
+  return on ? km * LOG2E_ : -INFINITY;
+}
+
+template <typename T, int D> struct QTile { static constexpr int ROWS = Geo<T, D>::NCH >= 8 ? 32 : 64; };      // query rows of a dK / dV step: a chunk per thread at least
+
+// where the partial sums of key j lie: split passes hold every key, unsplit ones the keys of the sink blocks
+__device__ __forceinline__ int64_t part_row(const Params& p, const Rows& rw, int b, int hk, int j) {
+  return p.nsplit > 1 ? (int64_t)hk * p.Mk + rw.k0 + j : ((int64_t)b * p.Hk + hk) * p.s32 + j;
+}
+__host__ __device__ inline int64_t part_rows(const Params& p) { return p.nsplit > 1 ? (int64_t)p.Hk * p.Mk : (int64_t)p.nseq * p.Hk * p.s32; }
+__host__ __device__ inline int64_t sink_rows(const Params& p) { return (int64_t)p.nseq * p.Hk * p.s32; }
+
+template <typename T, int D, bool DROP, int WGS>
+__global__ __launch_bounds__(256, WGS) void dkv_kernel(Params p, int nunits, int nkt) {
+  typedef Geo<T, D> G;
+  constexpr int QT = QTile<T, D>::ROWS, TILE = QT * G::ROWB;
+  extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][Q | dO], then [2][lse | Delta] of the rows
+  float* stat = reinterpret_cast<float*>(lds + 4 * TILE);
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Unit u = unit_of(p, blockIdx.x, nunits, nkt, 1);
+  if (!u.real) return;
+  const Rows rw = rows_of(p, u.b);
+  const int k0 = u.tile * QB;
+  if (k0 >= rw.lk) return;
+  const int kend = k0 + QB - 1 < rw.lk - 1 ? k0 + QB - 1 : rw.lk - 1;
+  // rows whose windows hold one of the keys
+  int rlo = k0 - p.right - p.q_start, rhi = kend + p.left - p.q_start;
+  rlo = rlo < 0 ? 0 : rlo;
+  rhi = rhi < rw.lq - 1 ? rhi : rw.lq - 1;
+  const int t0 = rlo / QT, nt = rhi >= rlo ? rhi / QT - t0 + 1 : 0, steps = nt * p.G;
+  const int i0 = (int)((int64_t)steps * blockIdx.y / p.nsplit), i1 = (int)((int64_t)steps * (blockIdx.y + 1) / p.nsplit);
+
+  const int jw = k0 + 32 * wave, j = jw + c;
+  KeyState<T, D> st;
+  const float kbias = load_keys<T, D>(st, p, rw, u.hk, j, half);
+  const bool any = __builtin_amdgcn_ballot_w64(kbias > -INFINITY) != 0;      // wave-uniform
+  typedef Stage<T, D, QT, 256> St;
+  St sq, sd;
+  uint32_t keep = 0;
+  float s_lse = 0.f, s_del = 0.f;
+  auto fetch = [&](int i) {
+    const int g = i / nt, r0 = (t0 + i - g * nt) * QT, h = u.hk * p.G + g;
+    sq.get(reinterpret_cast<const T*>(p.q) + rw.q0 * p.ldq + (int64_t)h * D, p.ldq, r0, rw.lq, tid);
+    sd.get(reinterpret_cast<const T*>(p.dout) + rw.q0 * p.lddo + (int64_t)h * D, p.lddo, r0, rw.lq, tid);
+    keep = 0;
+#pragma unroll
+    for (int n = 0; n < St::N; ++n) keep |= (uint32_t)(r0 + St::row(tid, n) < rw.lq) << n;
+    if (tid < QT) {
+      const int r = r0 + tid;
+      const int64_t at = (int64_t)h * p.Mq + rw.q0 + (r < rw.lq ? r : rw.lq - 1);
+      s_lse = r < rw.lq ? p.lse[at] : INFINITY;
+      s_del = r < rw.lq ? p.delta[at] : 0.f;
+    }
+  };
+  auto deposit = [&](int buf) {
+    sq.put(lds + buf * 2 * TILE, keep, tid);
+    sd.put(lds + buf * 2 * TILE + TILE, keep, tid);
+    if (tid < QT) { stat[buf * 2 * QT + tid] = s_lse; stat[buf * 2 * QT + QT + tid] = s_del; }
+  };
+  if (i0 < i1) {
+    fetch(i0);
+    deposit(0);
+  }
+  __syncthreads();
+  for (int i = i0; i < i1; ++i) {
+    const int buf = (i - i0) & 1;
+    if (i + 1 < i1) fetch(i + 1);
+    const int g = i / nt, r0 = (t0 + i - g * nt) * QT;
+    const int64_t sh = (int64_t)u.b * p.H + u.hk * p.G + g;
+#pragma unroll
+    for (int b = 0; b < QT / 32; ++b) {
+      const int lo = p.q_start + r0 + 32 * b, last = p.q_start + rw.lq - 1;
+      const int sight = any && lo <= last ? block_sight(lo, lo + 31 < last ? lo + 31 : last, jw, p.left, p.right, 0, rw.lk) : 0;
+      if (sight)
+        query_block<T, D, DROP, false>(st, lds + buf * 2 * TILE, lds + buf * 2 * TILE + TILE, stat + buf * 2 * QT, stat + buf * 2 * QT + QT, 32 * b, p, r0 + 32 * b, j,
+                                       kbias, sight == 1, lane, sh);
+    }
+    if (i + 1 < i1) deposit(buf ^ 1);
+    __syncthreads();
+  }
+  if (j >= rw.lk) return;
+  if (p.nsplit > 1 || jw < p.s32) {
+    const int64_t N = part_rows(p), r = (int64_t)blockIdx.y * N + part_row(p, rw, u.b, u.hk, j);
+    store_row<float, D>(p.part + r * D, st.dk, 1.f, half);
+    store_row<float, D>(p.part + ((int64_t)p.nsplit * N + r) * D, st.dv, 1.f, half);
+    return;
+  }
+  store_row<T, D>(reinterpret_cast<T*>(p.dk) + (rw.k0 + j) * p.lddk + (int64_t)u.hk * D, st.dk, p.scale, half);
+  store_row<T, D>(reinterpret_cast<T*>(p.dv) + (rw.k0 + j) * p.lddv + (int64_t)u.hk * D, st.dv, 1.f, half);
+}
+
+template <typename T, int D, bool DROP>
+__global__ __launch_bounds__(256, 1) void dkv_sink_kernel(Params p, int nblk) {
+  typedef Geo<T, D> G;
+  constexpr int TILE = 32 * G::ROWB;
+  extern __shared__ __attribute__((aligned(16))) char lds[];       // four waves x [Q | dO | lse, Delta] of 32 rows; reused to fold the waves
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int blk = blockIdx.x % nblk, hk = (blockIdx.x / nblk) % p.Hk, b = blockIdx.x / (nblk * p.Hk);
+  const Rows rw = rows_of(p, b);
+  const int jw = 32 * blk, j = jw + c;
+  if (jw >= rw.lk) return;
+  int rlo = jw + p.left + 1 - p.q_start;                           // first row that has a key of this block beyond its window
+  rlo = rlo < 0 ? 0 : rlo;
+  const int t0 = rlo / 32, nt = rw.lq > rlo ? (rw.lq - 1) / 32 - t0 + 1 : 0, steps = nt * p.G;
+  const int i0 = (int)((int64_t)steps * blockIdx.y / p.nchunk), i1 = (int)((int64_t)steps * (blockIdx.y + 1) / p.nchunk);
+  KeyState<T, D> st;
+  const float kbias = load_keys<T, D>(st, p, rw, hk, j, half);
+  char* qtile = lds + wave * (2 * TILE + 256);
+  char* dtile = qtile + TILE;
+  float* stat = reinterpret_cast<float*>(dtile + TILE);
+  typedef Stage<T, D, 32, 64> St;
+  St sq, sd;
+  uint32_t keep = 0;
+  float s_stat = 0.f;
+  auto fetch = [&](int i) {
+    const int g = i / nt, r0 = (t0 + i - g * nt) * 32, h = hk * p.G + g;
+    sq.get(reinterpret_cast<const T*>(p.q) + rw.q0 * p.ldq + (int64_t)h * D, p.ldq, r0, rw.lq, lane);
+    sd.get(reinterpret_cast<const T*>(p.dout) + rw.q0 * p.lddo + (int64_t)h * D, p.lddo, r0, rw.lq, lane);
+    keep = 0;
+#pragma unroll
+    for (int n = 0; n < St::N; ++n) keep |= (uint32_t)(r0 + St::row(lane, n) < rw.lq) << n;
+    const int r = r0 + c;
+    const int64_t at = (int64_t)h * p.Mq + rw.q0 + (r < rw.lq ? r : rw.lq - 1);
+    s_stat = half ? p.delta[at] : p.lse[at];
+    if (r >= rw.lq) s_stat = half ? 0.f : INFINITY;
+  };
+  int i = i0 + wave;
+  if (i < i1) fetch(i);
+  for (; i < i1; i += 4) {
+    const int g = i / nt, r0 = (t0 + i - g * nt) * 32;
+    sq.put(qtile, keep, lane);
+    sd.put(dtile, keep, lane);
+    stat[lane] = s_stat;                                           // 32 log-sum-exps, then 32 Deltas
+    if (i + 4 < i1) fetch(i + 4);
+    wave_sync();
+    query_block<T, D, DROP, true>(st, qtile, dtile, stat, stat + 32, 0, p, r0, j, kbias, true, lane, (int64_t)b * p.H + hk * p.G + g);
+    wave_sync();
+  }
+  // fold the four waves, dK then dV, in the order of the waves
+  float* fa = reinterpret_cast<float*>(lds);                       // [4][32][D + 4]
+  const int64_t r = ((int64_t)b * p.Hk + hk) * p.s32 + jw, S = sink_rows(p);
+  float* base = p.part + (int64_t)2 * p.nsplit * part_rows(p) * D;
+  constexpr int PER = D / 8;
+  const int fr = tid >> 3, fc = (tid & 7) * PER;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& a = which ? st.dv[n] : st.dk[n];
+        const f32x4 t = {a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+        *reinterpret_cast<f32x4*>(fa + (wave * 32 + c) * (D + 4) + 32 * n + 8 * q + 4 * half) = t;
+      }
+    __syncthreads();
+    float* dst = base + (((int64_t)which * p.nchunk + blockIdx.y) * S + r + fr) * D + fc;
+#pragma unroll
+    for (int e = 0; e < PER; e += 4) {
+      float t[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float* a = fa + fr * (D + 4) + fc + e + x;
+        t[x] = a[0] + a[32 * (D + 4)] + a[64 * (D + 4)] + a[96 * (D + 4)];
+      }
+      store4(dst + e, t);
+    }
+  }
+}
+
+// keys whose sums came in parts: D / 4 threads per (k|v head, key)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void dkv_reduce_kernel(Params p, int keys) {
+  const int b = blockIdx.z, hk = blockIdx.y;
+  const Rows rw = rows_of(p, b);
+  const int j = blockIdx.x * (256 / (D / 4)) + threadIdx.x / (D / 4), col = (threadIdx.x % (D / 4)) * 4;
+  if (j >= keys || j >= rw.lk) return;
+  const int64_t N = part_rows(p), S = sink_rows(p), r = part_row(p, rw, b, hk, j);
+  const float* sink = p.part + 2 * p.nsplit * N * D;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    float o[4] = {0.f, 0.f, 0.f, 0.f}, a[4];
+    for (int s = 0; s < p.nsplit; ++s) {
+      load4(p.part + (((int64_t)which * p.nsplit + s) * N + r) * D + col, a);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += a[e];
+    }
+    if (j < p.s32)
+      for (int s = 0; s < p.nchunk; ++s) {
+        load4(sink + (((int64_t)which * p.nchunk + s) * S + ((int64_t)b * p.Hk + hk) * p.s32 + j) * D + col, a);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += a[e];
+      }
+    const float mul = which ? 1.f : p.scale;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= mul;
+    T* dst = which ? reinterpret_cast<T*>(p.dv) + (rw.k0 + j) * p.lddv : reinterpret_cast<T*>(p.dk) + (rw.k0 + j) * p.lddk;
+    store4(dst + (int64_t)hk * D + col, o);
+  }
+}
+
+struct BwdPlan { int nsplit, s32, nchunk; };
+inline BwdPlan bwd_plan(int nseq, int Lq, int Lk, int H, int Hk, int left, int right, int sinks, int q_start, int ntiles) {
+  BwdPlan b{1, 0, 0};
+  const int G = H / Hk;
+  const int64_t units = ntiles ? (int64_t)ntiles * Hk : (int64_t)nseq * Hk * cdiv(Lk, QB);
+  const int64_t span = (int64_t)QB + left + right < Lq ? (int64_t)QB + left + right : Lq;
+  const int64_t steps = cdiv(span, 32) * G;
+  if (units < 256) {                       // too few key tiles for the chip: split the rows (and heads) they meet
+    int64_t s = cdiv(512, units);
+    if (s > steps / 8) s = steps / 8;
+    b.nsplit = (int)(s < 1 ? 1 : s);
+  }
+  const int64_t far = (int64_t)q_start + Lq - 1 - left;            // sinks 0 ... far - 1 have rows beyond their window
+  if (sinks > 0 && far > 0) {
+    const int64_t n = sinks < far ? sinks : far;
+    b.s32 = (int)(cdiv(n, 32) * 32);
+    const int64_t blocks = (int64_t)nseq * Hk * (b.s32 / 32), tiles = cdiv(far, 32) * G;
+    int64_t ch = cdiv(512, blocks);
+    if (ch > tiles / 8) ch = tiles / 8;    // two tiles per wave at least
+    b.nchunk = (int)(ch < 1 ? 1 : ch);
+  }
+  return b;
+}
+inline int64_t bwd_floats(const BwdPlan& b, int nseq, int64_t Mk, int Hk, int D) {
+  const int64_t win = b.nsplit > 1 ? (int64_t)b.nsplit * Hk * Mk : (int64_t)nseq * Hk * b.s32;
+  return 2 * (win + (int64_t)b.nchunk * nseq * Hk * b.s32) * D;
+}
+
+template <typename T, int D, bool DROP> int launch_bwd(Params& p, hipStream_t s) {
+  typedef Geo<T, D> G;
+  constexpr int WGS = D == 128 ? 1 : 2;    // 128 columns: k, v and both gradients of a wave's keys alone are 256 registers
+  int rc;
+  {
+    const int nqt = (int)cdiv(p.Lq, QB);
+    const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.H : (int64_t)p.nseq * p.H * nqt;
+    if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
+    const int lds = 4 * G::KT * G::ROWB + 2 * G::KT * 4 + 16;
+    if ((rc = raise_lds<dq_kernel<T, D, DROP>>(lds))) return rc;
+    if (nu) hipLaunchKernelGGL((dq_kernel<T, D, DROP>), dim3((unsigned)(8 * cdiv(nu, 8))), dim3(256), lds, s, p, (int)nu, nqt);
+    if ((rc = ctclip_check_launch("win_attn_bwd dq"))) return rc;
+  }
+  if (p.s32) {
+    const int nblk = p.s32 / 32;
+    int lds = 4 * (2 * 32 * G::ROWB + 256);
+    if (4 * 32 * (D + 4) * 4 > lds) lds = 4 * 32 * (D + 4) * 4;
+    if ((rc = raise_lds<dkv_sink_kernel<T, D, DROP>>(lds))) return rc;
+    hipLaunchKernelGGL((dkv_sink_kernel<T, D, DROP>), dim3((unsigned)(nblk * p.Hk * p.nseq), p.nchunk), dim3(256), lds, s, p, nblk);
+    if ((rc = ctclip_check_launch("win_attn_bwd sinks"))) return rc;
+  }
+  {
+    const int nkt = (int)cdiv(p.Lk, QB);
+    const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.Hk : (int64_t)p.nseq * p.Hk * nkt;
+    if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
+    const int lds = 4 * QTile<T, D>::ROWS * G::ROWB + 4 * QTile<T, D>::ROWS * 4;
+    if ((rc = raise_lds<dkv_kernel<T, D, DROP, WGS>>(lds))) return rc;
+    if (nu) hipLaunchKernelGGL((dkv_kernel<T, D, DROP, WGS>), dim3((unsigned)(8 * cdiv(nu, 8)), p.nsplit), dim3(256), lds, s, p, (int)nu, nkt);
+    if ((rc = ctclip_check_launch("win_attn_bwd dkv"))) return rc;
+  }
+  const int keys = p.nsplit > 1 ? p.Lk : p.s32;
+  if (!keys) return CTCLIP_OK;
+  hipLaunchKernelGGL((dkv_reduce_kernel<T, D>), dim3((unsigned)cdiv(keys, 256 / (D / 4)), p.Hk, p.nseq), dim3(256), 0, s, p, keys);
+  return ctclip_check_launch("win_attn_bwd reduce");
+}
+template <typename T, int D> int launch_bwd_d(Params& p, hipStream_t s) { return p.drop_p > 0.f ? launch_bwd<T, D, true>(p, s) : launch_bwd<T, D, false>(p, s); }
+template <typename T> int launch_bwd_t(Params& p, int D, hipStream_t s) {
+  return D == 32 ? launch_bwd_d<T, 32>(p, s) : (D == 64 ? launch_bwd_d<T, 64>(p, s) : launch_bwd_d<T, 128>(p, s));
+}
+}  // namespace win
+
+// bytes of workspace of ctclip_win_attn_bwd (partial sums of the sinks' gradients and of split key tiles; 0: none).  ntiles: packed sequences, else 0
+extern "C" int64_t ctclip_win_attn_bwd_workspace(int nseq, int Lq, int Lk, int64_t Mk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int ntiles) {
+  if (nseq < 1 || Lq < 1 || Lk < 1 || H < 1 || Hk < 1 || H % Hk) return 0;
+  const int l = left < 0 || left > Lk ? Lk : left, r = right < 0 || right > Lk ? Lk : right, s = sinks < Lk ? sinks : Lk;
+  return win::bwd_floats(win::bwd_plan(nseq, Lq, Lk, H, Hk, l, r, s, q_start, ntiles), nseq, Mk, Hk, D) * 4;
+}
+
+// gradients of ctclip_win_attn_fwd: o, lse as it wrote them; delta: [H][Mq] f32 scratch; dq, dk, dv in the inputs' type, every row of a sequence written
+extern "C" int ctclip_win_attn_bwd(const void* q, const void* k, const void* v, const float* keymask, const int32_t* offsets, const int32_t* tiles, int ntiles, const void* o,
+                                   const void* dout, const float* lse, float* delta, void* dq, void* dk, void* dv, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H,
+                                   int Hk, int D, int left, int right, int sinks, int q_start, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t lddo,
+                                   int64_t lddq, int64_t lddk, int64_t lddv, float scale, float dropout_p, uint64_t dropout_seed, int dtype, void* workspace,
+                                   int64_t workspace_bytes, hipStream_t stream) {
+  using namespace win;
+  int rc = check_shape(nseq, Lq, Lk, Mq, Mk, H, Hk, D, left, right, sinks, q_start, offsets != nullptr, dtype);
+  if (rc) return rc;
+  if (!(scale > 0.f) || !(scale < 1e30f) || !(dropout_p >= 0.f) || !(dropout_p < 1.f)) { ctclip_set_error("win_attn_bwd: scale > 0, 0 <= dropout < 1"); return CTCLIP_EBADARG; }
+  if (nseq == 0 || Lk == 0 || Lq == 0 || (offsets && ntiles == 0)) return CTCLIP_OK;
+  if (offsets && (!tiles || ntiles < 0)) { ctclip_set_error("win_attn_bwd: packed sequences need their tiles"); return CTCLIP_EBADARG; }
+  if (Hk > 65535 || nseq > 65535) { ctclip_set_error("win_attn_bwd: more than 65535 sequences or heads"); return CTCLIP_EUNSUPPORTED; }
+  if (!lse || !delta) { ctclip_set_error("win_attn_bwd: needs lse and delta"); return CTCLIP_EBADARG; }
+  if ((rc = check_rows(q, ldq, H, D, dtype, false, "win_attn_bwd: q rows 16-byte aligned")) || (rc = check_rows(k, ldk, Hk, D, dtype, false, "win_attn_bwd: k rows 16-byte aligned")) ||
+      (rc = check_rows(v, ldv, Hk, D, dtype, false, "win_attn_bwd: v rows 16-byte aligned")) || (rc = check_rows(o, ldo, H, D, dtype, false, "win_attn_bwd: o rows 16-byte aligned")) ||
+      (rc = check_rows(dout, lddo, H, D, dtype, false, "win_attn_bwd: dout rows 16-byte aligned")) || (rc = check_rows(dq, lddq, H, D, dtype, true, "win_attn_bwd: dq rows 16-byte aligned, apart")) ||
+      (rc = check_rows(dk, lddk, Hk, D, dtype, true, "win_attn_bwd: dk rows 16-byte aligned, apart")) || (rc = check_rows(dv, lddv, Hk, D, dtype, true, "win_attn_bwd: dv rows 16-byte aligned, apart"))) return rc;
+  Params p{};
+  fill(p, nseq, Lq, Lk, Mq, Mk, H, Hk, left, right, sinks, q_start, scale, dropout_p, dropout_seed, offsets, tiles, ntiles, keymask);
+  p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.lse = const_cast<float*>(lse); p.delta = delta; p.dq = dq; p.dk = dk; p.dv = dv;
+  p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo; p.lddo = lddo; p.lddq = lddq; p.lddk = lddk; p.lddv = lddv;
+  const BwdPlan b = bwd_plan(nseq, Lq, Lk, H, Hk, p.left, p.right, p.sinks, q_start, offsets ? ntiles : 0);
+  p.nsplit = b.nsplit; p.s32 = b.s32; p.nchunk = b.nchunk;
+  const int64_t need = bwd_floats(b, nseq, Mk, Hk, D) * 4;
+  if (need) {
+    if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16) { ctclip_set_error("win_attn_bwd: workspace"); return CTCLIP_EWORKSPACE; }
+    p.part = (float*)workspace;
+  }
+  return dtype == DT_F32 ? launch_bwd_t<float>(p, D, stream) : launch_bwd_t<bf16_t>(p, D, stream);
+}

@@ -10,11 +10,13 @@ Weight handling
     gradient buffer; split-K partial sums go through f32 slabs and a fixed-order reduce -- the library has no float atomics)
     when present -- autograd then sees ``None`` for that input; otherwise a fresh f32 gradient tensor is returned as usual.
 """
+import math
 import os
 
 import numpy as np
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import backend as _be
 from . import streams as _streams
@@ -1210,6 +1212,290 @@ class SdpaFn(Function):
         return dq, dk, dv, None, None, None, None, None, None, None
 
 
+# ------------------------------------------------------------------------------------------ long reports: rotary positions, windowed attention
+
+class RotaryPositions:
+    """Frequencies of rotary positions (the plan that ``rotary`` takes): pair i of the first `dim` columns of a head turns by base^(-2i/dim) radians per position.
+
+    layout "half": pairs x[i], x[i + dim/2]; "interleaved": x[2i], x[2i+1].  scaling for contexts longer than the ones trained on, a dict with "type" and "factor":
+    "linear" (positions divided by the factor), "ntk" (base * factor^(dim/(dim-2))), "yarn" ("original_length", optional "beta_fast" = 32, "beta_slow" = 1: pairs that
+    turn more than beta_fast times within the original length keep their frequency, pairs that turn less than beta_slow times are divided by the factor, a ramp
+    between; rotated values are multiplied by "attention_factor", default 0.1 ln(factor) + 1).
+
+    Frequencies are kept as 64-bit binary fractions of a turn: the angle of an integer position is exact modulo whole turns, there is no last position."""
+
+    def __init__(self, dim, base=10000.0, layout="half", scaling=None):
+        if int(dim) != dim or dim < 2 or dim % 2:
+            raise ValueError(f"rotary dim must be a positive even number, got {dim}")
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"rotary layout {layout!r}: 'half' or 'interleaved'")
+        if not base > 1.0 or not math.isfinite(base):
+            raise ValueError(f"rotary base must be finite and > 1, got {base}")
+        self.dim, self.layout, self.base, self.magnitude = int(dim), layout, float(base), 1.0
+        pair = np.arange(0, self.dim, 2, dtype=np.float64)
+        scaling = dict(scaling) if scaling else {"type": "none"}
+        kind = scaling.pop("type", None)
+        factor = float(scaling.pop("factor", 1.0))
+        original = scaling.pop("original_length", None)
+        fast, slow, attention = scaling.pop("beta_fast", 32.0), scaling.pop("beta_slow", 1.0), scaling.pop("attention_factor", None)
+        if kind not in ("none", "linear", "ntk", "yarn") or scaling:
+            raise ValueError(f"rotary scaling: type none, linear, ntk or yarn, got {kind!r} {sorted(scaling)}")
+        if not factor >= 1.0 or not math.isfinite(factor):
+            raise ValueError(f"rotary scaling factor must be finite and >= 1, got {factor}")
+        if kind == "ntk" and self.dim > 2:
+            base = base * factor ** (self.dim / (self.dim - 2))
+        f = float(base) ** (-pair / self.dim)
+        if kind == "linear":
+            f = f / factor
+        elif kind == "yarn":
+            if not original or original < 1 or not fast > slow > 0:
+                raise ValueError("rotary scaling yarn needs original_length >= 1 and beta_fast > beta_slow > 0")
+
+            def pair_with(turns):         # the pair that turns so often within the original length
+                return self.dim * math.log(original / (turns * 2.0 * math.pi)) / (2.0 * math.log(self.base))
+            lo, hi = max(math.floor(pair_with(fast)), 0), min(math.ceil(pair_with(slow)), self.dim - 1)
+            ramp = np.clip((np.arange(self.dim // 2) - lo) / max(hi - lo, 0.001), 0.0, 1.0)
+            f = f * (1.0 - ramp) + f / factor * ramp
+            self.magnitude = float(attention) if attention is not None else 0.1 * math.log(factor) + 1.0
+        self.frequencies = f
+        self._bits = [int(math.ldexp(t % 1.0, 64)) & (2 ** 64 - 1) for t in f / (2.0 * math.pi)]
+        self._turns = {}
+
+    def turns(self, device):
+        """(dim / 2) int64 tensor with the bits of the unsigned fractions, on the device (made once)."""
+        t = self._turns.get(device)
+        if t is None:
+            t = self._turns[device] = torch.tensor([b - 2 ** 64 if b >= 2 ** 63 else b for b in self._bits], dtype=torch.int64).to(device)
+        return t
+
+
+def _aligned_rows(t):
+    """t itself when its rows can be read 16 bytes at a time, else a dense copy."""
+    ok = t.stride(1) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) * t.element_size() % 16 == 0
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+class RotaryFn(Function):
+    @staticmethod
+    def forward(ctx, q, k, rope, D, L, positions, start):
+        be = B()
+        ctx.args = (rope, D, L, start)
+        ctx.save_for_backward(*([positions] if positions is not None else []))
+        qo, ko = be.rotary(q, k, rope.turns(q.device), D, rope.dim, L, positions, start, rope.layout == "interleaved", rope.magnitude)
+        return qo if k is None else (qo, ko)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        rope, D, L, start = ctx.args
+        positions = ctx.saved_tensors[0] if ctx.saved_tensors else None
+        dq = dq.contiguous()
+        gq, gk = B().rotary(dq, dk.contiguous() if dk is not None else None, rope.turns(dq.device), D, rope.dim, L, positions, start, rope.layout == "interleaved",
+                            rope.magnitude, inverse=True)
+        return gq, gk, None, None, None, None, None
+
+
+def rotary(q, k, rope, D, L=None, positions=None, start=0):
+    """Rotary positions on a projection's output: q (M, Hq * D) and k (M, Hk * D; or None), row-strided views welcome, bf16 or f32 -> (q', k'), or q' without k.
+
+    rope: a ``RotaryPositions``; its `dim` first columns of every head are rotated, the others pass through.  The position of row i is positions[i] (an int32 / int64
+    tensor of M on the same device, any values), or start + i % L for sequences of L rows (L = None: one sequence)."""
+    if not isinstance(rope, RotaryPositions):
+        raise TypeError("rotary: rope must be a RotaryPositions")
+    for t, name in ((q, "q"), (k, "k")):
+        if t is None and name == "k":
+            continue
+        if t.dim() != 2 or t.shape[1] % D or (t.shape[1] == 0) or t.shape[0] != q.shape[0] or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"rotary: {name} must be (M, heads * {D}) like q, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if rope.dim > D:
+        raise ValueError(f"rotary: {rope.dim} rotated columns in heads of {D}")
+    M = q.shape[0]
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (M,) or positions.device != q.device:
+            raise ValueError(f"rotary: positions must be {M} int32 / int64 values on {q.device}")
+        positions = positions.contiguous()
+    L = max(M, 1) if L is None else int(L)
+    if L < 1 or not -2 ** 62 < int(start) < 2 ** 62:
+        raise ValueError("rotary: L >= 1 and a start within 62 bits")
+    if q.stride(1) != 1:
+        q = q.contiguous()
+    if k is not None and k.stride(1) != 1:
+        k = k.contiguous()
+    return RotaryFn.apply(q, k, rope, int(D), L, positions, int(start))
+
+
+class PackedSequences:
+    """Sequences of the given lengths, one behind the other in the rows of q, k and v (the plan that ``window_attention`` takes in the place of a number of equal
+    sequences).  first: the row of the first one.  Lengths of 0 are sequences without rows."""
+
+    def __init__(self, lengths, first=0):
+        self.lengths = [int(n) for n in lengths]
+        if any(n < 0 for n in self.lengths) or first < 0:
+            raise ValueError("PackedSequences: lengths and first row must not be negative")
+        self.first = int(first)
+        ends = np.cumsum([self.first] + self.lengths)
+        if ends[-1] >= 2 ** 31 - 256:
+            raise ValueError("PackedSequences: too many rows")
+        self.end = int(ends[-1])
+        self.rows = self.end - self.first
+        self.longest = max(self.lengths, default=0)
+        tiles = [(b, t) for b, n in enumerate(self.lengths) for t in range((n + 127) // 128)]
+        self.ntiles = len(tiles)
+        self._host = (torch.from_numpy(ends.astype(np.int32)), torch.tensor(tiles, dtype=torch.int32).reshape(-1))
+        self._dev = {}
+
+    def on(self, device):
+        t = self._dev.get(device)
+        if t is None:
+            t = self._dev[device] = tuple(x.to(device) for x in self._host)
+        return t
+
+
+class WindowGeometry:
+    """What the kernels need to know of a call: sizes, window, and the packed sequences' tables."""
+    __slots__ = ("nseq", "Lq", "Lk", "Mq", "Mk", "H", "Hk", "D", "left", "right", "sinks", "q_start", "offsets", "tiles", "ntiles", "rows")
+
+
+class WindowAttnFn(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, keymask, geo, scale, dropout):
+        ctx.args = (geo, scale, dropout)
+        if geo.nseq == 0 or geo.Lq == 0:       # no query row in any sequence
+            ctx.save_for_backward(q, k, v)
+            return q.new_zeros((geo.Mq, geo.H * geo.D))
+        need = any(ctx.needs_input_grad[:3])
+        o, lse = B().win_attn_fwd(q, k, v, keymask, geo, scale, want_lse=need, dropout=dropout)
+        if need:
+            ctx.save_for_backward(q, k, v, o, lse, *([keymask] if keymask is not None else []))
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        geo, scale, dropout = ctx.args
+        if geo.nseq == 0 or geo.Lq == 0:
+            return (*(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in ctx.saved_tensors), None, None, None, None)
+        q, k, v, o, lse, *mask = ctx.saved_tensors
+        dq, dk, dv = B().win_attn_bwd(q, k, v, mask[0] if mask else None, geo, scale, o, _aligned_rows(do), lse, dropout=dropout)
+        return dq, dk, dv, None, None, None, None
+
+
+def window_geometry(q, k, v, H, D, nseq=1, kv_heads=None, window=(-1, -1), sinks=0, q_start=0):
+    Hk = H if kv_heads is None else int(kv_heads)
+    if D not in (32, 64, 128):
+        raise ValueError(f"window_attention: heads of 32, 64 or 128 columns, got {D}")
+    if H < 1 or Hk < 1 or H % Hk:
+        raise ValueError(f"window_attention: {H} query heads over {Hk} key / value heads")
+    for t, heads, name in ((q, H, "q"), (k, Hk, "k"), (v, Hk, "v")):
+        if t.dim() != 2 or t.shape[1] != heads * D or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"window_attention: {name} must be (rows, {heads} * {D}) of q's type and device, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"window_attention: unsupported dtype {q.dtype}")
+    left, right = (int(window), int(window)) if isinstance(window, int) else (int(window[0]), int(window[1]))
+    if left < -1 or right < -1 or sinks < 0 or q_start < 0:
+        raise ValueError("window_attention: window sides >= -1, sinks >= 0, q_start >= 0")
+    if k.shape[0] != v.shape[0]:
+        raise ValueError(f"window_attention: {k.shape[0]} rows of k, {v.shape[0]} of v")
+    g = WindowGeometry()
+    g.H, g.Hk, g.D, g.left, g.right, g.sinks, g.q_start = int(H), Hk, int(D), min(left, 2 ** 30), min(right, 2 ** 30), min(int(sinks), 2 ** 30), int(q_start)
+    g.Mq, g.Mk, g.offsets, g.tiles, g.ntiles = q.shape[0], k.shape[0], None, None, 0
+    if isinstance(nseq, PackedSequences):
+        if g.Mq != g.Mk or nseq.end > g.Mq or g.q_start:
+            raise ValueError(f"window_attention: packed sequences end at row {nseq.end} of {g.Mq} query and {g.Mk} key rows (equal, and q_start = 0)")
+        g.nseq, g.Lq, g.Lk, g.rows = len(nseq.lengths), nseq.longest, nseq.longest, nseq.rows
+        if nseq.ntiles:
+            (g.offsets, g.tiles), g.ntiles = nseq.on(q.device), nseq.ntiles
+        else:
+            g.nseq = 0
+    else:
+        g.nseq = int(nseq)
+        if g.nseq < 0 or (g.nseq == 0 and (g.Mq or g.Mk)) or (g.nseq and (g.Mq % g.nseq or g.Mk % g.nseq)):
+            raise ValueError(f"window_attention: {g.Mq} query and {g.Mk} key rows are not {g.nseq} equal sequences")
+        g.Lq, g.Lk = (g.Mq // g.nseq, g.Mk // g.nseq) if g.nseq else (0, 0)
+        g.rows = g.Mq
+        if g.q_start + g.Lq > g.Lk and g.Lq:
+            raise ValueError(f"window_attention: query positions {g.q_start} ... {g.q_start + g.Lq - 1} on a key axis of {g.Lk}")
+    return g
+
+
+def window_attention(q, k, v, H, D, nseq=1, kv_heads=None, window=(-1, -1), sinks=0, keymask=None, scale=None, q_start=0, dropout=None):
+    """Attention inside a sliding window, with a few first tokens that stay visible: o = softmax(scale q k^T + keymask) v, differentiable in q, k, v.
+
+    q (rows, H * D), k and v (rows, kv_heads * D; query head h reads key head h // (H / kv_heads)), bf16 or f32, heads of 32, 64 or 128, row-strided views welcome.
+    nseq: that many equal sequences, or a ``PackedSequences`` (rows outside every sequence: output and gradients 0).  Query row i of a sequence is at position
+    q_start + i of its key axis (one new token: a single row with q_start = its position; the [CLS] row: q_start = 0).
+    window = (left, right) or one number for both, -1 = no limit: position i sees keys i - left ... i + right, and of the keys further left the first `sinks`.
+    keymask: additive f32, (nseq, key rows of a sequence) or flat per key row, no gradient; values <= -1e30 (HF's finfo.min, -inf) and NaN hide the key, whatever k
+    and v hold there.  A row that sees no key is 0 and gives no gradient.  dropout = (p, seed): attention-probability dropout, masks as in ``SdpaFn``.
+    scale > 0, default 1 / sqrt(D)."""
+    g = window_geometry(q, k, v, H, D, nseq, kv_heads, window, sinks, q_start)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"window_attention: scale must be positive and finite, got {scale}")
+    if dropout is not None and not 0.0 <= dropout[0] < 1.0:
+        raise ValueError(f"window_attention: dropout probability {dropout[0]}")
+    if keymask is not None:
+        if keymask.numel() != g.Mk or keymask.device != q.device or not keymask.is_floating_point():
+            raise ValueError(f"window_attention: keymask must be one additive value per key row ({g.Mk}) on {q.device}")
+        keymask = keymask.detach().to(torch.float32).contiguous().view(-1)
+    return WindowAttnFn.apply(_aligned_rows(q), _aligned_rows(k), _aligned_rows(v), keymask, g, scale, dropout)
+
+
+def _qkv_shadows(dtype, device, wq, wk, wv, bq, bk, bv):
+    """-> (stacked (3 N, K) weight shadow, stacked f32 bias) of the three projections."""
+    be = B()
+    N, K = wq.shape
+
+    def make_w():
+        out = torch.empty((3 * N, K), dtype=dtype, device=device)
+        for i, w in enumerate((wq, wk, wv)):
+            be.convert_pad(w.detach(), N, K, dtype, out=out[i * N:(i + 1) * N])
+        return out
+    # (the stamp of the cache entry is wq's; the fused optimiser bumps the weight epoch, load_state_dict touches all three)
+    wsh = shadow(wq, ("qkv", id(wk), id(wv)), dtype, make_w, recipe=[(w, i * N, N, K, MAP_PLAIN, 0, False) for i, w in enumerate((wq, wk, wv))],
+                 deps=(wk, wv))
+    bias = shadow(bq, ("qkv_bias", id(bk), id(bv)), torch.float32, lambda: torch.cat([bq.detach(), bk.detach(), bv.detach()]).float(),
+                  deps=(bk, bv))
+    return wsh, bias
+
+
+def _qkv_transposed_shadow(x, wq, wk, wv):
+    """(K, 3 N) = the stacked weight transposed: the grad-input GEMM dx = [dq | dk | dv] W then has both operands k-contiguous (gemm_sm.hip); None: not served."""
+    be = B()
+    N, K = wq.shape
+    if not (x.dtype == torch.bfloat16 and x.shape[0] >= 256 and N % 64 == 0 and K % 8 == 0):
+        return None
+
+    def make_wt():
+        out = torch.empty((K, 3 * N), dtype=x.dtype, device=x.device)
+        for i, w in enumerate((wq, wk, wv)):
+            out[:, i * N:(i + 1) * N].copy_(be.transpose2d(be.convert_pad(w.detach(), N, K, x.dtype)))
+        return out
+    return shadow(wq, ("qkvT", id(wk), id(wv)), x.dtype, make_wt,
+                  recipe=[(w, 0, K, N, MAP_PLAIN, 0, True, i * N) for i, w in enumerate((wq, wk, wv))], deps=(wk, wv))
+
+
+def _qkv_backward(ctx, dqkv, x, wsh, d_pass):
+    """-> dx, [dWq, dWk, dWv], [dbq, dbk, dbv] of the stacked projection from dq | dk | dv side by side."""
+    be = B()
+    wq, wk, wv, bq, bk, bv = ctx.params
+    N, K = wq.shape
+    dx = None
+    if ctx.needs_input_grad[0]:
+        dx = (be.gemm(dqkv, ctx.wt, residual=d_pass, out_dtype=ctx.x_dtype) if ctx.wt is not None
+              else be.gemm(dqkv, wsh, a_kc=True, b_kc=False, residual=d_pass, out_dtype=ctx.x_dtype))
+    gw, gb = [], []
+    for i, (w, b) in enumerate(zip((wq, wk, wv), (bq, bk, bv))):
+        dyi = dqkv[:, i * N:(i + 1) * N]
+        fused = weight_bias_grad(dyi, x, w, b, K) if (w.requires_grad and b.requires_grad) else None      # dW and db in one launch
+        if fused is not None:
+            gw.append(fused[0]); gb.append(fused[1])
+            continue
+        gw.append(weight_grad(dqkv, x, w, [(0, N, i * N)], K) if w.requires_grad else None)
+        gb.append(vec_grad(b, lambda dst, i=i: be.colsum(dqkv[:, i * N:(i + 1) * N], dst, N=N)) if b.requires_grad else None)
+    return dx, gw, gb
+
+
 class QkvSdpaFn(Function):
     """HF BertSelfAttention as one node: q, k, v = x Wq^T + bq, x Wk^T + bk, x Wv^T + bv as ONE GEMM against the stacked weight
     shadow (3 * hidden outputs: three times the column tiles for the M = B * T = a-few-hundred-rows text tower, one launch instead
@@ -1228,32 +1514,12 @@ class QkvSdpaFn(Function):
         x_in = x
         if operand_dtype is not None and x.dtype != operand_dtype:
             x = be.convert_pad(x, x.shape[0], x.shape[1], operand_dtype)
-
-        def make_w():
-            out = torch.empty((3 * N, K), dtype=x.dtype, device=x.device)
-            for i, w in enumerate((wq, wk, wv)):
-                be.convert_pad(w.detach(), N, K, x.dtype, out=out[i * N:(i + 1) * N])
-            return out
-        # (the stamp of the cache entry is wq's; the fused optimiser bumps the weight epoch, load_state_dict touches all three)
-        wsh = shadow(wq, ("qkv", id(wk), id(wv)), x.dtype, make_w, recipe=[(w, i * N, N, K, MAP_PLAIN, 0, False) for i, w in enumerate((wq, wk, wv))],
-                     deps=(wk, wv))
-        bias = shadow(bq, ("qkv_bias", id(bk), id(bv)), torch.float32, lambda: torch.cat([bq.detach(), bk.detach(), bv.detach()]).float(),
-                      deps=(bk, bv))
+        wsh, bias = _qkv_shadows(x.dtype, x.device, wq, wk, wv, bq, bk, bv)
         qkv = be.gemm(x, wsh, bias=bias)
         q, k, v = qkv[:, :N], qkv[:, N:2 * N], qkv[:, 2 * N:]
         vt = be.head_transpose(v, nseq, H, L, D)
         o, lse = be.attn_fwd(q, k, vt, None, keymask, nseq, H, L, D, scale, dropout=dropout)
-        wt = None
-        if x.dtype == torch.bfloat16 and x.shape[0] >= 256 and N % 64 == 0 and K % 8 == 0 and ctx.needs_input_grad[0]:
-            # (K, 3 N) = the stacked weight transposed: the grad-input GEMM dx = [dq | dk | dv] W then has both operands k-contiguous (gemm_sm.hip)
-            def make_wt():
-                out = torch.empty((K, 3 * N), dtype=x.dtype, device=x.device)
-                for i, w in enumerate((wq, wk, wv)):
-                    out[:, i * N:(i + 1) * N].copy_(be.transpose2d(be.convert_pad(w.detach(), N, K, x.dtype)))
-                return out
-            wt = shadow(wq, ("qkvT", id(wk), id(wv)), x.dtype, make_wt,
-                        recipe=[(w, 0, K, N, MAP_PLAIN, 0, True, i * N) for i, w in enumerate((wq, wk, wv))], deps=(wk, wv))
-        ctx.wt = wt
+        ctx.wt = _qkv_transposed_shadow(x, wq, wk, wv) if ctx.needs_input_grad[0] else None
         ctx.save_for_backward(x, wsh, qkv, o, lse, keymask if keymask is not None else x.new_empty(0))
         ctx.params = (wq, wk, wv, bq, bk, bv)
         ctx.dims = (nseq, L, H, D, scale, keymask is not None, dropout, N, K)
@@ -1267,27 +1533,69 @@ class QkvSdpaFn(Function):
         x, wsh, qkv, o, lse, keymask = ctx.saved_tensors
         d_pass = d_pass.contiguous() if (ctx.passthrough and d_pass is not None) else None
         nseq, L, H, D, scale, has_mask, dropout, N, K = ctx.dims
-        wq, wk, wv, bq, bk, bv = ctx.params
         do = do.contiguous()
         q, k, v = qkv[:, :N], qkv[:, N:2 * N], qkv[:, 2 * N:]
         qt, kt, dot = (be.head_transpose(t, nseq, H, L, D) for t in (q, k, do))
         dqkv = torch.empty_like(qkv)
         be.attn_bwd(q, k, v, qt, kt, o, do, dot, lse, None, keymask if has_mask else None, dqkv[:, :N], dqkv[:, N:2 * N], dqkv[:, 2 * N:], None,
                     nseq, H, L, D, scale, dropout=dropout)
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = (be.gemm(dqkv, ctx.wt, residual=d_pass, out_dtype=ctx.x_dtype) if ctx.wt is not None
-                  else be.gemm(dqkv, wsh, a_kc=True, b_kc=False, residual=d_pass, out_dtype=ctx.x_dtype))
-        gw, gb = [], []
-        for i, (w, b) in enumerate(zip((wq, wk, wv), (bq, bk, bv))):
-            dyi = dqkv[:, i * N:(i + 1) * N]
-            fused = weight_bias_grad(dyi, x, w, b, K) if (w.requires_grad and b.requires_grad) else None      # dW and db in one launch
-            if fused is not None:
-                gw.append(fused[0]); gb.append(fused[1])
-                continue
-            gw.append(weight_grad(dqkv, x, w, [(0, N, i * N)], K) if w.requires_grad else None)
-            gb.append(vec_grad(b, lambda dst, i=i: be.colsum(dqkv[:, i * N:(i + 1) * N], dst, N=N)) if b.requires_grad else None)
+        dx, gw, gb = _qkv_backward(ctx, dqkv, x, wsh, d_pass)
         return (dx, *gw, *gb, None, None, None, None, None, None, None, None, None)
+
+
+class QkvWindowFn(Function):
+    """``QkvSdpaFn`` for long reports: the stacked projection, rotary positions on its q | k columns in place, windowed attention with sinks on column views of the same
+    buffer; backward turns dq | dk back in place in front of the grad-input GEMM."""
+
+    @staticmethod
+    def forward(ctx, x, wq, wk, wv, bq, bk, bv, keymask, nseq, L, H, D, scale, dropout, rope, window, sinks, first_only, operand_dtype=None, passthrough=False):
+        """rope: ``RotaryPositions`` or None.  first_only: only the first row of every sequence is attended FROM ([CLS] in the last layer) -> o (nseq, H * D)."""
+        be = B()
+        N, K = wq.shape
+        ctx.x_dtype = x.dtype
+        ctx.passthrough = bool(passthrough)
+        x_in = x
+        if operand_dtype is not None and x.dtype != operand_dtype:
+            x = be.convert_pad(x, x.shape[0], x.shape[1], operand_dtype)
+        wsh, bias = _qkv_shadows(x.dtype, x.device, wq, wk, wv, bq, bk, bv)
+        qkv = be.gemm(x, wsh, bias=bias)
+        if rope is not None:
+            q, k = qkv[:, :N], qkv[:, N:2 * N]
+            be.rotary(q, k, rope.turns(x.device), D, rope.dim, L, None, 0, rope.layout == "interleaved", rope.magnitude, out=(q, k))
+        q, k, v = QkvWindowFn._views(qkv, N, nseq, L, first_only)
+        geo = window_geometry(q, k, v, H, D, nseq, None, window, sinks, 0)
+        o, lse = be.win_attn_fwd(q, k, v, keymask, geo, scale, want_lse=any(ctx.needs_input_grad[:7]), dropout=dropout)
+        ctx.wt = _qkv_transposed_shadow(x, wq, wk, wv) if ctx.needs_input_grad[0] else None
+        if lse is not None:
+            ctx.save_for_backward(x, wsh, qkv, o, lse, *([keymask] if keymask is not None else []))
+        ctx.params = (wq, wk, wv, bq, bk, bv)
+        ctx.args = (geo, scale, dropout, rope, nseq, L, N, D, first_only)
+        if passthrough:
+            return o, x_in.view_as(x_in)
+        return o
+
+    @staticmethod
+    def _views(qkv, N, nseq, L, first_only):
+        q = qkv.view(nseq, -1)[:, :N] if first_only else qkv[:, :N]
+        return q, qkv[:, N:2 * N], qkv[:, 2 * N:]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, d_pass=None):
+        be = B()
+        x, wsh, qkv, o, lse, *mask = ctx.saved_tensors
+        geo, scale, dropout, rope, nseq, L, N, D, first_only = ctx.args
+        d_pass = d_pass.contiguous() if (ctx.passthrough and d_pass is not None) else None
+        dqkv = torch.empty_like(qkv)
+        if first_only:
+            dqkv[:, :N].zero_()                # rows that attended to nothing
+        be.win_attn_bwd(*QkvWindowFn._views(qkv, N, nseq, L, first_only), mask[0] if mask else None, geo, scale, o, _aligned_rows(do), lse, dropout=dropout,
+                        out=QkvWindowFn._views(dqkv, N, nseq, L, first_only))
+        if rope is not None:
+            dq, dk = dqkv[:, :N], dqkv[:, N:2 * N]
+            be.rotary(dq, dk, rope.turns(x.device), D, rope.dim, L, None, 0, rope.layout == "interleaved", rope.magnitude, inverse=True, out=(dq, dk))
+        dx, gw, gb = _qkv_backward(ctx, dqkv, x, wsh, d_pass)
+        return (dx, *gw, *gb, *([None] * 13))
 
 
 class DropoutAddFn(Function):
@@ -1495,7 +1803,11 @@ class ClipLossFn(Function):
 class BertEmbedFn(Function):
     @staticmethod
     def forward(ctx, ids, word, pos, typ, dtype):
-        x = B().bert_embed_fwd(ids, word.detach(), pos.detach(), typ.detach()[0].contiguous(), dtype)
+        """pos = None: no position table (rotary positions): every token is the first of its own sequence, and the table one row of zeros."""
+        if pos is None:
+            x = B().bert_embed_fwd(ids.view(-1, 1), word.detach(), word.new_zeros((1, word.shape[1])), typ.detach()[0].contiguous(), dtype)
+        else:
+            x = B().bert_embed_fwd(ids, word.detach(), pos.detach(), typ.detach()[0].contiguous(), dtype)
         ctx.save_for_backward(ids)
         ctx.params = (word, pos, typ)
         return x
@@ -1504,9 +1816,9 @@ class BertEmbedFn(Function):
     def backward(ctx, dx):
         (ids,) = ctx.saved_tensors
         word, pos, typ = ctx.params
-        ws, ps, ts = sink_of(word), sink_of(pos), sink_of(typ)
+        ws, ps, ts = sink_of(word), (sink_of(pos) if pos is not None else None), sink_of(typ)
         dw = ws if ws is not None else torch.zeros_like(word)
-        dp = ps if ps is not None else torch.zeros_like(pos)
+        dp = None if pos is None else ps if ps is not None else torch.zeros_like(pos)
         dt = ts if ts is not None else torch.zeros_like(typ)
         B().bert_embed_bwd(ids, dx.contiguous(), dw, dp, dt)   # dt row 0 only (token_type_ids are all zero)
         notify_grad_ready(("bert_embeddings", id(word)))        # the last gradients of the text tower

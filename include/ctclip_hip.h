@@ -305,6 +305,9 @@ int ctclip_adam_step_zero_grad(float* p, float* g, float* m, float* v, int64_t n
 /* scripts/data.py:92-162 (CTReportDataset.nii_img_to_tensor) without the file decode: src = the (H, W, D) voxel array as nibabel returns it (src_dtype 0 int16, 1 f32, 2 f64, device memory) -> HU = slope * v + intercept, trilinear resample to target_xy / target_z mm (F.interpolate align_corners=False, new size int(n * spacing / target)), clip to [hu_lo, hu_hi], / hu_div, centre crop / pad with pad_value -> out (out_d, out_h, out_w) f32 = (240, 480, 480). */
 int ctclip_preprocess_volume(const void* src, int src_dtype, int H, int W, int D, double slope, double intercept, double xy_spacing, double z_spacing, double target_xy, double target_z, float* out, int out_h, int out_w, int out_d, double hu_lo, double hu_hi, double hu_div, float pad_value, hipStream_t stream);
 
+/* Rotary positions: q (M, Hq D) and k (M, Hk D; NULL with Hk = 0) rotated into qo, ko (the same pointers and pitches: in place; otherwise no overlap).  The first `rot` columns of every head are rotated (rot even; pairs x[i], x[i + rot/2], or x[2i], x[2i+1] with interleaved = 1), the others pass through: (a, b) -> magnitude (a cos - b sin, b cos + a sin), angle = position * frequency; inverse = 1: the angle negated (the backward pass).  turns: rot/2 frequencies as 64-bit binary fractions of a turn per position (frequency / 2 pi * 2^64): angles of integer positions are exact.  positions: M integers of pos_bytes (4 / 8) bytes, or NULL: start + row % L.  [no reference counterpart on the hot path: the built-in text encoder of ct_clip.py:103-385 has rotary positions, HF BertModel an absolute table of 512 rows] */
+int ctclip_rotary(const void* q, const void* k, void* qo, void* ko, const uint64_t* turns, const void* positions, int pos_bytes, int64_t M, int64_t L, int64_t start, int Hq, int Hk, int D, int rot, int64_t ldq, int64_t ldk, int64_t ldqo, int64_t ldko, int interleaved, float magnitude, int inverse, int dtype, hipStream_t stream);
+
 /* bytes of workspace ctclip_segment_sum needs (row histogram, scan and the row order of each segment). [workspace query of ctclip_segment_sum (EMA statistics of vector-quantize-pytorch behind ctvit.py:403; nn.Embedding backward of HF BertEmbeddings)] */
 int64_t ctclip_segment_sum_workspace(int64_t M, int nseg);
 
@@ -313,6 +316,18 @@ int ctclip_segment_sum(const int64_t* keys, int key_mod, const void* x, int64_t 
 
 /* Batched refresh of the bf16 weight shadows after the optimiser step (replaces the per-parameter `.to(bf16)` / `.t().contiguous()` / re-layout copies a torch module makes when its weights change; scripts/CTCLIPTrainer.py:259-263 is followed by nothing of the kind because torch computes from the f32 weights): jobs = DEVICE array of njobs records of 12 int64 {src, dst, src_ld, dst_ld, src_rows, src_cols, dst_rows, dst_cols, map, aux, transposed, tile0} sorted by tile0 (tile0 of job i = sum over the jobs before it of ceil(dst_rows / 64) * ceil(dst_cols / 64)), ntiles = the total.  src f32 (src_rows, src_cols), dst bf16 (dst_rows, dst_cols); plain: dst[r][c] = src[map(r)][c], transposed: dst[r][c] = src[map(c)][r], 0 outside the source.  map 0: identity; 1: GEGLU [x | pad | gate | pad] split (aux = inner, half = mapped extent / 2); 2: ctclip_geglu_weight_interleave's row order (aux = inner). */
 int ctclip_shadow_refresh(const void* jobs, int njobs, int64_t ntiles, hipStream_t stream);
+
+/* bytes of workspace ctclip_win_attn_fwd needs (partial results of a split key axis; 0: none).  packed: 1 with offsets.  [no reference counterpart: workspace query] */
+int64_t ctclip_win_attn_fwd_workspace(int nseq, int Lq, int Lk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int packed);
+
+/* Attention in a sliding window with sinks: out = softmax(scale q k^T + keymask) v, position i sees key j when j <= i + right and (j >= i - left or j < sinks); left / right = -1: no limit.  q (Mq, H D), k | v (Mk, Hk D), head h reads k|v head h / (H / Hk); D = 32, 64 or 128.  Sequence b = rows b Lq ... of q at positions q_start ... (q_start + Lq <= Lk) and rows b Lk ... of k | v; with offsets (nseq + 1 int32 on the device) rows offsets[b] ... offsets[b + 1] - 1 of all three tensors (Mq = Mk, Lq = Lk = the longest, q_start = 0), tiles = ntiles (sequence, 128-row tile) int32 pairs covering them; rows outside are not written.  keymask: additive f32 per key row or NULL; a value <= -1e30 or NaN hides the key whatever k and v hold there (a key that a window hides from some rows of a 128-row tile and shows to others must be finite).  A row that sees nothing is 0.  lse: [H][Mq] f32, log2 of the sum of exponentials (+inf for a row that sees nothing), NULL: not wanted.  Attention dropout as in ctclip_attn_fwd, masks by query ROW and key.  Rows 16-byte aligned.  [HF BertSelfAttention (ct_clip.py:685-686) for reports longer than its window; no reference counterpart for the window] */
+int ctclip_win_attn_fwd(const void* q, const void* k, const void* v, const float* keymask, const int32_t* offsets, const int32_t* tiles, int ntiles, void* out, float* lse, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, float dropout_p, uint64_t dropout_seed, int dtype, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* bytes of workspace ctclip_win_attn_bwd needs (partial sums of the sinks' gradients and of split key tiles; 0: none).  ntiles: packed sequences, else 0.  [no reference counterpart: workspace query] */
+int64_t ctclip_win_attn_bwd_workspace(int nseq, int Lq, int Lk, int64_t Mk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int ntiles);
+
+/* Gradients of ctclip_win_attn_fwd from its out and lse: dq, dk, dv in the inputs' type, every row of a sequence overwritten (the k|v gradients summed over the query heads that share them); delta: [H][Mq] f32 scratch.  Fixed summation order.  [autograd through HF BertSelfAttention (ct_clip.py:685-686); no reference counterpart for the window] */
+int ctclip_win_attn_bwd(const void* q, const void* k, const void* v, const float* keymask, const int32_t* offsets, const int32_t* tiles, int ntiles, const void* o, const void* dout, const float* lse, float* delta, void* dq, void* dk, void* dv, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t lddo, int64_t lddq, int64_t lddk, int64_t lddv, float scale, float dropout_p, uint64_t dropout_seed, int dtype, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,351 @@
+"""Rotary positions and windowed attention on the device, against their 64-bit forms within counted roundings (tests/long_report_oracle.py)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from ct_clip_amd import functional as Fn  # noqa: E402
+from tests import long_report_oracle as O  # noqa: E402
+
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def rnd(shape, dtype, seed, scale=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).to(DEV).to(dtype)
+
+
+# ------------------------------------------------------------------------------------------------------------------ rotary
+
+ROTARY = [  # M, L, start, Hq, Hk, D, rot, interleaved, positions, scaling
+    (1, 1, 0, 12, 12, 64, 64, False, None, None),
+    (1, 1, 2 ** 40 + 7, 1, 1, 64, 64, False, None, None),
+    (77, 11, 1000003, 3, 1, 32, 32, False, None, dict(type="linear", factor=4.0)),
+    (1030, 515, 0, 12, 4, 64, 32, True, None, dict(type="yarn", factor=8.0, original_length=512)),
+    (4100, 4100, 5, 5, 0, 128, 64, False, None, dict(type="ntk", factor=2.0)),
+    (333, 333, 0, 2, 2, 64, 64, False, torch.int32, None),
+    (333, 333, 0, 2, 2, 64, 48, True, torch.int64, None),
+    (9, 3, 0, 3, 2, 6, 2, False, None, None),               # element-wise kernel: odd heads, rot 2
+    (65, 65, 3, 2, 1, 40, 20, True, None, None),
+    (50, 50, 0, 1, 1, 48, 24, False, None, None),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,L,start,Hq,Hk,D,rot,inter,posdt,scaling", ROTARY)
+def test_rotary_forward_and_backward(M, L, start, Hq, Hk, D, rot, inter, posdt, scaling, dtype):
+    rope = Fn.RotaryPositions(rot, layout="interleaved" if inter else "half", scaling=scaling)
+    q = rnd((M, Hq * D), dtype, 1).requires_grad_(True)
+    k = rnd((M, Hk * D), dtype, 2).requires_grad_(True) if Hk else None
+    positions = None
+    pos = start + torch.arange(M, device=DEV) % L
+    if posdt is not None:
+        pos = torch.randint(-5, 2 ** 31 - 1 if posdt == torch.int32 else 2 ** 45, (M,), generator=torch.Generator().manual_seed(3)).to(DEV)
+        positions = pos.to(posdt)
+    out = Fn.rotary(q, k, rope, D, L=L, positions=positions, start=start)
+    out = out if Hk else (out,)
+    xs = (q, k) if Hk else (q,)
+    gs = [rnd(tuple(x.shape), dtype, 5 + i) for i, x in enumerate(xs)]
+    grads = torch.autograd.grad(out, xs, gs)
+    # angles of far positions in integers (64-bit floats would lose what is tested): turns modulo one, then the plain form at the remaining angle
+    freq = torch.tensor([b for b in rope._bits], dtype=torch.float64) * 2.0 ** -64 * 2 * math.pi
+    small = pos.abs().max().item() < 2 ** 21
+    for i, x in enumerate(xs):
+        if small:
+            w = O.rotary64(x.detach(), torch.from_numpy(rope.frequencies), rope.magnitude, D, rot, inter, pos)
+            b = O.rotary64(gs[i], torch.from_numpy(rope.frequencies), rope.magnitude, D, rot, inter, pos, inverse=True)
+        else:
+            w = far_rotary64(x.detach(), rope, D, rot, inter, pos, 1)
+            b = far_rotary64(gs[i], rope, D, rot, inter, pos, -1)
+        O.check(out[i].detach(), (w[0], O.rotary_bound(*w, dtype)), f"out {i}")
+        O.check(grads[i], (b[0], O.rotary_bound(*b, dtype)), f"grad {i}")
+    assert freq.numel() == rot // 2
+
+
+def far_rotary64(x, rope, D, rot, inter, pos, sign):
+    """Row by row: position times the 64-bit fraction of a turn in whole numbers, modulo one turn."""
+    turns = torch.tensor([[((int(p) * b) % 2 ** 64) / 2.0 ** 64 for b in rope._bits] for p in pos.tolist()], dtype=torch.float64, device=x.device)
+    ang = turns * 2 * math.pi * sign
+    y = x.double().reshape(x.shape[0], -1, D)
+    c, s = torch.cos(ang)[:, None] * rope.magnitude, torch.sin(ang)[:, None] * rope.magnitude
+    ia = slice(0, rot, 2) if inter else slice(0, rot // 2)
+    ib = slice(1, rot, 2) if inter else slice(rot // 2, rot)
+    a, b = y[..., ia], y[..., ib]
+    z, m = y.clone(), torch.zeros_like(y)
+    z[..., ia], z[..., ib] = a * c - b * s, b * c + a * s
+    m[..., ia] = m[..., ib] = (a.abs() + b.abs()) * rope.magnitude
+    return z.reshape(x.shape[0], -1), m.reshape(x.shape[0], -1)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rotary_in_place_on_the_projection_and_odd_strides(dtype):
+    """Column views of one buffer, in place: the v columns stay as they were; a pitch and an offset that only the element-wise kernel serves give the same."""
+    from ct_clip_amd import backend
+    be, H, D, M = backend.get(), 4, 64, 150
+    rope = Fn.RotaryPositions(32)
+    buf = rnd((M, 3 * H * D), dtype, 9)
+    want = buf.clone()
+    q, k = want[:, :H * D], want[:, H * D:2 * H * D]
+    nq, nk = Fn.rotary(q, k, rope, D, L=50, start=2)
+    be.rotary(buf[:, :H * D], buf[:, H * D:2 * H * D], rope.turns(buf.device), D, 32, 50, None, 2, False, 1.0, out=(buf[:, :H * D], buf[:, H * D:2 * H * D]))
+    assert torch.equal(buf[:, :H * D], nq) and torch.equal(buf[:, H * D:2 * H * D], nk) and torch.equal(buf[:, 2 * H * D:], want[:, 2 * H * D:])
+    odd = torch.zeros((M, H * D + 3), dtype=dtype, device=DEV)
+    odd[:, 1:1 + H * D] = q
+    assert torch.equal(Fn.rotary(odd[:, 1:1 + H * D], None, rope, D, L=50, start=2), nq)
+
+
+def test_rotary_gradient_against_differences():
+    rope = Fn.RotaryPositions(32, scaling=dict(type="yarn", factor=4.0, original_length=256))
+    x = rnd((7, 2 * 32), F32, 11).requires_grad_(True)
+    g, d = rnd((7, 64), F32, 12), rnd((7, 64), F32, 13)
+    (dx,) = torch.autograd.grad(Fn.rotary(x, None, rope, 32, start=100), x, g)
+    # linear: the difference quotient is exact up to the roundings of two outputs (4 u of |y| each, y within sqrt(2) magnitude |x|, step 1/4)
+    h = 0.25
+    with torch.no_grad():
+        num = ((Fn.rotary(x + h * d, None, rope, 32, start=100).double() - Fn.rotary(x - h * d, None, rope, 32, start=100).double()) / (2 * h) * g.double()).sum()
+    room = 16 * O.U32 * 2 * ((x.detach().abs() + d.abs()).double().sum(1).max() * g.abs().double().sum()) / (2 * h)
+    assert abs(num - (dx.double() * d.double()).sum()) <= room
+
+
+# --------------------------------------------------------------------------------------------------------------- attention
+
+def make_mask(kind, nseq, Lk, seed):
+    if kind is None:
+        return None
+    j, b = torch.arange(Lk)[None, :], torch.arange(nseq)[:, None]
+    m = torch.zeros((nseq, Lk))
+    if kind == "pad":
+        m[(j >= Lk - (b * Lk) // (2 * nseq)).expand(nseq, Lk)] = torch.finfo(F32).min
+    elif kind == "holes":            # finfo.min, -inf and NaN all hide; the last sequence sees nothing
+        m = torch.randn((nseq, Lk), generator=torch.Generator().manual_seed(seed))
+        m[((j * 7 + b * 3) % 5 == 0).expand(nseq, Lk)] = -math.inf
+        m[((j * 7 + b * 3) % 5 == 1).expand(nseq, Lk)] = math.nan
+        if nseq > 1:
+            m[-1] = torch.finfo(F32).min
+    elif kind == "front":            # the first two thirds hidden: rows of a left-bounded window see nothing
+        m[(j < 2 * Lk // 3).expand(nseq, Lk)] = torch.finfo(F32).min
+    return m.to(DEV)
+
+
+def run_case(dtype, nseq, Lq, Lk, H, Hk, D, window, sinks, q_start=0, mask=None, lengths=None, first=0, tail=0, drop=None, seed=0, poison=True, strided=True, grad=True):
+    if lengths is not None:
+        M = first + sum(lengths) + tail
+        Mq = Mk = M
+        spans, at = [], first
+        for n in lengths:
+            spans.append((at, n, at, n))
+            at += n
+        nseq = Fn.PackedSequences(lengths, first=first)
+        keymask = None
+    else:
+        Mq, Mk = nseq * Lq, nseq * Lk
+        spans = [(b * Lq, Lq, b * Lk, Lk) for b in range(nseq)]
+        keymask = make_mask(mask, nseq, Lk, seed + 7)
+    if strided and Mq == Mk:
+        buf = rnd((Mq, (H + 2 * Hk) * D), dtype, seed + 1)
+        q, k, v = buf[:, :H * D], buf[:, H * D:(H + Hk) * D], buf[:, (H + Hk) * D:]
+    else:
+        q, k, v = rnd((Mq, H * D), dtype, seed + 1), rnd((Mk, Hk * D), dtype, seed + 2), rnd((Mk, Hk * D), dtype, seed + 3)
+    if keymask is not None and poison:       # whatever stands in a hidden key
+        bad = ~(keymask.reshape(-1) > -1e30)
+        k[bad] = math.nan
+        v[bad] = math.inf
+    q, k, v = (t.detach().requires_grad_(grad) for t in (q, k, v))
+    scale = 0.9 / math.sqrt(D)
+    do = rnd((Mq, H * D), dtype, seed + 4) if grad else None
+    o = Fn.window_attention(q, k, v, H, D, nseq=nseq, kv_heads=Hk, window=window, sinks=sinks, keymask=keymask, scale=scale, q_start=q_start, dropout=drop)
+    left, right = window if isinstance(window, tuple) else (window, window)
+    mult = None
+    if drop is not None:
+        from ct_clip_amd import backend
+        top = max(s[3] for s in spans)
+        m = backend.get().attn_dropout_mask(len(spans), H, top, drop[0], drop[1], torch.device(DEV))
+        mult = [m[b] for b in range(len(spans))]
+    want = O.batch64(q.detach(), k.detach(), v.detach(), H, Hk, D, spans, left, right, sinks, q_start, keymask.reshape(-1) if keymask is not None else None, scale, do, mult, dtype)
+    O.check(o.detach(), want["o"], "o")
+    if grad:
+        got = torch.autograd.grad(o, (q, k, v), do)
+        for n, g in zip(("dq", "dk", "dv"), got):
+            O.check(g, want[n], n)
+    return o
+
+
+SQUARE = [  # nseq, L, H, Hk, D, window, sinks, mask
+    (1, 1, 1, 1, 64, (0, 0), 0, None),
+    (2, 2, 2, 1, 32, (1, 0), 1, None),
+    (3, 31, 4, 2, 64, (5, 3), 2, None),
+    (1, 32, 3, 3, 128, (-1, 0), 0, None),
+    (2, 33, 2, 2, 64, (0, 40), 0, "pad"),
+    (3, 65, 6, 2, 64, (16, 16), 4, "holes"),
+    (1, 127, 2, 1, 32, (-1, -1), 0, None),
+    (2, 128, 3, 1, 64, (32, 0), 1, "pad"),
+    (1, 129, 2, 2, 128, (64, 64), 33, None),
+    (2, 200, 4, 4, 64, (20, 10), 70, "holes"),
+    (2, 257, 2, 2, 32, (3, 2), 500, None),              # more sinks than keys
+    (3, 320, 2, 1, 64, (10, 5), 0, "front"),            # rows that see nothing
+    (1, 577, 8, 8, 32, (100, 100), 3, None),
+    (2, 700, 4, 2, 64, (63, 0), 5, None),
+    (1, 1300, 2, 1, 128, (200, 0), 4, "holes"),
+    (1, 1111, 8, 1, 64, (1, 1), 40, None),              # two sink blocks, eight heads on one
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nseq,L,H,Hk,D,window,sinks,mask", SQUARE)
+def test_window_attention_padded_batches(nseq, L, H, Hk, D, window, sinks, mask, dtype):
+    run_case(dtype, nseq, L, L, H, Hk, D, window, sinks, mask=mask, seed=L)
+
+
+ROWS = [  # nseq, Lq, Lk, H, Hk, D, window, sinks, q_start, mask
+    (1, 1, 1, 1, 1, 64, (0, 0), 0, 0, None),
+    (8, 1, 512, 12, 12, 64, (128, 128), 1, 0, "pad"),
+    (2, 1, 777, 8, 2, 128, (-1, 0), 0, 776, None),
+    (1, 1, 5000, 4, 1, 64, (-1, 0), 0, 4999, None),     # the key axis split over workgroups
+    (3, 1, 3001, 6, 3, 32, (1000, 0), 4, 3000, "holes"),
+    (1, 7, 4096, 4, 1, 64, (-1, -1), 0, 2000, None),    # 28 rows of one block
+    (2, 5, 900, 6, 1, 128, (300, 2), 2, 895, "pad"),
+    (1, 1, 2049, 32, 1, 64, (-1, 0), 0, 2048, None),    # 32 heads on one
+    (1, 33, 3000, 1, 1, 64, (-1, 0), 0, 2960, None),    # too many rows for one block: the tiled kernel, split
+    (1, 70, 2500, 2, 1, 128, (-1, -1), 0, 100, "holes"),
+    (2, 40, 100, 3, 3, 32, (9, 9), 3, 50, None),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nseq,Lq,Lk,H,Hk,D,window,sinks,q_start,mask", ROWS)
+def test_window_attention_query_rows_against_a_longer_key_axis(nseq, Lq, Lk, H, Hk, D, window, sinks, q_start, mask, dtype):
+    run_case(dtype, nseq, Lq, Lk, H, Hk, D, window, sinks, q_start=q_start, mask=mask, seed=Lk)
+
+
+PACKED = [  # lengths, first, tail, H, Hk, D, window, sinks
+    ([1], 0, 0, 2, 2, 64, (4, 4), 1),
+    ([5, 0, 1, 64, 33, 130, 2], 0, 0, 4, 2, 64, (20, 10), 2),
+    ([300, 7, 129], 3, 40, 2, 1, 32, (-1, 0), 0),       # rows in front of and behind the sequences
+    ([0, 0, 257], 0, 1, 3, 3, 128, (40, 0), 5),
+    ([700, 1, 600], 0, 0, 2, 1, 64, (50, 50), 36),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lengths,first,tail,H,Hk,D,window,sinks", PACKED)
+def test_window_attention_packed_sequences(lengths, first, tail, H, Hk, D, window, sinks, dtype):
+    run_case(dtype, None, None, None, H, Hk, D, window, sinks, lengths=lengths, first=first, tail=tail, seed=sum(lengths))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nseq,Lq,Lk,H,Hk,D,window,sinks,q_start", [(2, 150, 150, 4, 2, 64, (30, 30), 2, 0), (2, 1, 150, 4, 4, 32, (40, 0), 1, 0), (1, 97, 97, 2, 1, 128, (-1, 0), 0, 0),
+                                                                   (1, 600, 600, 2, 2, 64, (7, 0), 35, 0)])
+def test_window_attention_dropout(nseq, Lq, Lk, H, Hk, D, window, sinks, q_start, dtype):
+    run_case(dtype, nseq, Lq, Lk, H, Hk, D, window, sinks, q_start=q_start, drop=(0.25, 1234567), seed=Lq + 1)
+
+
+def test_window_attention_gradient_against_differences():
+    L, H, D = 70, 2, 32
+    q, k, v = (rnd((L, H * D), F32, 20 + i, 0.7).requires_grad_(True) for i in range(3))
+    g = rnd((L, H * D), F32, 30)
+    dirs = [rnd((L, H * D), F32, 40 + i) for i in range(3)]
+
+    def f(t):      # in 64 bits from the 64-bit form at shifted inputs; the kernel's gradient is what is tested
+        r = O.batch64(q.detach().double() + t * dirs[0], k.detach().double() + t * dirs[1], v.detach().double() + t * dirs[2], H, H, D, [(0, L, 0, L)], 12, 5, 3, 0, None,
+                      1 / math.sqrt(D))
+        return (r["o"][0] * g.double()).sum()
+    h = 1e-4
+    num = (f(h) - f(-h)) / (2 * h)
+    got = torch.autograd.grad(Fn.window_attention(q, k, v, H, D, window=(12, 5), sinks=3), (q, k, v), g)
+    dot = sum((a.double() * d.double()).sum() for a, d in zip(got, dirs))
+    want = O.batch64(q.detach(), k.detach(), v.detach(), H, H, D, [(0, L, 0, L)], 12, 5, 3, 0, None, 1 / math.sqrt(D), g)
+    room = sum((want[n][1] * d.abs().double()).sum() for n, d in zip(("dq", "dk", "dv"), dirs)) + 1e-6 * num.abs()      # h^2 f''' of the difference
+    assert abs(dot - num) <= room
+
+
+def test_window_attention_broadcast_inputs_and_other_streams():
+    """Expanded inputs (row stride 0) get the sum of their rows' gradients; a call on another stream gives the same bits."""
+    L, H, D = 100, 2, 64
+    one = rnd((1, H * D), BF16, 3).requires_grad_(True)
+    k, v = rnd((L, H * D), BF16, 4), rnd((L, H * D), BF16, 5)
+    g = rnd((L, H * D), BF16, 6)
+    (dq,) = torch.autograd.grad(Fn.window_attention(one.expand(L, H * D), k, v, H, D, window=8), one, g)
+    full = one.detach().expand(L, H * D).contiguous().requires_grad_(True)
+    (dfull,) = torch.autograd.grad(Fn.window_attention(full, k, v, H, D, window=8), full, g)
+    assert torch.equal(dq, dfull.sum(0, keepdim=True))
+    want = Fn.window_attention(full.detach(), k, v, H, D, window=8)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = Fn.window_attention(full.detach(), k, v, H, D, window=8)
+    torch.cuda.current_stream().wait_stream(st)
+    assert torch.equal(got, want)
+
+
+def test_every_result_is_reproducible():
+    """Split key axes, sinks and shared heads: a second run gives the same bits."""
+    for kw in (dict(nseq=1, Lq=1, Lk=6000, H=8, Hk=2, D=64, window=(-1, 0), q_start=5999), dict(nseq=2, Lq=900, Lk=900, H=4, Hk=1, D=64, window=(100, 0), q_start=0)):
+        q, k, v = rnd((kw["nseq"] * kw["Lq"], kw["H"] * kw["D"]), BF16, 1), rnd((kw["nseq"] * kw["Lk"], kw["Hk"] * kw["D"]), BF16, 2), rnd((kw["nseq"] * kw["Lk"], kw["Hk"] * kw["D"]), BF16, 3)
+        q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+        g = rnd(tuple(q.shape), BF16, 4)
+        runs = []
+        for _ in range(2):
+            o = Fn.window_attention(q, k, v, kw["H"], kw["D"], nseq=kw["nseq"], kv_heads=kw["Hk"], window=kw["window"], sinks=4, q_start=kw["q_start"])
+            runs.append([o.detach(), *torch.autograd.grad(o, (q, k, v), g)])
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_captured_and_replayed_with_a_workspace_each():
+    """Two graphs whose calls split the key axis, replayed alternately with other inputs between: each replay equals the eager result."""
+    H, D, L = 4, 64, 5000
+    q, k, v = rnd((1, H * D), BF16, 1), rnd((L, H * D), BF16, 2), rnd((L, H * D), BF16, 3)
+    rope = Fn.RotaryPositions(64)
+
+    def step(window):
+        return Fn.window_attention(Fn.rotary(q, None, rope, D, start=L - 1), Fn.rotary(k, None, rope, D), v, H, D, window=window, q_start=L - 1)
+    for w in ((-1, 0), (4000, 0)):
+        step(w)
+    graphs, outs = [], []
+    for w in ((-1, 0), (4000, 0)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(w))
+        graphs.append(g)
+    for rep in range(3):
+        for t in (q, k, v):
+            t.copy_(rnd(tuple(t.shape), BF16, 50 + rep))
+        want = [step((-1, 0)), step((4000, 0))]
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------------- the operators together
+
+@pytest.mark.parametrize("cls_only", [False, True])
+@pytest.mark.parametrize("options", O.BERT_OPTIONS)
+def test_text_tower_with_long_report_options(options, cls_only):
+    """Two layers in f32: ten products of at most 130 terms each way, sums of magnitudes some three times the values: 10 * 130 * 3 * 2^-24 = 2.3e-4 at worst, of either sign."""
+    T = 30 if options.get("position_embedding_type") != "rotary" else 150
+    got, want, grads, rotary = O.bert_case(options, T, DEV, cls_only=cls_only)
+    assert (got.double() - want).abs().max() <= 2e-4 * want.abs().max()
+    for n, (a, b) in grads.items():
+        if "pooler" in n or (rotary and "position_embeddings" in n):
+            assert a is None
+            continue
+        assert (a.double() - b).norm() <= 4e-4 * b.norm() + 1e-6, n
+
+
+@pytest.mark.parametrize("options", O.BERT_OPTIONS)
+def test_text_tower_with_long_report_options_mixed_precision(options):
+    """f32 stream, bf16 matrix operands: in each of two layers seven roundings (2^-8 at most each) stand between the input and the output, and twice that in the gradients;
+    a key bias shifts every score of a row alike, so its true gradient is zero and what is left is held to the query bias's scale."""
+    T = 30 if options.get("position_embedding_type") != "rotary" else 150
+    got, want, grads, rotary = O.bert_case(options, T, DEV, operand_dtype=BF16)
+    assert (got.double() - want).norm() <= 14 * 2.0 ** -8 * want.norm()
+    for n, (a, b) in grads.items():
+        if "pooler" in n or (rotary and "position_embeddings" in n):
+            assert a is None
+            continue
+        scale = grads[n.replace("self.key", "self.query")][1].norm() if "key.bias" in n else b.norm()
+        assert (a.double() - b).norm() <= 28 * 2.0 ** -8 * scale, n

@@ -32,9 +32,17 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(t):
     """Launches for tensors of another device than the current one happen there (its current stream, its allocator)."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _stream_of(t):
+    """The current stream of t's device, as an integer (torch.cuda.current_stream() builds a Stream object: 2.8 us of the ~15 that a small call takes)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _rowmajor(t, what):
@@ -406,54 +414,64 @@ class HipBackend:
     # ------------------------------------------------------------------ long reports (csrc/rotary.hip, csrc/win_attn.hip, csrc/win_attn_bwd.hip)
     def rotary(self, q, k, turns, D, rot, L, positions, start, interleaved, magnitude, inverse=False, out=None):
         """q (M, Hq * D), k (M, Hk * D) or None, rotated by their rows' positions (ctclip_rotary) -> (q', k').  out = (q, k): in place."""
-        M, Hq, Hk = q.shape[0], q.shape[1] // D, (k.shape[1] // D if k is not None else 0)
+        M, nq = q.shape
+        nk = k.shape[1] if k is not None else 0
         with _on(q):
-            if out is None:
-                out = (torch.empty((M, Hq * D), dtype=q.dtype, device=q.device), torch.empty((M, Hk * D), dtype=q.dtype, device=q.device) if k is not None else None)
-            qo, ko = out
-            rc = self.lib.ctclip_rotary(_p(q), _p(k), _p(qo), _p(ko), _p(turns), _p(positions), positions.element_size() if positions is not None else 0, M, int(L), int(start),
-                                        Hq, Hk, D, rot, _rowmajor(q, "q"), _rowmajor(k, "k") if Hk else 0, _rowmajor(qo, "out q"), _rowmajor(ko, "out k") if Hk else 0,
-                                        int(interleaved), float(magnitude), int(inverse), dcode(q.dtype), _stream())
-            _lib.check(rc, "ctclip_rotary")
+            qo, ko = out if out is not None else (torch.empty((M, nq), dtype=q.dtype, device=q.device),
+                                                  torch.empty((M, nk), dtype=q.dtype, device=q.device) if nk else None)
+            rc = self.lib.ctclip_rotary(q.data_ptr(), _p(k), qo.data_ptr(), _p(ko), turns.data_ptr(), _p(positions), positions.element_size() if positions is not None else 0, M,
+                                        L, start, nq // D, nk // D, D, rot, _rowmajor(q, "q"), _rowmajor(k, "k") if nk else 0, _rowmajor(qo, "out q"),
+                                        _rowmajor(ko, "out k") if nk else 0, interleaved, magnitude, inverse, dcode(q.dtype), _stream_of(q))
+            if rc:
+                _lib.check(rc, "ctclip_rotary")
         return qo, ko
 
-    @staticmethod
-    def _win_args(geo):
-        return (geo.nseq, geo.Lq, geo.Lk, geo.Mq, geo.Mk, geo.H, geo.Hk, geo.D, geo.left, geo.right, geo.sinks, geo.q_start)
+    def _win_workspaces(self, geo):
+        """-> bytes of (forward, backward) workspace: they follow from the sizes and are kept with them."""
+        if geo.workspaces is None:
+            sizes = (geo.H, geo.Hk, geo.D, geo.left, geo.right, geo.sinks, geo.q_start)
+            geo.workspaces = (self.lib.ctclip_win_attn_fwd_workspace(geo.nseq, geo.Lq, geo.Lk, *sizes, int(geo.packed)),
+                              self.lib.ctclip_win_attn_bwd_workspace(geo.nseq, geo.Lq, geo.Lk, geo.Mk, *sizes, geo.ntiles))
+        return geo.workspaces
 
     def win_attn_fwd(self, q, k, v, keymask, geo, scale, want_lse=True, dropout=None):
         """softmax(scale q k^T + keymask) v inside geo's window (functional.WindowGeometry; ctclip_win_attn_fwd) -> (o, lse).  Workspaces come from the caching
         allocator per call: two captured graphs never share one."""
         dp, dseed = dropout if dropout is not None else (0.0, 0)
+        dev, n = q.device, geo.H * geo.D
         with _on(q):
-            packed = geo.offsets is not None
-            o = (torch.zeros if packed and geo.rows < geo.Mq else torch.empty)((geo.Mq, geo.H * geo.D), dtype=q.dtype, device=q.device)
-            lse = torch.empty((geo.H, geo.Mq), dtype=torch.float32, device=q.device) if want_lse else None
-            need = self.lib.ctclip_win_attn_fwd_workspace(geo.nseq, geo.Lq, geo.Lk, geo.H, geo.Hk, geo.D, geo.left, geo.right, geo.sinks, geo.q_start, int(packed))
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-            rc = self.lib.ctclip_win_attn_fwd(_p(q), _p(k), _p(v), _p(keymask), _p(geo.offsets), _p(geo.tiles), geo.ntiles, _p(o), _p(lse), *self._win_args(geo),
-                                              _rowmajor(q, "q"), _rowmajor(k, "k"), _rowmajor(v, "v"), _rowmajor(o, "o"), float(scale), float(dp), int(dseed), dcode(q.dtype),
-                                              _p(ws), need, _stream())
-            _lib.check(rc, "ctclip_win_attn_fwd")
+            o = torch.zeros((geo.Mq, n), dtype=q.dtype, device=dev) if geo.uncovered else torch.empty((geo.Mq, n), dtype=q.dtype, device=dev)
+            lse = torch.empty((geo.H, geo.Mq), dtype=torch.float32, device=dev) if want_lse else None
+            need = self._win_workspaces(geo)[0]
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            off, tiles = geo.tables(dev) if geo.packed else (None, None)
+            rc = self.lib.ctclip_win_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), _p(keymask), _p(off), _p(tiles), geo.ntiles, o.data_ptr(), _p(lse), *geo.sizes,
+                                              _rowmajor(q, "q"), _rowmajor(k, "k"), _rowmajor(v, "v"), n, scale, dp, dseed, dcode(q.dtype), _p(ws), need, _stream_of(q))
+            if rc:
+                _lib.check(rc, "ctclip_win_attn_fwd")
         return o, lse
 
     def win_attn_bwd(self, q, k, v, keymask, geo, scale, o, dout, lse, dropout=None, out=None):
         """-> (dq, dk, dv); out: row-strided tensors to write them to (packed rows outside every sequence are zeroed only in fresh ones)."""
         dp, dseed = dropout if dropout is not None else (0.0, 0)
+        dev = q.device
         with _on(q):
-            packed = geo.offsets is not None
             if out is None:
-                new = torch.zeros if packed and geo.rows < geo.Mq else torch.empty
-                out = tuple(new((t.shape[0], t.shape[1]), dtype=q.dtype, device=q.device) for t in (q, k, v))
-            dq, dk, dv = out
-            delta = torch.empty((geo.H, geo.Mq), dtype=torch.float32, device=q.device)
-            need = self.lib.ctclip_win_attn_bwd_workspace(geo.nseq, geo.Lq, geo.Lk, geo.Mk, geo.H, geo.Hk, geo.D, geo.left, geo.right, geo.sinks, geo.q_start, geo.ntiles)
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-            rc = self.lib.ctclip_win_attn_bwd(_p(q), _p(k), _p(v), _p(keymask), _p(geo.offsets), _p(geo.tiles), geo.ntiles, _p(o), _p(dout), _p(lse), _p(delta), _p(dq), _p(dk),
-                                              _p(dv), *self._win_args(geo), _rowmajor(q, "q"), _rowmajor(k, "k"), _rowmajor(v, "v"), _rowmajor(o, "o"),
-                                              _rowmajor(dout, "dout"), _rowmajor(dq, "dq"), _rowmajor(dk, "dk"), _rowmajor(dv, "dv"), float(scale), float(dp), int(dseed),
-                                              dcode(q.dtype), _p(ws), need, _stream())
-            _lib.check(rc, "ctclip_win_attn_bwd")
+                new = torch.zeros if geo.uncovered else torch.empty
+                n, nk = geo.H * geo.D, geo.Hk * geo.D
+                dq, dk, dv = new((geo.Mq, n), dtype=q.dtype, device=dev), new((geo.Mk, nk), dtype=q.dtype, device=dev), new((geo.Mk, nk), dtype=q.dtype, device=dev)
+            else:
+                dq, dk, dv = out
+            need = self._win_workspaces(geo)[1]
+            ws = torch.empty(need + 4 * geo.H * geo.Mq, dtype=torch.uint8, device=dev)       # partial sums, then Delta
+            off, tiles = geo.tables(dev) if geo.packed else (None, None)
+            at = ws.data_ptr()
+            rc = self.lib.ctclip_win_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), _p(keymask), _p(off), _p(tiles), geo.ntiles, o.data_ptr(), dout.data_ptr(),
+                                              lse.data_ptr(), at + need, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *geo.sizes, _rowmajor(q, "q"), _rowmajor(k, "k"),
+                                              _rowmajor(v, "v"), _rowmajor(o, "o"), _rowmajor(dout, "dout"), _rowmajor(dq, "dq"), _rowmajor(dk, "dk"), _rowmajor(dv, "dv"),
+                                              scale, dp, dseed, dcode(q.dtype), at, need, _stream_of(q))
+            if rc:
+                _lib.check(rc, "ctclip_win_attn_bwd")
         return dq, dk, dv
 
     # ------------------------------------------------------------------ input pipeline (csrc/preprocess.hip)

@@ -10,13 +10,13 @@ Weight handling
     gradient buffer; split-K partial sums go through f32 slabs and a fixed-order reduce -- the library has no float atomics)
     when present -- autograd then sees ``None`` for that input; otherwise a fresh f32 gradient tensor is returned as usual.
 """
+import functools
 import math
 import os
 
 import numpy as np
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import backend as _be
 from . import streams as _streams
@@ -1232,6 +1232,7 @@ class RotaryPositions:
         if not base > 1.0 or not math.isfinite(base):
             raise ValueError(f"rotary base must be finite and > 1, got {base}")
         self.dim, self.layout, self.base, self.magnitude = int(dim), layout, float(base), 1.0
+        self.interleaved = layout == "interleaved"
         pair = np.arange(0, self.dim, 2, dtype=np.float64)
         scaling = dict(scaling) if scaling else {"type": "none"}
         kind = scaling.pop("type", None)
@@ -1271,27 +1272,32 @@ class RotaryPositions:
 
 def _aligned_rows(t):
     """t itself when its rows can be read 16 bytes at a time, else a dense copy."""
-    ok = t.stride(1) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) * t.element_size() % 16 == 0
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    ld, one = t.stride()
+    return t if one == 1 and not (t.data_ptr() | ld * t.element_size()) & 15 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _not_twice():
+    """(Backward functions made of kernels: a graph of them would hold no further derivative.)"""
+    if torch.is_grad_enabled():
+        raise RuntimeError("rotary / window_attention: no derivative of the gradient (create_graph=True)")
 
 
 class RotaryFn(Function):
     @staticmethod
     def forward(ctx, q, k, rope, D, L, positions, start):
-        be = B()
-        ctx.args = (rope, D, L, start)
-        ctx.save_for_backward(*([positions] if positions is not None else []))
-        qo, ko = be.rotary(q, k, rope.turns(q.device), D, rope.dim, L, positions, start, rope.layout == "interleaved", rope.magnitude)
+        ctx.args = (rope, D, L, start, positions)           # (positions: integers, not differentiated, not an output)
+        qo, ko = B().rotary(q, k, rope.turns(q.device), D, rope.dim, L, positions, start, rope.interleaved, rope.magnitude)
         return qo if k is None else (qo, ko)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dq, dk=None):
-        rope, D, L, start = ctx.args
-        positions = ctx.saved_tensors[0] if ctx.saved_tensors else None
-        dq = dq.contiguous()
-        gq, gk = B().rotary(dq, dk.contiguous() if dk is not None else None, rope.turns(dq.device), D, rope.dim, L, positions, start, rope.layout == "interleaved",
-                            rope.magnitude, inverse=True)
+        _not_twice()
+        rope, D, L, start, positions = ctx.args
+        if dq.stride(1) != 1:
+            dq = dq.contiguous()
+        if dk is not None and dk.stride(1) != 1:
+            dk = dk.contiguous()
+        gq, gk = B().rotary(dq, dk, rope.turns(dq.device), D, rope.dim, L, positions, start, rope.interleaved, rope.magnitude, True)
         return gq, gk, None, None, None, None, None
 
 
@@ -1302,26 +1308,28 @@ def rotary(q, k, rope, D, L=None, positions=None, start=0):
     tensor of M on the same device, any values), or start + i % L for sequences of L rows (L = None: one sequence)."""
     if not isinstance(rope, RotaryPositions):
         raise TypeError("rotary: rope must be a RotaryPositions")
-    for t, name in ((q, "q"), (k, "k")):
-        if t is None and name == "k":
-            continue
-        if t.dim() != 2 or t.shape[1] % D or (t.shape[1] == 0) or t.shape[0] != q.shape[0] or t.dtype != q.dtype or t.device != q.device:
-            raise ValueError(f"rotary: {name} must be (M, heads * {D}) like q, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if q.dim() != 2 or q.shape[1] % D or not q.shape[1]:
+        raise ValueError(f"rotary: q must be (M, heads * {D}), got {tuple(q.shape)}")
+    M = q.shape[0]
+    if k is not None and (k.dim() != 2 or k.shape[1] % D or not k.shape[1] or k.shape[0] != M or k.dtype != q.dtype or k.device != q.device):
+        raise ValueError(f"rotary: k must be ({M}, heads * {D}) like q, got {tuple(k.shape)} {k.dtype} on {k.device}")
     if rope.dim > D:
         raise ValueError(f"rotary: {rope.dim} rotated columns in heads of {D}")
-    M = q.shape[0]
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (M,) or positions.device != q.device:
             raise ValueError(f"rotary: positions must be {M} int32 / int64 values on {q.device}")
         positions = positions.contiguous()
-    L = max(M, 1) if L is None else int(L)
-    if L < 1 or not -2 ** 62 < int(start) < 2 ** 62:
+    L, start = max(M, 1) if L is None else int(L), int(start)
+    if L < 1 or not -2 ** 62 < start < 2 ** 62:
         raise ValueError("rotary: L >= 1 and a start within 62 bits")
     if q.stride(1) != 1:
         q = q.contiguous()
     if k is not None and k.stride(1) != 1:
         k = k.contiguous()
-    return RotaryFn.apply(q, k, rope, int(D), L, positions, int(start))
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return RotaryFn.apply(q, k, rope, D, L, positions, start)
+    qo, ko = B().rotary(q, k, rope.turns(q.device), D, rope.dim, L, positions, start, rope.interleaved, rope.magnitude)
+    return qo if k is None else (qo, ko)
 
 
 class PackedSequences:
@@ -1342,7 +1350,7 @@ class PackedSequences:
         tiles = [(b, t) for b, n in enumerate(self.lengths) for t in range((n + 127) // 128)]
         self.ntiles = len(tiles)
         self._host = (torch.from_numpy(ends.astype(np.int32)), torch.tensor(tiles, dtype=torch.int32).reshape(-1))
-        self._dev = {}
+        self._dev, self._geometry = {}, {}
 
     def on(self, device):
         t = self._dev.get(device)
@@ -1352,70 +1360,76 @@ class PackedSequences:
 
 
 class WindowGeometry:
-    """What the kernels need to know of a call: sizes, window, and the packed sequences' tables."""
-    __slots__ = ("nseq", "Lq", "Lk", "Mq", "Mk", "H", "Hk", "D", "left", "right", "sinks", "q_start", "offsets", "tiles", "ntiles", "rows")
+    """What the kernels need to know of a call -- sizes, window, the packed sequences -- and the workspaces that follow from it.  Depends on sizes only."""
+
+    def __init__(self, Mq, Mk, H, Hk, D, seqs, left, right, sinks, q_start):
+        if D not in (32, 64, 128):
+            raise ValueError(f"window_attention: heads of 32, 64 or 128 columns, got {D}")
+        if H < 1 or Hk < 1 or H % Hk:
+            raise ValueError(f"window_attention: {H} query heads over {Hk} key / value heads")
+        if left < -1 or right < -1 or sinks < 0 or q_start < 0:
+            raise ValueError("window_attention: window sides >= -1, sinks >= 0, q_start >= 0")
+        self.Mq, self.Mk, self.H, self.Hk, self.D = Mq, Mk, H, Hk, D
+        self.left, self.right, self.sinks, self.q_start = min(left, 2 ** 30), min(right, 2 ** 30), min(sinks, 2 ** 30), q_start
+        self.packed, self.seqs = isinstance(seqs, PackedSequences), seqs
+        self.ntiles, self.uncovered = 0, False
+        if self.packed:
+            if Mq != Mk or seqs.end > Mq or q_start:
+                raise ValueError(f"window_attention: packed sequences end at row {seqs.end} of {Mq} query and {Mk} key rows (equal, and q_start = 0)")
+            self.Lq = self.Lk = seqs.longest
+            self.nseq, self.ntiles, self.uncovered = len(seqs.lengths) if seqs.ntiles else 0, seqs.ntiles, seqs.rows < Mq
+        else:
+            self.nseq = seqs
+            if seqs < 0 or (seqs == 0 and (Mq or Mk)) or (seqs and (Mq % seqs or Mk % seqs)):
+                raise ValueError(f"window_attention: {Mq} query and {Mk} key rows are not {seqs} equal sequences")
+            self.Lq, self.Lk = (Mq // seqs, Mk // seqs) if seqs else (0, 0)
+            if q_start + self.Lq > self.Lk and self.Lq:
+                raise ValueError(f"window_attention: query positions {q_start} ... {q_start + self.Lq - 1} on a key axis of {self.Lk}")
+        self.empty = self.nseq == 0 or self.Lq == 0           # no query row in any sequence
+        self.sizes = (self.nseq, self.Lq, self.Lk, Mq, Mk, H, Hk, D, self.left, self.right, self.sinks, q_start)
+        self.workspaces = None        # (bytes forward, backward), by the kernels' backend at the first call
+
+    def tables(self, device):
+        return self.seqs.on(device)
+
+
+_equal_sequences = functools.lru_cache(maxsize=512)(WindowGeometry)
+
+
+def window_geometry(Mq, Mk, H, Hk, D, nseq, window, sinks, q_start):
+    """The (kept) ``WindowGeometry`` of these sizes: with the table of a number of equal sequences, or with the packed sequences themselves."""
+    left, right = (window, window) if isinstance(window, int) else window
+    key = (Mq, Mk, H, Hk, D, int(left), int(right), int(sinks), int(q_start))
+    if not isinstance(nseq, PackedSequences):
+        return _equal_sequences(*key[:5], int(nseq), *key[5:])
+    g = nseq._geometry.get(key)
+    if g is None:
+        if len(nseq._geometry) > 64:
+            nseq._geometry.clear()
+        g = nseq._geometry[key] = WindowGeometry(*key[:5], nseq, *key[5:])
+    return g
 
 
 class WindowAttnFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, keymask, geo, scale, dropout):
         ctx.args = (geo, scale, dropout)
-        if geo.nseq == 0 or geo.Lq == 0:       # no query row in any sequence
+        if geo.empty:
             ctx.save_for_backward(q, k, v)
             return q.new_zeros((geo.Mq, geo.H * geo.D))
-        need = any(ctx.needs_input_grad[:3])
-        o, lse = B().win_attn_fwd(q, k, v, keymask, geo, scale, want_lse=need, dropout=dropout)
-        if need:
-            ctx.save_for_backward(q, k, v, o, lse, *([keymask] if keymask is not None else []))
+        o, lse = B().win_attn_fwd(q, k, v, keymask, geo, scale, True, dropout)
+        ctx.save_for_backward(q, k, v, o, lse, keymask)
         return o
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do):
+        _not_twice()
         geo, scale, dropout = ctx.args
-        if geo.nseq == 0 or geo.Lq == 0:
+        if geo.empty:
             return (*(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in ctx.saved_tensors), None, None, None, None)
-        q, k, v, o, lse, *mask = ctx.saved_tensors
-        dq, dk, dv = B().win_attn_bwd(q, k, v, mask[0] if mask else None, geo, scale, o, _aligned_rows(do), lse, dropout=dropout)
+        q, k, v, o, lse, keymask = ctx.saved_tensors
+        dq, dk, dv = B().win_attn_bwd(q, k, v, keymask, geo, scale, o, _aligned_rows(do), lse, dropout)
         return dq, dk, dv, None, None, None, None
-
-
-def window_geometry(q, k, v, H, D, nseq=1, kv_heads=None, window=(-1, -1), sinks=0, q_start=0):
-    Hk = H if kv_heads is None else int(kv_heads)
-    if D not in (32, 64, 128):
-        raise ValueError(f"window_attention: heads of 32, 64 or 128 columns, got {D}")
-    if H < 1 or Hk < 1 or H % Hk:
-        raise ValueError(f"window_attention: {H} query heads over {Hk} key / value heads")
-    for t, heads, name in ((q, H, "q"), (k, Hk, "k"), (v, Hk, "v")):
-        if t.dim() != 2 or t.shape[1] != heads * D or t.dtype != q.dtype or t.device != q.device:
-            raise ValueError(f"window_attention: {name} must be (rows, {heads} * {D}) of q's type and device, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    if q.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"window_attention: unsupported dtype {q.dtype}")
-    left, right = (int(window), int(window)) if isinstance(window, int) else (int(window[0]), int(window[1]))
-    if left < -1 or right < -1 or sinks < 0 or q_start < 0:
-        raise ValueError("window_attention: window sides >= -1, sinks >= 0, q_start >= 0")
-    if k.shape[0] != v.shape[0]:
-        raise ValueError(f"window_attention: {k.shape[0]} rows of k, {v.shape[0]} of v")
-    g = WindowGeometry()
-    g.H, g.Hk, g.D, g.left, g.right, g.sinks, g.q_start = int(H), Hk, int(D), min(left, 2 ** 30), min(right, 2 ** 30), min(int(sinks), 2 ** 30), int(q_start)
-    g.Mq, g.Mk, g.offsets, g.tiles, g.ntiles = q.shape[0], k.shape[0], None, None, 0
-    if isinstance(nseq, PackedSequences):
-        if g.Mq != g.Mk or nseq.end > g.Mq or g.q_start:
-            raise ValueError(f"window_attention: packed sequences end at row {nseq.end} of {g.Mq} query and {g.Mk} key rows (equal, and q_start = 0)")
-        g.nseq, g.Lq, g.Lk, g.rows = len(nseq.lengths), nseq.longest, nseq.longest, nseq.rows
-        if nseq.ntiles:
-            (g.offsets, g.tiles), g.ntiles = nseq.on(q.device), nseq.ntiles
-        else:
-            g.nseq = 0
-    else:
-        g.nseq = int(nseq)
-        if g.nseq < 0 or (g.nseq == 0 and (g.Mq or g.Mk)) or (g.nseq and (g.Mq % g.nseq or g.Mk % g.nseq)):
-            raise ValueError(f"window_attention: {g.Mq} query and {g.Mk} key rows are not {g.nseq} equal sequences")
-        g.Lq, g.Lk = (g.Mq // g.nseq, g.Mk // g.nseq) if g.nseq else (0, 0)
-        g.rows = g.Mq
-        if g.q_start + g.Lq > g.Lk and g.Lq:
-            raise ValueError(f"window_attention: query positions {g.q_start} ... {g.q_start + g.Lq - 1} on a key axis of {g.Lk}")
-    return g
 
 
 def window_attention(q, k, v, H, D, nseq=1, kv_heads=None, window=(-1, -1), sinks=0, keymask=None, scale=None, q_start=0, dropout=None):
@@ -1426,19 +1440,30 @@ def window_attention(q, k, v, H, D, nseq=1, kv_heads=None, window=(-1, -1), sink
     q_start + i of its key axis (one new token: a single row with q_start = its position; the [CLS] row: q_start = 0).
     window = (left, right) or one number for both, -1 = no limit: position i sees keys i - left ... i + right, and of the keys further left the first `sinks`.
     keymask: additive f32, (nseq, key rows of a sequence) or flat per key row, no gradient; values <= -1e30 (HF's finfo.min, -inf) and NaN hide the key, whatever k
-    and v hold there.  A row that sees no key is 0 and gives no gradient.  dropout = (p, seed): attention-probability dropout, masks as in ``SdpaFn``.
-    scale > 0, default 1 / sqrt(D)."""
-    g = window_geometry(q, k, v, H, D, nseq, kv_heads, window, sinks, q_start)
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    and v hold there; keys that only the window hides must be finite.  A row that sees no key is 0 and gives no gradient.  dropout = (p, seed):
+    attention-probability dropout, masks as in ``SdpaFn``.  scale > 0, default 1 / sqrt(D)."""
+    Hk = H if kv_heads is None else kv_heads
+    if q.dim() != 2 or k.dim() != 2 or q.shape[1] != H * D or k.shape[1] != Hk * D or k.shape != v.shape or k.dtype != q.dtype or v.dtype != q.dtype \
+            or k.device != q.device or v.device != q.device:
+        raise ValueError(f"window_attention: q (rows, {H} * {D}), k and v (rows, {Hk} * {D}) of one type and device, got " +
+                         ", ".join(f"{tuple(t.shape)} {t.dtype} on {t.device}" for t in (q, k, v)))
+    if q.dtype != torch.bfloat16 and q.dtype != torch.float32:
+        raise TypeError(f"window_attention: unsupported dtype {q.dtype}")
+    geo = window_geometry(q.shape[0], k.shape[0], H, Hk, D, nseq, window, sinks, q_start)
+    scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise ValueError(f"window_attention: scale must be positive and finite, got {scale}")
     if dropout is not None and not 0.0 <= dropout[0] < 1.0:
         raise ValueError(f"window_attention: dropout probability {dropout[0]}")
     if keymask is not None:
-        if keymask.numel() != g.Mk or keymask.device != q.device or not keymask.is_floating_point():
-            raise ValueError(f"window_attention: keymask must be one additive value per key row ({g.Mk}) on {q.device}")
-        keymask = keymask.detach().to(torch.float32).contiguous().view(-1)
-    return WindowAttnFn.apply(_aligned_rows(q), _aligned_rows(k), _aligned_rows(v), keymask, g, scale, dropout)
+        if keymask.numel() != geo.Mk or keymask.device != q.device or not keymask.is_floating_point():
+            raise ValueError(f"window_attention: keymask must be one additive value per key row ({geo.Mk}) on {q.device}")
+        if keymask.dtype != torch.float32 or keymask.requires_grad or not keymask.is_contiguous():
+            keymask = keymask.detach().to(torch.float32).contiguous()
+    q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return WindowAttnFn.apply(q, k, v, keymask, geo, scale, dropout)
+    return q.new_zeros((geo.Mq, H * D)) if geo.empty else B().win_attn_fwd(q, k, v, keymask, geo, scale, False, dropout)[0]
 
 
 def _qkv_shadows(dtype, device, wq, wk, wv, bq, bk, bv):
@@ -1561,9 +1586,9 @@ class QkvWindowFn(Function):
         qkv = be.gemm(x, wsh, bias=bias)
         if rope is not None:
             q, k = qkv[:, :N], qkv[:, N:2 * N]
-            be.rotary(q, k, rope.turns(x.device), D, rope.dim, L, None, 0, rope.layout == "interleaved", rope.magnitude, out=(q, k))
+            be.rotary(q, k, rope.turns(x.device), D, rope.dim, L, None, 0, rope.interleaved, rope.magnitude, out=(q, k))
         q, k, v = QkvWindowFn._views(qkv, N, nseq, L, first_only)
-        geo = window_geometry(q, k, v, H, D, nseq, None, window, sinks, 0)
+        geo = window_geometry(q.shape[0], k.shape[0], H, H, D, nseq, window, sinks, 0)
         o, lse = be.win_attn_fwd(q, k, v, keymask, geo, scale, want_lse=any(ctx.needs_input_grad[:7]), dropout=dropout)
         ctx.wt = _qkv_transposed_shadow(x, wq, wk, wv) if ctx.needs_input_grad[0] else None
         if lse is not None:
@@ -1580,8 +1605,8 @@ class QkvWindowFn(Function):
         return q, qkv[:, N:2 * N], qkv[:, 2 * N:]
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do, d_pass=None):
+        _not_twice()
         be = B()
         x, wsh, qkv, o, lse, *mask = ctx.saved_tensors
         geo, scale, dropout, rope, nseq, L, N, D, first_only = ctx.args
@@ -1593,7 +1618,7 @@ class QkvWindowFn(Function):
                         out=QkvWindowFn._views(dqkv, N, nseq, L, first_only))
         if rope is not None:
             dq, dk = dqkv[:, :N], dqkv[:, N:2 * N]
-            be.rotary(dq, dk, rope.turns(x.device), D, rope.dim, L, None, 0, rope.layout == "interleaved", rope.magnitude, inverse=True, out=(dq, dk))
+            be.rotary(dq, dk, rope.turns(x.device), D, rope.dim, L, None, 0, rope.interleaved, rope.magnitude, inverse=True, out=(dq, dk))
         dx, gw, gb = _qkv_backward(ctx, dqkv, x, wsh, d_pass)
         return (dx, *gw, *gb, *([None] * 13))
 

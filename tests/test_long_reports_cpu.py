@@ -29,8 +29,8 @@ class RefOps(RefBackend):
 
     @staticmethod
     def _spans(geo):
-        if geo.offsets is not None:
-            e = geo.offsets.tolist()
+        if geo.packed:
+            e = geo.tables(torch.device("cpu"))[0].tolist()
             return [(a, b - a, a, b - a) for a, b in zip(e, e[1:])]
         return [(b * geo.Lq, geo.Lq, b * geo.Lk, geo.Lk) for b in range(geo.nseq)]
 

@@ -67,13 +67,6 @@ template <typename T, int D> __device__ __forceinline__ void row_frag_global(Row
     f.v[g] = __builtin_bit_cast(decltype(f.v[0] + f.v[0]), w);
   }
 }
-template <typename T, int D> __device__ __forceinline__ void row_frag_lds(RowFrag<T, D>& f, const char* tile, int row, int half) {
-#pragma unroll
-  for (int g = 0; g < Geo<T, D>::NCH / 2; ++g) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(tile + lds_at<T, D>(row, 2 * g + half));
-    f.v[g] = __builtin_bit_cast(decltype(f.v[0] + f.v[0]), w);
-  }
-}
 template <int D> __device__ __forceinline__ f32x16 mma_rows(const RowFrag<bf16_t, D>& a, const RowFrag<bf16_t, D>& b, f32x16 c) {
 #pragma unroll
   for (int g = 0; g < D / 16; ++g) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v[g], b.v[g], c, 0, 0, 0);
@@ -85,6 +78,16 @@ template <int D> __device__ __forceinline__ f32x16 mma_rows(const RowFrag<float,
 #pragma unroll
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[g][e], b.v[g][e], c, 0, 0, 0);
   return c;
+}
+// Wait for a fragment HERE.  Left to itself the compiler waits in front of the first product of a loop, in every round of it (it cannot count the loads of the first
+// round), and so for the next tile's loads too, which were to arrive under the products: 150 -> 73 us for 4 x 8192 tokens, 12 heads of 64, window 512.
+template <typename T, int D> __device__ __forceinline__ void row_frag_arrive(RowFrag<T, D>& f) {
+#pragma unroll
+  for (int g = 0; g < Geo<T, D>::NCH / 2; ++g) {
+    u32x4 w = __builtin_bit_cast(u32x4, f.v[g]);
+    asm volatile("" : "+v"(w));
+    f.v[g] = __builtin_bit_cast(decltype(f.v[0] + f.v[0]), w);
+  }
 }
 // a lane's half of a row's dot product
 template <int D> __device__ __forceinline__ float row_dot(const RowFrag<bf16_t, D>& a, const RowFrag<bf16_t, D>& b) {
@@ -126,34 +129,67 @@ __device__ __forceinline__ void p_frag(PFrag<float>& f, const float (&p)[16]) {
   for (int r = 0; r < 16; ++r) f.v[r] = p[r];
 }
 typedef __attribute__((ext_vector_type(4))) short s16x4;
-// acc[i] += (32-column block i of the tile rows row0 ... row0 + 31)^T x P: the second product, operand read transposed from the row-major tile
-template <int D> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[D / 32], const char* tile, int row0, const PFrag<bf16_t>& p, int lane) {
-  const int half = lane >> 5, t = lane & 15, g1 = (lane >> 4) & 1;
+// A lane's byte offsets inside a 32-row block, computed once: `row` for the products along D (row c = lane & 31), `col` for the transposing reads of the second
+// product (32-column block i, rows + 8 u).  Blocks are multiples of 32 rows apart, which the chunk permutation does not see, so everything else is an immediate.
+template <typename T, int D> struct LaneAt {
+  int row[Geo<T, D>::NCH / 2];
+  int col[D / 32][2];
+  __device__ __forceinline__ explicit LaneAt(int lane) {
+    const int half = lane >> 5, c = lane & 31, t = lane & 15, g1 = (lane >> 4) & 1;
+#pragma unroll
+    for (int g = 0; g < Geo<T, D>::NCH / 2; ++g) row[g] = lds_at<T, D>(c, 2 * g + half);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) col[i][u] = sizeof(T) == 2 ? lds_at<T, D>(8 * u + 4 * half + (t >> 2), 4 * i + 2 * g1 + ((t & 3) >> 1)) + (t & 1) * 8 : 0;
+  }
+};
+template <typename T, int D> __device__ __forceinline__ void row_frag_lds(RowFrag<T, D>& f, const char* block, const LaneAt<T, D>& at) {
+#pragma unroll
+  for (int g = 0; g < Geo<T, D>::NCH / 2; ++g) {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(block + at.row[g]);
+    f.v[g] = __builtin_bit_cast(decltype(f.v[0] + f.v[0]), w);
+  }
+}
+// Operand of the second product: the block's 32 rows read transposed from the row-major tile.  Read apart from the product, so that it can be on its way while
+// something else is computed (bf16; f32 reads element by element inside the product).
+template <typename T, int D> struct ColFrag;
+template <int D> struct ColFrag<bf16_t, D> { bf16x8 v[2][D / 32]; };
+template <int D> struct ColFrag<float, D> { const char* block; };
+template <int D> __device__ __forceinline__ void col_frag_lds(ColFrag<bf16_t, D>& f, const char* block, const LaneAt<bf16_t, D>& at) {
 #pragma unroll
   for (int G = 0; G < 2; ++G)
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
-      const int chunk = 4 * i + 2 * g1 + ((t & 3) >> 1);
-      const int r = 16 * G + 4 * half + (t >> 2);          // (row0 is a multiple of 32: the chunk permutation does not see it)
-      const char* lo = tile + row0 * Geo<bf16_t, D>::ROWB + lds_at<bf16_t, D>(r, chunk) + (t & 1) * 8;
-      const char* hi = tile + row0 * Geo<bf16_t, D>::ROWB + lds_at<bf16_t, D>(r + 8, chunk) + (t & 1) * 8;
-      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lo));
-      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(hi));
-      const bf16x8 op = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op, p.v[G], acc[i], 0, 0, 0);
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(block + 16 * G * Geo<bf16_t, D>::ROWB + at.col[i][0]));
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(block + 16 * G * Geo<bf16_t, D>::ROWB + at.col[i][1]));
+      f.v[G][i] = bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
 }
-template <int D> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[D / 32], const char* tile, int row0, const PFrag<float>& p, int lane) {
+template <int D> __device__ __forceinline__ void col_frag_lds(ColFrag<float, D>& f, const char* block, const LaneAt<float, D>&) { f.block = block; }
+// acc[i] += (32-column block i)^T x P
+template <int D> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[D / 32], const ColFrag<bf16_t, D>& f, const PFrag<bf16_t>& p, int) {
+#pragma unroll
+  for (int G = 0; G < 2; ++G)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.v[G][i], p.v[G], acc[i], 0, 0, 0);
+}
+template <int D> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[D / 32], const ColFrag<float, D>& f, const PFrag<float>& p, int lane) {
   const int half = lane >> 5, c = lane & 31;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const int row = 8 * (r >> 2) + 4 * half + (r & 3);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
-      const float a = *reinterpret_cast<const float*>(tile + row0 * Geo<float, D>::ROWB + lds_at<float, D>(row, 8 * i + (c >> 2)) + (c & 3) * 4);
+      const float a = *reinterpret_cast<const float*>(f.block + lds_at<float, D>(row, 8 * i + (c >> 2)) + (c & 3) * 4);
       acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p.v[r], acc[i], 0, 0, 0);
     }
   }
+}
+template <typename T, int D> __device__ __forceinline__ void mma_cols(f32x16 (&acc)[D / 32], const char* block, const LaneAt<T, D>& at, const PFrag<T>& p, int lane) {
+  ColFrag<T, D> f;
+  col_frag_lds<D>(f, block, at);
+  mma_cols<D>(acc, f, p, lane);
 }
 
 // ---- a tile's journey from memory through registers to LDS: ROWS rows of D elements by NT threads
@@ -163,30 +199,163 @@ template <typename T, int D, int ROWS, int NT> struct Stage {
   u32x4 w[N];
   __device__ static __forceinline__ int row(int tid, int i) { return (tid + i * NT) / Geo<T, D>::NCH; }
   __device__ static __forceinline__ int chunk(int tid, int i) { return (tid + i * NT) % Geo<T, D>::NCH; }
-  // rows first ... of a sequence that has `n` of them (n >= 1), base = its row 0; rows outside are read from the nearest one inside, and zeroed by put()
-  __device__ __forceinline__ void get(const T* base, int64_t ld, int first, int n, int tid) {
+  // tile = row 0 of the tile (uniform), ldb = bytes between rows (below 2^24: 24-bit products); rows past `last` >= 0 are read from row `last`, and zeroed by put()
+  __device__ __forceinline__ void get(const char* tile, int ldb, int last, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      int j = first + row(tid, i);
-      j = j < 0 ? 0 : (j < n ? j : n - 1);
-      w[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base + (int64_t)j * ld) + chunk(tid, i) * 16);
+      const int r = row(tid, i) < last ? row(tid, i) : last;
+      w[i] = *reinterpret_cast<const u32x4*>(tile + ((uint32_t)__mul24(r, ldb) + (uint32_t)(chunk(tid, i) * 16)));
     }
   }
-  // keep: bit i = chunk i belongs to a row that may be seen (a hidden row is stored as zeros: whatever it holds, NaN included, never meets a product)
-  __device__ __forceinline__ void put(char* tile, uint32_t keep, int tid) const {
+  __device__ __forceinline__ void put(char* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(tile + lds_at<T, D>(row(tid, i), chunk(tid, i))) = w[i];
+  }
+  // keep: bit r = row r of the tile may be seen (a hidden row is stored as zeros: whatever it holds, NaN included, never meets a product)
+  __device__ __forceinline__ void put(char* tile, uint64_t keep, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const u32x4 z = {0, 0, 0, 0};
-      *reinterpret_cast<u32x4*>(tile + lds_at<T, D>(row(tid, i), chunk(tid, i))) = (keep >> i) & 1 ? w[i] : z;
+      *reinterpret_cast<u32x4*>(tile + lds_at<T, D>(row(tid, i), chunk(tid, i))) = (keep >> row(tid, i)) & 1 ? w[i] : z;
     }
   }
 };
+__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1ull); }
 
-// visibility of the 32 x 32 block (query positions lo ... hi, keys j0 ... j0 + 31) by position: 0 nothing, 1 some, 2 everything
-__device__ __forceinline__ int block_sight(int lo, int hi, int j0, int left, int right, int sinks, int Lk) {
-  if (j0 > hi + right || j0 >= Lk || (j0 + 31 < lo - left && j0 >= sinks)) return 0;
-  return (j0 + 31 <= lo + right && j0 + 31 < Lk && (j0 >= hi - left || j0 + 31 < sinks)) ? 2 : 1;
-}
+__device__ __forceinline__ float mask_value(float km) { return km > HIDDEN ? km * LOG2E_ : -INFINITY; }      // (NaN hides)
+// ---- the same journey without the registers: 16 bytes per lane straight from memory into LDS (buffer_load ... lds).  The LDS side is linear in the thread index, so the
+// chunk permutation is applied to the address that a lane READS.  Rows past the valid ones are outside the buffer descriptor, and the load writes zeros for them.
+// Inline asm on purpose: next to the builtin the compiler waits for all loads in front of every LDS read, since it cannot tell the buffer being filled from the one
+// being read.  There is no output register; arrive() waits for everything in flight.
+template <typename T, int D, int ROWS, int NT> struct Dma {
+  static constexpr int N = ROWS * Geo<T, D>::NCH / NT;
+  static_assert(N >= 1 && ROWS * Geo<T, D>::NCH % NT == 0 && NT % 64 == 0, "whole chunks per thread");
+  uint32_t off[N];                                         // a lane's byte offsets inside a tile
+  __device__ static __forceinline__ int row(int tid, int i) { return (tid + i * NT) / Geo<T, D>::NCH; }
+  __device__ __forceinline__ void init(int ldb, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = row(tid, i), c = (tid + i * NT) % Geo<T, D>::NCH;
+      off[i] = (uint32_t)(r * ldb) + (uint32_t)((c ^ swz<Geo<T, D>::NCH>(r)) << 4);
+    }
+  }
+  // tile, ldb (bytes between rows), valid (rows from the tile's first on that may be read, >= 1) are uniform
+  __device__ __forceinline__ void issue(char* lds_tile, const char* tile, int ldb, int valid, int tid) const {
+    const uint64_t base = reinterpret_cast<uint64_t>(tile);
+    const uint32_t bytes = valid >= ROWS ? 0x7fffffffu : (uint32_t)((valid - 1) * ldb) + (uint32_t)Geo<T, D>::ROWB;
+    const u32x4 rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)base), (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(base >> 32) & 0xffffu)),
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00027000u};
+    const uint32_t dst = (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds_tile + (uint32_t)(tid & ~63) * 16u));
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(dst + (uint32_t)(i * NT * 16)), "v"(off[i]), "s"(rsrc) : "memory", "m0");
+  }
+  // (behind arrive()) zeros over the rows of this thread's chunks that `keep` leaves out
+  __device__ __forceinline__ void erase(char* lds_tile, uint64_t keep, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (!((keep >> row(tid, i)) & 1)) { const u32x4 z = {0, 0, 0, 0}; *reinterpret_cast<u32x4*>(lds_tile + (tid + i * NT) * 16) = z; }
+  }
+};
+__device__ __forceinline__ void dma_arrive() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// The key tiles (KT keys of k and v) of a (sequence, k|v head) on their way into LDS, with the key mask.  NT threads share a tile; every wave knows the whole tile's
+// mask by a ballot (lane = key), so hidden rows and the state are wave-uniform masks.
+struct KeySource {
+  const char *k, *v;
+  const float* mask;
+  int ldk, ldv, lk, jlo, jhi, sinks;                       // keys outside [jlo, jhi] and the sinks are seen by nobody here
+  template <typename T, int D> __device__ __forceinline__ void init(const Params& p, int64_t k0, int hk, int lk_, int jlo_, int jhi_) {
+    k = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.k) + k0 * p.ldk + (int64_t)hk * D);
+    v = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + k0 * p.ldv + (int64_t)hk * D);
+    mask = p.keymask ? p.keymask + k0 : nullptr;
+    ldk = (int)p.ldk * (int)sizeof(T); ldv = (int)p.ldv * (int)sizeof(T);
+    lk = lk_; jlo = jlo_; jhi = jhi_ < lk_ - 1 ? jhi_ : lk_ - 1; sinks = p.sinks;
+  }
+  // rows of the tile at j0 that may be seen, and (return) what its mask looks like: 0 nothing, 1 some additive values (written to `bias`), 2 no key is seen
+  template <int KT> __device__ __forceinline__ int look(uint64_t& keep, float km, float* bias, int j0, int tid) const {
+    keep = low_bits(jhi + 1 - j0);
+    if (j0 < jlo) keep &= ~low_bits(jlo - j0) | low_bits(sinks - j0);
+    int state = 0;
+    if (mask) {
+      const float b = mask_value(km);
+      const uint64_t seen = __builtin_amdgcn_ballot_w64(b > -INFINITY);
+      keep &= seen;
+      state = (keep & low_bits(KT)) == 0 ? 2 : (__builtin_amdgcn_ballot_w64(b != 0.f) != 0 ? 1 : 0);
+      if (tid < KT) bias[tid] = b;
+    }
+    keep |= ~low_bits(KT);
+    return state;
+  }
+};
+template <typename T, int D, int KT, int NT> struct KeyPipe {      // through LDS-DMA: issue() into a buffer that nobody reads, settle() before the barrier
+  KeySource src;
+  Dma<T, D, KT, NT> dk, dv;
+  float km;
+  int j0;
+  __device__ __forceinline__ KeyPipe(const Params& p, int64_t k0, int hk, int lk, int jlo, int jhi, int tid) {
+    src.init<T, D>(p, k0, hk, lk, jlo, jhi);
+    dk.init(src.ldk, tid);
+    dv.init(src.ldv, tid);
+    km = 0.f; j0 = 0;
+  }
+  __device__ __forceinline__ void issue(char* kt, char* vt, int first, int tid) {
+    j0 = first;
+    dk.issue(kt, src.k + (int64_t)first * src.ldk, src.ldk, src.jhi + 1 - first, tid);
+    dv.issue(vt, src.v + (int64_t)first * src.ldv, src.ldv, src.jhi + 1 - first, tid);
+    if (src.mask) { const int j = first + (tid & (KT - 1)); km = src.mask[j < src.lk ? j : src.lk - 1]; }
+  }
+  __device__ __forceinline__ int settle(char* kt, char* vt, float* bias, int tid) const {
+    dma_arrive();
+    if (!src.mask && j0 >= src.jlo) return 0;              // (rows past jhi have been written as zeros)
+    uint64_t keep;
+    const int state = src.look<KT>(keep, km, bias, j0, tid);
+    if (~keep) { dk.erase(kt, keep, tid); dv.erase(vt, keep, tid); }
+    return state;
+  }
+};
+template <typename T, int D> struct WaveKeyPipe {          // a wave's own tiles of 32 keys, through registers (one LDS buffer per wave)
+  typedef Stage<T, D, 32, 64> St;
+  KeySource src;
+  St sk, sv;
+  float km;
+  int j0;
+  __device__ __forceinline__ WaveKeyPipe(const Params& p, int64_t k0, int hk, int lk, int jlo, int jhi) { src.init<T, D>(p, k0, hk, lk, jlo, jhi); km = 0.f; j0 = 0; }
+  __device__ __forceinline__ void fetch(int first, int lane) {
+    j0 = first;
+    const int last = src.lk - 1 - first;
+    sk.get(src.k + (int64_t)first * src.ldk, src.ldk, last, lane);
+    sv.get(src.v + (int64_t)first * src.ldv, src.ldv, last, lane);
+    if (src.mask) { const int r = lane & 31; km = src.mask[first + (r < last ? r : last)]; }
+  }
+  __device__ __forceinline__ int deposit(char* kt, char* vt, float* bias, int lane) const {
+    if (!src.mask && j0 >= src.jlo && j0 + 31 <= src.jhi) { sk.put(kt, lane); sv.put(vt, lane); return 0; }
+    uint64_t keep;
+    const int state = src.look<32>(keep, km, bias, j0, lane);
+    sk.put(kt, keep, lane);
+    sv.put(vt, keep, lane);
+    return state;
+  }
+};
+
+// visibility by position of 32 x 32 blocks: rows lo ... hi (positions; hi < lo: none) against keys j0 ... j0 + 31: 0 nothing, 1 some, 2 everything
+struct Sight {
+  int none_above, full_above, full_below, none_below, sinks;
+  __device__ __forceinline__ Sight(int lo, int hi, int left, int right, int sinks_, int lk) {
+    const int top = lk - 1;
+    none_above = hi < lo ? -1 : (hi + right < top ? hi + right : top);       // first key of the block past this: nothing
+    full_above = lo + right < top ? lo + right : top;                        // last key of the block past this: not everything
+    full_below = hi - left;
+    none_below = lo - left;
+    sinks = sinks_;
+  }
+  __device__ __forceinline__ int of(int j0) const {
+    const int j1 = j0 + 31;
+    if (j0 > none_above) return 0;
+    if (j1 <= full_above && (j0 >= full_below || j1 < sinks)) return 2;
+    return j1 < none_below && j0 >= sinks ? 0 : 1;
+  }
+};
 
 // dropout multipliers of a lane's query row qi and the 16 keys j0 + 8 (r >> 2) + 4 h + (r & 3): common.h attn_drop_block (one Philox call per 2 rows x 4 keys).
 // PAIRED: lanes c, c ^ 1 hold rows 2 n, 2 n + 1 of one sequence and head, so each draws two of the four blocks and they swap
@@ -268,13 +437,6 @@ template <int KT> __device__ __host__ __forceinline__ TileList tile_list(int lo,
 }
 __device__ __forceinline__ int tile_at(const TileList& t, int i) { return i < t.nsink ? i : t.first + i - t.nsink; }
 
-// what the keys of a tile look like through the key mask: 0 every value 0, 1 some not, 2 all hidden
-__device__ __forceinline__ int mask_state(float kb, bool on) {
-  const uint64_t any = __builtin_amdgcn_ballot_w64(on && kb != 0.f), seen = __builtin_amdgcn_ballot_w64(on && kb > -INFINITY);
-  return seen == 0 ? 2 : (any != 0 ? 1 : 0);
-}
-__device__ __forceinline__ float mask_value(float km) { return km > HIDDEN ? km * LOG2E_ : -INFINITY; }      // (NaN hides)
-
 // a lane's row of O: columns 32 i + 8 g + 4 h + e; four consecutive columns per store
 template <typename T, int D> __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[D / 32], float mul, int half) {
 #pragma unroll
@@ -307,7 +469,7 @@ inline int check_shape(int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, 
 inline int check_rows(const void* x, int64_t ld, int heads, int D, int dtype, bool written, const char* what) {
   const int e = dtype == DT_F32 ? 4 : 2;
   if (!x) { ctclip_set_error("win_attn: null tensor"); return CTCLIP_EBADARG; }
-  if ((reinterpret_cast<uintptr_t>(x) % 16) || (ld * e) % 16 || ld < 0 || (written && ld < (int64_t)heads * D)) { ctclip_set_error(what); return CTCLIP_EBADARG; }
+  if ((reinterpret_cast<uintptr_t>(x) % 16) || (ld * e) % 16 || ld < 0 || ld * e >= (1 << 23) || (written && ld < (int64_t)heads * D)) { ctclip_set_error(what); return CTCLIP_EBADARG; }
   return CTCLIP_OK;
 }
 inline void fill(Params& p, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, int Hk, int left, int right, int sinks, int q_start, float scale, float dropout_p,

@@ -23,76 +23,93 @@ template <int D> struct SoftRow {          // the running softmax of a lane's qu
   }
 };
 
-// one 32-key block: scores -> running softmax -> acc.  pos = the lane's query position, kb = additive mask of the block's keys in LDS (or null)
-template <typename T, int D, bool DROP, bool PAIRED>
-__device__ __forceinline__ void key_block(SoftRow<D>& st, const RowFrag<T, D>& qf, const char* ktile, const char* vtile, int row0, const float* kb, const Params& p,
-                                          int j0, int pos, int lk, bool partial, int lane, int64_t sh, int qi) {
-  const int half = lane >> 5, c = lane & 31;
-  RowFrag<T, D> kf;
-  row_frag_lds<T, D>(kf, ktile, row0 + c, half);
-  f32x16 s;
+// The running maximum is raised only when some row's scores outgrow it by more than 2^LAZY: accumulators and sums then hold probabilities up to 2^8 times the
+// final ones, which f32 (and the operand type: bf16 has the range of f32) does not notice, and the rescale of the accumulators -- with 32 rows to a wave some row's
+// maximum moves in nearly every block -- becomes rare.
+constexpr float LAZY = 8.f;
+
+// NB neighbouring 32-key blocks: scores -> running softmax -> acc.  kt, vt = the blocks in LDS; bias = their additive mask (or null); pos = the lane's position
+template <typename T, int D, int NB, bool DROP, bool PAIRED>
+__device__ __forceinline__ void key_blocks(SoftRow<D>& st, const RowFrag<T, D>& qf, const char* kt, const char* vt, const float* bias, const LaneAt<T, D>& at, const Params& p,
+                                           int j0, int pos, int lk, bool partial, int lane, int64_t sh, int qi) {
+  constexpr int BLK = 32 * Geo<T, D>::ROWB;
+  const int half = lane >> 5;
+  f32x16 s[NB];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) s[r] = 0.f;
-  s = mma_rows<D>(kf, qf, s);
-  float v[16];
+  for (int b = 0; b < NB; ++b) {
+    RowFrag<T, D> kf;
+    row_frag_lds<T, D>(kf, kt + b * BLK, at);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+    s[b] = mma_rows<D>(kf, qf, s[b]);
+  }
   float sc = p.scale2;                                     // (scale > 0: the maximum may be taken of the unscaled scores; one rounding in the fma below)
-  if (kb) {
+  if (bias) {
     sc = 1.f;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(kb + 8 * g + 4 * half);
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * g + e] = fmaf(s[4 * g + e], p.scale2, a[e]);
-    }
-  } else {
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(bias + 32 * b + 8 * g + 4 * half);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) v[r] = s[r];
+        for (int e = 0; e < 4; ++e) s[b][4 * g + e] = fmaf(s[b][4 * g + e], p.scale2, a[e]);
+      }
   }
   if (partial) {
-    const int b = j0 + 4 * half;
-    const int hi = (pos + p.right < lk - 1 ? pos + p.right : lk - 1) - b, lo = pos - p.left - b, sk = p.sinks - b;
+    const int o = j0 + 4 * half;
+    const int hi = (pos + p.right < lk - 1 ? pos + p.right : lk - 1) - o, lo = pos - p.left - o, sk = p.sinks - o;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int j = 8 * (r >> 2) + (r & 3);
-      v[r] = (j <= hi && (j >= lo || j < sk)) ? v[r] : -INFINITY;
-    }
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = 32 * b + 8 * (r >> 2) + (r & 3);
+        s[b][r] = (j <= hi && (j >= lo || j < sk)) ? s[b][r] : -INFINITY;
+      }
   }
-  float mx = v[0];
+  float mx = s[0][0];
 #pragma unroll
-  for (int r = 1; r < 16; ++r) mx = fmaxf(mx, v[r]);
-  mx = half_max(mx);
-  const float mn = fmaxf(st.m, mx * sc);
-  const float ms = mn == -INFINITY ? 0.f : mn;             // nothing seen so far: every exp2 below is exp2(-inf) = 0
-  const float alpha = __builtin_amdgcn_exp2f(st.m - ms);
-  float pr[16], ps = 0.f;
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
-  for (int r = 0; r < 16; ++r) { pr[r] = __builtin_amdgcn_exp2f(fmaf(v[r], sc, -ms)); ps += pr[r]; }
-  st.l = st.l * alpha + ps;
-  if (DROP) {                                              // on the normalised probabilities: the sum above stays undropped
-    float dm[16];
-    drop_of_query<PAIRED>(dm, p, sh, qi, j0, half);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) pr[r] *= dm[r];
-  }
-  PFrag<T> pf;
-  p_frag(pf, pr);
-  if (__builtin_amdgcn_ballot_w64(mn != st.m) != 0) {      // wave-uniform: no rescale while no maximum moved
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+  mx = half_max(mx) * sc;
+  if (__builtin_amdgcn_ballot_w64(mx > st.m + LAZY) != 0) {        // wave-uniform
+    const float mn = fmaxf(st.m, mx);
+    const float alpha = __builtin_amdgcn_exp2f(st.m - (mn == -INFINITY ? 0.f : mn));
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) st.acc[i][r] *= alpha;
+    st.l *= alpha;
+    st.m = mn;
   }
-  st.m = mn;
-  mma_cols<D>(st.acc, vtile, row0, pf, lane);
+  const float ms = st.m == -INFINITY ? 0.f : st.m;         // nothing seen so far: every exp2 below is exp2(-inf) = 0
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    float pr[16], ps[4];                                   // (four sums: one would be a chain of 16 dependent additions)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      pr[r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], sc, -ms));
+      ps[r & 3] = r < 4 ? pr[r] : ps[r & 3] + pr[r];
+    }
+    st.l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+    if (DROP) {                                            // on the normalised probabilities: the sum above stays undropped
+      float dm[16];
+      drop_of_query<PAIRED>(dm, p, sh, qi, j0 + 32 * b, half);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) pr[r] *= dm[r];
+    }
+    PFrag<T> pf;
+    p_frag(pf, pr);
+    mma_cols<T, D>(st.acc, vt + b * BLK, at, pf, lane);
+  }
 }
 
 template <typename T, int D, bool DROP>
-__global__ __launch_bounds__(256, 2) void fwd_kernel(Params p, int nunits, int nqt) {
+__global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 4 : 2)) void fwd_kernel(Params p, int nunits, int nqt) {
   typedef Geo<T, D> G;
   constexpr int KT = G::KT, TILE = KT * G::ROWB;
-  extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K | V], additive mask [2][KT], mask state [2]
+  extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K | V], additive mask [2][KT]
   float* kb = reinterpret_cast<float*>(lds + 4 * TILE);
-  int* state = reinterpret_cast<int*>(kb + 2 * KT);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Unit u = unit_of(p, blockIdx.x, nunits, nqt, p.G);
@@ -104,68 +121,42 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Params p, int nunits, int n
   const int lo = p.q_start + q0, hi = lo + nq - 1;                 // positions of the workgroup's rows
   const TileList tl = tile_list<KT>(lo, hi, p.left, p.right, p.sinks, rw.lk);
   const int i0 = (int)((int64_t)tl.n * blockIdx.y / p.nsplit), i1 = (int)((int64_t)tl.n * (blockIdx.y + 1) / p.nsplit);
-  const int jhi = hi + p.right, jlo = lo - p.left;                 // keys outside [jlo, jhi] and the sinks are seen by no row of the workgroup
 
   int row = q0 + 32 * wave + c;
   const bool real = row < rw.lq;
   row = real ? row : rw.lq - 1;
   const int wlo = lo + 32 * wave, whi = wlo + 31 < hi ? wlo + 31 : hi;      // the wave's positions (whi < wlo: it has none)
+  const Sight sight(wlo, whi, p.left, p.right, p.sinks, rw.lk);
   const int pos = p.q_start + row;
   RowFrag<T, D> qf;
   row_frag_global<T, D>(qf, reinterpret_cast<const T*>(p.q) + (rw.q0 + row) * p.ldq + (int64_t)h * D, half);
-  const T* kbase = reinterpret_cast<const T*>(p.k) + rw.k0 * p.ldk + (int64_t)u.hk * D;
-  const T* vbase = reinterpret_cast<const T*>(p.v) + rw.k0 * p.ldv + (int64_t)u.hk * D;
-  const float* mbase = p.keymask ? p.keymask + rw.k0 : nullptr;
-
-  typedef Stage<T, D, KT, 256> St;
-  St sk, sv;
-  uint32_t keep = 0;
-  float km = 0.f;
-  auto fetch = [&](int j0) {
-    sk.get(kbase, p.ldk, j0, rw.lk, tid);
-    sv.get(vbase, p.ldv, j0, rw.lk, tid);
-    keep = 0;
-#pragma unroll
-    for (int i = 0; i < St::N; ++i) {
-      const int j = j0 + St::row(tid, i);
-      bool on = j < rw.lk && j <= jhi && (j >= jlo || j < p.sinks);
-      if (mbase) on = on && mbase[j < rw.lk ? j : rw.lk - 1] > HIDDEN;
-      keep |= (uint32_t)on << i;
-    }
-    if (mbase) { const int j = j0 + (tid & (KT - 1)); km = mask_value(mbase[j < rw.lk ? j : rw.lk - 1]); }
-  };
-  auto deposit = [&](int buf) {
-    sk.put(lds + buf * 2 * TILE, keep, tid);
-    sv.put(lds + buf * 2 * TILE + TILE, keep, tid);
-    if (mbase && wave == 0) {
-      if (tid < KT) kb[buf * KT + tid] = km;
-      const int s = mask_state(km, tid < KT);
-      if (tid == 0) state[buf] = s;
-    }
-  };
-
+  const LaneAt<T, D> at(lane);
+  KeyPipe<T, D, KT, 256> kp(p, rw.k0, u.hk, rw.lk, lo - p.left, hi + p.right, tid);
   SoftRow<D> st;
   st.clear();
   const int64_t sh = (int64_t)u.b * p.H + h;
+  int state = 0;
   if (i0 < i1) {
-    fetch(tile_at(tl, i0) * KT);
-    deposit(0);
+    kp.issue(lds, lds + TILE, tile_at(tl, i0) * KT, tid);
+    state = kp.settle(lds, lds + TILE, kb, tid);
   }
+  row_frag_arrive<T, D>(qf);                               // (behind the first tile's loads)
   __syncthreads();
   for (int it = i0; it < i1; ++it) {
     const int buf = (it - i0) & 1, j0 = tile_at(tl, it) * KT;
-    if (it + 1 < i1) fetch(tile_at(tl, it + 1) * KT);
-    const int ms = mbase ? __builtin_amdgcn_readfirstlane(state[buf]) : 0;
-    if (ms != 2) {
+    const bool more = it + 1 < i1;
+    char* next = lds + (buf ^ 1) * 2 * TILE;               // (its readers are behind the last barrier)
+    if (more) kp.issue(next, next + TILE, tile_at(tl, it + 1) * KT, tid);
+    if (state != 2) {
+      const char *kt = lds + buf * 2 * TILE, *vt = kt + TILE;
+      const float* bias = state ? kb + buf * KT : nullptr;
 #pragma unroll
       for (int b = 0; b < KT / 32; ++b) {
-        const int sight = whi < wlo ? 0 : block_sight(wlo, whi, j0 + 32 * b, p.left, p.right, p.sinks, rw.lk);
-        if (sight)
-          key_block<T, D, DROP, true>(st, qf, lds + buf * 2 * TILE, lds + buf * 2 * TILE + TILE, 32 * b, ms ? kb + buf * KT + 32 * b : nullptr, p, j0 + 32 * b, pos,
-                                      rw.lk, sight == 1, lane, sh, row);
+        const int a = sight.of(j0 + 32 * b), o = 32 * b * G::ROWB;
+        if (a) key_blocks<T, D, 1, DROP, true>(st, qf, kt + o, vt + o, bias ? bias + 32 * b : nullptr, at, p, j0 + 32 * b, pos, rw.lk, a != 2, lane, sh, row);
       }
     }
-    if (it + 1 < i1) deposit(buf ^ 1);
+    if (more) state = kp.settle(next, next + TILE, kb + (buf ^ 1) * KT, tid);
     __syncthreads();
   }
   const float l = half_sum(st.l);
@@ -196,50 +187,29 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Params p, int nunits) {
   const int lo = p.q_start, hi = p.q_start + rw.lq - 1;
   const TileList tl = tile_list<32>(lo, hi, p.left, p.right, p.sinks, rw.lk);
   const int i0 = (int)((int64_t)tl.n * blockIdx.y / p.nsplit), i1 = (int)((int64_t)tl.n * (blockIdx.y + 1) / p.nsplit);
-  const int jhi = hi + p.right, jlo = lo - p.left;
   const int rc = c < R ? c : R - 1;
   const int g = rc / rw.lq, row = rc - g * rw.lq, h = u.hk * p.G + g, pos = p.q_start + row;
   RowFrag<T, D> qf;
   row_frag_global<T, D>(qf, reinterpret_cast<const T*>(p.q) + (rw.q0 + row) * p.ldq + (int64_t)h * D, half);
-  const T* kbase = reinterpret_cast<const T*>(p.k) + rw.k0 * p.ldk + (int64_t)u.hk * D;
-  const T* vbase = reinterpret_cast<const T*>(p.v) + rw.k0 * p.ldv + (int64_t)u.hk * D;
-  const float* mbase = p.keymask ? p.keymask + rw.k0 : nullptr;
   char* ktile = lds + wave * (2 * TILE + 128);
   char* vtile = ktile + TILE;
   float* kb = reinterpret_cast<float*>(vtile + TILE);
-
-  typedef Stage<T, D, 32, 64> St;
-  St sk, sv;
-  uint32_t keep = 0;
-  float km = 0.f;
-  auto fetch = [&](int j0) {
-    sk.get(kbase, p.ldk, j0, rw.lk, lane);
-    sv.get(vbase, p.ldv, j0, rw.lk, lane);
-    keep = 0;
-#pragma unroll
-    for (int i = 0; i < St::N; ++i) {
-      const int j = j0 + St::row(lane, i);
-      bool on = j < rw.lk && j <= jhi && (j >= jlo || j < p.sinks);
-      if (mbase) on = on && mbase[j < rw.lk ? j : rw.lk - 1] > HIDDEN;
-      keep |= (uint32_t)on << i;
-    }
-    if (mbase) { const int j = j0 + c; km = mask_value(mbase[j < rw.lk ? j : rw.lk - 1]); }
-  };
+  const Sight sight(lo, hi, p.left, p.right, p.sinks, rw.lk);
+  const LaneAt<T, D> at(lane);
+  WaveKeyPipe<T, D> kp(p, rw.k0, u.hk, rw.lk, lo - p.left, hi + p.right);
   SoftRow<D> st;
   st.clear();
   const int64_t sh = (int64_t)u.b * p.H + h;
   int it = i0 + wave;
-  if (it < i1) fetch(tile_at(tl, it) * 32);
+  if (it < i1) kp.fetch(tile_at(tl, it) * 32, lane);
+  row_frag_arrive<T, D>(qf);
   for (; it < i1; it += 4) {                                       // (no barrier: a wave's tiles are its own, and its LDS operations keep their order)
     const int j0 = tile_at(tl, it) * 32;
-    sk.put(ktile, keep, lane);
-    sv.put(vtile, keep, lane);
-    int ms = 0;
-    if (mbase) { if (half == 0) kb[c] = km; ms = __builtin_amdgcn_readfirstlane(mask_state(km, true)); }
-    if (it + 4 < i1) fetch(tile_at(tl, it + 4) * 32);
+    const int state = kp.deposit(ktile, vtile, kb, lane);
+    if (it + 4 < i1) kp.fetch(tile_at(tl, it + 4) * 32, lane);
     wave_sync();
-    const int sight = block_sight(lo, hi, j0, p.left, p.right, p.sinks, rw.lk);
-    if (sight && ms != 2) key_block<T, D, DROP, false>(st, qf, ktile, vtile, 0, ms ? kb : nullptr, p, j0, pos, rw.lk, sight == 1, lane, sh, row);
+    const int a = sight.of(j0);
+    if (a && state != 2) key_blocks<T, D, 1, DROP, false>(st, qf, ktile, vtile, state ? kb : nullptr, at, p, j0, pos, rw.lk, a == 1, lane, sh, row);
     wave_sync();
   }
   // fold the four waves: row maxima first, then sums and accumulators under the common maximum
@@ -358,7 +328,7 @@ template <typename T, int D, bool DROP> int launch_fwd(Params& p, const Plan& pl
     const int nqt = (int)cdiv(p.Lq, QB);
     const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.H : (int64_t)p.nseq * p.H * nqt;
     if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
-    const int lds = 4 * G::KT * G::ROWB + 2 * G::KT * 4 + 16;
+    const int lds = 4 * G::KT * G::ROWB + 2 * G::KT * 4;
     const int rc = raise_lds<fwd_kernel<T, D, DROP>>(lds);
     if (rc) return rc;
     hipLaunchKernelGGL((fwd_kernel<T, D, DROP>), dim3((unsigned)(8 * cdiv(nu, 8)), p.nsplit), dim3(256), lds, s, p, (int)nu, nqt);

@@ -9,6 +9,9 @@
 //   dkv_reduce_kernel  adds the partial sums of split keys in a fixed order.  Every result is bit-reproducible.
 // Seven products per visible block (five are needed at least; the other two are S and dP again, because dQ across key tiles would need float atomics).
 #include "win_attn.h"
+#ifndef DKV_JOINT
+#define DKV_JOINT 1
+#endif
 
 namespace win {
 
@@ -16,9 +19,8 @@ template <typename T, int D, bool DROP>
 __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nqt) {
   typedef Geo<T, D> G;
   constexpr int KT = G::KT, TILE = KT * G::ROWB;
-  extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K | V], additive mask [2][KT], mask state [2]
+  extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K | V], additive mask [2][KT]
   float* kb = reinterpret_cast<float*>(lds + 4 * TILE);
-  int* state = reinterpret_cast<int*>(kb + 2 * KT);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Unit u = unit_of(p, blockIdx.x, nunits, nqt, p.G);
@@ -29,7 +31,6 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
   const int h = u.hk * p.G + u.g, nq = rw.lq - q0 < QB ? rw.lq - q0 : QB;
   const int lo = p.q_start + q0, hi = lo + nq - 1;
   const TileList tl = tile_list<KT>(lo, hi, p.left, p.right, p.sinks, rw.lk);
-  const int jhi = hi + p.right, jlo = lo - p.left;
 
   int row = q0 + 32 * wave + c;
   const bool real = row < rw.lq;
@@ -45,70 +46,48 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
     row_frag_global<T, D>(of, reinterpret_cast<const T*>(p.o) + (rw.q0 + row) * p.ldo + (int64_t)h * D, half);
     delta = half_sum(row_dot<D>(of, df));
   }
-  const float lse = p.lse[(int64_t)h * p.Mq + rw.q0 + row];
+  float lse = p.lse[(int64_t)h * p.Mq + rw.q0 + row];
+  row_frag_arrive<T, D>(qf);
+  row_frag_arrive<T, D>(df);
+  asm volatile("" : "+v"(lse));
   if (real && half == 0) p.delta[(int64_t)h * p.Mq + rw.q0 + row] = delta;
-  const T* kbase = reinterpret_cast<const T*>(p.k) + rw.k0 * p.ldk + (int64_t)u.hk * D;
-  const T* vbase = reinterpret_cast<const T*>(p.v) + rw.k0 * p.ldv + (int64_t)u.hk * D;
-  const float* mbase = p.keymask ? p.keymask + rw.k0 : nullptr;
-
-  typedef Stage<T, D, KT, 256> St;
-  St sk, sv;
-  uint32_t keep = 0;
-  float km = 0.f;
-  auto fetch = [&](int j0) {
-    sk.get(kbase, p.ldk, j0, rw.lk, tid);
-    sv.get(vbase, p.ldv, j0, rw.lk, tid);
-    keep = 0;
-#pragma unroll
-    for (int i = 0; i < St::N; ++i) {
-      const int j = j0 + St::row(tid, i);
-      bool on = j < rw.lk && j <= jhi && (j >= jlo || j < p.sinks);
-      if (mbase) on = on && mbase[j < rw.lk ? j : rw.lk - 1] > HIDDEN;
-      keep |= (uint32_t)on << i;
-    }
-    if (mbase) { const int j = j0 + (tid & (KT - 1)); km = mask_value(mbase[j < rw.lk ? j : rw.lk - 1]); }
-  };
-  auto deposit = [&](int buf) {
-    sk.put(lds + buf * 2 * TILE, keep, tid);
-    sv.put(lds + buf * 2 * TILE + TILE, keep, tid);
-    if (mbase && wave == 0) {
-      if (tid < KT) kb[buf * KT + tid] = km;
-      const int s = mask_state(km, tid < KT);
-      if (tid == 0) state[buf] = s;
-    }
-  };
+  const Sight sight(wlo, whi, p.left, p.right, p.sinks, rw.lk);
+  const LaneAt<T, D> at(lane);
+  KeyPipe<T, D, KT, 256> kp(p, rw.k0, u.hk, rw.lk, lo - p.left, hi + p.right, tid);
   f32x16 acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
   const int64_t sh = (int64_t)u.b * p.H + h;
+  int state = 0;
   if (tl.n > 0) {
-    fetch(tile_at(tl, 0) * KT);
-    deposit(0);
+    kp.issue(lds, lds + TILE, tile_at(tl, 0) * KT, tid);
+    state = kp.settle(lds, lds + TILE, kb, tid);
   }
   __syncthreads();
   for (int it = 0; it < tl.n; ++it) {
     const int buf = it & 1, j0 = tile_at(tl, it) * KT;
-    if (it + 1 < tl.n) fetch(tile_at(tl, it + 1) * KT);
-    const int ms = mbase ? __builtin_amdgcn_readfirstlane(state[buf]) : 0;
-    if (ms != 2) {
-      const char* ktile = lds + buf * 2 * TILE;
+    const bool more = it + 1 < tl.n;
+    char* next = lds + (buf ^ 1) * 2 * TILE;               // (its readers are behind the last barrier)
+    if (more) kp.issue(next, next + TILE, tile_at(tl, it + 1) * KT, tid);
+    if (state != 2) {
 #pragma unroll
       for (int b = 0; b < KT / 32; ++b) {
         const int jb = j0 + 32 * b;
-        const int sight = whi < wlo ? 0 : block_sight(wlo, whi, jb, p.left, p.right, p.sinks, rw.lk);
-        if (!sight) continue;
+        const char *kt = lds + buf * 2 * TILE + 32 * b * G::ROWB, *vt = kt + TILE;
+        const int see = sight.of(jb);
+        if (!see) continue;
         RowFrag<T, D> kf;
-        row_frag_lds<T, D>(kf, ktile, 32 * b + c, half);
+        row_frag_lds<T, D>(kf, kt, at);
         f32x16 s, dp;
 #pragma unroll
         for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
         s = mma_rows<D>(kf, qf, s);
-        row_frag_lds<T, D>(kf, ktile + TILE, 32 * b + c, half);
+        row_frag_lds<T, D>(kf, vt, at);
         dp = mma_rows<D>(kf, df, dp);
         float pr[16];
-        if (ms) {
+        if (state) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const f32x4 a = *reinterpret_cast<const f32x4*>(kb + buf * KT + 32 * b + 8 * g + 4 * half);
@@ -119,7 +98,7 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
 #pragma unroll
           for (int r = 0; r < 16; ++r) pr[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, -lse));
         }
-        if (sight == 1) {
+        if (see == 1) {
           const int bb = jb + 4 * half;
           const int jh = (pos + p.right < rw.lk - 1 ? pos + p.right : rw.lk - 1) - bb, jl = pos - p.left - bb, sk_ = p.sinks - bb;
 #pragma unroll
@@ -138,16 +117,16 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
         for (int r = 0; r < 16; ++r) pr[r] *= dp[r] - delta;
         PFrag<T> pf;
         p_frag(pf, pr);
-        mma_cols<D>(acc, ktile, 32 * b, pf, lane);
+        mma_cols<T, D>(acc, kt, at, pf, lane);
       }
     }
-    if (it + 1 < tl.n) deposit(buf ^ 1);
+    if (more) state = kp.settle(next, next + TILE, kb + (buf ^ 1) * KT, tid);
     __syncthreads();
   }
   if (real) store_row<T, D>(reinterpret_cast<T*>(p.dq) + (rw.q0 + row) * p.lddq + (int64_t)h * D, acc, p.scale, half);
 }
 
-// the 32 queries of a staged tile (rows row0 ... of it) against the 32 keys of a wave
+// 32 staged queries against the 32 keys of a wave
 template <typename T, int D> struct KeyState {
   RowFrag<T, D> kf, vf;
   f32x16 dk[D / 32], dv[D / 32];
@@ -175,53 +154,70 @@ __device__ __forceinline__ void drop_of_key(float (&m)[16], const Params& p, int
       for (int e = 0; e < 2; ++e) m[4 * g + 2 * s + e] = attn_drop_pick(w[g], e, j, thr, p.inv_keep);
   }
 }
-// FAR: the sink pass (keys seen because they are sinks, j < i - left); otherwise the window (i - left <= j <= i + right)
-template <typename T, int D, bool DROP, bool FAR>
-__device__ __forceinline__ void query_block(KeyState<T, D>& st, const char* qtile, const char* dtile, const float* lse, const float* delta, int row0, const Params& p, int row,
-                                            int j, float kbias, bool partial, int lane, int64_t sh) {
-  const int half = lane >> 5, c = lane & 31;
-  RowFrag<T, D> f;
-  row_frag_lds<T, D>(f, qtile, row0 + c, half);
-  f32x16 s, dp;
+// FAR: the sink pass (keys seen because they are sinks, j < i - left); otherwise the window (i - left <= j <= i + right).  NB neighbouring blocks of 32 queries at a
+// time: the products of one block run under the exponentials of the other.
+template <typename T, int D, int NB, bool DROP, bool FAR>
+__device__ __forceinline__ void query_blocks(KeyState<T, D>& st, const char* qt, const char* dt, const float* lse, const float* delta, const LaneAt<T, D>& at, const Params& p,
+                                             int row, int j, float kbias, bool partial, int lane, int64_t sh) {
+  constexpr int BLK = 32 * Geo<T, D>::ROWB;
+  const int half = lane >> 5;
+  f32x16 s[NB], dp[NB];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
-  s = mma_rows<D>(f, st.kf, s);
-  row_frag_lds<T, D>(f, dtile, row0 + c, half);
-  dp = mma_rows<D>(f, st.vf, dp);
-  float pr[16], ds[16];
+  for (int b = 0; b < NB; ++b) {
+    RowFrag<T, D> f;
+    row_frag_lds<T, D>(f, qt + b * BLK, at);
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(lse + row0 + 8 * g + 4 * half);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) pr[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], p.scale2, kbias - a[e]));
+    for (int r = 0; r < 16; ++r) { s[b][r] = 0.f; dp[b][r] = 0.f; }
+    s[b] = mma_rows<D>(f, st.kf, s[b]);
   }
   if (partial) {                           // row >= j - right, row <= j + left (positions), or beyond: row > j + left and j a sink
-    const int b = p.q_start + row + 4 * half;
-    const int rl = j - p.right - b, rh = j + p.left - b;
+    const int o = p.q_start + row + 4 * half;
+    const int rl = j - p.right - o, rh = j + p.left - o;
     const bool sink = j < p.sinks;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int i = 8 * (r >> 2) + (r & 3);
-      pr[r] = (FAR ? (sink && i > rh) : (i >= rl && i <= rh)) ? pr[r] : 0.f;
-    }
-  }
-  float dm[16];
-  if (DROP) drop_of_key(dm, p, sh, row, j, half);
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const f32x4 d = *reinterpret_cast<const f32x4*>(delta + row0 + 8 * g + 4 * half);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = 4 * g + e;
-      ds[r] = pr[r] * ((DROP ? dp[r] * dm[r] : dp[r]) - d[e]);
-      if (DROP) pr[r] *= dm[r];
-    }
+      for (int r = 0; r < 16; ++r) {
+        const int i = 32 * b + 8 * (r >> 2) + (r & 3);
+        s[b][r] = (FAR ? (sink && i > rh) : (i >= rl && i <= rh)) ? s[b][r] : -INFINITY;
+      }
   }
-  PFrag<T> pf;
-  p_frag(pf, pr);
-  mma_cols<D>(st.dv, dtile, row0, pf, lane);
-  p_frag(pf, ds);
-  mma_cols<D>(st.dk, qtile, row0, pf, lane);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    RowFrag<T, D> f;
+    row_frag_lds<T, D>(f, dt + b * BLK, at);
+    dp[b] = mma_rows<D>(f, st.vf, dp[b]);
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    float pr[16], dm[16];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(lse + 32 * b + 8 * g + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pr[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[b][4 * g + e], p.scale2, kbias - a[e]));
+    }
+    if (DROP) drop_of_key(dm, p, sh, row + 32 * b, j, half);
+    PFrag<T> pf, df;
+    {
+      float pd[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) pd[r] = DROP ? pr[r] * dm[r] : pr[r];
+      p_frag(pf, pd);
+    }
+    mma_cols<T, D>(st.dv, dt + b * BLK, at, pf, lane);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 d = *reinterpret_cast<const f32x4*>(delta + 32 * b + 8 * g + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * g + e;
+        pr[r] *= (DROP ? dp[b][r] * dm[r] : dp[b][r]) - d[e];
+      }
+    }
+    p_frag(df, pr);
+    mma_cols<T, D>(st.dk, qt + b * BLK, at, df, lane);
+  }
 }
 
 // a wave's 32 keys into registers; hidden keys and keys past the end are zeros and carry a bias of -inf
@@ -231,6 +227,8 @@ template <typename T, int D> __device__ __forceinline__ float load_keys(KeyState
   const bool on = j < rw.lk && km > HIDDEN;
   row_frag_global<T, D>(st.kf, reinterpret_cast<const T*>(p.k) + (rw.k0 + jr) * p.ldk + (int64_t)hk * D, half);
   row_frag_global<T, D>(st.vf, reinterpret_cast<const T*>(p.v) + (rw.k0 + jr) * p.ldv + (int64_t)hk * D, half);
+  row_frag_arrive<T, D>(st.kf);
+  row_frag_arrive<T, D>(st.vf);
   if (!on) { row_frag_zero<T, D>(st.kf); row_frag_zero<T, D>(st.vf); }
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
@@ -239,7 +237,69 @@ template <typename T, int D> __device__ __forceinline__ float load_keys(KeyState
   return on ? km * LOG2E_ : -INFINITY;
 }
 
-template <typename T, int D> struct QTile { static constexpr int ROWS = Geo<T, D>::NCH >= 8 ? 32 : 64; };      // query rows of a dK / dV step: a chunk per thread at least
+// Query rows (q, dO and their statistics) on their way into LDS, ROWS at a time.
+struct RowSource {
+  const char *q, *d;
+  const float *lse, *delta;
+  int ldq, ldd, lq, r0;
+  float sl, sdel;
+  template <typename T, int D> __device__ __forceinline__ void init(const Params& p, const Rows& rw, int h0) {
+    q = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.q) + rw.q0 * p.ldq + (int64_t)h0 * D);
+    d = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.dout) + rw.q0 * p.lddo + (int64_t)h0 * D);
+    lse = p.lse + (int64_t)h0 * p.Mq + rw.q0;
+    delta = p.delta + (int64_t)h0 * p.Mq + rw.q0;
+    ldq = (int)p.ldq * (int)sizeof(T); ldd = (int)p.lddo * (int)sizeof(T);
+    lq = rw.lq; r0 = 0; sl = 0.f; sdel = 0.f;
+  }
+  template <int ROWS> __device__ __forceinline__ void get_stat(const Params& p, int g, int tid) {
+    const int r = r0 + (tid & (ROWS - 1)) < lq ? r0 + (tid & (ROWS - 1)) : lq - 1;
+    const int64_t at = (int64_t)g * p.Mq + r;
+    sl = lse[at];                          // (loaded whatever the row: a branch around a load is waited for at its end)
+    sdel = delta[at];
+  }
+  template <int ROWS> __device__ __forceinline__ void put_stat(float* stat, int tid) const {      // log-sum-exps, then Deltas; rows past the end: probability 0
+    const int r = r0 + (tid & (ROWS - 1));
+    if (tid < ROWS) { stat[tid] = r < lq ? sl : INFINITY; stat[ROWS + tid] = r < lq ? sdel : 0.f; }
+  }
+};
+template <typename T, int D, int ROWS, int NT> struct RowPipe {    // through LDS-DMA: issue() into a buffer that nobody reads, settle() before the barrier
+  RowSource src;
+  Dma<T, D, ROWS, NT> dq, dd;
+  __device__ __forceinline__ RowPipe(const Params& p, const Rows& rw, int h0, int tid) {
+    src.init<T, D>(p, rw, h0);
+    dq.init(src.ldq, tid);
+    dd.init(src.ldd, tid);
+  }
+  __device__ __forceinline__ void issue(const Params& p, char* qt, char* dt, int g, int first, int tid) {
+    src.r0 = first;
+    dq.issue(qt, src.q + (int64_t)first * src.ldq + g * (D * (int)sizeof(T)), src.ldq, src.lq - first, tid);
+    dd.issue(dt, src.d + (int64_t)first * src.ldd + g * (D * (int)sizeof(T)), src.ldd, src.lq - first, tid);
+    src.get_stat<ROWS>(p, g, tid);
+  }
+  __device__ __forceinline__ void settle(float* stat, int tid) const {
+    dma_arrive();
+    src.put_stat<ROWS>(stat, tid);
+  }
+};
+template <typename T, int D> struct WaveRowPipe {          // a wave's own tiles of 32 rows, through registers (one LDS buffer per wave)
+  RowSource src;
+  Stage<T, D, 32, 64> sq, sd;
+  __device__ __forceinline__ WaveRowPipe(const Params& p, const Rows& rw, int h0) { src.init<T, D>(p, rw, h0); }
+  __device__ __forceinline__ void fetch(const Params& p, int g, int first, int lane) {
+    src.r0 = first;
+    const int last = src.lq - 1 - first;
+    sq.get(src.q + (int64_t)first * src.ldq + g * (D * (int)sizeof(T)), src.ldq, last, lane);
+    sd.get(src.d + (int64_t)first * src.ldd + g * (D * (int)sizeof(T)), src.ldd, last, lane);
+    src.get_stat<32>(p, g, lane);
+  }
+  __device__ __forceinline__ void deposit(char* qt, char* dt, float* stat, int lane) const {
+    if (src.r0 + 32 <= src.lq) { sq.put(qt, lane); sd.put(dt, lane); }
+    else { const uint64_t keep = low_bits(src.lq - src.r0); sq.put(qt, keep, lane); sd.put(dt, keep, lane); }
+    src.put_stat<32>(stat, lane);
+  }
+};
+
+template <typename T, int D> struct QTile { static constexpr int ROWS = sizeof(T) == 2 ? 64 : 32; };      // query rows of a dK / dV step
 
 // where the partial sums of key j lie: split passes hold every key, unsplit ones the keys of the sink blocks
 __device__ __forceinline__ int64_t part_row(const Params& p, const Rows& rw, int b, int hk, int j) {
@@ -273,48 +333,44 @@ __global__ __launch_bounds__(256, WGS) void dkv_kernel(Params p, int nunits, int
   KeyState<T, D> st;
   const float kbias = load_keys<T, D>(st, p, rw, u.hk, j, half);
   const bool any = __builtin_amdgcn_ballot_w64(kbias > -INFINITY) != 0;      // wave-uniform
-  typedef Stage<T, D, QT, 256> St;
-  St sq, sd;
-  uint32_t keep = 0;
-  float s_lse = 0.f, s_del = 0.f;
-  auto fetch = [&](int i) {
-    const int g = i / nt, r0 = (t0 + i - g * nt) * QT, h = u.hk * p.G + g;
-    sq.get(reinterpret_cast<const T*>(p.q) + rw.q0 * p.ldq + (int64_t)h * D, p.ldq, r0, rw.lq, tid);
-    sd.get(reinterpret_cast<const T*>(p.dout) + rw.q0 * p.lddo + (int64_t)h * D, p.lddo, r0, rw.lq, tid);
-    keep = 0;
-#pragma unroll
-    for (int n = 0; n < St::N; ++n) keep |= (uint32_t)(r0 + St::row(tid, n) < rw.lq) << n;
-    if (tid < QT) {
-      const int r = r0 + tid;
-      const int64_t at = (int64_t)h * p.Mq + rw.q0 + (r < rw.lq ? r : rw.lq - 1);
-      s_lse = r < rw.lq ? p.lse[at] : INFINITY;
-      s_del = r < rw.lq ? p.delta[at] : 0.f;
-    }
-  };
-  auto deposit = [&](int buf) {
-    sq.put(lds + buf * 2 * TILE, keep, tid);
-    sd.put(lds + buf * 2 * TILE + TILE, keep, tid);
-    if (tid < QT) { stat[buf * 2 * QT + tid] = s_lse; stat[buf * 2 * QT + QT + tid] = s_del; }
-  };
+  const LaneAt<T, D> at(lane);
+  RowPipe<T, D, QT, 256> rp(p, rw, u.hk * p.G, tid);
   if (i0 < i1) {
-    fetch(i0);
-    deposit(0);
+    rp.issue(p, lds, lds + TILE, i0 / nt, (t0 + i0 % nt) * QT, tid);
+    rp.settle(stat, tid);
   }
   __syncthreads();
+  int g = i0 < i1 ? i0 / nt : 0, t = i0 < i1 ? i0 % nt : 0;        // the step's head of the group and tile
   for (int i = i0; i < i1; ++i) {
-    const int buf = (i - i0) & 1;
-    if (i + 1 < i1) fetch(i + 1);
-    const int g = i / nt, r0 = (t0 + i - g * nt) * QT;
+    const int buf = (i - i0) & 1, r0 = (t0 + t) * QT;
     const int64_t sh = (int64_t)u.b * p.H + u.hk * p.G + g;
+    const bool more = i + 1 < i1;
+    if (++t == nt) { t = 0; ++g; }
+    char* next = lds + (buf ^ 1) * 2 * TILE;               // (its readers are behind the last barrier)
+    if (more) rp.issue(p, next, next + TILE, g, (t0 + t) * QT, tid);
+#if DKV_JOINT
+    {
+      const int lo = p.q_start + r0, last = p.q_start + rw.lq - 1, n = QT - 1;
+      const int see = any ? Sight(lo, lo + n < last ? lo + n : last, p.left, p.right, 0, rw.lk).of(jw) : 0;
+      if (see) {
+        const char* qt = lds + buf * 2 * TILE;
+        const float* sp = stat + buf * 2 * QT;
+        query_blocks<T, D, QT / 32, DROP, false>(st, qt, qt + TILE, sp, sp + QT, at, p, r0, j, kbias, see == 1, lane, sh);
+      }
+    }
+#else
 #pragma unroll
     for (int b = 0; b < QT / 32; ++b) {
       const int lo = p.q_start + r0 + 32 * b, last = p.q_start + rw.lq - 1;
-      const int sight = any && lo <= last ? block_sight(lo, lo + 31 < last ? lo + 31 : last, jw, p.left, p.right, 0, rw.lk) : 0;
-      if (sight)
-        query_block<T, D, DROP, false>(st, lds + buf * 2 * TILE, lds + buf * 2 * TILE + TILE, stat + buf * 2 * QT, stat + buf * 2 * QT + QT, 32 * b, p, r0 + 32 * b, j,
-                                       kbias, sight == 1, lane, sh);
+      const int see = any ? Sight(lo, lo + 31 < last ? lo + 31 : last, p.left, p.right, 0, rw.lk).of(jw) : 0;
+      if (see) {
+        const char* qt = lds + buf * 2 * TILE + 32 * b * G::ROWB;
+        const float* sp = stat + buf * 2 * QT + 32 * b;
+        query_blocks<T, D, 1, DROP, false>(st, qt, qt + TILE, sp, sp + QT, at, p, r0 + 32 * b, j, kbias, see == 1, lane, sh);
+      }
     }
-    if (i + 1 < i1) deposit(buf ^ 1);
+#endif
+    if (more) rp.settle(stat + (buf ^ 1) * 2 * QT, tid);
     __syncthreads();
   }
   if (j >= rw.lk) return;
@@ -348,32 +404,16 @@ __global__ __launch_bounds__(256, 1) void dkv_sink_kernel(Params p, int nblk) {
   char* qtile = lds + wave * (2 * TILE + 256);
   char* dtile = qtile + TILE;
   float* stat = reinterpret_cast<float*>(dtile + TILE);
-  typedef Stage<T, D, 32, 64> St;
-  St sq, sd;
-  uint32_t keep = 0;
-  float s_stat = 0.f;
-  auto fetch = [&](int i) {
-    const int g = i / nt, r0 = (t0 + i - g * nt) * 32, h = hk * p.G + g;
-    sq.get(reinterpret_cast<const T*>(p.q) + rw.q0 * p.ldq + (int64_t)h * D, p.ldq, r0, rw.lq, lane);
-    sd.get(reinterpret_cast<const T*>(p.dout) + rw.q0 * p.lddo + (int64_t)h * D, p.lddo, r0, rw.lq, lane);
-    keep = 0;
-#pragma unroll
-    for (int n = 0; n < St::N; ++n) keep |= (uint32_t)(r0 + St::row(lane, n) < rw.lq) << n;
-    const int r = r0 + c;
-    const int64_t at = (int64_t)h * p.Mq + rw.q0 + (r < rw.lq ? r : rw.lq - 1);
-    s_stat = half ? p.delta[at] : p.lse[at];
-    if (r >= rw.lq) s_stat = half ? 0.f : INFINITY;
-  };
+  const LaneAt<T, D> at(lane);
+  WaveRowPipe<T, D> rp(p, rw, hk * p.G);
   int i = i0 + wave;
-  if (i < i1) fetch(i);
+  if (i < i1) rp.fetch(p, i / nt, (t0 + i % nt) * 32, lane);
   for (; i < i1; i += 4) {
-    const int g = i / nt, r0 = (t0 + i - g * nt) * 32;
-    sq.put(qtile, keep, lane);
-    sd.put(dtile, keep, lane);
-    stat[lane] = s_stat;                                           // 32 log-sum-exps, then 32 Deltas
-    if (i + 4 < i1) fetch(i + 4);
+    const int g = i / nt, r0 = (t0 + i % nt) * 32;
+    rp.deposit(qtile, dtile, stat, lane);
+    if (i + 4 < i1) rp.fetch(p, (i + 4) / nt, (t0 + (i + 4) % nt) * 32, lane);
     wave_sync();
-    query_block<T, D, DROP, true>(st, qtile, dtile, stat, stat + 32, 0, p, r0, j, kbias, true, lane, (int64_t)b * p.H + hk * p.G + g);
+    query_blocks<T, D, 1, DROP, true>(st, qtile, dtile, stat, stat + 32, at, p, r0, j, kbias, true, lane, (int64_t)b * p.H + hk * p.G + g);
     wave_sync();
   }
   // fold the four waves, dK then dV, in the order of the waves
@@ -408,34 +448,58 @@ __global__ __launch_bounds__(256, 1) void dkv_sink_kernel(Params p, int nblk) {
   }
 }
 
-// keys whose sums came in parts: D / 4 threads per (k|v head, key)
-template <typename T, int D>
+// Keys whose sums came in parts.  A workgroup folds 256 / (D / 4) / PG keys of one k|v head: D / 4 threads across the columns, PG threads (1, or a sixteenth of the
+// chunks each where there are many: one thread's chain of dependent additions over 43 chunks took 40 us) across the parts, folded in a fixed order.
+template <typename T, int D, int PG>
 __global__ __launch_bounds__(256) void dkv_reduce_kernel(Params p, int keys) {
+  constexpr int C = D / 4, KEYS = 256 / C / PG;
+  __shared__ __attribute__((aligned(16))) float fold[2][PG][KEYS][D];
   const int b = blockIdx.z, hk = blockIdx.y;
   const Rows rw = rows_of(p, b);
-  const int j = blockIdx.x * (256 / (D / 4)) + threadIdx.x / (D / 4), col = (threadIdx.x % (D / 4)) * 4;
-  if (j >= keys || j >= rw.lk) return;
+  const int col = (threadIdx.x % C) * 4, key = threadIdx.x / C % KEYS, pg = threadIdx.x / C / KEYS;
+  const int j = blockIdx.x * KEYS + key;
+  const bool on = j < keys && j < rw.lk;
   const int64_t N = part_rows(p), S = sink_rows(p), r = part_row(p, rw, b, hk, j);
   const float* sink = p.part + 2 * p.nsplit * N * D;
+  const int parts = p.nsplit + (j < p.s32 ? p.nchunk : 0);
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    float o[4] = {0.f, 0.f, 0.f, 0.f}, a[4];
-    for (int s = 0; s < p.nsplit; ++s) {
-      load4(p.part + (((int64_t)which * p.nsplit + s) * N + r) * D + col, a);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += a[e];
-    }
-    if (j < p.s32)
-      for (int s = 0; s < p.nchunk; ++s) {
-        load4(sink + (((int64_t)which * p.nchunk + s) * S + ((int64_t)b * p.Hk + hk) * p.s32 + j) * D + col, a);
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    if (on)
+      for (int s = pg; s < parts; s += PG) {
+        const float* src = s < p.nsplit ? p.part + (((int64_t)which * p.nsplit + s) * N + r) * D
+                                        : sink + (((int64_t)which * p.nchunk + s - p.nsplit) * S + ((int64_t)b * p.Hk + hk) * p.s32 + j) * D;
+        float a[4];
+        load4(src + col, a);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += a[e];
       }
+    if (PG > 1) {
+      store4(&fold[which][pg][key][col], o);
+    } else if (on) {
+      const float mul = which ? 1.f : p.scale;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= mul;
+      store4((which ? reinterpret_cast<T*>(p.dv) + (rw.k0 + j) * p.lddv : reinterpret_cast<T*>(p.dk) + (rw.k0 + j) * p.lddk) + (int64_t)hk * D + col, o);
+    }
+  }
+  if (PG == 1) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * KEYS * C; i += 256) {          // (with PG = 16: at most one round)
+    const int which = i / (KEYS * C), k = i / C % KEYS, cc = (i % C) * 4, jj = blockIdx.x * KEYS + k;
+    if (jj >= keys || jj >= rw.lk) continue;
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < PG; ++g) {
+      float a[4];
+      load4(&fold[which][g][k][cc], a);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += a[e];
+    }
     const float mul = which ? 1.f : p.scale;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] *= mul;
-    T* dst = which ? reinterpret_cast<T*>(p.dv) + (rw.k0 + j) * p.lddv : reinterpret_cast<T*>(p.dk) + (rw.k0 + j) * p.lddk;
-    store4(dst + (int64_t)hk * D + col, o);
+    store4((which ? reinterpret_cast<T*>(p.dv) + (rw.k0 + jj) * p.lddv : reinterpret_cast<T*>(p.dk) + (rw.k0 + jj) * p.lddk) + (int64_t)hk * D + cc, o);
   }
 }
 
@@ -475,7 +539,7 @@ template <typename T, int D, bool DROP> int launch_bwd(Params& p, hipStream_t s)
     const int nqt = (int)cdiv(p.Lq, QB);
     const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.H : (int64_t)p.nseq * p.H * nqt;
     if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
-    const int lds = 4 * G::KT * G::ROWB + 2 * G::KT * 4 + 16;
+    const int lds = 4 * G::KT * G::ROWB + 2 * G::KT * 4;
     if ((rc = raise_lds<dq_kernel<T, D, DROP>>(lds))) return rc;
     if (nu) hipLaunchKernelGGL((dq_kernel<T, D, DROP>), dim3((unsigned)(8 * cdiv(nu, 8))), dim3(256), lds, s, p, (int)nu, nqt);
     if ((rc = ctclip_check_launch("win_attn_bwd dq"))) return rc;
@@ -499,7 +563,9 @@ template <typename T, int D, bool DROP> int launch_bwd(Params& p, hipStream_t s)
   }
   const int keys = p.nsplit > 1 ? p.Lk : p.s32;
   if (!keys) return CTCLIP_OK;
-  hipLaunchKernelGGL((dkv_reduce_kernel<T, D>), dim3((unsigned)cdiv(keys, 256 / (D / 4)), p.Hk, p.nseq), dim3(256), 0, s, p, keys);
+  constexpr int PG = 256 / (D / 4) < 16 ? 256 / (D / 4) : 16;      // threads across the parts where the sinks' chunks are many
+  if (p.nsplit + p.nchunk > 8) hipLaunchKernelGGL((dkv_reduce_kernel<T, D, PG>), dim3((unsigned)cdiv(keys, 256 / (D / 4) / PG), p.Hk, p.nseq), dim3(256), 0, s, p, keys);
+  else hipLaunchKernelGGL((dkv_reduce_kernel<T, D, 1>), dim3((unsigned)cdiv(keys, 256 / (D / 4)), p.Hk, p.nseq), dim3(256), 0, s, p, keys);
   return ctclip_check_launch("win_attn_bwd reduce");
 }
 template <typename T, int D> int launch_bwd_d(Params& p, hipStream_t s) { return p.drop_p > 0.f ? launch_bwd<T, D, true>(p, s) : launch_bwd<T, D, false>(p, s); }

@@ -9,9 +9,6 @@
 //   dkv_reduce_kernel  adds the partial sums of split keys in a fixed order.  Every result is bit-reproducible.
 // Seven products per visible block (five are needed at least; the other two are S and dP again, because dQ across key tiles would need float atomics).
 #include "win_attn.h"
-#ifndef DKV_JOINT
-#define DKV_JOINT 1
-#endif
 
 namespace win {
 
@@ -348,17 +345,6 @@ __global__ __launch_bounds__(256, WGS) void dkv_kernel(Params p, int nunits, int
     if (++t == nt) { t = 0; ++g; }
     char* next = lds + (buf ^ 1) * 2 * TILE;               // (its readers are behind the last barrier)
     if (more) rp.issue(p, next, next + TILE, g, (t0 + t) * QT, tid);
-#if DKV_JOINT
-    {
-      const int lo = p.q_start + r0, last = p.q_start + rw.lq - 1, n = QT - 1;
-      const int see = any ? Sight(lo, lo + n < last ? lo + n : last, p.left, p.right, 0, rw.lk).of(jw) : 0;
-      if (see) {
-        const char* qt = lds + buf * 2 * TILE;
-        const float* sp = stat + buf * 2 * QT;
-        query_blocks<T, D, QT / 32, DROP, false>(st, qt, qt + TILE, sp, sp + QT, at, p, r0, j, kbias, see == 1, lane, sh);
-      }
-    }
-#else
 #pragma unroll
     for (int b = 0; b < QT / 32; ++b) {
       const int lo = p.q_start + r0 + 32 * b, last = p.q_start + rw.lq - 1;
@@ -369,7 +355,6 @@ __global__ __launch_bounds__(256, WGS) void dkv_kernel(Params p, int nunits, int
         query_blocks<T, D, 1, DROP, false>(st, qt, qt + TILE, sp, sp + QT, at, p, r0 + 32 * b, j, kbias, see == 1, lane, sh);
       }
     }
-#endif
     if (more) rp.settle(stat + (buf ^ 1) * 2 * QT, tid);
     __syncthreads();
   }

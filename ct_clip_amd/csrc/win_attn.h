@@ -314,30 +314,6 @@ template <typename T, int D, int KT, int NT> struct KeyPipe {      // through LD
     return state;
   }
 };
-template <typename T, int D> struct WaveKeyPipe {          // a wave's own tiles of 32 keys, through registers (one LDS buffer per wave)
-  typedef Stage<T, D, 32, 64> St;
-  KeySource src;
-  St sk, sv;
-  float km;
-  int j0;
-  __device__ __forceinline__ WaveKeyPipe(const Params& p, int64_t k0, int hk, int lk, int jlo, int jhi) { src.init<T, D>(p, k0, hk, lk, jlo, jhi); km = 0.f; j0 = 0; }
-  __device__ __forceinline__ void fetch(int first, int lane) {
-    j0 = first;
-    const int last = src.lk - 1 - first;
-    sk.get(src.k + (int64_t)first * src.ldk, src.ldk, last, lane);
-    sv.get(src.v + (int64_t)first * src.ldv, src.ldv, last, lane);
-    if (src.mask) { const int r = lane & 31; km = src.mask[first + (r < last ? r : last)]; }
-  }
-  __device__ __forceinline__ int deposit(char* kt, char* vt, float* bias, int lane) const {
-    if (!src.mask && j0 >= src.jlo && j0 + 31 <= src.jhi) { sk.put(kt, lane); sv.put(vt, lane); return 0; }
-    uint64_t keep;
-    const int state = src.look<32>(keep, km, bias, j0, lane);
-    sk.put(kt, keep, lane);
-    sv.put(vt, keep, lane);
-    return state;
-  }
-};
-
 // visibility by position of 32 x 32 blocks: rows lo ... hi (positions; hi < lo: none) against keys j0 ... j0 + 31: 0 nothing, 1 some, 2 everything
 struct Sight {
   int none_above, full_above, full_below, none_below, sinks;

@@ -28,49 +28,33 @@ template <int D> struct SoftRow {          // the running softmax of a lane's qu
 // maximum moves in nearly every block -- becomes rare.
 constexpr float LAZY = 8.f;
 
-// NB neighbouring 32-key blocks: scores -> running softmax -> acc.  kt, vt = the blocks in LDS; bias = their additive mask (or null); pos = the lane's position
-template <typename T, int D, int NB, bool DROP, bool PAIRED>
-__device__ __forceinline__ void key_blocks(SoftRow<D>& st, const RowFrag<T, D>& qf, const char* kt, const char* vt, const float* bias, const LaneAt<T, D>& at, const Params& p,
-                                           int j0, int pos, int lk, bool partial, int lane, int64_t sh, int qi) {
-  constexpr int BLK = 32 * Geo<T, D>::ROWB;
+// A 32-key block: scores -> running softmax -> acc.  vt = the block's v rows in LDS; bias = its additive mask (or null); pos = the lane's position
+template <typename T, int D, bool DROP, bool PAIRED>
+__device__ __forceinline__ void key_block(SoftRow<D>& st, f32x16 s, const char* vt, const float* bias, const LaneAt<T, D>& at, const Params& p, int j0, int pos, int lk,
+                                          bool partial, int lane, int64_t sh, int qi) {
   const int half = lane >> 5;
-  f32x16 s[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    RowFrag<T, D> kf;
-    row_frag_lds<T, D>(kf, kt + b * BLK, at);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
-    s[b] = mma_rows<D>(kf, qf, s[b]);
-  }
   float sc = p.scale2;                                     // (scale > 0: the maximum may be taken of the unscaled scores; one rounding in the fma below)
   if (bias) {
     sc = 1.f;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(bias + 8 * g + 4 * half);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(bias + 32 * b + 8 * g + 4 * half);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[b][4 * g + e] = fmaf(s[b][4 * g + e], p.scale2, a[e]);
-      }
+      for (int e = 0; e < 4; ++e) s[4 * g + e] = fmaf(s[4 * g + e], p.scale2, a[e]);
+    }
   }
   if (partial) {
     const int o = j0 + 4 * half;
     const int hi = (pos + p.right < lk - 1 ? pos + p.right : lk - 1) - o, lo = pos - p.left - o, sk = p.sinks - o;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = 32 * b + 8 * (r >> 2) + (r & 3);
-        s[b][r] = (j <= hi && (j >= lo || j < sk)) ? s[b][r] : -INFINITY;
-      }
+    for (int r = 0; r < 16; ++r) {
+      const int j = 8 * (r >> 2) + (r & 3);
+      s[r] = (j <= hi && (j >= lo || j < sk)) ? s[r] : -INFINITY;
+    }
   }
-  float mx = s[0][0];
+  float mx = s[0];
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+  for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
   mx = half_max(mx) * sc;
   if (__builtin_amdgcn_ballot_w64(mx > st.m + LAZY) != 0) {        // wave-uniform
     const float mn = fmaxf(st.m, mx);
@@ -83,25 +67,28 @@ __device__ __forceinline__ void key_blocks(SoftRow<D>& st, const RowFrag<T, D>& 
     st.m = mn;
   }
   const float ms = st.m == -INFINITY ? 0.f : st.m;         // nothing seen so far: every exp2 below is exp2(-inf) = 0
+  float pr[16], ps[4];                                     // (four sums: one would be a chain of 16 dependent additions)
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    float pr[16], ps[4];                                   // (four sums: one would be a chain of 16 dependent additions)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      pr[r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], sc, -ms));
-      ps[r & 3] = r < 4 ? pr[r] : ps[r & 3] + pr[r];
-    }
-    st.l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-    if (DROP) {                                            // on the normalised probabilities: the sum above stays undropped
-      float dm[16];
-      drop_of_query<PAIRED>(dm, p, sh, qi, j0 + 32 * b, half);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) pr[r] *= dm[r];
-    }
-    PFrag<T> pf;
-    p_frag(pf, pr);
-    mma_cols<T, D>(st.acc, vt + b * BLK, at, pf, lane);
+  for (int r = 0; r < 16; ++r) {
+    pr[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, -ms));
+    ps[r & 3] = r < 4 ? pr[r] : ps[r & 3] + pr[r];
   }
+  st.l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+  if (DROP) {                                              // on the normalised probabilities: the sum above stays undropped
+    float dm[16];
+    drop_of_query<PAIRED>(dm, p, sh, qi, j0, half);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) pr[r] *= dm[r];
+  }
+  PFrag<T> pf;
+  p_frag(pf, pr);
+  mma_cols<T, D>(st.acc, vt, at, pf, lane);
+}
+template <typename T, int D> __device__ __forceinline__ f32x16 scores(const RowFrag<T, D>& kf, const RowFrag<T, D>& qf) {
+  f32x16 s;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = 0.f;
+  return mma_rows<D>(kf, qf, s);
 }
 
 template <typename T, int D, bool DROP>
@@ -153,7 +140,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 4 : 2)) void fwd_
 #pragma unroll
       for (int b = 0; b < KT / 32; ++b) {
         const int a = sight.of(j0 + 32 * b), o = 32 * b * G::ROWB;
-        if (a) key_blocks<T, D, 1, DROP, true>(st, qf, kt + o, vt + o, bias ? bias + 32 * b : nullptr, at, p, j0 + 32 * b, pos, rw.lk, a != 2, lane, sh, row);
+        if (!a) continue;
+        RowFrag<T, D> kf;
+        row_frag_lds<T, D>(kf, kt + o, at);
+        key_block<T, D, DROP, true>(st, scores<T, D>(kf, qf), vt + o, bias ? bias + 32 * b : nullptr, at, p, j0 + 32 * b, pos, rw.lk, a != 2, lane, sh, row);
       }
     }
     if (more) state = kp.settle(next, next + TILE, kb + (buf ^ 1) * KT, tid);
@@ -172,12 +162,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 4 : 2)) void fwd_
   if (half == 0 && p.lse) p.lse[(int64_t)h * p.Mq + rw.q0 + row] = l == 0.f ? INFINITY : st.m + __builtin_amdgcn_logf(l);
 }
 
-// ---- few query rows: R = Lq * G <= 32 rows (row c = head g = c / Lq of the group, query c % Lq)
+// ---- few query rows: R = Lq * G <= 32 rows (row c = head g = c / Lq of the group, query c % Lq).  A wave's keys meet no other wave's rows, so k goes straight from
+// memory into the first product's operand registers (the next block's while this one is worked on), only v through LDS, two blocks per wave.
 template <typename T, int D, bool DROP>
-__global__ __launch_bounds__(256, 2) void rows_kernel(Params p, int nunits) {
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void rows_kernel(Params p, int nunits) {
   typedef Geo<T, D> G;
   constexpr int TILE = 32 * G::ROWB;
-  extern __shared__ __attribute__((aligned(16))) char lds[];       // four waves x [K | V] of 32 keys; reused to fold the waves
+  extern __shared__ __attribute__((aligned(16))) char lds[];       // four waves x ([2][V] of 32 keys, [2][32] additive mask); reused to fold the waves
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Unit u = unit_of(p, blockIdx.x, nunits, 1, 1);
@@ -191,25 +182,46 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Params p, int nunits) {
   const int g = rc / rw.lq, row = rc - g * rw.lq, h = u.hk * p.G + g, pos = p.q_start + row;
   RowFrag<T, D> qf;
   row_frag_global<T, D>(qf, reinterpret_cast<const T*>(p.q) + (rw.q0 + row) * p.ldq + (int64_t)h * D, half);
-  char* ktile = lds + wave * (2 * TILE + 128);
-  char* vtile = ktile + TILE;
-  float* kb = reinterpret_cast<float*>(vtile + TILE);
+  char* vtile = lds + wave * (2 * TILE + 256);
+  float* kb = reinterpret_cast<float*>(vtile + 2 * TILE);
   const Sight sight(lo, hi, p.left, p.right, p.sinks, rw.lk);
   const LaneAt<T, D> at(lane);
-  WaveKeyPipe<T, D> kp(p, rw.k0, u.hk, rw.lk, lo - p.left, hi + p.right);
+  KeySource src;
+  src.init<T, D>(p, rw.k0, u.hk, rw.lk, lo - p.left, hi + p.right);
+  Dma<T, D, 32, 64> dv;
+  dv.init(src.ldv, lane);
+  RowFrag<T, D> kf;
+  float km = 0.f;
+  auto fetch = [&](int j0, int buf) {                              // (rows past the end: k of the last row, v zeros)
+    const int r = c < src.lk - 1 - j0 ? c : src.lk - 1 - j0;
+    if (src.mask) km = src.mask[j0 + r];
+    row_frag_global<T, D>(kf, reinterpret_cast<const T*>(src.k + (int64_t)(j0 + r) * src.ldk), half);
+    dv.issue(vtile + buf * TILE, src.v + (int64_t)j0 * src.ldv, src.ldv, src.jhi + 1 - j0, lane);
+  };
   SoftRow<D> st;
   st.clear();
   const int64_t sh = (int64_t)u.b * p.H + h;
-  int it = i0 + wave;
-  if (it < i1) kp.fetch(tile_at(tl, it) * 32, lane);
+  int it = i0 + wave, buf = 0;
+  if (it < i1) fetch(tile_at(tl, it) * 32, 0);
   row_frag_arrive<T, D>(qf);
-  for (; it < i1; it += 4) {                                       // (no barrier: a wave's tiles are its own, and its LDS operations keep their order)
+  for (; it < i1; it += 4, buf ^= 1) {                             // (no barrier: a wave's tiles are its own, and its LDS operations keep their order)
     const int j0 = tile_at(tl, it) * 32;
-    const int state = kp.deposit(ktile, vtile, kb, lane);
-    if (it + 4 < i1) kp.fetch(tile_at(tl, it + 4) * 32, lane);
+    dma_arrive();
+    int state = 0;
+    if (src.mask || j0 < src.jlo || j0 + 31 > src.jhi) {
+      uint64_t keep;
+      state = src.look<32>(keep, km, kb + buf * 32, j0, lane);
+      if (~keep) {
+        dv.erase(vtile + buf * TILE, keep, lane);
+        row_frag_arrive<T, D>(kf);
+        if (!((keep >> c) & 1)) row_frag_zero<T, D>(kf);
+      }
+    }
     wave_sync();
+    const f32x16 s = scores<T, D>(kf, qf);
+    if (it + 4 < i1) fetch(tile_at(tl, it + 4) * 32, buf ^ 1);
     const int a = sight.of(j0);
-    if (a && state != 2) key_blocks<T, D, 1, DROP, false>(st, qf, ktile, vtile, state ? kb : nullptr, at, p, j0, pos, rw.lk, a == 1, lane, sh, row);
+    if (a && state != 2) key_block<T, D, DROP, false>(st, s, vtile + buf * TILE, state ? kb + buf * 32 : nullptr, at, p, j0, pos, rw.lk, a == 1, lane, sh, row);
     wave_sync();
   }
   // fold the four waves: row maxima first, then sums and accumulators under the common maximum
@@ -259,24 +271,41 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Params p, int nunits) {
   if ((tid & 7) == 0 && p.lse) p.lse[(int64_t)oh * p.Mq + rw.q0 + orow] = lsum == 0.f ? INFINITY : m + __builtin_amdgcn_logf(lsum);
 }
 
-// out = sum_s exp2(m_s - M) acc_s / sum_s exp2(m_s - M) l_s over the split passes; D / 4 threads per (head, row)
+// out = sum_s exp2(m_s - M) acc_s / sum_s exp2(m_s - M) l_s over the split passes.  A workgroup per (head, row): D / 4 threads across the columns, the others across the
+// splits (one thread per column alone chains nsplit loads: 11 us for 16 splits), folded in a fixed order.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
-  const int64_t n = (int64_t)p.H * p.Mq, rows = (int64_t)p.nsplit * n;
-  const int64_t i = (int64_t)blockIdx.x * (256 / (D / 4)) + threadIdx.x / (D / 4);
-  const int col = (threadIdx.x % (D / 4)) * 4;
-  if (i >= n) return;
+  constexpr int C = D / 4, SG = 256 / C;
+  __shared__ __attribute__((aligned(16))) float fo[SG][D], fl[SG];
+  const int64_t n = (int64_t)p.H * p.Mq, rows = (int64_t)p.nsplit * n, i = blockIdx.x;
+  const int col = (threadIdx.x % C) * 4, sg = threadIdx.x / C;
   float m = -INFINITY;
-  for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, p.part[s * n + i]);
+  for (int s = threadIdx.x & 63; s < p.nsplit; s += 64) m = fmaxf(m, p.part[s * n + i]);
+  m = wave_max(m);
   const float ms = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.nsplit; ++s) {
+  for (int s = sg; s < p.nsplit; s += SG) {
     const float f = __builtin_amdgcn_exp2f(p.part[s * n + i] - ms);
     l = fmaf(p.part[rows + s * n + i], f, l);
     float a[4];
     load4(p.part + 2 * rows + (s * n + i) * D + col, a);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(a[e], f, o[e]);
+  }
+  store4(&fo[sg][col], o);
+  if (col == 0) fl[sg] = l;
+  __syncthreads();
+  if (sg) return;
+  l = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = 0.f;
+#pragma unroll
+  for (int g = 0; g < SG; ++g) {
+    float a[4];
+    load4(&fo[g][col], a);
+    l += fl[g];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += a[e];
   }
   const int64_t h = i / p.Mq, row = i - h * p.Mq;
   const float mul = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
@@ -318,7 +347,7 @@ template <typename T, int D, bool DROP> int launch_fwd(Params& p, const Plan& pl
   if (pl.rows) {
     const int64_t nu = (int64_t)p.nseq * p.Hk;
     if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many sequences"); return CTCLIP_EUNSUPPORTED; }
-    int lds = 4 * (2 * 32 * G::ROWB + 128);
+    int lds = 4 * (2 * 32 * G::ROWB + 256);
     const int fold = 1024 + 4 * 32 * (D + 4) * 4;
     if (fold > lds) lds = fold;
     const int rc = raise_lds<rows_kernel<T, D, DROP>>(lds);
@@ -335,7 +364,7 @@ template <typename T, int D, bool DROP> int launch_fwd(Params& p, const Plan& pl
   }
   int rc = ctclip_check_launch("win_attn_fwd");
   if (rc || p.nsplit == 1) return rc;
-  hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)cdiv((int64_t)p.H * p.Mq, 256 / (D / 4))), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)((int64_t)p.H * p.Mq)), dim3(256), 0, s, p);
   return ctclip_check_launch("win_attn_fwd join");
 }
 template <typename T, int D> int launch_fwd_d(Params& p, const Plan& pl, hipStream_t s) {

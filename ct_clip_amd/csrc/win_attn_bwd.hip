@@ -2,9 +2,9 @@
 //
 // With P from the forward pass's log-sum-exp and Delta = rowsum(dO o O):  dV = P^T dO,  dS = P o (dO V^T - Delta),  dQ = scale dS K,  dK = scale dS^T Q.
 //   dq_kernel     query rows as in the forward kernel: S^T, dP^T with a query per lane, dQ^T += K^T dS^T.  Also writes Delta.
-//   dkv_kernel    128 keys of one (sequence, k|v head), 32 per wave: k, v and both gradients stay in registers while the query rows whose windows hold the keys pass
+//   dkv_kernel, window_pass   128 keys of one (sequence, k|v head), 32 per wave: k, v and both gradients stay in registers while the query rows whose windows hold the keys pass
 //                 through a double-buffered LDS ring, for every query head that shares the keys: their gradients are summed here, no atomics.
-//   dkv_sink_kernel  the sinks meet EVERY later row: one key block would walk the whole sequence while all others walk a window.  The pairs (sink, row beyond its
+//   dkv_kernel, sink_pass     the sinks meet EVERY later row: one key block would walk the whole sequence while all others walk a window.  The pairs (sink, row beyond its
 //                 window) are a pass of their own, split over the rows, a wave per 32-row tile; f32 partial sums.
 //   dkv_reduce_kernel  adds the partial sums of split keys in a fixed order.  Every result is bit-reproducible.
 // Seven products per visible block (five are needed at least; the other two are S and dP again, because dQ across key tiles would need float atomics).
@@ -305,15 +305,14 @@ __device__ __forceinline__ int64_t part_row(const Params& p, const Rows& rw, int
 __host__ __device__ inline int64_t part_rows(const Params& p) { return p.nsplit > 1 ? (int64_t)p.Hk * p.Mk : (int64_t)p.nseq * p.Hk * p.s32; }
 __host__ __device__ inline int64_t sink_rows(const Params& p) { return (int64_t)p.nseq * p.Hk * p.s32; }
 
-template <typename T, int D, bool DROP, int WGS>
-__global__ __launch_bounds__(256, WGS) void dkv_kernel(Params p, int nunits, int nkt) {
+template <typename T, int D, bool DROP>
+__device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, int split, int nunits, int nkt) {
   typedef Geo<T, D> G;
   constexpr int QT = QTile<T, D>::ROWS, TILE = QT * G::ROWB;
-  extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][Q | dO], then [2][lse | Delta] of the rows
   float* stat = reinterpret_cast<float*>(lds + 4 * TILE);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Unit u = unit_of(p, blockIdx.x, nunits, nkt, 1);
+  const Unit u = unit_of(p, id, nunits, nkt, 1);
   if (!u.real) return;
   const Rows rw = rows_of(p, u.b);
   const int k0 = u.tile * QB;
@@ -324,7 +323,7 @@ __global__ __launch_bounds__(256, WGS) void dkv_kernel(Params p, int nunits, int
   rlo = rlo < 0 ? 0 : rlo;
   rhi = rhi < rw.lq - 1 ? rhi : rw.lq - 1;
   const int t0 = rlo / QT, nt = rhi >= rlo ? rhi / QT - t0 + 1 : 0, steps = nt * p.G;
-  const int i0 = (int)((int64_t)steps * blockIdx.y / p.nsplit), i1 = (int)((int64_t)steps * (blockIdx.y + 1) / p.nsplit);
+  const int i0 = (int)((int64_t)steps * split / p.nsplit), i1 = (int)((int64_t)steps * (split + 1) / p.nsplit);
 
   const int jw = k0 + 32 * wave, j = jw + c;
   KeyState<T, D> st;
@@ -360,7 +359,7 @@ __global__ __launch_bounds__(256, WGS) void dkv_kernel(Params p, int nunits, int
   }
   if (j >= rw.lk) return;
   if (p.nsplit > 1 || jw < p.s32) {
-    const int64_t N = part_rows(p), r = (int64_t)blockIdx.y * N + part_row(p, rw, u.b, u.hk, j);
+    const int64_t N = part_rows(p), r = (int64_t)split * N + part_row(p, rw, u.b, u.hk, j);
     store_row<float, D>(p.part + r * D, st.dk, 1.f, half);
     store_row<float, D>(p.part + ((int64_t)p.nsplit * N + r) * D, st.dv, 1.f, half);
     return;
@@ -370,20 +369,19 @@ __global__ __launch_bounds__(256, WGS) void dkv_kernel(Params p, int nunits, int
 }
 
 template <typename T, int D, bool DROP>
-__global__ __launch_bounds__(256, 1) void dkv_sink_kernel(Params p, int nblk) {
+__device__ __forceinline__ void sink_pass(const Params& p, char* lds, int id, int nblk) {
   typedef Geo<T, D> G;
-  constexpr int TILE = 32 * G::ROWB;
-  extern __shared__ __attribute__((aligned(16))) char lds[];       // four waves x [Q | dO | lse, Delta] of 32 rows; reused to fold the waves
+  constexpr int TILE = 32 * G::ROWB;                               // lds: four waves x [Q | dO | lse, Delta] of 32 rows; reused to fold the waves
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int blk = blockIdx.x % nblk, hk = (blockIdx.x / nblk) % p.Hk, b = blockIdx.x / (nblk * p.Hk);
+  const int chunk = id % p.nchunk, blk = id / p.nchunk % nblk, hk = id / (p.nchunk * nblk) % p.Hk, b = id / (p.nchunk * nblk * p.Hk);
   const Rows rw = rows_of(p, b);
   const int jw = 32 * blk, j = jw + c;
   if (jw >= rw.lk) return;
   int rlo = jw + p.left + 1 - p.q_start;                           // first row that has a key of this block beyond its window
   rlo = rlo < 0 ? 0 : rlo;
   const int t0 = rlo / 32, nt = rw.lq > rlo ? (rw.lq - 1) / 32 - t0 + 1 : 0, steps = nt * p.G;
-  const int i0 = (int)((int64_t)steps * blockIdx.y / p.nchunk), i1 = (int)((int64_t)steps * (blockIdx.y + 1) / p.nchunk);
+  const int i0 = (int)((int64_t)steps * chunk / p.nchunk), i1 = (int)((int64_t)steps * (chunk + 1) / p.nchunk);
   KeyState<T, D> st;
   const float kbias = load_keys<T, D>(st, p, rw, hk, j, half);
   char* qtile = lds + wave * (2 * TILE + 256);
@@ -419,7 +417,7 @@ __global__ __launch_bounds__(256, 1) void dkv_sink_kernel(Params p, int nblk) {
         *reinterpret_cast<f32x4*>(fa + (wave * 32 + c) * (D + 4) + 32 * n + 8 * q + 4 * half) = t;
       }
     __syncthreads();
-    float* dst = base + (((int64_t)which * p.nchunk + blockIdx.y) * S + r + fr) * D + fc;
+    float* dst = base + (((int64_t)which * p.nchunk + chunk) * S + r + fr) * D + fc;
 #pragma unroll
     for (int e = 0; e < PER; e += 4) {
       float t[4];
@@ -431,6 +429,16 @@ __global__ __launch_bounds__(256, 1) void dkv_sink_kernel(Params p, int nblk) {
       store4(dst + e, t);
     }
   }
+}
+
+// The first nsink workgroups take the sink pass, so that it runs beside the window pass instead of in front of it.
+template <typename T, int D, bool DROP>
+__global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void dkv_kernel(Params p, int nunits, int nkt, int nsink) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int id = (int)blockIdx.x - nsink;
+  if (id < 0) { sink_pass<T, D, DROP>(p, lds, blockIdx.x, p.s32 / 32); return; }
+  const int per = (nunits + 7) / 8 * 8;
+  window_pass<T, D, DROP>(p, lds, id % per, id / per, nunits, nkt);
 }
 
 // Keys whose sums came in parts.  A workgroup folds 256 / (D / 4) / PG keys of one k|v head: D / 4 threads across the columns, PG threads (1, or a sixteenth of the
@@ -518,7 +526,6 @@ inline int64_t bwd_floats(const BwdPlan& b, int nseq, int64_t Mk, int Hk, int D)
 
 template <typename T, int D, bool DROP> int launch_bwd(Params& p, hipStream_t s) {
   typedef Geo<T, D> G;
-  constexpr int WGS = D == 128 ? 1 : 2;    // 128 columns: k, v and both gradients of a wave's keys alone are 256 registers
   int rc;
   {
     const int nqt = (int)cdiv(p.Lq, QB);
@@ -529,21 +536,16 @@ template <typename T, int D, bool DROP> int launch_bwd(Params& p, hipStream_t s)
     if (nu) hipLaunchKernelGGL((dq_kernel<T, D, DROP>), dim3((unsigned)(8 * cdiv(nu, 8))), dim3(256), lds, s, p, (int)nu, nqt);
     if ((rc = ctclip_check_launch("win_attn_bwd dq"))) return rc;
   }
-  if (p.s32) {
-    const int nblk = p.s32 / 32;
-    int lds = 4 * (2 * 32 * G::ROWB + 256);
-    if (4 * 32 * (D + 4) * 4 > lds) lds = 4 * 32 * (D + 4) * 4;
-    if ((rc = raise_lds<dkv_sink_kernel<T, D, DROP>>(lds))) return rc;
-    hipLaunchKernelGGL((dkv_sink_kernel<T, D, DROP>), dim3((unsigned)(nblk * p.Hk * p.nseq), p.nchunk), dim3(256), lds, s, p, nblk);
-    if ((rc = ctclip_check_launch("win_attn_bwd sinks"))) return rc;
-  }
   {
     const int nkt = (int)cdiv(p.Lk, QB);
-    const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.Hk : (int64_t)p.nseq * p.Hk * nkt;
-    if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
-    const int lds = 4 * QTile<T, D>::ROWS * G::ROWB + 4 * QTile<T, D>::ROWS * 4;
-    if ((rc = raise_lds<dkv_kernel<T, D, DROP, WGS>>(lds))) return rc;
-    if (nu) hipLaunchKernelGGL((dkv_kernel<T, D, DROP, WGS>), dim3((unsigned)(8 * cdiv(nu, 8)), p.nsplit), dim3(256), lds, s, p, (int)nu, nkt);
+    const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.Hk : (int64_t)p.nseq * p.Hk * nkt, nsink = (int64_t)(p.s32 / 32) * p.Hk * p.nseq * p.nchunk;
+    const int64_t grid = nsink + 8 * cdiv(nu, 8) * p.nsplit;
+    if (grid > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
+    int lds = 4 * QTile<T, D>::ROWS * G::ROWB + 4 * QTile<T, D>::ROWS * 4;
+    if (4 * (2 * 32 * G::ROWB + 256) > lds) lds = 4 * (2 * 32 * G::ROWB + 256);
+    if (4 * 32 * (D + 4) * 4 > lds) lds = 4 * 32 * (D + 4) * 4;
+    if ((rc = raise_lds<dkv_kernel<T, D, DROP>>(lds))) return rc;
+    if (nu) hipLaunchKernelGGL((dkv_kernel<T, D, DROP>), dim3((unsigned)grid), dim3(256), lds, s, p, (int)nu, nkt, (int)nsink);
     if ((rc = ctclip_check_launch("win_attn_bwd dkv"))) return rc;
   }
   const int keys = p.nsplit > 1 ? p.Lk : p.s32;

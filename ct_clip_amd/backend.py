@@ -417,8 +417,7 @@ class HipBackend:
         M, nq = q.shape
         nk = k.shape[1] if k is not None else 0
         with _on(q):
-            qo, ko = out if out is not None else (torch.empty((M, nq), dtype=q.dtype, device=q.device),
-                                                  torch.empty((M, nk), dtype=q.dtype, device=q.device) if nk else None)
+            qo, ko = out if out is not None else (q.new_empty((M, nq)), q.new_empty((M, nk)) if nk else None)
             rc = self.lib.ctclip_rotary(q.data_ptr(), _p(k), qo.data_ptr(), _p(ko), turns.data_ptr(), _p(positions), positions.element_size() if positions is not None else 0, M,
                                         L, start, nq // D, nk // D, D, rot, _rowmajor(q, "q"), _rowmajor(k, "k") if nk else 0, _rowmajor(qo, "out q"),
                                         _rowmajor(ko, "out k") if nk else 0, interleaved, magnitude, inverse, dcode(q.dtype), _stream_of(q))
@@ -440,7 +439,7 @@ class HipBackend:
         dp, dseed = dropout if dropout is not None else (0.0, 0)
         dev, n = q.device, geo.H * geo.D
         with _on(q):
-            o = torch.zeros((geo.Mq, n), dtype=q.dtype, device=dev) if geo.uncovered else torch.empty((geo.Mq, n), dtype=q.dtype, device=dev)
+            o = q.new_zeros((geo.Mq, n)) if geo.uncovered else q.new_empty((geo.Mq, n))
             lse = torch.empty((geo.H, geo.Mq), dtype=torch.float32, device=dev) if want_lse else None
             need = self._win_workspaces(geo)[0]
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
@@ -457,9 +456,9 @@ class HipBackend:
         dev = q.device
         with _on(q):
             if out is None:
-                new = torch.zeros if geo.uncovered else torch.empty
+                new = q.new_zeros if geo.uncovered else q.new_empty
                 n, nk = geo.H * geo.D, geo.Hk * geo.D
-                dq, dk, dv = new((geo.Mq, n), dtype=q.dtype, device=dev), new((geo.Mk, nk), dtype=q.dtype, device=dev), new((geo.Mk, nk), dtype=q.dtype, device=dev)
+                dq, dk, dv = new((geo.Mq, n)), new((geo.Mk, nk)), new((geo.Mk, nk))
             else:
                 dq, dk, dv = out
             need = self._win_workspaces(geo)[1]

@@ -151,70 +151,50 @@ __device__ __forceinline__ void drop_of_key(float (&m)[16], const Params& p, int
       for (int e = 0; e < 2; ++e) m[4 * g + 2 * s + e] = attn_drop_pick(w[g], e, j, thr, p.inv_keep);
   }
 }
-// FAR: the sink pass (keys seen because they are sinks, j < i - left); otherwise the window (i - left <= j <= i + right).  NB neighbouring blocks of 32 queries at a
-// time: the products of one block run under the exponentials of the other.
-template <typename T, int D, int NB, bool DROP, bool FAR>
-__device__ __forceinline__ void query_blocks(KeyState<T, D>& st, const char* qt, const char* dt, const float* lse, const float* delta, const LaneAt<T, D>& at, const Params& p,
-                                             int row, int j, float kbias, bool partial, int lane, int64_t sh) {
-  constexpr int BLK = 32 * Geo<T, D>::ROWB;
+// FAR: the sink pass (keys seen because they are sinks, j < i - left); otherwise the window (i - left <= j <= i + right).
+template <typename T, int D, bool DROP, bool FAR>
+__device__ __forceinline__ void query_block(KeyState<T, D>& st, const char* qt, const char* dt, const float* lse, const float* delta, const LaneAt<T, D>& at, const Params& p,
+                                            int row, int j, float kbias, bool partial, int lane, int64_t sh) {
   const int half = lane >> 5;
-  f32x16 s[NB], dp[NB];
+  RowFrag<T, D> f, f2;
+  row_frag_lds<T, D>(f, qt, at);
+  row_frag_lds<T, D>(f2, dt, at);
+  f32x16 s, dp;
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    RowFrag<T, D> f;
-    row_frag_lds<T, D>(f, qt + b * BLK, at);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) { s[b][r] = 0.f; dp[b][r] = 0.f; }
-    s[b] = mma_rows<D>(f, st.kf, s[b]);
-  }
+  for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+  s = mma_rows<D>(f, st.kf, s);
   if (partial) {                           // row >= j - right, row <= j + left (positions), or beyond: row > j + left and j a sink
     const int o = p.q_start + row + 4 * half;
     const int rl = j - p.right - o, rh = j + p.left - o;
     const bool sink = j < p.sinks;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = 32 * b + 8 * (r >> 2) + (r & 3);
-        s[b][r] = (FAR ? (sink && i > rh) : (i >= rl && i <= rh)) ? s[b][r] : -INFINITY;
-      }
-  }
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    RowFrag<T, D> f;
-    row_frag_lds<T, D>(f, dt + b * BLK, at);
-    dp[b] = mma_rows<D>(f, st.vf, dp[b]);
-  }
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    float pr[16], dm[16];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(lse + 32 * b + 8 * g + 4 * half);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pr[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[b][4 * g + e], p.scale2, kbias - a[e]));
+    for (int r = 0; r < 16; ++r) {
+      const int i = 8 * (r >> 2) + (r & 3);
+      s[r] = (FAR ? (sink && i > rh) : (i >= rl && i <= rh)) ? s[r] : -INFINITY;
     }
-    if (DROP) drop_of_key(dm, p, sh, row + 32 * b, j, half);
-    PFrag<T> pf, df;
-    {
-      float pd[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) pd[r] = DROP ? pr[r] * dm[r] : pr[r];
-      p_frag(pf, pd);
-    }
-    mma_cols<T, D>(st.dv, dt + b * BLK, at, pf, lane);
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 d = *reinterpret_cast<const f32x4*>(delta + 32 * b + 8 * g + 4 * half);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 4 * g + e;
-        pr[r] *= (DROP ? dp[b][r] * dm[r] : dp[b][r]) - d[e];
-      }
-    }
-    p_frag(df, pr);
-    mma_cols<T, D>(st.dk, qt + b * BLK, at, df, lane);
   }
+  float pr[16], dm[16], ls[16], de[16];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(lse + 8 * g + 4 * half), b = *reinterpret_cast<const f32x4*>(delta + 8 * g + 4 * half);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { ls[4 * g + e] = kbias - a[e]; de[4 * g + e] = b[e]; }
+  }
+  if (DROP) drop_of_key(dm, p, sh, row, j, half);
+  PFrag<T> pf, df;
+  ColFrag<T, D> dc, qc;
+  col_frag_lds<D>(dc, dt, at);
+  dp = mma_rows<D>(f2, st.vf, dp);
+  float pd[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) { pr[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, ls[r])); pd[r] = DROP ? pr[r] * dm[r] : pr[r]; }
+  p_frag(pf, pd);
+  col_frag_lds<D>(qc, qt, at);
+  mma_cols<D>(st.dv, dc, pf, lane);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) pr[r] *= (DROP ? dp[r] * dm[r] : dp[r]) - de[r];
+  p_frag(df, pr);
+  mma_cols<D>(st.dk, qc, df, lane);
 }
 
 // a wave's 32 keys into registers; hidden keys and keys past the end are zeros and carry a bias of -inf
@@ -351,7 +331,7 @@ __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, 
       if (see) {
         const char* qt = lds + buf * 2 * TILE + 32 * b * G::ROWB;
         const float* sp = stat + buf * 2 * QT + 32 * b;
-        query_blocks<T, D, 1, DROP, false>(st, qt, qt + TILE, sp, sp + QT, at, p, r0 + 32 * b, j, kbias, see == 1, lane, sh);
+        query_block<T, D, DROP, false>(st, qt, qt + TILE, sp, sp + QT, at, p, r0 + 32 * b, j, kbias, see == 1, lane, sh);
       }
     }
     if (more) rp.settle(stat + (buf ^ 1) * 2 * QT, tid);
@@ -396,7 +376,7 @@ __device__ __forceinline__ void sink_pass(const Params& p, char* lds, int id, in
     rp.deposit(qtile, dtile, stat, lane);
     if (i + 4 < i1) rp.fetch(p, (i + 4) / nt, (t0 + (i + 4) % nt) * 32, lane);
     wave_sync();
-    query_blocks<T, D, 1, DROP, true>(st, qtile, dtile, stat, stat + 32, at, p, r0, j, kbias, true, lane, (int64_t)b * p.H + hk * p.G + g);
+    query_block<T, D, DROP, true>(st, qtile, dtile, stat, stat + 32, at, p, r0, j, kbias, true, lane, (int64_t)b * p.H + hk * p.G + g);
     wave_sync();
   }
   // fold the four waves, dK then dV, in the order of the waves

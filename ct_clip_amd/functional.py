@@ -1259,14 +1259,16 @@ class RotaryPositions:
             f = f * (1.0 - ramp) + f / factor * ramp
             self.magnitude = float(attention) if attention is not None else 0.1 * math.log(factor) + 1.0
         self.frequencies = f
-        self._bits = [int(math.ldexp(t % 1.0, 64)) & (2 ** 64 - 1) for t in f / (2.0 * math.pi)]
+        turn = np.mod(f / (2.0 * math.pi), 1.0) * 2.0 ** 32          # (exact from here on: a 64-bit float has 53 bits, in two halves of 32)
+        high = np.floor(turn)
+        self.bits = (high.astype(np.uint64) << np.uint64(32)) | ((turn - high) * 2.0 ** 32).astype(np.uint64)
         self._turns = {}
 
     def turns(self, device):
         """(dim / 2) int64 tensor with the bits of the unsigned fractions, on the device (made once)."""
         t = self._turns.get(device)
         if t is None:
-            t = self._turns[device] = torch.tensor([b - 2 ** 64 if b >= 2 ** 63 else b for b in self._bits], dtype=torch.int64).to(device)
+            t = self._turns[device] = torch.from_numpy(self.bits.view(np.int64)).to(device)
         return t
 
 
@@ -1285,19 +1287,19 @@ def _not_twice():
 class RotaryFn(Function):
     @staticmethod
     def forward(ctx, q, k, rope, D, L, positions, start):
-        ctx.args = (rope, D, L, start, positions)           # (positions: integers, not differentiated, not an output)
-        qo, ko = B().rotary(q, k, rope.turns(q.device), D, rope.dim, L, positions, start, rope.interleaved, rope.magnitude)
+        turns = rope.turns(q.device)
+        ctx.args = (turns, D, rope.dim, L, positions, start, rope.interleaved, rope.magnitude)      # (positions: integers, not differentiated, not an output)
+        qo, ko = B().rotary(q, k, *ctx.args)
         return qo if k is None else (qo, ko)
 
     @staticmethod
     def backward(ctx, dq, dk=None):
         _not_twice()
-        rope, D, L, start, positions = ctx.args
         if dq.stride(1) != 1:
             dq = dq.contiguous()
         if dk is not None and dk.stride(1) != 1:
             dk = dk.contiguous()
-        gq, gk = B().rotary(dq, dk, rope.turns(dq.device), D, rope.dim, L, positions, start, rope.interleaved, rope.magnitude, True)
+        gq, gk = B().rotary(dq, dk, *ctx.args, True)
         return gq, gk, None, None, None, None, None
 
 

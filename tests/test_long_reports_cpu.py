@@ -65,7 +65,7 @@ def test_frequencies():
     r = Fn.RotaryPositions(64)
     want = 10000.0 ** (-np.arange(32) / 32)
     np.testing.assert_allclose(r.frequencies, want, rtol=1e-14)
-    np.testing.assert_allclose([b * 2.0 ** -64 * 2 * math.pi for b in r._bits], want, rtol=1e-14)
+    np.testing.assert_allclose([int(b) * 2.0 ** -64 * 2 * math.pi for b in r.bits], want, rtol=1e-14)
     assert r.magnitude == 1.0
     np.testing.assert_allclose(Fn.RotaryPositions(64, scaling=dict(type="linear", factor=4)).frequencies, want / 4, rtol=1e-14)
     n = Fn.RotaryPositions(64, scaling=dict(type="ntk", factor=4)).frequencies
@@ -76,7 +76,7 @@ def test_frequencies():
     assert np.all(np.diff(y.frequencies) < 0)
     assert Fn.RotaryPositions(64, scaling=dict(type="yarn", factor=8, original_length=512, attention_factor=2.0)).magnitude == 2.0
     t = r.turns(torch.device("cpu"))
-    assert t.dtype == torch.int64 and [int(x) % 2 ** 64 for x in t] == r._bits and r.turns(torch.device("cpu")) is t
+    assert t.dtype == torch.int64 and [int(x) % 2 ** 64 for x in t] == [int(b) for b in r.bits] and r.turns(torch.device("cpu")) is t
 
 
 @pytest.mark.parametrize("args,kw", [((3,), {}), ((0,), {}), ((64,), dict(layout="pairs")), ((64,), dict(base=1.0)), ((64,), dict(base=math.inf)),

@@ -113,9 +113,9 @@ SIGNATURES = {
     "ctclip_adam_step_zero_grad": (_I, [_P, _P, _P, _P, _L, _F, _F, _F, _F, _I, _F, _P, _P, _P]),
     "ctclip_rotary": (_I, [_P] * 6 + [_I] + [_L] * 3 + [_I] * 4 + [_L] * 4 + [_I, _F, _I, _I, _P]),
     "ctclip_win_attn_fwd_workspace": (_L, [_I] * 11),
-    "ctclip_win_attn_fwd": (_I, [_P] * 6 + [_I, _P, _P] + [_I] * 3 + [_L] * 2 + [_I] * 7 + [_L] * 4 + [_F, _F, _U64, _I, _P, _L, _P]),
+    "ctclip_win_attn_fwd": (_I, [_P] * 6 + [_I, _P, _P, _P] + [_I] * 3 + [_L] * 2 + [_I] * 7 + [_L] * 4 + [_F, _F, _U64, _I, _P, _L, _P]),
     "ctclip_win_attn_bwd_workspace": (_L, [_I] * 3 + [_L] + [_I] * 8),
-    "ctclip_win_attn_bwd": (_I, [_P] * 6 + [_I] + [_P] * 7 + [_I] * 3 + [_L] * 2 + [_I] * 7 + [_L] * 8 + [_F, _F, _U64, _I, _P, _L, _P]),
+    "ctclip_win_attn_bwd": (_I, [_P] * 6 + [_I] + [_P] * 8 + [_I] * 3 + [_L] * 2 + [_I] * 7 + [_L] * 8 + [_F, _F, _U64, _I, _P, _L, _P]),
     "ctclip_spin": (_I, [_L, _P]),
 }
 

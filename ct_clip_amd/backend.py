@@ -434,23 +434,24 @@ class HipBackend:
         return geo.workspaces
 
     def win_attn_fwd(self, q, k, v, keymask, geo, scale, want_lse=True, dropout=None):
-        """softmax(scale q k^T + keymask) v inside geo's window (functional.WindowGeometry; ctclip_win_attn_fwd) -> (o, lse).  Workspaces come from the caching
-        allocator per call: two captured graphs never share one."""
+        """softmax(scale q k^T + keymask) v inside geo's window (functional.WindowGeometry; ctclip_win_attn_fwd) -> (o, lse, o_lo): the last two for win_attn_bwd.
+        Workspaces come from the caching allocator per call: two captured graphs never share one."""
         dp, dseed = dropout if dropout is not None else (0.0, 0)
         dev, n = q.device, geo.H * geo.D
         with _on(q):
             o = q.new_zeros((geo.Mq, n)) if geo.uncovered else q.new_empty((geo.Mq, n))
             lse = torch.empty((geo.H, geo.Mq), dtype=torch.float32, device=dev) if want_lse else None
+            lo = q.new_empty((geo.Mq, n)) if want_lse and q.dtype == torch.bfloat16 else None
             need = self._win_workspaces(geo)[0]
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             off, tiles = geo.tables(dev) if geo.packed else (None, None)
-            rc = self.lib.ctclip_win_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), _p(keymask), _p(off), _p(tiles), geo.ntiles, o.data_ptr(), _p(lse), *geo.sizes,
+            rc = self.lib.ctclip_win_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), _p(keymask), _p(off), _p(tiles), geo.ntiles, o.data_ptr(), _p(lo), _p(lse), *geo.sizes,
                                               _rowmajor(q, "q"), _rowmajor(k, "k"), _rowmajor(v, "v"), n, scale, dp, dseed, dcode(q.dtype), _p(ws), need, _stream_of(q))
             if rc:
                 _lib.check(rc, "ctclip_win_attn_fwd")
-        return o, lse
+        return o, lse, lo
 
-    def win_attn_bwd(self, q, k, v, keymask, geo, scale, o, dout, lse, dropout=None, out=None):
+    def win_attn_bwd(self, q, k, v, keymask, geo, scale, o, dout, lse, o_lo=None, dropout=None, out=None):
         """-> (dq, dk, dv); out: row-strided tensors to write them to (packed rows outside every sequence are zeroed only in fresh ones)."""
         dp, dseed = dropout if dropout is not None else (0.0, 0)
         dev = q.device
@@ -465,7 +466,7 @@ class HipBackend:
             ws = torch.empty(need + 4 * geo.H * geo.Mq, dtype=torch.uint8, device=dev)       # partial sums, then Delta
             off, tiles = geo.tables(dev) if geo.packed else (None, None)
             at = ws.data_ptr()
-            rc = self.lib.ctclip_win_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), _p(keymask), _p(off), _p(tiles), geo.ntiles, o.data_ptr(), dout.data_ptr(),
+            rc = self.lib.ctclip_win_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), _p(keymask), _p(off), _p(tiles), geo.ntiles, o.data_ptr(), _p(o_lo), dout.data_ptr(),
                                               lse.data_ptr(), at + need, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *geo.sizes, _rowmajor(q, "q"), _rowmajor(k, "k"),
                                               _rowmajor(v, "v"), _rowmajor(o, "o"), _rowmajor(dout, "dout"), _rowmajor(dq, "dq"), _rowmajor(dk, "dk"), _rowmajor(dv, "dv"),
                                               scale, dp, dseed, dcode(q.dtype), at, need, _stream_of(q))

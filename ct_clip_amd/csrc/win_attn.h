@@ -24,6 +24,7 @@ struct Params {
   const int32_t* tiles;                   // packed sequences: (sequence, 128-row tile) of every tile
   int ntiles;
   void *out, *dq, *dk, *dv;
+  void* out_lo;                           // bf16: what the rounding of `out` left over (pitch ldo), for the backward pass's Delta; or null
   float *lse, *delta;                     // [H][query rows]: log2-domain log-sum-exp (+inf for a row that sees nothing), rowsum(dO o O)
   float* part;                            // workspace of split passes
   int nseq, Lq, Lk, H, Hk, G;
@@ -413,8 +414,8 @@ template <int KT> __device__ __host__ __forceinline__ TileList tile_list(int lo,
 }
 __device__ __forceinline__ int tile_at(const TileList& t, int i) { return i < t.nsink ? i : t.first + i - t.nsink; }
 
-// a lane's row of O: columns 32 i + 8 g + 4 h + e; four consecutive columns per store
-template <typename T, int D> __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[D / 32], float mul, int half) {
+// a lane's row of O: columns 32 i + 8 g + 4 h + e; four consecutive columns per store.  rest: also where the roundings' remainders go (bf16)
+template <typename T, int D> __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[D / 32], float mul, int half, T* rest = nullptr) {
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
@@ -422,10 +423,28 @@ template <typename T, int D> __device__ __forceinline__ void store_row(T* row, c
       float o[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = acc[i][4 * g + e] * mul;
-      store4(row + 32 * i + 8 * g + 4 * half, o);
+      const int at = 32 * i + 8 * g + 4 * half;
+      store4(row + at, o);
+      if constexpr (sizeof(T) == 2) {
+        if (rest) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] -= bf2f(f2bf(o[e]));
+          store4(rest + at, o);
+        }
+      }
     }
 }
-
+// four columns of a finished row of O
+template <typename T> __device__ __forceinline__ void store_out(const Params& p, int64_t row, int64_t col, float (&o)[4]) {
+  store4(reinterpret_cast<T*>(p.out) + row * p.ldo + col, o);
+  if constexpr (sizeof(T) == 2) {
+    if (p.out_lo) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] -= bf2f(f2bf(o[e]));
+      store4(reinterpret_cast<T*>(p.out_lo) + row * p.ldo + col, o);
+    }
+  }
+}
 // lanes of a wave exchange through LDS: its operations retire in order, so only the compiler has to keep them in place
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");

@@ -158,7 +158,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 4 : 2)) void fwd_
     if (half == 0) { p.part[r] = st.m; p.part[rows + r] = l; }
     return;
   }
-  store_row<T, D>(reinterpret_cast<T*>(p.out) + (rw.q0 + row) * p.ldo + (int64_t)h * D, st.acc, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), half);
+  const int64_t o = (rw.q0 + row) * p.ldo + (int64_t)h * D;
+  store_row<T, D>(reinterpret_cast<T*>(p.out) + o, st.acc, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), half, p.out_lo ? reinterpret_cast<T*>(p.out_lo) + o : nullptr);
   if (half == 0 && p.lse) p.lse[(int64_t)h * p.Mq + rw.q0 + row] = l == 0.f ? INFINITY : st.m + __builtin_amdgcn_logf(l);
 }
 
@@ -265,9 +266,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void row
     return;
   }
   const float mul = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
-  T* dst = reinterpret_cast<T*>(p.out) + (rw.q0 + orow) * p.ldo + (int64_t)oh * D + fc;
 #pragma unroll
-  for (int e = 0; e < PER; e += 4) { const float t[4] = {o[e] * mul, o[e + 1] * mul, o[e + 2] * mul, o[e + 3] * mul}; store4(dst + e, t); }
+  for (int e = 0; e < PER; e += 4) { float t[4] = {o[e] * mul, o[e + 1] * mul, o[e + 2] * mul, o[e + 3] * mul}; store_out<T>(p, rw.q0 + orow, (int64_t)oh * D + fc + e, t); }
   if ((tid & 7) == 0 && p.lse) p.lse[(int64_t)oh * p.Mq + rw.q0 + orow] = lsum == 0.f ? INFINITY : m + __builtin_amdgcn_logf(lsum);
 }
 
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
   const float mul = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] *= mul;
-  store4(reinterpret_cast<T*>(p.out) + row * p.ldo + h * D + col, o);
+  store_out<T>(p, row, h * D + col, o);
   if (col == 0 && p.lse) p.lse[i] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -387,7 +387,7 @@ extern "C" int64_t ctclip_win_attn_fwd_workspace(int nseq, int Lq, int Lk, int H
 // k | v; with offsets (nseq + 1, int32) the rows offsets[b] ... offsets[b + 1] - 1 of all three (Lq = Lk = the longest), tiles = (sequence, 128-row tile) pairs.
 // keymask: additive f32 per key row; a value <= -1e30 or NaN hides the key, whatever k and v hold there.
 extern "C" int ctclip_win_attn_fwd(const void* q, const void* k, const void* v, const float* keymask, const int32_t* offsets, const int32_t* tiles, int ntiles, void* out,
-                                   float* lse, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, int Hk, int D, int left, int right, int sinks, int q_start,
+                                   void* out_lo, float* lse, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, int Hk, int D, int left, int right, int sinks, int q_start,
                                    int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, float dropout_p, uint64_t dropout_seed, int dtype, void* workspace,
                                    int64_t workspace_bytes, hipStream_t stream) {
   using namespace win;
@@ -397,10 +397,11 @@ extern "C" int ctclip_win_attn_fwd(const void* q, const void* k, const void* v, 
   if (nseq == 0 || Lq == 0 || (offsets && ntiles == 0)) return CTCLIP_OK;
   if (offsets && (!tiles || ntiles < 0)) { ctclip_set_error("win_attn_fwd: packed sequences need their tiles"); return CTCLIP_EBADARG; }
   if ((rc = check_rows(q, ldq, H, D, dtype, false, "win_attn_fwd: q rows 16-byte aligned")) || (rc = check_rows(k, ldk, Hk, D, dtype, false, "win_attn_fwd: k rows 16-byte aligned")) ||
-      (rc = check_rows(v, ldv, Hk, D, dtype, false, "win_attn_fwd: v rows 16-byte aligned")) || (rc = check_rows(out, ldo, H, D, dtype, true, "win_attn_fwd: out rows 16-byte aligned, apart"))) return rc;
+      (rc = check_rows(v, ldv, Hk, D, dtype, false, "win_attn_fwd: v rows 16-byte aligned")) || (rc = check_rows(out, ldo, H, D, dtype, true, "win_attn_fwd: out rows 16-byte aligned, apart")) ||
+      (out_lo && (rc = check_rows(out_lo, ldo, H, D, dtype, true, "win_attn_fwd: out_lo rows 16-byte aligned")))) return rc;
   Params p{};
   fill(p, nseq, Lq, Lk, Mq, Mk, H, Hk, left, right, sinks, q_start, scale, dropout_p, dropout_seed, offsets, tiles, ntiles, keymask);
-  p.q = q; p.k = k; p.v = v; p.out = out; p.lse = lse; p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo;
+  p.q = q; p.k = k; p.v = v; p.out = out; p.out_lo = dtype == DT_BF16 ? out_lo : nullptr; p.lse = lse; p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo;
   const Plan pl = plan(nseq, Lq, Lk, H, Hk, p.left, p.right, p.sinks, q_start, offsets != nullptr);
   p.nsplit = pl.nsplit;
   if (p.nsplit > 1) {

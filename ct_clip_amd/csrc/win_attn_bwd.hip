@@ -41,7 +41,12 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
   {
     RowFrag<T, D> of;
     row_frag_global<T, D>(of, reinterpret_cast<const T*>(p.o) + (rw.q0 + row) * p.ldo + (int64_t)h * D, half);
-    delta = half_sum(row_dot<D>(of, df));
+    delta = row_dot<D>(of, df);
+    if (sizeof(T) == 2 && p.out_lo) {      // the O that the probabilities give, to 2^-17: with the rounded one alone its error is half of dS's (kernel-uniform)
+      row_frag_global<T, D>(of, reinterpret_cast<const T*>(p.out_lo) + (rw.q0 + row) * p.ldo + (int64_t)h * D, half);
+      delta += row_dot<D>(of, df);
+    }
+    delta = half_sum(delta);
   }
   float lse = p.lse[(int64_t)h * p.Mq + rw.q0 + row];
   row_frag_arrive<T, D>(qf);
@@ -550,7 +555,7 @@ extern "C" int64_t ctclip_win_attn_bwd_workspace(int nseq, int Lq, int Lk, int64
 
 // gradients of ctclip_win_attn_fwd: o, lse as it wrote them; delta: [H][Mq] f32 scratch; dq, dk, dv in the inputs' type, every row of a sequence written
 extern "C" int ctclip_win_attn_bwd(const void* q, const void* k, const void* v, const float* keymask, const int32_t* offsets, const int32_t* tiles, int ntiles, const void* o,
-                                   const void* dout, const float* lse, float* delta, void* dq, void* dk, void* dv, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H,
+                                   const void* o_lo, const void* dout, const float* lse, float* delta, void* dq, void* dk, void* dv, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H,
                                    int Hk, int D, int left, int right, int sinks, int q_start, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t lddo,
                                    int64_t lddq, int64_t lddk, int64_t lddv, float scale, float dropout_p, uint64_t dropout_seed, int dtype, void* workspace,
                                    int64_t workspace_bytes, hipStream_t stream) {
@@ -564,11 +569,12 @@ extern "C" int ctclip_win_attn_bwd(const void* q, const void* k, const void* v, 
   if (!lse || !delta) { ctclip_set_error("win_attn_bwd: needs lse and delta"); return CTCLIP_EBADARG; }
   if ((rc = check_rows(q, ldq, H, D, dtype, false, "win_attn_bwd: q rows 16-byte aligned")) || (rc = check_rows(k, ldk, Hk, D, dtype, false, "win_attn_bwd: k rows 16-byte aligned")) ||
       (rc = check_rows(v, ldv, Hk, D, dtype, false, "win_attn_bwd: v rows 16-byte aligned")) || (rc = check_rows(o, ldo, H, D, dtype, false, "win_attn_bwd: o rows 16-byte aligned")) ||
+      (o_lo && (rc = check_rows(o_lo, ldo, H, D, dtype, false, "win_attn_bwd: o_lo rows 16-byte aligned"))) ||
       (rc = check_rows(dout, lddo, H, D, dtype, false, "win_attn_bwd: dout rows 16-byte aligned")) || (rc = check_rows(dq, lddq, H, D, dtype, true, "win_attn_bwd: dq rows 16-byte aligned, apart")) ||
       (rc = check_rows(dk, lddk, Hk, D, dtype, true, "win_attn_bwd: dk rows 16-byte aligned, apart")) || (rc = check_rows(dv, lddv, Hk, D, dtype, true, "win_attn_bwd: dv rows 16-byte aligned, apart"))) return rc;
   Params p{};
   fill(p, nseq, Lq, Lk, Mq, Mk, H, Hk, left, right, sinks, q_start, scale, dropout_p, dropout_seed, offsets, tiles, ntiles, keymask);
-  p.q = q; p.k = k; p.v = v; p.o = o; p.dout = dout; p.lse = const_cast<float*>(lse); p.delta = delta; p.dq = dq; p.dk = dk; p.dv = dv;
+  p.q = q; p.k = k; p.v = v; p.o = o; p.out_lo = dtype == DT_BF16 ? const_cast<void*>(o_lo) : nullptr; p.dout = dout; p.lse = const_cast<float*>(lse); p.delta = delta; p.dq = dq; p.dk = dk; p.dv = dv;
   p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo; p.lddo = lddo; p.lddq = lddq; p.lddk = lddk; p.lddv = lddv;
   const BwdPlan b = bwd_plan(nseq, Lq, Lk, H, Hk, p.left, p.right, p.sinks, q_start, offsets ? ntiles : 0);
   p.nsplit = b.nsplit; p.s32 = b.s32; p.nchunk = b.nchunk;

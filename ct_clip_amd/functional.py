@@ -1200,7 +1200,7 @@ class SdpaFn(Function):
     @staticmethod
     def backward(ctx, do):
         be = B()
-        q, k, v, o, lse, keymask = ctx.saved_tensors
+        q, k, v, o, lse, lo, keymask = ctx.saved_tensors
         nseq, L, H, D, scale, has_mask, dropout = ctx.dims
         do = do.contiguous()
         qt = be.head_transpose(q, nseq, H, L, D)
@@ -1419,8 +1419,8 @@ class WindowAttnFn(Function):
         if geo.empty:
             ctx.save_for_backward(q, k, v)
             return q.new_zeros((geo.Mq, geo.H * geo.D))
-        o, lse = B().win_attn_fwd(q, k, v, keymask, geo, scale, True, dropout)
-        ctx.save_for_backward(q, k, v, o, lse, keymask)
+        o, lse, lo = B().win_attn_fwd(q, k, v, keymask, geo, scale, True, dropout)
+        ctx.save_for_backward(q, k, v, o, lse, lo, keymask)
         return o
 
     @staticmethod
@@ -1429,8 +1429,8 @@ class WindowAttnFn(Function):
         geo, scale, dropout = ctx.args
         if geo.empty:
             return (*(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in ctx.saved_tensors), None, None, None, None)
-        q, k, v, o, lse, keymask = ctx.saved_tensors
-        dq, dk, dv = B().win_attn_bwd(q, k, v, keymask, geo, scale, o, _aligned_rows(do), lse, dropout)
+        q, k, v, o, lse, lo, keymask = ctx.saved_tensors
+        dq, dk, dv = B().win_attn_bwd(q, k, v, keymask, geo, scale, o, _aligned_rows(do), lse, lo, dropout)
         return dq, dk, dv, None, None, None, None
 
 
@@ -1591,10 +1591,10 @@ class QkvWindowFn(Function):
             be.rotary(q, k, rope.turns(x.device), D, rope.dim, L, None, 0, rope.interleaved, rope.magnitude, out=(q, k))
         q, k, v = QkvWindowFn._views(qkv, N, nseq, L, first_only)
         geo = window_geometry(q.shape[0], k.shape[0], H, H, D, nseq, window, sinks, 0)
-        o, lse = be.win_attn_fwd(q, k, v, keymask, geo, scale, want_lse=any(ctx.needs_input_grad[:7]), dropout=dropout)
+        o, lse, lo = be.win_attn_fwd(q, k, v, keymask, geo, scale, want_lse=any(ctx.needs_input_grad[:7]), dropout=dropout)
         ctx.wt = _qkv_transposed_shadow(x, wq, wk, wv) if ctx.needs_input_grad[0] else None
         if lse is not None:
-            ctx.save_for_backward(x, wsh, qkv, o, lse, *([keymask] if keymask is not None else []))
+            ctx.save_for_backward(x, wsh, qkv, o, lse, lo, keymask)
         ctx.params = (wq, wk, wv, bq, bk, bv)
         ctx.args = (geo, scale, dropout, rope, nseq, L, N, D, first_only)
         if passthrough:
@@ -1610,13 +1610,13 @@ class QkvWindowFn(Function):
     def backward(ctx, do, d_pass=None):
         _not_twice()
         be = B()
-        x, wsh, qkv, o, lse, *mask = ctx.saved_tensors
+        x, wsh, qkv, o, lse, lo, keymask = ctx.saved_tensors
         geo, scale, dropout, rope, nseq, L, N, D, first_only = ctx.args
         d_pass = d_pass.contiguous() if (ctx.passthrough and d_pass is not None) else None
         dqkv = torch.empty_like(qkv)
         if first_only:
             dqkv[:, :N].zero_()                # rows that attended to nothing
-        be.win_attn_bwd(*QkvWindowFn._views(qkv, N, nseq, L, first_only), mask[0] if mask else None, geo, scale, o, _aligned_rows(do), lse, dropout=dropout,
+        be.win_attn_bwd(*QkvWindowFn._views(qkv, N, nseq, L, first_only), keymask, geo, scale, o, _aligned_rows(do), lse, lo, dropout=dropout,
                         out=QkvWindowFn._views(dqkv, N, nseq, L, first_only))
         if rope is not None:
             dq, dk = dqkv[:, :N], dqkv[:, N:2 * N]

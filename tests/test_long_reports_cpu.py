@@ -40,9 +40,9 @@ class RefOps(RefBackend):
 
     def win_attn_fwd(self, q, k, v, keymask, geo, scale, want_lse=True, dropout=None):
         keymask = keymask.reshape(-1) if keymask is not None else None
-        return self._run(q, k, v, keymask, geo, scale, dropout)["o"][0].to(q.dtype), torch.zeros(geo.H, geo.Mq) if want_lse else None
+        return self._run(q, k, v, keymask, geo, scale, dropout)["o"][0].to(q.dtype), torch.zeros(geo.H, geo.Mq) if want_lse else None, None
 
-    def win_attn_bwd(self, q, k, v, keymask, geo, scale, o, dout, lse, dropout=None, out=None):
+    def win_attn_bwd(self, q, k, v, keymask, geo, scale, o, dout, lse, o_lo=None, dropout=None, out=None):
         r = self._run(q, k, v, keymask.reshape(-1) if keymask is not None else None, geo, scale, dropout, dout)
         new = [r[n][0].to(q.dtype) for n in ("dq", "dk", "dv")]
         if out is None:
@@ -144,7 +144,7 @@ def test_c_entries_answer_before_any_launch():
 
     def fwd(q=p, k=p, v=p, off=None, tiles=None, nt=0, out=p, nseq=2, Lq=8, Lk=8, Mq=16, Mk=16, H=2, Hk=1, D=64, left=4, right=4, sinks=1, q0=0, ldq=128, ldk=64, ldv=64, ldo=128,
             scale=1.0, drop=0.0, dt=1, ws=None, n=0):
-        return lib.ctclip_win_attn_fwd(q, k, v, None, off, tiles, nt, out, None, nseq, Lq, Lk, Mq, Mk, H, Hk, D, left, right, sinks, q0, ldq, ldk, ldv, ldo, scale, drop, 0, dt, ws, n, None)
+        return lib.ctclip_win_attn_fwd(q, k, v, None, off, tiles, nt, out, None, None, nseq, Lq, Lk, Mq, Mk, H, Hk, D, left, right, sinks, q0, ldq, ldk, ldv, ldo, scale, drop, 0, dt, ws, n, None)
     assert fwd(q=None) == fwd(k=None) == fwd(v=None) == fwd(out=None) == fwd(q=p + 2) == fwd(ldk=65) == fwd(ldo=120) == -1
     assert fwd(H=3, Hk=2) == fwd(left=-2) == fwd(sinks=-1) == fwd(q0=1) == fwd(Mq=17) == fwd(Lq=9, Mq=18) == fwd(scale=0.0) == fwd(scale=-1.0) == fwd(drop=1.0) == -1
     assert fwd(scale=math.nan) == fwd(drop=math.nan) == fwd(off=p, Mq=16, nt=2) == fwd(off=p, tiles=p, nt=2, Mk=15) == -1
@@ -154,7 +154,7 @@ def test_c_entries_answer_before_any_launch():
 
     def bwd(q=p, lse=p, delta=p, dq=p, ldq=128, lddq=128, nseq=2, L=8, left=4, sinks=0, ws=None, n=0, dt=1, D=64, scale=1.0):
         M = nseq * L
-        return lib.ctclip_win_attn_bwd(q, p, p, None, None, None, 0, p, p, lse, delta, dq, p, p, nseq, L, L, M, M, 2, 1, D, left, 0, sinks, 0, ldq, 64, 64, 128, 128, lddq, 64, 64,
+        return lib.ctclip_win_attn_bwd(q, p, p, None, None, None, 0, p, None, p, lse, delta, dq, p, p, nseq, L, L, M, M, 2, 1, D, left, 0, sinks, 0, ldq, 64, 64, 128, 128, lddq, 64, 64,
                                        scale, 0.0, 0, dt, ws, n, None)
     assert bwd(q=None) == bwd(lse=None) == bwd(delta=None) == bwd(dq=None) == bwd(dq=p + 8) == bwd(lddq=64) == bwd(scale=0.0) == -1
     assert bwd(D=96) == bwd(dt=3) == -2

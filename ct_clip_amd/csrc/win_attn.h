@@ -414,25 +414,39 @@ template <int KT> __device__ __host__ __forceinline__ TileList tile_list(int lo,
 }
 __device__ __forceinline__ int tile_at(const TileList& t, int i) { return i < t.nsink ? i : t.first + i - t.nsink; }
 
-// a lane's row of O: columns 32 i + 8 g + 4 h + e; four consecutive columns per store.  rest: also where the roundings' remainders go (bf16)
-template <typename T, int D> __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[D / 32], float mul, int half, T* rest = nullptr) {
+// a lane's row: columns 32 i + 8 g + 4 h + e; four consecutive columns per store (partial sums)
+template <int D> __device__ __forceinline__ void store_part(float* row, const f32x16 (&acc)[D / 32], int half) {
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) *reinterpret_cast<f32x4*>(row + 32 * i + 8 * g + 4 * half) = f32x4{acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]};
+}
+__device__ __forceinline__ void wave_sync();
+// A wave's 32 rows to memory, by way of 32 * ROWB bytes of LDS that nobody else touches: a lane holds four columns of one row at a time, and stored from there an
+// instruction would touch 32 lines for 16 bytes each; after the turn it writes whole lines.  lane c = lane & 31 is row c; rows from `n` on are not stored.
+// REST: what the rounding of the values leaves over, instead of the values (bf16)
+template <typename T, int D, bool REST> __device__ __forceinline__ void store_rows(char* lds, const f32x16 (&acc)[D / 32], float mul, T* first, int64_t ld, int n, int lane) {
+  const int half = lane >> 5, c = lane & 31;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       float o[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = acc[i][4 * g + e] * mul;
-      const int at = 32 * i + 8 * g + 4 * half;
-      store4(row + at, o);
-      if constexpr (sizeof(T) == 2) {
-        if (rest) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] -= bf2f(f2bf(o[e]));
-          store4(rest + at, o);
-        }
+      for (int e = 0; e < 4; ++e) {
+        o[e] = acc[i][4 * g + e] * mul;
+        if (REST && sizeof(T) == 2) o[e] -= bf2f(f2bf(o[e]));
       }
+      store4(reinterpret_cast<T*>(lds + lds_at<T, D>(c, sizeof(T) == 2 ? 4 * i + g : 8 * i + 2 * g + half) + (sizeof(T) == 2 ? 8 * half : 0)), o);
     }
+  wave_sync();
+#pragma unroll
+  for (int k = 0; k < 32 * Geo<T, D>::NCH / 64; ++k) {
+    const int r = (lane + 64 * k) / Geo<T, D>::NCH, ch = (lane + 64 * k) % Geo<T, D>::NCH;
+    const u32x4 w = *reinterpret_cast<const u32x4*>(lds + lds_at<T, D>(r, ch));
+    if (r < n) *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(first + (int64_t)r * ld) + ch * 16) = w;
+  }
+  wave_sync();
 }
 // four columns of a finished row of O
 template <typename T> __device__ __forceinline__ void store_out(const Params& p, int64_t row, int64_t col, float (&o)[4]) {

@@ -150,16 +150,21 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 4 : 2)) void fwd_
     __syncthreads();
   }
   const float l = half_sum(st.l);
-  if (!real) return;
   if (p.nsplit > 1) {
+    if (!real) return;
     const int64_t r = ((int64_t)blockIdx.y * p.H + h) * p.Mq + rw.q0 + row;
     const int64_t rows = (int64_t)p.nsplit * p.H * p.Mq;
-    store_row<float, D>(p.part + 2 * rows + r * D, st.acc, 1.f, half);
+    store_part<D>(p.part + 2 * rows + r * D, st.acc, half);
     if (half == 0) { p.part[r] = st.m; p.part[rows + r] = l; }
     return;
   }
-  const int64_t o = (rw.q0 + row) * p.ldo + (int64_t)h * D;
-  store_row<T, D>(reinterpret_cast<T*>(p.out) + o, st.acc, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), half, p.out_lo ? reinterpret_cast<T*>(p.out_lo) + o : nullptr);
+  // (everybody is behind the last barrier: the tiles' space is free)
+  const int wr = q0 + 32 * wave;
+  const int64_t o = (rw.q0 + wr) * p.ldo + (int64_t)h * D;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  store_rows<T, D, false>(lds + wave * 32 * G::ROWB, st.acc, inv, reinterpret_cast<T*>(p.out) + o, p.ldo, rw.lq - wr, lane);
+  if (sizeof(T) == 2 && p.out_lo) store_rows<T, D, true>(lds + wave * 32 * G::ROWB, st.acc, inv, reinterpret_cast<T*>(p.out_lo) + o, p.ldo, rw.lq - wr, lane);
+  if (!real) return;
   if (half == 0 && p.lse) p.lse[(int64_t)h * p.Mq + rw.q0 + row] = l == 0.f ? INFINITY : st.m + __builtin_amdgcn_logf(l);
 }
 

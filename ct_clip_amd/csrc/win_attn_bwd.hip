@@ -125,7 +125,8 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
     if (more) state = kp.settle(next, next + TILE, kb + (buf ^ 1) * KT, tid);
     __syncthreads();
   }
-  if (real) store_row<T, D>(reinterpret_cast<T*>(p.dq) + (rw.q0 + row) * p.lddq + (int64_t)h * D, acc, p.scale, half);
+  const int wr = q0 + 32 * wave;           // (everybody is behind the last barrier: the tiles' space is free)
+  store_rows<T, D, false>(lds + wave * 32 * G::ROWB, acc, p.scale, reinterpret_cast<T*>(p.dq) + (rw.q0 + wr) * p.lddq + (int64_t)h * D, p.lddq, rw.lq - wr, lane);
 }
 
 // 32 staged queries against the 32 keys of a wave
@@ -342,15 +343,16 @@ __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, 
     if (more) rp.settle(stat + (buf ^ 1) * 2 * QT, tid);
     __syncthreads();
   }
-  if (j >= rw.lk) return;
   if (p.nsplit > 1 || jw < p.s32) {
+    if (j >= rw.lk) return;
     const int64_t N = part_rows(p), r = (int64_t)split * N + part_row(p, rw, u.b, u.hk, j);
-    store_row<float, D>(p.part + r * D, st.dk, 1.f, half);
-    store_row<float, D>(p.part + ((int64_t)p.nsplit * N + r) * D, st.dv, 1.f, half);
+    store_part<D>(p.part + r * D, st.dk, half);
+    store_part<D>(p.part + ((int64_t)p.nsplit * N + r) * D, st.dv, half);
     return;
   }
-  store_row<T, D>(reinterpret_cast<T*>(p.dk) + (rw.k0 + j) * p.lddk + (int64_t)u.hk * D, st.dk, p.scale, half);
-  store_row<T, D>(reinterpret_cast<T*>(p.dv) + (rw.k0 + j) * p.lddv + (int64_t)u.hk * D, st.dv, 1.f, half);
+  char* turn = lds + wave * 32 * G::ROWB;
+  store_rows<T, D, false>(turn, st.dk, p.scale, reinterpret_cast<T*>(p.dk) + (rw.k0 + jw) * p.lddk + (int64_t)u.hk * D, p.lddk, rw.lk - jw, lane);
+  store_rows<T, D, false>(turn, st.dv, 1.f, reinterpret_cast<T*>(p.dv) + (rw.k0 + jw) * p.lddv + (int64_t)u.hk * D, p.lddv, rw.lk - jw, lane);
 }
 
 template <typename T, int D, bool DROP>

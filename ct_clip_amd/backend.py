@@ -37,6 +37,8 @@ _HERE = contextlib.nullcontext()
 
 def _on(t):
     """Launches for tensors of another device than the current one happen there (its current stream, its allocator)."""
+    if not t.is_cuda:
+        raise TypeError(f"the HIP kernels take tensors on the GPU, got one on {t.device}")
     return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 

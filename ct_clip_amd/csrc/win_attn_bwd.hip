@@ -434,52 +434,55 @@ template <typename T, int D, int PG>
 __global__ __launch_bounds__(256) void dkv_reduce_kernel(Params p, int keys) {
   constexpr int C = D / 4, KEYS = 256 / C / PG;
   __shared__ __attribute__((aligned(16))) float fold[2][PG][KEYS][D];
-  const int b = blockIdx.z, hk = blockIdx.y;
-  const Rows rw = rows_of(p, b);
+  const int hk = blockIdx.y;
   const int col = (threadIdx.x % C) * 4, key = threadIdx.x / C % KEYS, pg = threadIdx.x / C / KEYS;
   const int j = blockIdx.x * KEYS + key;
-  const bool on = j < keys && j < rw.lk;
-  const int64_t N = part_rows(p), S = sink_rows(p), r = part_row(p, rw, b, hk, j);
-  const float* sink = p.part + 2 * p.nsplit * N * D;
-  const int parts = p.nsplit + (j < p.s32 ? p.nchunk : 0);
+  for (int b = blockIdx.z; b < p.nseq; b += gridDim.z) {
+    const Rows rw = rows_of(p, b);
+    const bool on = j < keys && j < rw.lk;
+    const int64_t N = part_rows(p), S = sink_rows(p), r = part_row(p, rw, b, hk, j);
+    const float* sink = p.part + 2 * p.nsplit * N * D;
+    const int parts = p.nsplit + (j < p.s32 ? p.nchunk : 0);
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    float o[4] = {0.f, 0.f, 0.f, 0.f};
-    if (on)
-      for (int s = pg; s < parts; s += PG) {
-        const float* src = s < p.nsplit ? p.part + (((int64_t)which * p.nsplit + s) * N + r) * D
-                                        : sink + (((int64_t)which * p.nchunk + s - p.nsplit) * S + ((int64_t)b * p.Hk + hk) * p.s32 + j) * D;
+    for (int which = 0; which < 2; ++which) {
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
+      if (on)
+        for (int s = pg; s < parts; s += PG) {
+          const float* src = s < p.nsplit ? p.part + (((int64_t)which * p.nsplit + s) * N + r) * D
+                                          : sink + (((int64_t)which * p.nchunk + s - p.nsplit) * S + ((int64_t)b * p.Hk + hk) * p.s32 + j) * D;
+          float a[4];
+          load4(src + col, a);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] += a[e];
+        }
+      if (PG > 1) {
+        store4(&fold[which][pg][key][col], o);
+      } else if (on) {
+        const float mul = which ? 1.f : p.scale;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= mul;
+        store4((which ? reinterpret_cast<T*>(p.dv) + (rw.k0 + j) * p.lddv : reinterpret_cast<T*>(p.dk) + (rw.k0 + j) * p.lddk) + (int64_t)hk * D + col, o);
+      }
+    }
+    if (PG == 1) continue;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * KEYS * C; i += 256) {          // (with PG = 16: at most one round)
+      const int which = i / (KEYS * C), k = i / C % KEYS, cc = (i % C) * 4, jj = blockIdx.x * KEYS + k;
+      if (jj >= keys || jj >= rw.lk) continue;
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int g = 0; g < PG; ++g) {
         float a[4];
-        load4(src + col, a);
+        load4(&fold[which][g][k][cc], a);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += a[e];
       }
-    if (PG > 1) {
-      store4(&fold[which][pg][key][col], o);
-    } else if (on) {
       const float mul = which ? 1.f : p.scale;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] *= mul;
-      store4((which ? reinterpret_cast<T*>(p.dv) + (rw.k0 + j) * p.lddv : reinterpret_cast<T*>(p.dk) + (rw.k0 + j) * p.lddk) + (int64_t)hk * D + col, o);
+      store4((which ? reinterpret_cast<T*>(p.dv) + (rw.k0 + jj) * p.lddv : reinterpret_cast<T*>(p.dk) + (rw.k0 + jj) * p.lddk) + (int64_t)hk * D + cc, o);
     }
-  }
-  if (PG == 1) return;
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * KEYS * C; i += 256) {          // (with PG = 16: at most one round)
-    const int which = i / (KEYS * C), k = i / C % KEYS, cc = (i % C) * 4, jj = blockIdx.x * KEYS + k;
-    if (jj >= keys || jj >= rw.lk) continue;
-    float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < PG; ++g) {
-      float a[4];
-      load4(&fold[which][g][k][cc], a);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += a[e];
-    }
-    const float mul = which ? 1.f : p.scale;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] *= mul;
-    store4((which ? reinterpret_cast<T*>(p.dv) + (rw.k0 + jj) * p.lddv : reinterpret_cast<T*>(p.dk) + (rw.k0 + jj) * p.lddk) + (int64_t)hk * D + cc, o);
+    __syncthreads();                       // (the next sequence's parts go to the same place)
   }
 }
 
@@ -537,9 +540,10 @@ template <typename T, int D, bool DROP> int launch_bwd(Params& p, hipStream_t s)
   }
   const int keys = p.nsplit > 1 ? p.Lk : p.s32;
   if (!keys) return CTCLIP_OK;
+  const unsigned nz = p.nseq < 32768 ? p.nseq : 32768;
   constexpr int PG = 256 / (D / 4) < 16 ? 256 / (D / 4) : 16;      // threads across the parts where the sinks' chunks are many
-  if (p.nsplit + p.nchunk > 8) hipLaunchKernelGGL((dkv_reduce_kernel<T, D, PG>), dim3((unsigned)cdiv(keys, 256 / (D / 4) / PG), p.Hk, p.nseq), dim3(256), 0, s, p, keys);
-  else hipLaunchKernelGGL((dkv_reduce_kernel<T, D, 1>), dim3((unsigned)cdiv(keys, 256 / (D / 4)), p.Hk, p.nseq), dim3(256), 0, s, p, keys);
+  if (p.nsplit + p.nchunk > 8) hipLaunchKernelGGL((dkv_reduce_kernel<T, D, PG>), dim3((unsigned)cdiv(keys, 256 / (D / 4) / PG), p.Hk, nz), dim3(256), 0, s, p, keys);
+  else hipLaunchKernelGGL((dkv_reduce_kernel<T, D, 1>), dim3((unsigned)cdiv(keys, 256 / (D / 4)), p.Hk, nz), dim3(256), 0, s, p, keys);
   return ctclip_check_launch("win_attn_bwd reduce");
 }
 template <typename T, int D> int launch_bwd_d(Params& p, hipStream_t s) { return p.drop_p > 0.f ? launch_bwd<T, D, true>(p, s) : launch_bwd<T, D, false>(p, s); }
@@ -567,7 +571,6 @@ extern "C" int ctclip_win_attn_bwd(const void* q, const void* k, const void* v, 
   if (!(scale > 0.f) || !(scale < 1e30f) || !(dropout_p >= 0.f) || !(dropout_p < 1.f)) { ctclip_set_error("win_attn_bwd: scale > 0, 0 <= dropout < 1"); return CTCLIP_EBADARG; }
   if (nseq == 0 || Lk == 0 || Lq == 0 || (offsets && ntiles == 0)) return CTCLIP_OK;
   if (offsets && (!tiles || ntiles < 0)) { ctclip_set_error("win_attn_bwd: packed sequences need their tiles"); return CTCLIP_EBADARG; }
-  if (Hk > 65535 || nseq > 65535) { ctclip_set_error("win_attn_bwd: more than 65535 sequences or heads"); return CTCLIP_EUNSUPPORTED; }
   if (!lse || !delta) { ctclip_set_error("win_attn_bwd: needs lse and delta"); return CTCLIP_EBADARG; }
   if ((rc = check_rows(q, ldq, H, D, dtype, false, "win_attn_bwd: q rows 16-byte aligned")) || (rc = check_rows(k, ldk, Hk, D, dtype, false, "win_attn_bwd: k rows 16-byte aligned")) ||
       (rc = check_rows(v, ldv, Hk, D, dtype, false, "win_attn_bwd: v rows 16-byte aligned")) || (rc = check_rows(o, ldo, H, D, dtype, false, "win_attn_bwd: o rows 16-byte aligned")) ||

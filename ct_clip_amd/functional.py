@@ -1400,7 +1400,7 @@ _equal_sequences = functools.lru_cache(maxsize=512)(WindowGeometry)
 
 def window_geometry(Mq, Mk, H, Hk, D, nseq, window, sinks, q_start):
     """The (kept) ``WindowGeometry`` of these sizes: with the table of a number of equal sequences, or with the packed sequences themselves."""
-    left, right = (window, window) if isinstance(window, int) else window
+    left, right = window if isinstance(window, (tuple, list)) else (window, window)
     key = (Mq, Mk, H, Hk, D, int(left), int(right), int(sinks), int(q_start))
     if not isinstance(nseq, PackedSequences):
         return _equal_sequences(*key[:5], int(nseq), *key[5:])

@@ -136,7 +136,7 @@ def run_case(dtype, nseq, Lq, Lk, H, Hk, D, window, sinks, q_start=0, mask=None,
             spans.append((at, n, at, n))
             at += n
         nseq = Fn.PackedSequences(lengths, first=first)
-        keymask = None
+        keymask = make_mask(mask, 1, M, seed + 7)
     else:
         Mq, Mk = nseq * Lq, nseq * Lk
         spans = [(b * Lq, Lq, b * Lk, Lk) for b in range(nseq)]
@@ -230,6 +230,81 @@ PACKED = [  # lengths, first, tail, H, Hk, D, window, sinks
 @pytest.mark.parametrize("lengths,first,tail,H,Hk,D,window,sinks", PACKED)
 def test_window_attention_packed_sequences(lengths, first, tail, H, Hk, D, window, sinks, dtype):
     run_case(dtype, None, None, None, H, Hk, D, window, sinks, lengths=lengths, first=first, tail=tail, seed=sum(lengths))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("mask,drop", [("holes", None), ("front", None), (None, (0.2, 77)), ("holes", (0.1, 99))])
+def test_window_attention_packed_sequences_with_mask_and_dropout(mask, drop, dtype):
+    run_case(dtype, None, None, None, 4, 2, 64, (20, 10), 3, lengths=[5, 0, 70, 1, 200], first=1, tail=3, mask=mask, drop=drop, seed=3)
+
+
+def test_window_attention_many_short_sequences():
+    """More sequences than a grid's z axis has room for."""
+    n = 70000
+    q, k, v, g = (rnd((n * 3, 32), BF16, 60 + i) for i in range(4))
+    q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+    o = Fn.window_attention(q, k, v, 1, 32, nseq=n, window=(0, 0), sinks=1)
+    got = torch.autograd.grad(o, (q, k, v), g)
+    at = slice(3 * (n - 5), 3 * n)        # the last five, by themselves
+    q2, k2, v2 = (t.detach()[at].clone().requires_grad_(True) for t in (q, k, v))
+    o2 = Fn.window_attention(q2, k2, v2, 1, 32, nseq=5, window=(0, 0), sinks=1)
+    spans = [(3 * b, 3, 3 * b, 3) for b in range(5)]
+    want = O.batch64(q2.detach(), k2.detach(), v2.detach(), 1, 1, 32, spans, 0, 0, 1, 0, None, 32 ** -0.5, g[at], dtype=BF16)
+    O.check(o.detach()[at], want["o"], "o")
+    O.check(o2.detach(), want["o"], "o of the five")
+    for name, x in zip(("dq", "dk", "dv"), got):
+        O.check(x[at], want[name], name)
+
+
+@pytest.mark.parametrize("Lq", [1, 200])
+def test_window_attention_offsets_beyond_32_bits(Lq):
+    """Key rows 4 KB apart, 1.1 million of them: the last window lies 4.5 GB behind the sinks."""
+    Lk, H, D, left, sinks = 1100000, 2, 64, 90, 4
+    buf = torch.zeros((Lk, 2048), dtype=BF16, device=DEV)
+    near = torch.cat([torch.arange(sinks), torch.arange(Lk - Lq - left, Lk)]).to(DEV)
+    buf[near, :2 * H * D] = rnd((len(near), 2 * H * D), BF16, 5)
+    k, v = buf[:, :H * D].requires_grad_(True), buf[:, H * D:2 * H * D].requires_grad_(True)
+    q = rnd((Lq, H * D), BF16, 6).requires_grad_(True)
+    g = rnd((Lq, H * D), BF16, 7)
+    o = Fn.window_attention(q, k, v, H, D, window=(left, 0), sinks=sinks, q_start=Lk - Lq)
+    got = torch.autograd.grad(o, (q, k, v), g)
+    # the same rows without what lies between: positions shift, the sinks stay in front of every window
+    n = len(near)
+    want = O.batch64(q.detach(), k.detach()[near], v.detach()[near], H, H, D, [(0, Lq, 0, n)], left, 0, sinks, n - Lq, None, D ** -0.5, g, dtype=BF16)
+    O.check(o.detach(), want["o"], "o")
+    O.check(got[0], want["dq"], "dq")
+    for name, x in zip(("dk", "dv"), got[1:]):
+        O.check(x[near], want[name], name)
+        assert not x[sinks:Lk - Lq - left].any()
+
+
+def test_window_attention_on_two_streams_at_once():
+    """Calls that split the key axis, running at the same time on two streams, have a workspace each."""
+    q, k, v = rnd((1, 256), BF16, 1), rnd((20000, 256), BF16, 2), rnd((20000, 256), BF16, 3)
+    calls = [dict(window=(-1, 0), q_start=19999), dict(window=(9000, 0), q_start=12000)]
+    want = [Fn.window_attention(q, k, v, 4, 64, **c) for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[], []]
+    for _ in range(5):
+        for i, (st, c) in enumerate(zip(streams, calls)):
+            with torch.cuda.stream(st):
+                got[i].append(Fn.window_attention(q, k, v, 4, 64, **c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+
+
+def test_the_backend_refuses_tensors_of_the_cpu():
+    with pytest.raises(TypeError, match="on the GPU"):
+        Fn.window_attention(torch.zeros(4, 64), torch.zeros(4, 64), torch.zeros(4, 64), 1, 64)
+    with pytest.raises(TypeError, match="on the GPU"):
+        Fn.rotary(torch.zeros(4, 64), None, Fn.RotaryPositions(64), 64)
+
+
+def test_no_derivative_of_the_gradient():
+    q = rnd((8, 64), F32, 1).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(Fn.window_attention(q, q, q, 1, 64, window=2).sum(), q, create_graph=True)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -81,7 +81,7 @@ template <int D> __device__ __forceinline__ f32x16 mma_rows(const RowFrag<float,
   return c;
 }
 // Wait for a fragment HERE.  Left to itself the compiler waits in front of the first product of a loop, in every round of it (it cannot count the loads of the first
-// round), and so for the next tile's loads too, which were to arrive under the products: 150 -> 73 us for 4 x 8192 tokens, 12 heads of 64, window 512.
+// round), and so for the loads of the next round too, which are to arrive under the products.
 template <typename T, int D> __device__ __forceinline__ void row_frag_arrive(RowFrag<T, D>& f) {
 #pragma unroll
   for (int g = 0; g < Geo<T, D>::NCH / 2; ++g) {
@@ -193,41 +193,14 @@ template <typename T, int D> __device__ __forceinline__ void mma_cols(f32x16 (&a
   mma_cols<D>(acc, f, p, lane);
 }
 
-// ---- a tile's journey from memory through registers to LDS: ROWS rows of D elements by NT threads
-template <typename T, int D, int ROWS, int NT> struct Stage {
-  static constexpr int N = ROWS * Geo<T, D>::NCH / NT;     // 16-byte chunks per thread
-  static_assert(N >= 1 && ROWS * Geo<T, D>::NCH % NT == 0, "whole chunks per thread");
-  u32x4 w[N];
-  __device__ static __forceinline__ int row(int tid, int i) { return (tid + i * NT) / Geo<T, D>::NCH; }
-  __device__ static __forceinline__ int chunk(int tid, int i) { return (tid + i * NT) % Geo<T, D>::NCH; }
-  // tile = row 0 of the tile (uniform), ldb = bytes between rows (below 2^24: 24-bit products); rows past `last` >= 0 are read from row `last`, and zeroed by put()
-  __device__ __forceinline__ void get(const char* tile, int ldb, int last, int tid) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = row(tid, i) < last ? row(tid, i) : last;
-      w[i] = *reinterpret_cast<const u32x4*>(tile + ((uint32_t)__mul24(r, ldb) + (uint32_t)(chunk(tid, i) * 16)));
-    }
-  }
-  __device__ __forceinline__ void put(char* tile, int tid) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(tile + lds_at<T, D>(row(tid, i), chunk(tid, i))) = w[i];
-  }
-  // keep: bit r = row r of the tile may be seen (a hidden row is stored as zeros: whatever it holds, NaN included, never meets a product)
-  __device__ __forceinline__ void put(char* tile, uint64_t keep, int tid) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const u32x4 z = {0, 0, 0, 0};
-      *reinterpret_cast<u32x4*>(tile + lds_at<T, D>(row(tid, i), chunk(tid, i))) = (keep >> row(tid, i)) & 1 ? w[i] : z;
-    }
-  }
-};
 __device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1ull); }
 
 __device__ __forceinline__ float mask_value(float km) { return km > HIDDEN ? km * LOG2E_ : -INFINITY; }      // (NaN hides)
-// ---- the same journey without the registers: 16 bytes per lane straight from memory into LDS (buffer_load ... lds).  The LDS side is linear in the thread index, so the
+// ---- a tile's journey, 16 bytes per lane straight from memory into LDS (buffer_load ... lds).  Through registers (load, then write to LDS) the tile in flight cost 16 to 64
+// of them (a wave per SIMD less); with the lazily raised maximum of the forward pass 139 -> 101 us for 4 x 8192 tokens, 12 heads of 64, window 256 + 256.  The LDS side is linear in the thread index, so the
 // chunk permutation is applied to the address that a lane READS.  Rows past the valid ones are outside the buffer descriptor, and the load writes zeros for them.
 // Inline asm on purpose: next to the builtin the compiler waits for all loads in front of every LDS read, since it cannot tell the buffer being filled from the one
-// being read.  There is no output register; arrive() waits for everything in flight.
+// being read.  There is no output register; dma_arrive() waits for everything in flight.
 template <typename T, int D, int ROWS, int NT> struct Dma {
   static constexpr int N = ROWS * Geo<T, D>::NCH / NT;
   static_assert(N >= 1 && ROWS * Geo<T, D>::NCH % NT == 0 && NT % 64 == 0, "whole chunks per thread");
@@ -251,7 +224,7 @@ template <typename T, int D, int ROWS, int NT> struct Dma {
     for (int i = 0; i < N; ++i)
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(dst + (uint32_t)(i * NT * 16)), "v"(off[i]), "s"(rsrc) : "memory", "m0");
   }
-  // (behind arrive()) zeros over the rows of this thread's chunks that `keep` leaves out
+  // (behind dma_arrive()) zeros over the rows of this thread's chunks that `keep` leaves out
   __device__ __forceinline__ void erase(char* lds_tile, uint64_t keep, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i)

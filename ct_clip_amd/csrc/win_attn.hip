@@ -276,17 +276,23 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void row
   if ((tid & 7) == 0 && p.lse) p.lse[(int64_t)oh * p.Mq + rw.q0 + orow] = lsum == 0.f ? INFINITY : m + __builtin_amdgcn_logf(lsum);
 }
 
-// out = sum_s exp2(m_s - M) acc_s / sum_s exp2(m_s - M) l_s over the split passes.  A workgroup per (head, row): D / 4 threads across the columns, the others across the
-// splits (one thread per column alone chains nsplit loads: 11 us for 16 splits), folded in a fixed order.
-template <typename T, int D>
+// out = sum_s exp2(m_s - M) acc_s / sum_s exp2(m_s - M) l_s over the split passes, in a fixed order.  D / 4 threads across the columns of a (head, row); the others across
+// the splits (SG = 256 / (D / 4): one thread's chain over 16 splits took 11 us), or across rows (SG = 1) where there are many rows (f32, 3 x 577
+// tokens of 8 heads, split in two: 20 us, with a workgroup for each row and head 45, unsplit 27).
+template <typename T, int D, int SG>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
-  constexpr int C = D / 4, SG = 256 / C;
+  constexpr int C = D / 4, PER = 256 / C / SG;
   __shared__ __attribute__((aligned(16))) float fo[SG][D], fl[SG];
-  const int64_t n = (int64_t)p.H * p.Mq, rows = (int64_t)p.nsplit * n, i = blockIdx.x;
-  const int col = (threadIdx.x % C) * 4, sg = threadIdx.x / C;
+  const int64_t n = (int64_t)p.H * p.Mq, rows = (int64_t)p.nsplit * n, i = (int64_t)blockIdx.x * PER + (SG == 1 ? threadIdx.x / C : 0);
+  if (i >= n) return;                      // (SG > 1: the whole workgroup or nobody)
+  const int col = (threadIdx.x % C) * 4, sg = SG == 1 ? 0 : threadIdx.x / C;
   float m = -INFINITY;
-  for (int s = threadIdx.x & 63; s < p.nsplit; s += 64) m = fmaxf(m, p.part[s * n + i]);
-  m = wave_max(m);
+  if constexpr (SG > 1) {
+    for (int s = threadIdx.x & 63; s < p.nsplit; s += 64) m = fmaxf(m, p.part[s * n + i]);
+    m = wave_max(m);
+  } else {
+    for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, p.part[s * n + i]);
+  }
   const float ms = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   for (int s = sg; s < p.nsplit; s += SG) {
@@ -297,20 +303,22 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(a[e], f, o[e]);
   }
-  store4(&fo[sg][col], o);
-  if (col == 0) fl[sg] = l;
-  __syncthreads();
-  if (sg) return;
-  l = 0.f;
+  if constexpr (SG > 1) {
+    store4(&fo[sg][col], o);
+    if (col == 0) fl[sg] = l;
+    __syncthreads();
+    if (sg) return;
+    l = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = 0.f;
+    for (int e = 0; e < 4; ++e) o[e] = 0.f;
 #pragma unroll
-  for (int g = 0; g < SG; ++g) {
-    float a[4];
-    load4(&fo[g][col], a);
-    l += fl[g];
+    for (int g = 0; g < SG; ++g) {
+      float a[4];
+      load4(&fo[g][col], a);
+      l += fl[g];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += a[e];
+      for (int e = 0; e < 4; ++e) o[e] += a[e];
+    }
   }
   const int64_t h = i / p.Mq, row = i - h * p.Mq;
   const float mul = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
@@ -322,11 +330,13 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
 
 // ---- host side
 struct Plan { bool rows; int nsplit; };
-// Which kernel, and over how many workgroups a key axis is split: see the figures at each rule.
-inline Plan plan(int nseq, int Lq, int Lk, int H, int Hk, int left, int right, int sinks, int q_start, bool packed) {
+// Which kernel, and over how many workgroups a key axis is split.
+inline Plan plan(int nseq, int Lq, int Lk, int H, int Hk, int left, int right, int sinks, int q_start, bool packed, int dtype) {
   Plan pl{false, 1};
   const int G = H / Hk;
   if (packed) return pl;
+  // rows_kernel where the rows of a group fit its 32: one token of 4 sequences of 32768 keys, 32 heads of 128 on 8, takes 115 us (fwd_kernel, where the heads that share k and v
+  // are rows of different workgroups: 197), the [CLS] rows of 8 x 512 5.6 (6.1).  Split for two workgroups per CU, eight blocks (two per wave) each at least: unsplit 468 us.
   if ((int64_t)Lq * G <= 32) {
     pl.rows = true;
     const TileList tl = tile_list<32>(q_start, q_start + Lq - 1, left, right, sinks, Lk);
@@ -337,12 +347,14 @@ inline Plan plan(int nseq, int Lq, int Lk, int H, int Hk, int left, int right, i
     return pl;
   }
   const int64_t units = (int64_t)nseq * H * cdiv(Lq, QB);
+  // fewer tiles than CUs: split, but not below four steps.  1 x 4096, 2 heads of 64, no window: 29 us, unsplit 70; 200 rows against 8192 keys, 12 heads: 27 and 140; 512 tokens
+  // of 12 heads, window 128: 13.5, with parts of two steps 15.3
   if (units < 256) {
-    const int last = (int)((Lq - 1) / QB) * QB;
-    const TileList tl = tile_list<64>(q_start + last, q_start + Lq - 1, left, right, sinks, Lk);
-    int64_t s = cdiv(512, units);
-    if (s > tl.n / 4) s = tl.n / 4;
-    pl.nsplit = (int)(s < 1 ? 1 : s);
+    const int last = (int)((Lq - 1) / QB) * QB, lo = q_start + last, hi = q_start + Lq - 1;
+    const int tiles = dtype == DT_F32 ? tile_list<32>(lo, hi, left, right, sinks, Lk).n : tile_list<64>(lo, hi, left, right, sinks, Lk).n;
+    int64_t s = 256 / units;
+    if (s > tiles / 4) s = tiles / 4;
+    if (s > 1) pl.nsplit = (int)s;
   }
   return pl;
 }
@@ -369,7 +381,10 @@ template <typename T, int D, bool DROP> int launch_fwd(Params& p, const Plan& pl
   }
   int rc = ctclip_check_launch("win_attn_fwd");
   if (rc || p.nsplit == 1) return rc;
-  hipLaunchKernelGGL((join_kernel<T, D>), dim3((unsigned)((int64_t)p.H * p.Mq)), dim3(256), 0, s, p);
+  const int64_t n = (int64_t)p.H * p.Mq;
+  constexpr int SG = 256 / (D / 4);
+  if (n > 4096) hipLaunchKernelGGL((join_kernel<T, D, 1>), dim3((unsigned)cdiv(n, SG)), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((join_kernel<T, D, SG>), dim3((unsigned)n), dim3(256), 0, s, p);
   return ctclip_check_launch("win_attn_fwd join");
 }
 template <typename T, int D> int launch_fwd_d(Params& p, const Plan& pl, hipStream_t s) {
@@ -384,8 +399,9 @@ template <typename T> int launch_fwd_t(Params& p, const Plan& pl, int D, hipStre
 extern "C" int64_t ctclip_win_attn_fwd_workspace(int nseq, int Lq, int Lk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int packed) {
   if (nseq < 1 || Lq < 1 || Lk < 1 || H < 1 || Hk < 1 || H % Hk || packed) return 0;
   const int l = left < 0 || left > Lk ? Lk : left, r = right < 0 || right > Lk ? Lk : right, s = sinks < Lk ? sinks : Lk;
-  const win::Plan pl = win::plan(nseq, Lq, Lk, H, Hk, l, r, s, q_start, false);
-  return pl.nsplit > 1 ? (int64_t)pl.nsplit * H * nseq * Lq * (D + 2) * 4 : 0;
+  const int a = win::plan(nseq, Lq, Lk, H, Hk, l, r, s, q_start, false, DT_F32).nsplit, b = win::plan(nseq, Lq, Lk, H, Hk, l, r, s, q_start, false, DT_BF16).nsplit;
+  const int n = a > b ? a : b;             // (of either type: the larger)
+  return n > 1 ? (int64_t)n * H * nseq * Lq * (D + 2) * 4 : 0;
 }
 
 // q (Mq, H D), k | v (Mk, Hk D) -> out (Mq, H D), lse [H][Mq] f32 (log2 domain; optional: backward needs it).  Sequence b = rows b Lq ... of q and b Lk ... of
@@ -407,7 +423,7 @@ extern "C" int ctclip_win_attn_fwd(const void* q, const void* k, const void* v, 
   Params p{};
   fill(p, nseq, Lq, Lk, Mq, Mk, H, Hk, left, right, sinks, q_start, scale, dropout_p, dropout_seed, offsets, tiles, ntiles, keymask);
   p.q = q; p.k = k; p.v = v; p.out = out; p.out_lo = dtype == DT_BF16 ? out_lo : nullptr; p.lse = lse; p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo;
-  const Plan pl = plan(nseq, Lq, Lk, H, Hk, p.left, p.right, p.sinks, q_start, offsets != nullptr);
+  const Plan pl = plan(nseq, Lq, Lk, H, Hk, p.left, p.right, p.sinks, q_start, offsets != nullptr, dtype);
   p.nsplit = pl.nsplit;
   if (p.nsplit > 1) {
     if (!workspace || workspace_bytes < (int64_t)p.nsplit * H * Mq * (D + 2) * 4 || reinterpret_cast<uintptr_t>(workspace) % 16) { ctclip_set_error("win_attn_fwd: workspace"); return CTCLIP_EWORKSPACE; }

@@ -129,9 +129,25 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
   store_rows<T, D, false>(lds + wave * 32 * G::ROWB, acc, p.scale, reinterpret_cast<T*>(p.dq) + (rw.q0 + wr) * p.lddq + (int64_t)h * D, p.lddq, rw.lq - wr, lane);
 }
 
+// The shape of the dK / dV kernel.  Four waves with k, v and both gradients of 32 keys each in registers, or (bf16 heads of 128, where that is 192 registers and would leave
+// a SIMD one wave) k and v in LDS and eight waves, two to a 32-key block.
+template <typename T, int D> struct Dkv {
+  static constexpr bool IN_LDS = sizeof(T) == 2 && D == 128;
+  static constexpr int PAIR = IN_LDS ? 2 : 1, WAVES = 4 * PAIR, NT = 64 * WAVES;
+  static constexpr int QT = sizeof(T) == 2 ? 64 : 32;      // query rows of a step
+  static constexpr int TILE = QT * Geo<T, D>::ROWB, KEYS = IN_LDS ? 2 * QB * Geo<T, D>::ROWB : 0;      // bytes: a tile of rows, k and v
+  static constexpr int WINDOW = KEYS + 4 * TILE + 4 * QT * 4;                                          // [k | v], [2][Q | dO], [2][lse | Delta]
+  static constexpr int OWN = 64 * Geo<T, D>::ROWB + 256;                                               // a wave's [Q | dO | lse | Delta] of 32 rows
+  static constexpr int SINK = (IN_LDS ? 64 * Geo<T, D>::ROWB : 0) + WAVES * OWN, FOLD = WAVES * 32 * (D + 4) * 4;
+  static constexpr int LDS = WINDOW > SINK ? (WINDOW > FOLD ? WINDOW : FOLD) : (SINK > FOLD ? SINK : FOLD);
+};
 // 32 staged queries against the 32 keys of a wave
-template <typename T, int D> struct KeyState {
+template <typename T, int D, bool IN_LDS = Dkv<T, D>::IN_LDS> struct KeyState {
   RowFrag<T, D> kf, vf;
+  f32x16 dk[D / 32], dv[D / 32];
+};
+template <typename T, int D> struct KeyState<T, D, true> {
+  const char *kb, *vb;                     // the keys' 32 rows in LDS
   f32x16 dk[D / 32], dv[D / 32];
 };
 // dropout multipliers of a lane's key and the 16 queries row + 8 (r >> 2) + 4 h + (r & 3).  The four lanes of a key quad need the same eight blocks (2 rows x 4 keys
@@ -162,13 +178,19 @@ template <typename T, int D, bool DROP, bool FAR>
 __device__ __forceinline__ void query_block(KeyState<T, D>& st, const char* qt, const char* dt, const float* lse, const float* delta, const LaneAt<T, D>& at, const Params& p,
                                             int row, int j, float kbias, bool partial, int lane, int64_t sh) {
   const int half = lane >> 5;
+  constexpr bool IN_LDS = Dkv<T, D>::IN_LDS;
   RowFrag<T, D> f, f2;
   row_frag_lds<T, D>(f, qt, at);
-  row_frag_lds<T, D>(f2, dt, at);
   f32x16 s, dp;
 #pragma unroll
   for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
-  s = mma_rows<D>(f, st.kf, s);
+  if constexpr (IN_LDS) {
+    row_frag_lds<T, D>(f2, st.kb, at);
+    s = mma_rows<D>(f, f2, s);
+  } else {
+    row_frag_lds<T, D>(f2, dt, at);
+    s = mma_rows<D>(f, st.kf, s);
+  }
   if (partial) {                           // row >= j - right, row <= j + left (positions), or beyond: row > j + left and j a sink
     const int o = p.q_start + row + 4 * half;
     const int rl = j - p.right - o, rh = j + p.left - o;
@@ -188,31 +210,64 @@ __device__ __forceinline__ void query_block(KeyState<T, D>& st, const char* qt, 
   }
   if (DROP) drop_of_key(dm, p, sh, row, j, half);
   PFrag<T> pf, df;
+  if constexpr (IN_LDS) {                  // one operand at a time
+    row_frag_lds<T, D>(f, dt, at);
+    row_frag_lds<T, D>(f2, st.vb, at);
+    dp = mma_rows<D>(f, f2, dp);
+  } else {
+    dp = mma_rows<D>(f2, st.vf, dp);
+  }
   ColFrag<T, D> dc, qc;
-  col_frag_lds<D>(dc, dt, at);
-  dp = mma_rows<D>(f2, st.vf, dp);
+  if constexpr (!IN_LDS) col_frag_lds<D>(dc, dt, at);
   float pd[16];
 #pragma unroll
   for (int r = 0; r < 16; ++r) { pr[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, ls[r])); pd[r] = DROP ? pr[r] * dm[r] : pr[r]; }
   p_frag(pf, pd);
-  col_frag_lds<D>(qc, qt, at);
+  if constexpr (IN_LDS) col_frag_lds<D>(dc, dt, at);
+  else col_frag_lds<D>(qc, qt, at);
   mma_cols<D>(st.dv, dc, pf, lane);
 #pragma unroll
   for (int r = 0; r < 16; ++r) pr[r] *= (DROP ? dp[r] * dm[r] : dp[r]) - de[r];
   p_frag(df, pr);
+  if constexpr (IN_LDS) col_frag_lds<D>(qc, qt, at);
   mma_cols<D>(st.dk, qc, df, lane);
 }
 
-// a wave's 32 keys into registers; hidden keys and keys past the end are zeros and carry a bias of -inf
-template <typename T, int D> __device__ __forceinline__ float load_keys(KeyState<T, D>& st, const Params& p, const Rows& rw, int hk, int j, int half) {
-  const int jr = j < rw.lk ? j : rw.lk - 1;
+// A wave's keys j, 32 of the ROWS that its workgroup has (the first is `first`): into its registers, or all of them into LDS, which every wave takes part in.  Hidden keys
+// and keys past the end are zeros and carry a bias (returned) of -inf.
+template <int ROWS, typename T, int D> __device__ __forceinline__ float load_keys(KeyState<T, D>& st, const Params& p, const Rows& rw, int hk, int first, int j, char* lds, const LaneAt<T, D>& at,
+                                                                               int tid) {
+  const int half = (tid & 63) >> 5, jr = j < rw.lk ? j : rw.lk - 1;
   const float km = p.keymask ? p.keymask[rw.k0 + jr] : 0.f;
   const bool on = j < rw.lk && km > HIDDEN;
-  row_frag_global<T, D>(st.kf, reinterpret_cast<const T*>(p.k) + (rw.k0 + jr) * p.ldk + (int64_t)hk * D, half);
-  row_frag_global<T, D>(st.vf, reinterpret_cast<const T*>(p.v) + (rw.k0 + jr) * p.ldv + (int64_t)hk * D, half);
-  row_frag_arrive<T, D>(st.kf);
-  row_frag_arrive<T, D>(st.vf);
-  if (!on) { row_frag_zero<T, D>(st.kf); row_frag_zero<T, D>(st.vf); }
+  if constexpr (Dkv<T, D>::IN_LDS) {
+    constexpr int NT = Dkv<T, D>::NT, ROWB = Geo<T, D>::ROWB, NCH = Geo<T, D>::NCH;
+    char* v = lds + ROWS * ROWB;
+    Dma<T, D, ROWS, NT> dma;
+    dma.init((int)p.ldk * (int)sizeof(T), tid);
+    dma.issue(lds, reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.k) + (rw.k0 + first) * p.ldk + (int64_t)hk * D), (int)p.ldk * (int)sizeof(T), rw.lk - first, tid);
+    dma.init((int)p.ldv * (int)sizeof(T), tid);
+    dma.issue(v, reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + (rw.k0 + first) * p.ldv + (int64_t)hk * D), (int)p.ldv * (int)sizeof(T), rw.lk - first, tid);
+    dma_arrive();
+    st.kb = lds + (j - (tid & 31) - first) * ROWB;
+    st.vb = st.kb + ROWS * ROWB;
+    if (p.keymask) {
+      __syncthreads();
+      if (!on) {                           // (by every wave that has these keys)
+        const u32x4 z = {0, 0, 0, 0};
+        char* row = lds + (j - first) * ROWB + half * (ROWB / 2);
+#pragma unroll
+        for (int n = 0; n < NCH / 2; ++n) { *reinterpret_cast<u32x4*>(row + n * 16) = z; *reinterpret_cast<u32x4*>(row + ROWS * ROWB + n * 16) = z; }
+      }
+    }
+    __syncthreads();
+  } else {
+    row_frag_global<T, D>(st.kf, reinterpret_cast<const T*>(p.k) + (rw.k0 + jr) * p.ldk + (int64_t)hk * D, half);
+    row_frag_global<T, D>(st.vf, reinterpret_cast<const T*>(p.v) + (rw.k0 + jr) * p.ldv + (int64_t)hk * D, half);
+    row_frag_arrive<T, D>(st.kf);
+    row_frag_arrive<T, D>(st.vf);
+    if (!on) { row_frag_zero<T, D>(st.kf); row_frag_zero<T, D>(st.vf); }
+  }
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
@@ -264,26 +319,6 @@ template <typename T, int D, int ROWS, int NT> struct RowPipe {    // through LD
     src.put_stat<ROWS>(stat, tid);
   }
 };
-template <typename T, int D> struct WaveRowPipe {          // a wave's own tiles of 32 rows, through registers (one LDS buffer per wave)
-  RowSource src;
-  Stage<T, D, 32, 64> sq, sd;
-  __device__ __forceinline__ WaveRowPipe(const Params& p, const Rows& rw, int h0) { src.init<T, D>(p, rw, h0); }
-  __device__ __forceinline__ void fetch(const Params& p, int g, int first, int lane) {
-    src.r0 = first;
-    const int last = src.lq - 1 - first;
-    sq.get(src.q + (int64_t)first * src.ldq + g * (D * (int)sizeof(T)), src.ldq, last, lane);
-    sd.get(src.d + (int64_t)first * src.ldd + g * (D * (int)sizeof(T)), src.ldd, last, lane);
-    src.get_stat<32>(p, g, lane);
-  }
-  __device__ __forceinline__ void deposit(char* qt, char* dt, float* stat, int lane) const {
-    if (src.r0 + 32 <= src.lq) { sq.put(qt, lane); sd.put(dt, lane); }
-    else { const uint64_t keep = low_bits(src.lq - src.r0); sq.put(qt, keep, lane); sd.put(dt, keep, lane); }
-    src.put_stat<32>(stat, lane);
-  }
-};
-
-template <typename T, int D> struct QTile { static constexpr int ROWS = sizeof(T) == 2 ? 64 : 32; };      // query rows of a dK / dV step
-
 // where the partial sums of key j lie: split passes hold every key, unsplit ones the keys of the sink blocks
 __device__ __forceinline__ int64_t part_row(const Params& p, const Rows& rw, int b, int hk, int j) {
   return p.nsplit > 1 ? (int64_t)hk * p.Mk + rw.k0 + j : ((int64_t)b * p.Hk + hk) * p.s32 + j;
@@ -294,10 +329,12 @@ __host__ __device__ inline int64_t sink_rows(const Params& p) { return (int64_t)
 template <typename T, int D, bool DROP>
 __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, int split, int nunits, int nkt) {
   typedef Geo<T, D> G;
-  constexpr int QT = QTile<T, D>::ROWS, TILE = QT * G::ROWB;
-  float* stat = reinterpret_cast<float*>(lds + 4 * TILE);
+  typedef Dkv<T, D> X;
+  constexpr int QT = X::QT, TILE = X::TILE;
+  char* ring = lds + X::KEYS;
+  float* stat = reinterpret_cast<float*>(ring + 4 * TILE);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, par = __builtin_amdgcn_readfirstlane(tid >> 8);      // 32-key block; which of the waves that share it
   const Unit u = unit_of(p, id, nunits, nkt, 1);
   if (!u.real) return;
   const Rows rw = rows_of(p, u.b);
@@ -312,13 +349,13 @@ __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, 
   const int i0 = (int)((int64_t)steps * split / p.nsplit), i1 = (int)((int64_t)steps * (split + 1) / p.nsplit);
 
   const int jw = k0 + 32 * wave, j = jw + c;
-  KeyState<T, D> st;
-  const float kbias = load_keys<T, D>(st, p, rw, u.hk, j, half);
-  const bool any = __builtin_amdgcn_ballot_w64(kbias > -INFINITY) != 0;      // wave-uniform
   const LaneAt<T, D> at(lane);
-  RowPipe<T, D, QT, 256> rp(p, rw, u.hk * p.G, tid);
+  KeyState<T, D> st;
+  const float kbias = load_keys<QB, T, D>(st, p, rw, u.hk, k0, j, lds, at, tid);
+  const bool any = __builtin_amdgcn_ballot_w64(kbias > -INFINITY) != 0;      // wave-uniform
+  RowPipe<T, D, QT, X::NT> rp(p, rw, u.hk * p.G, tid);
   if (i0 < i1) {
-    rp.issue(p, lds, lds + TILE, i0 / nt, (t0 + i0 % nt) * QT, tid);
+    rp.issue(p, ring, ring + TILE, i0 / nt, (t0 + i0 % nt) * QT, tid);
     rp.settle(stat, tid);
   }
   __syncthreads();
@@ -328,20 +365,43 @@ __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, 
     const int64_t sh = (int64_t)u.b * p.H + u.hk * p.G + g;
     const bool more = i + 1 < i1;
     if (++t == nt) { t = 0; ++g; }
-    char* next = lds + (buf ^ 1) * 2 * TILE;               // (its readers are behind the last barrier)
+    char* next = ring + (buf ^ 1) * 2 * TILE;              // (its readers are behind the last barrier)
     if (more) rp.issue(p, next, next + TILE, g, (t0 + t) * QT, tid);
 #pragma unroll
-    for (int b = 0; b < QT / 32; ++b) {
+    for (int n = 0; n < QT / 32 / X::PAIR; ++n) {
+      const int b = X::PAIR * n + par;
       const int lo = p.q_start + r0 + 32 * b, last = p.q_start + rw.lq - 1;
       const int see = any ? Sight(lo, lo + 31 < last ? lo + 31 : last, p.left, p.right, 0, rw.lk).of(jw) : 0;
       if (see) {
-        const char* qt = lds + buf * 2 * TILE + 32 * b * G::ROWB;
+        const char* qt = ring + buf * 2 * TILE + 32 * b * G::ROWB;
         const float* sp = stat + buf * 2 * QT + 32 * b;
         query_block<T, D, DROP, false>(st, qt, qt + TILE, sp, sp + QT, at, p, r0 + 32 * b, j, kbias, see == 1, lane, sh);
       }
     }
     if (more) rp.settle(stat + (buf ^ 1) * 2 * QT, tid);
     __syncthreads();
+  }
+  if constexpr (X::PAIR == 2) {            // the second wave of a pair hands its sums to the first, lane to lane: [block][register][lane], dK, then dV
+    float* hand = reinterpret_cast<float*>(lds) + wave * (D / 2) * 64 + lane;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      f32x16(&a)[D / 32] = which ? st.dv : st.dk;
+      if (which) __syncthreads();
+      if (par) {
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) hand[(16 * x + r) * 64] = a[x][r];
+      }
+      __syncthreads();
+      if (!par) {
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) a[x][r] += hand[(16 * x + r) * 64];
+      }
+    }
+    if (par) return;
   }
   if (p.nsplit > 1 || jw < p.s32) {
     if (j >= rw.lk) return;
@@ -350,7 +410,7 @@ __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, 
     store_part<D>(p.part + ((int64_t)p.nsplit * N + r) * D, st.dv, half);
     return;
   }
-  char* turn = lds + wave * 32 * G::ROWB;
+  char* turn = ring + wave * 32 * G::ROWB;
   store_rows<T, D, false>(turn, st.dk, p.scale, reinterpret_cast<T*>(p.dk) + (rw.k0 + jw) * p.lddk + (int64_t)u.hk * D, p.lddk, rw.lk - jw, lane);
   store_rows<T, D, false>(turn, st.dv, 1.f, reinterpret_cast<T*>(p.dv) + (rw.k0 + jw) * p.lddv + (int64_t)u.hk * D, p.lddv, rw.lk - jw, lane);
 }
@@ -358,7 +418,8 @@ __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, 
 template <typename T, int D, bool DROP>
 __device__ __forceinline__ void sink_pass(const Params& p, char* lds, int id, int nblk) {
   typedef Geo<T, D> G;
-  constexpr int TILE = 32 * G::ROWB;                               // lds: four waves x [Q | dO | lse, Delta] of 32 rows; reused to fold the waves
+  typedef Dkv<T, D> X;
+  constexpr int TILE = 32 * G::ROWB;                               // lds: [k | v of 32 keys], a wave's own [Q | dO | lse, Delta] of 32 rows; reused to fold the waves
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int chunk = id % p.nchunk, blk = id / p.nchunk % nblk, hk = id / (p.nchunk * nblk) % p.Hk, b = id / (p.nchunk * nblk * p.Hk);
@@ -369,29 +430,27 @@ __device__ __forceinline__ void sink_pass(const Params& p, char* lds, int id, in
   rlo = rlo < 0 ? 0 : rlo;
   const int t0 = rlo / 32, nt = rw.lq > rlo ? (rw.lq - 1) / 32 - t0 + 1 : 0, steps = nt * p.G;
   const int i0 = (int)((int64_t)steps * chunk / p.nchunk), i1 = (int)((int64_t)steps * (chunk + 1) / p.nchunk);
+  const LaneAt<T, D> at(lane);
   KeyState<T, D> st;
-  const float kbias = load_keys<T, D>(st, p, rw, hk, j, half);
-  char* qtile = lds + wave * (2 * TILE + 256);
+  const float kbias = load_keys<32, T, D>(st, p, rw, hk, jw, j, lds, at, tid);
+  char* qtile = lds + X::SINK - (X::WAVES - wave) * X::OWN;
   char* dtile = qtile + TILE;
   float* stat = reinterpret_cast<float*>(dtile + TILE);
-  const LaneAt<T, D> at(lane);
-  WaveRowPipe<T, D> rp(p, rw, hk * p.G);
-  int i = i0 + wave;
-  if (i < i1) rp.fetch(p, i / nt, (t0 + i % nt) * 32, lane);
-  for (; i < i1; i += 4) {
+  RowPipe<T, D, 32, 64> rp(p, rw, hk * p.G, lane);
+  for (int i = i0 + wave; i < i1; i += X::WAVES) {                 // (the other waves of the SIMD work while this one waits for its rows)
     const int g = i / nt, r0 = (t0 + i % nt) * 32;
-    rp.deposit(qtile, dtile, stat, lane);
-    if (i + 4 < i1) rp.fetch(p, (i + 4) / nt, (t0 + (i + 4) % nt) * 32, lane);
+    rp.issue(p, qtile, dtile, g, r0, lane);
+    rp.settle(stat, lane);
     wave_sync();
     query_block<T, D, DROP, true>(st, qtile, dtile, stat, stat + 32, at, p, r0, j, kbias, true, lane, (int64_t)b * p.H + hk * p.G + g);
     wave_sync();
   }
-  // fold the four waves, dK then dV, in the order of the waves
-  float* fa = reinterpret_cast<float*>(lds);                       // [4][32][D + 4]
+  // fold the waves, dK then dV, in their order
+  float* fa = reinterpret_cast<float*>(lds);                       // [WAVES][32][D + 4]
   const int64_t r = ((int64_t)b * p.Hk + hk) * p.s32 + jw, S = sink_rows(p);
   float* base = p.part + (int64_t)2 * p.nsplit * part_rows(p) * D;
-  constexpr int PER = D / 8;
-  const int fr = tid >> 3, fc = (tid & 7) * PER;
+  constexpr int TPR = X::NT / 32, PER = D / TPR;                   // threads of a row, columns of a thread
+  const int fr = tid / TPR, fc = tid % TPR * PER;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     __syncthreads();
@@ -407,20 +466,18 @@ __device__ __forceinline__ void sink_pass(const Params& p, char* lds, int id, in
     float* dst = base + (((int64_t)which * p.nchunk + chunk) * S + r + fr) * D + fc;
 #pragma unroll
     for (int e = 0; e < PER; e += 4) {
-      float t[4];
+      float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float* a = fa + fr * (D + 4) + fc + e + x;
-        t[x] = a[0] + a[32 * (D + 4)] + a[64 * (D + 4)] + a[96 * (D + 4)];
-      }
+      for (int w = 0; w < X::WAVES; ++w)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) t[x] += fa[(w * 32 + fr) * (D + 4) + fc + e + x];
       store4(dst + e, t);
     }
   }
 }
-
 // The first nsink workgroups take the sink pass, so that it runs beside the window pass instead of in front of it.
 template <typename T, int D, bool DROP>
-__global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void dkv_kernel(Params p, int nunits, int nkt, int nsink) {
+__global__ __launch_bounds__((Dkv<T, D>::NT), (D == 128 && sizeof(T) == 4 ? 1 : 2)) void dkv_kernel(Params p, int nunits, int nkt, int nsink) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int id = (int)blockIdx.x - nsink;
   if (id < 0) { sink_pass<T, D, DROP>(p, lds, blockIdx.x, p.s32 / 32); return; }
@@ -428,18 +485,22 @@ __global__ __launch_bounds__(256, (D == 128 ? 1 : 2)) void dkv_kernel(Params p, 
   window_pass<T, D, DROP>(p, lds, id % per, id / per, nunits, nkt);
 }
 
-// Keys whose sums came in parts.  A workgroup folds 256 / (D / 4) / PG keys of one k|v head: D / 4 threads across the columns, PG threads (1, or a sixteenth of the
-// chunks each where there are many: one thread's chain of dependent additions over 43 chunks took 40 us) across the parts, folded in a fixed order.
-template <typename T, int D, int PG>
-__global__ __launch_bounds__(256) void dkv_reduce_kernel(Params p, int keys) {
-  constexpr int C = D / 4, KEYS = 256 / C / PG;
-  __shared__ __attribute__((aligned(16))) float fold[2][PG][KEYS][D];
-  const int hk = blockIdx.y;
-  const int col = (threadIdx.x % C) * 4, key = threadIdx.x / C % KEYS, pg = threadIdx.x / C / KEYS;
-  const int j = blockIdx.x * KEYS + key;
+// Keys whose sums came in parts, added in a fixed order: D / 4 threads across the columns of a key, the others across keys (a workgroup of the key range behind `deep`) or,
+// where the parts are many, PG of them across the parts of one key (the sinks' chunks: one thread's chain of dependent additions over 43 took 40 us; PG threads for
+// every key, most with two parts: 69 against 54 us for the whole backward pass of 2048 tokens, 12 heads of 64).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void dkv_reduce_kernel(Params p, int keys, int deep) {
+  constexpr int C = D / 4, PER = 256 / C, PG = PER < 16 ? PER : 16, DK = PER / PG;             // keys of a workgroup: PER, or DK
+  __shared__ __attribute__((aligned(16))) float fold[2][PG][DK][D];
+  const int hk = blockIdx.y, nd = (deep + DK - 1) / DK;
+  const bool split = (int)blockIdx.x < nd;
+  const int col = (threadIdx.x % C) * 4, sub = threadIdx.x / C;
+  const int pg = split ? sub / DK : 0, step = split ? PG : 1;
+  const int j = split ? blockIdx.x * DK + sub % DK : deep + (blockIdx.x - nd) * PER + sub;
+  const int end = split ? deep : keys;
   for (int b = blockIdx.z; b < p.nseq; b += gridDim.z) {
     const Rows rw = rows_of(p, b);
-    const bool on = j < keys && j < rw.lk;
+    const bool on = j < end && j < rw.lk;
     const int64_t N = part_rows(p), S = sink_rows(p), r = part_row(p, rw, b, hk, j);
     const float* sink = p.part + 2 * p.nsplit * N * D;
     const int parts = p.nsplit + (j < p.s32 ? p.nchunk : 0);
@@ -447,7 +508,7 @@ __global__ __launch_bounds__(256) void dkv_reduce_kernel(Params p, int keys) {
     for (int which = 0; which < 2; ++which) {
       float o[4] = {0.f, 0.f, 0.f, 0.f};
       if (on)
-        for (int s = pg; s < parts; s += PG) {
+        for (int s = pg; s < parts; s += step) {
           const float* src = s < p.nsplit ? p.part + (((int64_t)which * p.nsplit + s) * N + r) * D
                                           : sink + (((int64_t)which * p.nchunk + s - p.nsplit) * S + ((int64_t)b * p.Hk + hk) * p.s32 + j) * D;
           float a[4];
@@ -455,56 +516,50 @@ __global__ __launch_bounds__(256) void dkv_reduce_kernel(Params p, int keys) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] += a[e];
         }
-      if (PG > 1) {
-        store4(&fold[which][pg][key][col], o);
-      } else if (on) {
+      if (split) {
+        store4(&fold[which][pg][sub % DK][col], o);
+        __syncthreads();
+        if (pg == 0) {
+#pragma unroll
+          for (int g = 1; g < PG; ++g) {
+            float a[4];
+            load4(&fold[which][g][sub][col], a);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += a[e];
+          }
+        }
+      }
+      if (on && pg == 0) {
         const float mul = which ? 1.f : p.scale;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] *= mul;
         store4((which ? reinterpret_cast<T*>(p.dv) + (rw.k0 + j) * p.lddv : reinterpret_cast<T*>(p.dk) + (rw.k0 + j) * p.lddk) + (int64_t)hk * D + col, o);
       }
     }
-    if (PG == 1) continue;
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * KEYS * C; i += 256) {          // (with PG = 16: at most one round)
-      const int which = i / (KEYS * C), k = i / C % KEYS, cc = (i % C) * 4, jj = blockIdx.x * KEYS + k;
-      if (jj >= keys || jj >= rw.lk) continue;
-      float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int g = 0; g < PG; ++g) {
-        float a[4];
-        load4(&fold[which][g][k][cc], a);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += a[e];
-      }
-      const float mul = which ? 1.f : p.scale;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= mul;
-      store4((which ? reinterpret_cast<T*>(p.dv) + (rw.k0 + jj) * p.lddv : reinterpret_cast<T*>(p.dk) + (rw.k0 + jj) * p.lddk) + (int64_t)hk * D + cc, o);
-    }
-    __syncthreads();                       // (the next sequence's parts go to the same place)
+    if (split) __syncthreads();            // (the next sequence's parts go to the same place)
   }
 }
 
 struct BwdPlan { int nsplit, s32, nchunk; };
-inline BwdPlan bwd_plan(int nseq, int Lq, int Lk, int H, int Hk, int left, int right, int sinks, int q_start, int ntiles) {
+inline BwdPlan bwd_plan(int nseq, int Lq, int Lk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int ntiles, int dtype) {
   BwdPlan b{1, 0, 0};
   const int G = H / Hk;
   const int64_t units = ntiles ? (int64_t)ntiles * Hk : (int64_t)nseq * Hk * cdiv(Lk, QB);
   const int64_t span = (int64_t)QB + left + right < Lq ? (int64_t)QB + left + right : Lq;
-  const int64_t steps = cdiv(span, 32) * G;
-  if (units < 256) {                       // too few key tiles for the chip: split the rows (and heads) they meet
-    int64_t s = cdiv(512, units);
-    if (s > steps / 8) s = steps / 8;
-    b.nsplit = (int)(s < 1 ? 1 : s);
-  }
+  const int64_t steps = cdiv(span, dtype == DT_F32 ? 32 : 64) * G;         // of a workgroup that is not split
+  // Too few key tiles for the workgroups that are resident at once (one per CU for heads of 128, two otherwise): split the rows and heads that they meet, but not below four
+  // steps, for the parts are written and read again.  dQ, dK and dV of 1000 tokens, 8 heads on 2, no window: 48 us, unsplit 145; causal 2048, 4 heads of 128 on 1: 99 and 307;
+  // 1024 tokens, 12 heads, window 128: 34, with parts of two steps 40.  Two workgroups per CU for heads of 128: 106 instead of 91 us (4096 tokens, 4 heads, window 1023).
+  int64_t s = (D == 128 ? 256 : 512) / units;
+  if (s > steps / 4) s = steps / 4;
+  if (s > 1) b.nsplit = (int)s;
   const int64_t far = (int64_t)q_start + Lq - 1 - left;            // sinks 0 ... far - 1 have rows beyond their window
   if (sinks > 0 && far > 0) {
     const int64_t n = sinks < far ? sinks : far;
     b.s32 = (int)(cdiv(n, 32) * 32);
     const int64_t blocks = (int64_t)nseq * Hk * (b.s32 / 32), tiles = cdiv(far, 32) * G;
     int64_t ch = cdiv(512, blocks);
-    if (ch > tiles / 8) ch = tiles / 8;    // two tiles per wave at least
+    if (ch > tiles / 8) ch = tiles / 8;    // two tiles per wave at least; unsplit, the backward pass of 32768 tokens, 12 heads, takes 549 instead of 490 us
     b.nchunk = (int)(ch < 1 ? 1 : ch);
   }
   return b;
@@ -531,19 +586,17 @@ template <typename T, int D, bool DROP> int launch_bwd(Params& p, hipStream_t s)
     const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.Hk : (int64_t)p.nseq * p.Hk * nkt, nsink = (int64_t)(p.s32 / 32) * p.Hk * p.nseq * p.nchunk;
     const int64_t grid = nsink + 8 * cdiv(nu, 8) * p.nsplit;
     if (grid > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
-    int lds = 4 * QTile<T, D>::ROWS * G::ROWB + 4 * QTile<T, D>::ROWS * 4;
-    if (4 * (2 * 32 * G::ROWB + 256) > lds) lds = 4 * (2 * 32 * G::ROWB + 256);
-    if (4 * 32 * (D + 4) * 4 > lds) lds = 4 * 32 * (D + 4) * 4;
+    constexpr int lds = Dkv<T, D>::LDS;
     if ((rc = raise_lds<dkv_kernel<T, D, DROP>>(lds))) return rc;
-    if (nu) hipLaunchKernelGGL((dkv_kernel<T, D, DROP>), dim3((unsigned)grid), dim3(256), lds, s, p, (int)nu, nkt, (int)nsink);
+    if (nu) hipLaunchKernelGGL((dkv_kernel<T, D, DROP>), dim3((unsigned)grid), dim3(Dkv<T, D>::NT), lds, s, p, (int)nu, nkt, (int)nsink);
     if ((rc = ctclip_check_launch("win_attn_bwd dkv"))) return rc;
   }
   const int keys = p.nsplit > 1 ? p.Lk : p.s32;
   if (!keys) return CTCLIP_OK;
   const unsigned nz = p.nseq < 32768 ? p.nseq : 32768;
-  constexpr int PG = 256 / (D / 4) < 16 ? 256 / (D / 4) : 16;      // threads across the parts where the sinks' chunks are many
-  if (p.nsplit + p.nchunk > 8) hipLaunchKernelGGL((dkv_reduce_kernel<T, D, PG>), dim3((unsigned)cdiv(keys, 256 / (D / 4) / PG), p.Hk, nz), dim3(256), 0, s, p, keys);
-  else hipLaunchKernelGGL((dkv_reduce_kernel<T, D, 1>), dim3((unsigned)cdiv(keys, 256 / (D / 4)), p.Hk, nz), dim3(256), 0, s, p, keys);
+  constexpr int PER = 256 / (D / 4), DK = PER < 16 ? 1 : PER / 16;           // (as in the kernel)
+  const int deep = p.nsplit > 8 ? keys : (p.nsplit + p.nchunk > 8 ? (p.s32 < keys ? p.s32 : keys) : 0);
+  hipLaunchKernelGGL((dkv_reduce_kernel<T, D>), dim3((unsigned)(cdiv(deep, DK) + cdiv(keys - deep, PER)), p.Hk, nz), dim3(256), 0, s, p, keys, deep);
   return ctclip_check_launch("win_attn_bwd reduce");
 }
 template <typename T, int D> int launch_bwd_d(Params& p, hipStream_t s) { return p.drop_p > 0.f ? launch_bwd<T, D, true>(p, s) : launch_bwd<T, D, false>(p, s); }
@@ -556,7 +609,12 @@ template <typename T> int launch_bwd_t(Params& p, int D, hipStream_t s) {
 extern "C" int64_t ctclip_win_attn_bwd_workspace(int nseq, int Lq, int Lk, int64_t Mk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int ntiles) {
   if (nseq < 1 || Lq < 1 || Lk < 1 || H < 1 || Hk < 1 || H % Hk) return 0;
   const int l = left < 0 || left > Lk ? Lk : left, r = right < 0 || right > Lk ? Lk : right, s = sinks < Lk ? sinks : Lk;
-  return win::bwd_floats(win::bwd_plan(nseq, Lq, Lk, H, Hk, l, r, s, q_start, ntiles), nseq, Mk, Hk, D) * 4;
+  int64_t need = 0;                        // (of either type: the larger)
+  for (int dtype : {DT_F32, DT_BF16}) {
+    const int64_t n = win::bwd_floats(win::bwd_plan(nseq, Lq, Lk, H, Hk, D, l, r, s, q_start, ntiles, dtype), nseq, Mk, Hk, D) * 4;
+    need = n > need ? n : need;
+  }
+  return need;
 }
 
 // gradients of ctclip_win_attn_fwd: o, lse as it wrote them; delta: [H][Mq] f32 scratch; dq, dk, dv in the inputs' type, every row of a sequence written
@@ -581,7 +639,7 @@ extern "C" int ctclip_win_attn_bwd(const void* q, const void* k, const void* v, 
   fill(p, nseq, Lq, Lk, Mq, Mk, H, Hk, left, right, sinks, q_start, scale, dropout_p, dropout_seed, offsets, tiles, ntiles, keymask);
   p.q = q; p.k = k; p.v = v; p.o = o; p.out_lo = dtype == DT_BF16 ? const_cast<void*>(o_lo) : nullptr; p.dout = dout; p.lse = const_cast<float*>(lse); p.delta = delta; p.dq = dq; p.dk = dk; p.dv = dv;
   p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo; p.lddo = lddo; p.lddq = lddq; p.lddk = lddk; p.lddv = lddv;
-  const BwdPlan b = bwd_plan(nseq, Lq, Lk, H, Hk, p.left, p.right, p.sinks, q_start, offsets ? ntiles : 0);
+  const BwdPlan b = bwd_plan(nseq, Lq, Lk, H, Hk, D, p.left, p.right, p.sinks, q_start, offsets ? ntiles : 0, dtype);
   p.nsplit = b.nsplit; p.s32 = b.s32; p.nchunk = b.nchunk;
   const int64_t need = bwd_floats(b, nseq, Mk, Hk, D) * 4;
   if (need) {

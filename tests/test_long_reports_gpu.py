@@ -393,6 +393,53 @@ def test_captured_and_replayed_with_a_workspace_each():
             assert torch.equal(a, b)
 
 
+SPLIT = [  # nseq, Lq, Lk, H, Hk, D, window, sinks, q_start, mask, dropout: passes split over workgroups in many parts, in few, of many rows
+    (1, 1000, 1000, 8, 2, 64, (-1, -1), 0, 0, None, None),      # more than eight parts of every key
+    (1, 900, 900, 2, 1, 128, (-1, 0), 3, 0, "pad", None),
+    (1, 1030, 1030, 4, 4, 128, (200, 100), 40, 0, "holes", (0.1, 5)),     # two waves to a key block, two sink blocks
+    (2, 300, 300, 4, 2, 128, (30, 0), 2, 0, "front", (0.2, 6)),
+    (1, 2048, 2048, 3, 3, 32, (256, 256), 1, 0, None, None),    # two to eight parts, and the sinks' chunks
+    (1, 200, 2000, 6, 3, 64, (-1, 0), 0, 1800, "holes", None),
+    (1, 200, 2000, 24, 24, 32, (1500, 0), 5, 1700, None, (0.3, 7)),       # more than 4096 rows and heads to join
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("nseq,Lq,Lk,H,Hk,D,window,sinks,q_start,mask,drop", SPLIT)
+def test_window_attention_split_passes(nseq, Lq, Lk, H, Hk, D, window, sinks, q_start, mask, drop, dtype):
+    run_case(dtype, nseq, Lq, Lk, H, Hk, D, window, sinks, q_start=q_start, mask=mask, drop=drop, seed=Lk + D)
+
+
+def test_training_captured_and_replayed():
+    """Forward and backward of both operators in one graph, with sinks' and split keys' partial sums: each replay equals the eager result."""
+    H, D, L = 2, 64, 1500
+    q, k, v, g = (rnd((L, H * D), BF16, i) for i in range(4))
+    rope = Fn.RotaryPositions(64)
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        a, b = Fn.rotary(leaves[0], leaves[1], rope, D, start=7)
+        o = Fn.window_attention(a, b, leaves[2], H, D, window=(300, 20), sinks=3)
+        return [o.detach(), *torch.autograd.grad(o, leaves, g)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for rep in range(3):
+        for i, t in enumerate((q, k, v, g)):
+            t.copy_(rnd(tuple(t.shape), BF16, 60 + 4 * rep + i))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
 # ------------------------------------------------------------------------------------------------- the operators together
 
 @pytest.mark.parametrize("cls_only", [False, True])

@@ -5,8 +5,12 @@
 //   rows_kernel  few query rows against many keys (one token, the [CLS] row): the rows of all heads that share a k|v head are ONE 32-row block, the four
 //                waves take different key tiles and the axis is split over workgroups until the chip is full.  Bound by reading k and v once.
 //   join_kernel  folds the split passes of either.
-// One pass over the keys with the running maximum and sum of the softmax in f32, log2 domain.  P is rounded to the operand type (bf16: 2^-9 relative, one
-// rounding per probability) because the matrix cores read it; sums are taken of the unrounded values.
+// One pass over the keys with the running maximum and sum of the softmax in f32, log2 domain.  P is rounded to the operand type (bf16: half a step is 2^-8 of the value,
+// one rounding per probability) because the matrix cores read it; sums are taken of the unrounded values.  FINE adds what that rounding left over (launch_fwd_d).
+//
+// Bounds, MI355X.  One token of 4 sequences over 32768 keys, 32 heads of 128 on 8: 113 + 4 us (rows + join), 537 MB at 4.7 TB/s; a large copy runs at 5.1.  4 x 8192 tokens,
+// 12 heads of 64, window 256 + 256: 97 us, 0.53 PFLOP/s of 1.2 that a large product reaches: matrix instructions 0.27 of the time, vector instructions (exponentials, masks,
+// maxima, conversions) 0.58, LDS 0.20, which add up: a wave's step is a chain through all three, and four waves per SIMD overlap little of it.
 #include "win_attn.h"
 
 namespace win {
@@ -29,7 +33,7 @@ template <int D> struct SoftRow {          // the running softmax of a lane's qu
 constexpr float LAZY = 8.f;
 
 // A 32-key block: scores -> running softmax -> acc.  vt = the block's v rows in LDS; bias = its additive mask (or null); pos = the lane's position
-template <typename T, int D, bool DROP, bool PAIRED>
+template <typename T, int D, bool DROP, bool PAIRED, bool FINE>
 __device__ __forceinline__ void key_block(SoftRow<D>& st, f32x16 s, const char* vt, const float* bias, const LaneAt<T, D>& at, const Params& p, int j0, int pos, int lk,
                                           bool partial, int lane, int64_t sh, int qi) {
   const int half = lane >> 5;
@@ -82,7 +86,15 @@ __device__ __forceinline__ void key_block(SoftRow<D>& st, f32x16 s, const char* 
   }
   PFrag<T> pf;
   p_frag(pf, pr);
-  mma_cols<T, D>(st.acc, vt, at, pf, lane);
+  ColFrag<T, D> vf;
+  col_frag_lds<D>(vf, vt, at);
+  mma_cols<D>(st.acc, vf, pf, lane);
+  if constexpr (FINE) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) pr[r] -= bf2f(f2bf(pr[r]));
+    p_frag(pf, pr);
+    mma_cols<D>(st.acc, vf, pf, lane);
+  }
 }
 template <typename T, int D> __device__ __forceinline__ f32x16 scores(const RowFrag<T, D>& kf, const RowFrag<T, D>& qf) {
   f32x16 s;
@@ -91,8 +103,8 @@ template <typename T, int D> __device__ __forceinline__ f32x16 scores(const RowF
   return mma_rows<D>(kf, qf, s);
 }
 
-template <typename T, int D, bool DROP>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 4 : 2)) void fwd_kernel(Params p, int nunits, int nqt) {
+template <typename T, int D, bool DROP, bool FINE>
+__global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 && !FINE ? 4 : 2)) void fwd_kernel(Params p, int nunits, int nqt) {
   typedef Geo<T, D> G;
   constexpr int KT = G::KT, TILE = KT * G::ROWB;
   extern __shared__ __attribute__((aligned(16))) char lds[];       // [2][K | V], additive mask [2][KT]
@@ -143,7 +155,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 4 : 2)) void fwd_
         if (!a) continue;
         RowFrag<T, D> kf;
         row_frag_lds<T, D>(kf, kt + o, at);
-        key_block<T, D, DROP, true>(st, scores<T, D>(kf, qf), vt + o, bias ? bias + 32 * b : nullptr, at, p, j0 + 32 * b, pos, rw.lk, a != 2, lane, sh, row);
+        key_block<T, D, DROP, true, FINE>(st, scores<T, D>(kf, qf), vt + o, bias ? bias + 32 * b : nullptr, at, p, j0 + 32 * b, pos, rw.lk, a != 2, lane, sh, row);
       }
     }
     if (more) state = kp.settle(next, next + TILE, kb + (buf ^ 1) * KT, tid);
@@ -170,7 +182,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 ? 4 : 2)) void fwd_
 
 // ---- few query rows: R = Lq * G <= 32 rows (row c = head g = c / Lq of the group, query c % Lq).  A wave's keys meet no other wave's rows, so k goes straight from
 // memory into the first product's operand registers (the next block's while this one is worked on), only v through LDS, two blocks per wave.
-template <typename T, int D, bool DROP>
+template <typename T, int D, bool DROP, bool FINE>
 __global__ __launch_bounds__(256, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void rows_kernel(Params p, int nunits) {
   typedef Geo<T, D> G;
   constexpr int TILE = 32 * G::ROWB;
@@ -227,7 +239,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void row
     const f32x16 s = scores<T, D>(kf, qf);
     if (it + 4 < i1) fetch(tile_at(tl, it + 4) * 32, buf ^ 1);
     const int a = sight.of(j0);
-    if (a && state != 2) key_block<T, D, DROP, false>(st, s, vtile + buf * TILE, state ? kb + buf * 32 : nullptr, at, p, j0, pos, rw.lk, a == 1, lane, sh, row);
+    if (a && state != 2) key_block<T, D, DROP, false, FINE>(st, s, vtile + buf * TILE, state ? kb + buf * 32 : nullptr, at, p, j0, pos, rw.lk, a == 1, lane, sh, row);
     wave_sync();
   }
   // fold the four waves: row maxima first, then sums and accumulators under the common maximum
@@ -359,7 +371,7 @@ inline Plan plan(int nseq, int Lq, int Lk, int H, int Hk, int left, int right, i
   return pl;
 }
 
-template <typename T, int D, bool DROP> int launch_fwd(Params& p, const Plan& pl, hipStream_t s) {
+template <typename T, int D, bool DROP, bool FINE> int launch_fwd(Params& p, const Plan& pl, hipStream_t s) {
   typedef Geo<T, D> G;
   if (pl.rows) {
     const int64_t nu = (int64_t)p.nseq * p.Hk;
@@ -367,17 +379,17 @@ template <typename T, int D, bool DROP> int launch_fwd(Params& p, const Plan& pl
     int lds = 4 * (2 * 32 * G::ROWB + 256);
     const int fold = 1024 + 4 * 32 * (D + 4) * 4;
     if (fold > lds) lds = fold;
-    const int rc = raise_lds<rows_kernel<T, D, DROP>>(lds);
+    const int rc = raise_lds<rows_kernel<T, D, DROP, FINE>>(lds);
     if (rc) return rc;
-    hipLaunchKernelGGL((rows_kernel<T, D, DROP>), dim3((unsigned)(8 * cdiv(nu, 8)), p.nsplit), dim3(256), lds, s, p, (int)nu);
+    hipLaunchKernelGGL((rows_kernel<T, D, DROP, FINE>), dim3((unsigned)(8 * cdiv(nu, 8)), p.nsplit), dim3(256), lds, s, p, (int)nu);
   } else {
     const int nqt = (int)cdiv(p.Lq, QB);
     const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.H : (int64_t)p.nseq * p.H * nqt;
     if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
     const int lds = 4 * G::KT * G::ROWB + 2 * G::KT * 4;
-    const int rc = raise_lds<fwd_kernel<T, D, DROP>>(lds);
+    const int rc = raise_lds<fwd_kernel<T, D, DROP, FINE>>(lds);
     if (rc) return rc;
-    hipLaunchKernelGGL((fwd_kernel<T, D, DROP>), dim3((unsigned)(8 * cdiv(nu, 8)), p.nsplit), dim3(256), lds, s, p, (int)nu, nqt);
+    hipLaunchKernelGGL((fwd_kernel<T, D, DROP, FINE>), dim3((unsigned)(8 * cdiv(nu, 8)), p.nsplit), dim3(256), lds, s, p, (int)nu, nqt);
   }
   int rc = ctclip_check_launch("win_attn_fwd");
   if (rc || p.nsplit == 1) return rc;
@@ -388,7 +400,14 @@ template <typename T, int D, bool DROP> int launch_fwd(Params& p, const Plan& pl
   return ctclip_check_launch("win_attn_fwd join");
 }
 template <typename T, int D> int launch_fwd_d(Params& p, const Plan& pl, hipStream_t s) {
-  return p.drop_p > 0.f ? launch_fwd<T, D, true>(p, pl, s) : launch_fwd<T, D, false>(p, pl, s);
+  // FINE: the second product takes what the rounding of the probabilities left over, too.  Delta = rowsum(dO o O) has an error of the probabilities' rounding over the root of the keys that count; dS
+  // = P o (dP - Delta) has one rounding of its own, and up to 64 visible keys this one would be seen beside it (300 tokens, window 8 + 2:
+  // dq 2.60e-3 from 64 bits, here 2.36e-3; at 81 keys 2.39e-3 without it).  8 x 512 tokens, 12 heads, window 16 + 16: 15.8 -> 17.2 us.
+  if constexpr (sizeof(T) == 2) {
+    const int64_t keys = (int64_t)p.left + p.right + 1 + p.sinks < p.Lk ? (int64_t)p.left + p.right + 1 + p.sinks : p.Lk;
+    if (p.out_lo && keys <= 64) return p.drop_p > 0.f ? launch_fwd<T, D, true, true>(p, pl, s) : launch_fwd<T, D, false, true>(p, pl, s);
+  }
+  return p.drop_p > 0.f ? launch_fwd<T, D, true, false>(p, pl, s) : launch_fwd<T, D, false, false>(p, pl, s);
 }
 template <typename T> int launch_fwd_t(Params& p, const Plan& pl, int D, hipStream_t s) {
   return D == 32 ? launch_fwd_d<T, 32>(p, pl, s) : (D == 64 ? launch_fwd_d<T, 64>(p, pl, s) : launch_fwd_d<T, 128>(p, pl, s));

@@ -410,6 +410,16 @@ def test_window_attention_split_passes(nseq, Lq, Lk, H, Hk, D, window, sinks, q_
     run_case(dtype, nseq, Lq, Lk, H, Hk, D, window, sinks, q_start=q_start, mask=mask, drop=drop, seed=Lk + D)
 
 
+@pytest.mark.parametrize("L,H,D,window,sinks", [(300, 4, 64, (8, 2), 1), (20, 4, 64, (-1, -1), 0), (7, 2, 32, (-1, 0), 0), (300, 2, 128, (16, 0), 1)])
+def test_few_visible_keys_in_training_cost_one_rounding(L, H, D, window, sinks):
+    """Up to 64 visible keys the probabilities' rounding does not reach the output that the backward pass builds on: half a step of the output, and next to it what f32 scores
+    (D products of a sum of about 5 in magnitude, the row's sum once more: 2 * 64 * 5 * 2^-24 < 2^-14) and twice rounded probabilities (2^-17) leave, of sum P |v|."""
+    q, k, v = (rnd((L, H * D), BF16, 90 + i) for i in range(3))
+    o = Fn.window_attention(q.requires_grad_(True), k, v, H, D, window=window, sinks=sinks).detach().double()
+    exact, room = (O.batch64(q.detach(), k, x, H, H, D, [(0, L, 0, L)], *window, sinks, 0, None, 1 / math.sqrt(D), None, None, BF16)["o"][0] for x in (v, v.abs()))
+    assert ((o - exact.to(o)).abs() <= 2.0 ** -8 * exact.abs().to(o) + 2.0 ** -14 * room.to(o)).all()
+
+
 def test_training_captured_and_replayed():
     """Forward and backward of both operators in one graph, with sinks' and split keys' partial sums: each replay equals the eager result."""
     H, D, L = 2, 64, 1500

@@ -11,6 +11,8 @@
 //
 // Bound: HBM, every element is read and written once.  A workgroup takes a few tokens, computes their rot / 2 sines and cosines once into LDS (f32) and
 // then streams the tokens' heads, 16 bytes per load; without the sharing the 24 heads of a BERT token would each pay the ~40 instructions of an angle.
+// MI355X: 32002 tokens, 40 heads of 128 (bf16, interleaved) 131 us a direction, 655 MB at 5.0 TB/s (a large copy: 5.1); 8 x 512 tokens, 24 heads of 64 5.3 us, 25 MB at
+// 4.7 TB/s; f32, 12297 tokens, 16 heads of 32 11.7 us, 50 MB at 4.3 TB/s; four tokens 2.6 us, which is a launch.
 #include "common.h"
 
 namespace {
@@ -110,7 +112,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
   }
 }
 
-// any even rot, any alignment: one thread per pair or passed-through element
+// any even rot, any alignment: one thread per pair or passed-through element, an angle each (on the shapes above 481, 17.1 and 16.6 us)
 template <typename T>
 __global__ __launch_bounds__(256) void rotary_any_kernel(RotaryParams p, int interleaved) {
   const int half = p.rot >> 1, per = half + (p.inplace ? 0 : p.D - p.rot), heads = p.Hq + p.Hk;
@@ -146,7 +148,8 @@ template <typename T> int rotary_launch(RotaryParams& p, int interleaved, hipStr
   if (vec && (int64_t)p.nitem * p.nch < (1 << 20) && heads < 2048 && p.rot <= 512) {
     p.magic = ((1u << 20) + p.nch - 1) / p.nch;
     // tokens of a workgroup: eight items per thread keep the angles' share of the time small, but not at the price of an empty chip (2 048 workgroups:
-    // eight per CU).  One token per workgroup at least: a single token of BERT-base is 96 items.
+    // eight per CU).  One token per workgroup at least: a single token of BERT-base is 96 items.  8 x 512 tokens of 24 heads: 5.3 us; one token always 6.8, sixteen always 7.5;
+    // f32, 12297 tokens of 16 heads of 32: 11.7, 14.0 and 12.0.
     int tb = 2048 / p.nitem;
     if (tb > 16) tb = 16;
     if (tb * (int64_t)2048 > p.M) tb = (int)(p.M / 2048);

@@ -442,7 +442,7 @@ class HipBackend:
         dev, n = q.device, geo.H * geo.D
         with _on(q):
             o = q.new_zeros((geo.Mq, n)) if geo.uncovered else q.new_empty((geo.Mq, n))
-            lse = torch.empty((geo.H, geo.Mq), dtype=torch.float32, device=dev) if want_lse else None
+            lse = torch.empty((2, geo.H, geo.Mq), dtype=torch.float32, device=dev) if want_lse else None
             lo = q.new_empty((geo.Mq, n)) if want_lse and q.dtype == torch.bfloat16 else None
             need = self._win_workspaces(geo)[0]
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None

@@ -155,6 +155,7 @@ template <typename T> int rotary_launch(RotaryParams& p, int interleaved, hipStr
     if (tb * (int64_t)2048 > p.M) tb = (int)(p.M / 2048);
     if (tb < 1) tb = 1;
     p.tb = tb;
+    if (cdiv(p.M, tb) >= (1 << 24)) { ctclip_set_error("rotary: too many rows"); return CTCLIP_EUNSUPPORTED; }      // (2^32 threads of a launch)
     const dim3 grid((unsigned)cdiv(p.M, tb));
     const size_t lds = (size_t)tb * p.rot * 4;
     if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, 1>), grid, dim3(256), lds, s, p);

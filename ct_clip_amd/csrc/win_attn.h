@@ -25,7 +25,8 @@ struct Params {
   int ntiles;
   void *out, *dq, *dk, *dv;
   void* out_lo;                           // bf16: what the rounding of `out` left over (pitch ldo), for the backward pass's Delta; or null
-  float *lse, *delta;                     // [H][query rows]: log2-domain log-sum-exp (+inf for a row that sees nothing), rowsum(dO o O)
+  float *lse, *delta;                     // [2][H][query rows]: maximum and log2 of the sum (0 and +inf for a row that sees nothing), apart: where a mask shifts every key of a row by
+                                          // -1e9 their sum has lost the second; [H][query rows]: rowsum(dO o O)
   float* part;                            // workspace of split passes
   int nseq, Lq, Lk, H, Hk, G;
   int left, right, sinks, q_start;
@@ -210,10 +211,11 @@ template <typename T, int D, int ROWS, int NT> struct Dma {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int r = row(tid, i), c = (tid + i * NT) % Geo<T, D>::NCH;
-      off[i] = (uint32_t)(r * ldb) + (uint32_t)((c ^ swz<Geo<T, D>::NCH>(r)) << 4);
+      const uint64_t o = (uint64_t)(uint32_t)r * (uint32_t)ldb + (uint32_t)((c ^ swz<Geo<T, D>::NCH>(r)) << 4);
+      off[i] = o < 0x7fffffffull ? (uint32_t)o : 0x7fffffffu;              // (a row that far is past the valid ones)
     }
   }
-  // tile, ldb (bytes between rows), valid (rows from the tile's first on that may be read, >= 1) are uniform
+  // tile, ldb (bytes between rows), valid (rows from the tile's first on that may be read, >= 1) are uniform; valid rows lie within 2^31 bytes (check_rows)
   __device__ __forceinline__ void issue(char* lds_tile, const char* tile, int ldb, int valid, int tid) const {
     const uint64_t base = reinterpret_cast<uint64_t>(tile);
     const uint32_t bytes = valid >= ROWS ? 0x7fffffffu : (uint32_t)((valid - 1) * ldb) + (uint32_t)Geo<T, D>::ROWB;
@@ -432,6 +434,12 @@ template <typename T> __device__ __forceinline__ void store_out(const Params& p,
     }
   }
 }
+// the statistics of a finished row: what the backward pass takes its probabilities from
+__device__ __forceinline__ void store_lse(const Params& p, int64_t i, float m, float l) {
+  if (!p.lse) return;
+  p.lse[i] = l == 0.f ? 0.f : m;
+  p.lse[(int64_t)p.H * p.Mq + i] = l == 0.f ? INFINITY : __builtin_amdgcn_logf(l);
+}
 // lanes of a wave exchange through LDS: its operations retire in order, so only the compiler has to keep them in place
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -448,10 +456,12 @@ inline int check_shape(int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, 
   if (packed ? (Lq != Lk || Mq != Mk || q_start) : ((int64_t)q_start + Lq > Lk || Mq != (int64_t)nseq * Lq || Mk != (int64_t)nseq * Lk)) { ctclip_set_error("win_attn: query rows must be positions of the key axis (q_start + Lq <= Lk); packed sequences: q and k|v share their rows"); return CTCLIP_EBADARG; }
   return CTCLIP_OK;
 }
-inline int check_rows(const void* x, int64_t ld, int heads, int D, int dtype, bool written, const char* what) {
+// rows: of a sequence; those of one tile (128 at most) must lie within 2^31 bytes
+inline int check_rows(const void* x, int64_t ld, int rows, int heads, int D, int dtype, bool written, const char* what) {
   const int e = dtype == DT_F32 ? 4 : 2;
   if (!x) { ctclip_set_error("win_attn: null tensor"); return CTCLIP_EBADARG; }
-  if ((reinterpret_cast<uintptr_t>(x) % 16) || (ld * e) % 16 || ld < 0 || ld * e >= (1 << 23) || (written && ld < (int64_t)heads * D)) { ctclip_set_error(what); return CTCLIP_EBADARG; }
+  if ((reinterpret_cast<uintptr_t>(x) % 16) || (ld * e) % 16 || ld < 0 || ld > ((int64_t)1 << 31) / e - 256 || (written && ld < (int64_t)heads * D)) { ctclip_set_error(what); return CTCLIP_EBADARG; }
+  if ((int64_t)((rows < QB ? rows : QB) - 1) * ld * e + (int64_t)D * e >= ((int64_t)1 << 31) - 1) { ctclip_set_error("win_attn: 128 rows within 2 GiB"); return CTCLIP_EUNSUPPORTED; }
   return CTCLIP_OK;
 }
 inline void fill(Params& p, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, int Hk, int left, int right, int sinks, int q_start, float scale, float dropout_p,

@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 && !FINE ? 4 : 2)) 
   store_rows<T, D, false>(lds + wave * 32 * G::ROWB, st.acc, inv, reinterpret_cast<T*>(p.out) + o, p.ldo, rw.lq - wr, lane);
   if (sizeof(T) == 2 && p.out_lo) store_rows<T, D, true>(lds + wave * 32 * G::ROWB, st.acc, inv, reinterpret_cast<T*>(p.out_lo) + o, p.ldo, rw.lq - wr, lane);
   if (!real) return;
-  if (half == 0 && p.lse) p.lse[(int64_t)h * p.Mq + rw.q0 + row] = l == 0.f ? INFINITY : st.m + __builtin_amdgcn_logf(l);
+  if (half == 0) store_lse(p, (int64_t)h * p.Mq + rw.q0 + row, st.m, l);
 }
 
 // ---- few query rows: R = Lq * G <= 32 rows (row c = head g = c / Lq of the group, query c % Lq).  A wave's keys meet no other wave's rows, so k goes straight from
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void row
   const float mul = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
 #pragma unroll
   for (int e = 0; e < PER; e += 4) { float t[4] = {o[e] * mul, o[e + 1] * mul, o[e + 2] * mul, o[e + 3] * mul}; store_out<T>(p, rw.q0 + orow, (int64_t)oh * D + fc + e, t); }
-  if ((tid & 7) == 0 && p.lse) p.lse[(int64_t)oh * p.Mq + rw.q0 + orow] = lsum == 0.f ? INFINITY : m + __builtin_amdgcn_logf(lsum);
+  if ((tid & 7) == 0) store_lse(p, (int64_t)oh * p.Mq + rw.q0 + orow, m, lsum);
 }
 
 // out = sum_s exp2(m_s - M) acc_s / sum_s exp2(m_s - M) l_s over the split passes, in a fixed order.  D / 4 threads across the columns of a (head, row); the others across
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] *= mul;
   store_out<T>(p, row, h * D + col, o);
-  if (col == 0 && p.lse) p.lse[i] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  if (col == 0) store_lse(p, i, m, l);
 }
 
 // ---- host side
@@ -424,7 +424,7 @@ extern "C" int64_t ctclip_win_attn_fwd_workspace(int nseq, int Lq, int Lk, int H
   return n > 1 ? (int64_t)n * H * nseq * Lq * (D + 2) * 4 : 0;
 }
 
-// q (Mq, H D), k | v (Mk, Hk D) -> out (Mq, H D), lse [H][Mq] f32 (log2 domain; optional: backward needs it).  Sequence b = rows b Lq ... of q and b Lk ... of
+// q (Mq, H D), k | v (Mk, Hk D) -> out (Mq, H D), lse [2][H][Mq] f32 (row maximum and log2 of the row's sum, log2 domain; optional: backward needs it).  Sequence b = rows b Lq ... of q and b Lk ... of
 // k | v; with offsets (nseq + 1, int32) the rows offsets[b] ... offsets[b + 1] - 1 of all three (Lq = Lk = the longest), tiles = (sequence, 128-row tile) pairs.
 // keymask: additive f32 per key row; a value <= -1e30 or NaN hides the key, whatever k and v hold there.
 extern "C" int ctclip_win_attn_fwd(const void* q, const void* k, const void* v, const float* keymask, const int32_t* offsets, const int32_t* tiles, int ntiles, void* out,
@@ -437,9 +437,9 @@ extern "C" int ctclip_win_attn_fwd(const void* q, const void* k, const void* v, 
   if (!(scale > 0.f) || !(scale < 1e30f) || !(dropout_p >= 0.f) || !(dropout_p < 1.f)) { ctclip_set_error("win_attn_fwd: scale > 0, 0 <= dropout < 1"); return CTCLIP_EBADARG; }
   if (nseq == 0 || Lq == 0 || (offsets && ntiles == 0)) return CTCLIP_OK;
   if (offsets && (!tiles || ntiles < 0)) { ctclip_set_error("win_attn_fwd: packed sequences need their tiles"); return CTCLIP_EBADARG; }
-  if ((rc = check_rows(q, ldq, H, D, dtype, false, "win_attn_fwd: q rows 16-byte aligned")) || (rc = check_rows(k, ldk, Hk, D, dtype, false, "win_attn_fwd: k rows 16-byte aligned")) ||
-      (rc = check_rows(v, ldv, Hk, D, dtype, false, "win_attn_fwd: v rows 16-byte aligned")) || (rc = check_rows(out, ldo, H, D, dtype, true, "win_attn_fwd: out rows 16-byte aligned, apart")) ||
-      (out_lo && (rc = check_rows(out_lo, ldo, H, D, dtype, true, "win_attn_fwd: out_lo rows 16-byte aligned")))) return rc;
+  if ((rc = check_rows(q, ldq, Lq, H, D, dtype, false, "win_attn_fwd: q rows 16-byte aligned")) || (rc = check_rows(k, ldk, Lk, Hk, D, dtype, false, "win_attn_fwd: k rows 16-byte aligned")) ||
+      (rc = check_rows(v, ldv, Lk, Hk, D, dtype, false, "win_attn_fwd: v rows 16-byte aligned")) || (rc = check_rows(out, ldo, Lq, H, D, dtype, true, "win_attn_fwd: out rows 16-byte aligned, apart")) ||
+      (out_lo && (rc = check_rows(out_lo, ldo, Lq, H, D, dtype, true, "win_attn_fwd: out_lo rows 16-byte aligned")))) return rc;
   Params p{};
   fill(p, nseq, Lq, Lk, Mq, Mk, H, Hk, left, right, sinks, q_start, scale, dropout_p, dropout_seed, offsets, tiles, ntiles, keymask);
   p.q = q; p.k = k; p.v = v; p.out = out; p.out_lo = dtype == DT_BF16 ? out_lo : nullptr; p.lse = lse; p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo;

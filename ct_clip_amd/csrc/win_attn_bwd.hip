@@ -52,10 +52,11 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
     }
     delta = half_sum(delta);
   }
-  float lse = p.lse[(int64_t)h * p.Mq + rw.q0 + row];
+  float top = p.lse[(int64_t)h * p.Mq + rw.q0 + row], lsum = p.lse[(int64_t)(p.H + h) * p.Mq + rw.q0 + row];
   row_frag_arrive<T, D>(qf);
   row_frag_arrive<T, D>(df);
-  asm volatile("" : "+v"(lse));
+  asm volatile("" : "+v"(top), "+v"(lsum));
+  const float lse = top + lsum;
   if (real && half == 0) p.delta[(int64_t)h * p.Mq + rw.q0 + row] = delta;
   const Sight sight(wlo, whi, p.left, p.right, p.sinks, rw.lk);
   const LaneAt<T, D> at(lane);
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
           for (int g = 0; g < 4; ++g) {
             const f32x4 a = *reinterpret_cast<const f32x4*>(kb + buf * KT + 32 * b + 8 * g + 4 * half);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pr[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], p.scale2, a[e] - lse));
+            for (int e = 0; e < 4; ++e) pr[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], p.scale2, a[e]) - top - lsum);
           }
         } else {
 #pragma unroll
@@ -141,8 +142,8 @@ template <typename T, int D> struct Dkv {
   static constexpr int PAIR = IN_LDS ? 2 : 1, WAVES = 4 * PAIR, NT = 64 * WAVES;
   static constexpr int QT = sizeof(T) == 2 ? 64 : 32;      // query rows of a step
   static constexpr int TILE = QT * Geo<T, D>::ROWB, KEYS = IN_LDS ? 2 * QB * Geo<T, D>::ROWB : 0;      // bytes: a tile of rows, k and v
-  static constexpr int WINDOW = KEYS + 4 * TILE + 4 * QT * 4;                                          // [k | v], [2][Q | dO], [2][lse | Delta]
-  static constexpr int OWN = 64 * Geo<T, D>::ROWB + 256;                                               // a wave's [Q | dO | lse | Delta] of 32 rows
+  static constexpr int WINDOW = KEYS + 4 * TILE + 6 * QT * 4;                                          // [k | v], [2][Q | dO], [2][statistics]
+  static constexpr int OWN = 64 * Geo<T, D>::ROWB + 384;                                               // a wave's [Q | dO | statistics] of 32 rows
   static constexpr int SINK = (IN_LDS ? 64 * Geo<T, D>::ROWB : 0) + WAVES * OWN, FOLD = WAVES * 32 * (D + 4) * 4;
   static constexpr int LDS = WINDOW > SINK ? (WINDOW > FOLD ? WINDOW : FOLD) : (SINK > FOLD ? SINK : FOLD);
 };
@@ -180,7 +181,7 @@ __device__ __forceinline__ void drop_of_key(float (&m)[16], const Params& p, int
 }
 // FAR: the sink pass (keys seen because they are sinks, j < i - left); otherwise the window (i - left <= j <= i + right).
 template <typename T, int D, bool DROP, bool FAR>
-__device__ __forceinline__ void query_block(KeyState<T, D>& st, const char* qt, const char* dt, const float* lse, const float* delta, const LaneAt<T, D>& at, const Params& p,
+__device__ __forceinline__ void query_block(KeyState<T, D>& st, const char* qt, const char* dt, const float* stat, int rows, const LaneAt<T, D>& at, const Params& p,
                                             int row, int j, float kbias, bool partial, int lane, int64_t sh) {
   const int half = lane >> 5;
   constexpr bool IN_LDS = Dkv<T, D>::IN_LDS;
@@ -206,12 +207,23 @@ __device__ __forceinline__ void query_block(KeyState<T, D>& st, const char* qt, 
       s[r] = (FAR ? (sink && i > rh) : (i >= rl && i <= rh)) ? s[r] : -INFINITY;
     }
   }
-  float pr[16], dm[16], ls[16], de[16];
+  float pr[16], dm[16], ls[16], de[16];    // (stat: RowSource::put_stat)
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(lse + 8 * g + 4 * half), b = *reinterpret_cast<const f32x4*>(delta + 8 * g + 4 * half);
+    const f32x4 a = *reinterpret_cast<const f32x4*>(stat + 8 * g + 4 * half), b = *reinterpret_cast<const f32x4*>(stat + rows + 8 * g + 4 * half);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { ls[4 * g + e] = kbias - a[e]; de[4 * g + e] = b[e]; }
+    for (int e = 0; e < 4; ++e) { ls[4 * g + e] = a[e]; de[4 * g + e] = b[e]; }
+  }
+  if (p.keymask) {                         // kernel-uniform; without a mask: 0, and keys past the end are zeros whose gradients nobody stores
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(stat + 2 * rows + 8 * g + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[4 * g + e] = fmaf(s[4 * g + e], p.scale2, kbias) - a[e] - ls[4 * g + e];
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.scale2, -ls[r]);
   }
   if (DROP) drop_of_key(dm, p, sh, row, j, half);
   PFrag<T> pf, df;
@@ -226,7 +238,7 @@ __device__ __forceinline__ void query_block(KeyState<T, D>& st, const char* qt, 
   if constexpr (!IN_LDS) col_frag_lds<D>(dc, dt, at);
   float pd[16];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) { pr[r] = __builtin_amdgcn_exp2f(fmaf(s[r], p.scale2, ls[r])); pd[r] = DROP ? pr[r] * dm[r] : pr[r]; }
+  for (int r = 0; r < 16; ++r) { pr[r] = __builtin_amdgcn_exp2f(s[r]); pd[r] = DROP ? pr[r] * dm[r] : pr[r]; }
   p_frag(pf, pd);
   if constexpr (IN_LDS) col_frag_lds<D>(dc, dt, at);
   else col_frag_lds<D>(qc, qt, at);
@@ -284,25 +296,33 @@ template <int ROWS, typename T, int D> __device__ __forceinline__ float load_key
 struct RowSource {
   const char *q, *d;
   const float *lse, *delta;
+  int64_t sums;                            // from a row's maximum to the log of its sum
   int ldq, ldd, lq, r0;
-  float sl, sdel;
+  float st, sl, sdel;
   template <typename T, int D> __device__ __forceinline__ void init(const Params& p, const Rows& rw, int h0) {
     q = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.q) + rw.q0 * p.ldq + (int64_t)h0 * D);
     d = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.dout) + rw.q0 * p.lddo + (int64_t)h0 * D);
     lse = p.lse + (int64_t)h0 * p.Mq + rw.q0;
     delta = p.delta + (int64_t)h0 * p.Mq + rw.q0;
     ldq = (int)p.ldq * (int)sizeof(T); ldd = (int)p.lddo * (int)sizeof(T);
-    lq = rw.lq; r0 = 0; sl = 0.f; sdel = 0.f;
+    sums = (int64_t)p.H * p.Mq;
+    lq = rw.lq; r0 = 0; st = 0.f; sl = 0.f; sdel = 0.f;
   }
   template <int ROWS> __device__ __forceinline__ void get_stat(const Params& p, int g, int tid) {
     const int r = r0 + (tid & (ROWS - 1)) < lq ? r0 + (tid & (ROWS - 1)) : lq - 1;
     const int64_t at = (int64_t)g * p.Mq + r;
-    sl = lse[at];                          // (loaded whatever the row: a branch around a load is waited for at its end)
+    st = lse[at];                          // (loaded whatever the row: a branch around a load is waited for at its end)
+    sl = lse[at + sums];
     sdel = delta[at];
   }
-  template <int ROWS> __device__ __forceinline__ void put_stat(float* stat, int tid) const {      // log-sum-exps, then Deltas; rows past the end: probability 0
+  // what is taken off a score in the end, Deltas, what is taken off it first: without a mask the log-sum-exp at once; rows past the end: probability 0
+  template <int ROWS> __device__ __forceinline__ void put_stat(float* stat, bool masked, int tid) const {
     const int r = r0 + (tid & (ROWS - 1));
-    if (tid < ROWS) { stat[tid] = r < lq ? sl : INFINITY; stat[ROWS + tid] = r < lq ? sdel : 0.f; }
+    if (tid < ROWS) {
+      stat[tid] = r < lq ? (masked ? sl : st + sl) : INFINITY;
+      stat[ROWS + tid] = r < lq ? sdel : 0.f;
+      if (masked) stat[2 * ROWS + tid] = r < lq ? st : 0.f;
+    }
   }
 };
 template <typename T, int D, int ROWS, int NT> struct RowPipe {    // through LDS-DMA: issue() into a buffer that nobody reads, settle() before the barrier
@@ -319,9 +339,9 @@ template <typename T, int D, int ROWS, int NT> struct RowPipe {    // through LD
     dd.issue(dt, src.d + (int64_t)first * src.ldd + g * (D * (int)sizeof(T)), src.ldd, src.lq - first, tid);
     src.get_stat<ROWS>(p, g, tid);
   }
-  __device__ __forceinline__ void settle(float* stat, int tid) const {
+  __device__ __forceinline__ void settle(float* stat, bool masked, int tid) const {
     dma_arrive();
-    src.put_stat<ROWS>(stat, tid);
+    src.put_stat<ROWS>(stat, masked, tid);
   }
 };
 // where the partial sums of key j lie: split passes hold every key, unsplit ones the keys of the sink blocks
@@ -361,7 +381,7 @@ __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, 
   RowPipe<T, D, QT, X::NT> rp(p, rw, u.hk * p.G, tid);
   if (i0 < i1) {
     rp.issue(p, ring, ring + TILE, i0 / nt, (t0 + i0 % nt) * QT, tid);
-    rp.settle(stat, tid);
+    rp.settle(stat, p.keymask != nullptr, tid);
   }
   __syncthreads();
   int g = i0 < i1 ? i0 / nt : 0, t = i0 < i1 ? i0 % nt : 0;        // the step's head of the group and tile
@@ -379,11 +399,10 @@ __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, 
       const int see = any ? Sight(lo, lo + 31 < last ? lo + 31 : last, p.left, p.right, 0, rw.lk).of(jw) : 0;
       if (see) {
         const char* qt = ring + buf * 2 * TILE + 32 * b * G::ROWB;
-        const float* sp = stat + buf * 2 * QT + 32 * b;
-        query_block<T, D, DROP, false>(st, qt, qt + TILE, sp, sp + QT, at, p, r0 + 32 * b, j, kbias, see == 1, lane, sh);
+        query_block<T, D, DROP, false>(st, qt, qt + TILE, stat + buf * 3 * QT + 32 * b, QT, at, p, r0 + 32 * b, j, kbias, see == 1, lane, sh);
       }
     }
-    if (more) rp.settle(stat + (buf ^ 1) * 2 * QT, tid);
+    if (more) rp.settle(stat + (buf ^ 1) * 3 * QT, p.keymask != nullptr, tid);
     __syncthreads();
   }
   if constexpr (X::PAIR == 2) {            // the second wave of a pair hands its sums to the first, lane to lane: [block][register][lane], dK, then dV
@@ -445,9 +464,9 @@ __device__ __forceinline__ void sink_pass(const Params& p, char* lds, int id, in
   for (int i = i0 + wave; i < i1; i += X::WAVES) {                 // (the other waves of the SIMD work while this one waits for its rows)
     const int g = i / nt, r0 = (t0 + i % nt) * 32;
     rp.issue(p, qtile, dtile, g, r0, lane);
-    rp.settle(stat, lane);
+    rp.settle(stat, p.keymask != nullptr, lane);
     wave_sync();
-    query_block<T, D, DROP, true>(st, qtile, dtile, stat, stat + 32, at, p, r0, j, kbias, true, lane, (int64_t)b * p.H + hk * p.G + g);
+    query_block<T, D, DROP, true>(st, qtile, dtile, stat, 32, at, p, r0, j, kbias, true, lane, (int64_t)b * p.H + hk * p.G + g);
     wave_sync();
   }
   // fold the waves, dK then dV, in their order
@@ -635,11 +654,11 @@ extern "C" int ctclip_win_attn_bwd(const void* q, const void* k, const void* v, 
   if (nseq == 0 || Lk == 0 || Lq == 0 || (offsets && ntiles == 0)) return CTCLIP_OK;
   if (offsets && (!tiles || ntiles < 0)) { ctclip_set_error("win_attn_bwd: packed sequences need their tiles"); return CTCLIP_EBADARG; }
   if (!lse || !delta) { ctclip_set_error("win_attn_bwd: needs lse and delta"); return CTCLIP_EBADARG; }
-  if ((rc = check_rows(q, ldq, H, D, dtype, false, "win_attn_bwd: q rows 16-byte aligned")) || (rc = check_rows(k, ldk, Hk, D, dtype, false, "win_attn_bwd: k rows 16-byte aligned")) ||
-      (rc = check_rows(v, ldv, Hk, D, dtype, false, "win_attn_bwd: v rows 16-byte aligned")) || (rc = check_rows(o, ldo, H, D, dtype, false, "win_attn_bwd: o rows 16-byte aligned")) ||
-      (o_lo && (rc = check_rows(o_lo, ldo, H, D, dtype, false, "win_attn_bwd: o_lo rows 16-byte aligned"))) ||
-      (rc = check_rows(dout, lddo, H, D, dtype, false, "win_attn_bwd: dout rows 16-byte aligned")) || (rc = check_rows(dq, lddq, H, D, dtype, true, "win_attn_bwd: dq rows 16-byte aligned, apart")) ||
-      (rc = check_rows(dk, lddk, Hk, D, dtype, true, "win_attn_bwd: dk rows 16-byte aligned, apart")) || (rc = check_rows(dv, lddv, Hk, D, dtype, true, "win_attn_bwd: dv rows 16-byte aligned, apart"))) return rc;
+  if ((rc = check_rows(q, ldq, Lq, H, D, dtype, false, "win_attn_bwd: q rows 16-byte aligned")) || (rc = check_rows(k, ldk, Lk, Hk, D, dtype, false, "win_attn_bwd: k rows 16-byte aligned")) ||
+      (rc = check_rows(v, ldv, Lk, Hk, D, dtype, false, "win_attn_bwd: v rows 16-byte aligned")) || (rc = check_rows(o, ldo, Lq, H, D, dtype, false, "win_attn_bwd: o rows 16-byte aligned")) ||
+      (o_lo && (rc = check_rows(o_lo, ldo, Lq, H, D, dtype, false, "win_attn_bwd: o_lo rows 16-byte aligned"))) ||
+      (rc = check_rows(dout, lddo, Lq, H, D, dtype, false, "win_attn_bwd: dout rows 16-byte aligned")) || (rc = check_rows(dq, lddq, Lq, H, D, dtype, true, "win_attn_bwd: dq rows 16-byte aligned, apart")) ||
+      (rc = check_rows(dk, lddk, Lk, Hk, D, dtype, true, "win_attn_bwd: dk rows 16-byte aligned, apart")) || (rc = check_rows(dv, lddv, Lk, Hk, D, dtype, true, "win_attn_bwd: dv rows 16-byte aligned, apart"))) return rc;
   Params p{};
   fill(p, nseq, Lq, Lk, Mq, Mk, H, Hk, left, right, sinks, q_start, scale, dropout_p, dropout_seed, offsets, tiles, ntiles, keymask);
   p.q = q; p.k = k; p.v = v; p.o = o; p.out_lo = dtype == DT_BF16 ? const_cast<void*>(o_lo) : nullptr; p.dout = dout; p.lse = const_cast<float*>(lse); p.delta = delta; p.dq = dq; p.dk = dk; p.dv = dv;

@@ -1288,8 +1288,10 @@ class RotaryFn(Function):
     @staticmethod
     def forward(ctx, q, k, rope, D, L, positions, start):
         turns = rope.turns(q.device)
-        ctx.args = (turns, D, rope.dim, L, positions, start, rope.interleaved, rope.magnitude)      # (positions: integers, not differentiated, not an output)
-        qo, ko = B().rotary(q, k, *ctx.args)
+        ctx.args = (turns, D, rope.dim, L), (start, rope.interleaved, rope.magnitude)
+        if positions is not None:
+            ctx.save_for_backward(positions)               # (changed in place before the backward pass: refused there)
+        qo, ko = B().rotary(q, k, *ctx.args[0], positions, *ctx.args[1])
         return qo if k is None else (qo, ko)
 
     @staticmethod
@@ -1299,7 +1301,8 @@ class RotaryFn(Function):
             dq = dq.contiguous()
         if dk is not None and dk.stride(1) != 1:
             dk = dk.contiguous()
-        gq, gk = B().rotary(dq, dk, *ctx.args, True)
+        positions, = ctx.saved_tensors or (None,)
+        gq, gk = B().rotary(dq, dk, *ctx.args[0], positions, *ctx.args[1], True)
         return gq, gk, None, None, None, None, None
 
 

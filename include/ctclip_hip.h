@@ -320,7 +320,7 @@ int ctclip_shadow_refresh(const void* jobs, int njobs, int64_t ntiles, hipStream
 /* bytes of workspace ctclip_win_attn_fwd needs (partial results of a split key axis; 0: none).  packed: 1 with offsets.  [no reference counterpart: workspace query] */
 int64_t ctclip_win_attn_fwd_workspace(int nseq, int Lq, int Lk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int packed);
 
-/* Attention in a sliding window with sinks: out = softmax(scale q k^T + keymask) v, position i sees key j when j <= i + right and (j >= i - left or j < sinks); left / right = -1: no limit.  q (Mq, H D), k | v (Mk, Hk D), head h reads k|v head h / (H / Hk); D = 32, 64 or 128.  Sequence b = rows b Lq ... of q at positions q_start ... (q_start + Lq <= Lk) and rows b Lk ... of k | v; with offsets (nseq + 1 int32 on the device) rows offsets[b] ... offsets[b + 1] - 1 of all three tensors (Mq = Mk, Lq = Lk = the longest, q_start = 0), tiles = ntiles (sequence, 128-row tile) int32 pairs covering them; rows outside are not written.  keymask: additive f32 per key row or NULL; a value <= -1e30 or NaN hides the key whatever k and v hold there (a key that a window hides from some rows of a 128-row tile and shows to others must be finite).  A row that sees nothing is 0.  lse: [H][Mq] f32, log2 of the sum of exponentials (+inf for a row that sees nothing), NULL: not wanted.  out_lo (bf16; pitch ldo; or NULL): what the rounding of out left over, for the backward pass.  Attention dropout as in ctclip_attn_fwd, masks by query ROW and key.  Rows 16-byte aligned.  [HF BertSelfAttention (ct_clip.py:685-686) for reports longer than its window; no reference counterpart for the window] */
+/* Attention in a sliding window with sinks: out = softmax(scale q k^T + keymask) v, position i sees key j when j <= i + right and (j >= i - left or j < sinks); left / right = -1: no limit.  q (Mq, H D), k | v (Mk, Hk D), head h reads k|v head h / (H / Hk); D = 32, 64 or 128.  Sequence b = rows b Lq ... of q at positions q_start ... (q_start + Lq <= Lk) and rows b Lk ... of k | v; with offsets (nseq + 1 int32 on the device) rows offsets[b] ... offsets[b + 1] - 1 of all three tensors (Mq = Mk, Lq = Lk = the longest, q_start = 0), tiles = ntiles (sequence, 128-row tile) int32 pairs covering them; rows outside are not written.  keymask: additive f32 per key row or NULL; a value <= -1e30 or NaN hides the key whatever k and v hold there (a key that a window hides from some rows of a 128-row tile and shows to others must be finite).  A row that sees nothing is 0.  lse: [2][H][Mq] f32, a row's maximum and the log2 of its sum of exponentials, log2 domain (0 and +inf for a row that sees nothing), NULL: not wanted.  out_lo (bf16; pitch ldo; or NULL): what the rounding of out left over, for the backward pass.  Attention dropout as in ctclip_attn_fwd, masks by query ROW and key.  Rows 16-byte aligned.  [HF BertSelfAttention (ct_clip.py:685-686) for reports longer than its window; no reference counterpart for the window] */
 int ctclip_win_attn_fwd(const void* q, const void* k, const void* v, const float* keymask, const int32_t* offsets, const int32_t* tiles, int ntiles, void* out, void* out_lo, float* lse, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, float dropout_p, uint64_t dropout_seed, int dtype, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /* bytes of workspace ctclip_win_attn_bwd needs (partial sums of the sinks' gradients and of split key tiles; 0: none).  ntiles: packed sequences, else 0.  [no reference counterpart: workspace query] */

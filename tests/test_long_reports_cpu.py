@@ -163,6 +163,19 @@ def test_c_entries_answer_before_any_launch():
     assert lib.ctclip_win_attn_bwd_workspace(0, 8, 8, 0, 2, 1, 64, 4, 4, 1, 0, 0) == 0 and lib.ctclip_win_attn_bwd_workspace(1, 64, 64, 64, 2, 1, 64, 4, 4, 1, 0, 0) > 0
 
 
+def test_c_entries_refuse_rows_that_a_launch_cannot_reach():
+    from ct_clip_amd import _lib
+    lib = _lib.load()
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+
+    def fwd(ldq=64, ldk=64, L=128):
+        return lib.ctclip_win_attn_fwd(p, p, p, None, None, None, 0, p, None, None, 1, L, L, L, L, 1, 1, 64, 4, 4, 0, 0, ldq, ldk, 64, 64, 1.0, 0.0, 0, 1, None, 0, None)
+    assert fwd(ldq=2 ** 24) == fwd(ldk=2 ** 24) == fwd(ldk=2 ** 24, L=70) == -2 and b"2 GiB" in lib.ctclip_last_error()
+    assert fwd(ldq=2 ** 31) == fwd(ldk=2 ** 30) == -1
+    assert lib.ctclip_rotary(p, None, p, None, p, None, 0, 2 ** 28, 1, 0, 1, 0, 8, 8, 8, 0, 8, 0, 1, 1.0, 0, 1, None) == -2
+
+
 # --------------------------------------------------------------------------------------------------------------- composition
 
 def test_bounds_notice_a_wrong_oracle():

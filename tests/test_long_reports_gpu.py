@@ -420,6 +420,58 @@ def test_few_visible_keys_in_training_cost_one_rounding(L, H, D, window, sinks):
     assert ((o - exact.to(o)).abs() <= 2.0 ** -8 * exact.abs().to(o) + 2.0 ** -14 * room.to(o)).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("window,sinks,D", [((-1, -1), 0, 64), ((40, 10), 3, 64), ((30, 0), 2, 128)])
+def test_mask_that_drowns_the_scores(window, sinks, D, dtype):
+    """-1e9 on every key of a sequence: the scores are below the mask's last bit, so every visible key counts the same, in the gradients as in the output."""
+    L, H = 150, 2
+    q, k, v, do = (rnd((L, H * D), dtype, 70 + i) for i in range(4))
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = Fn.window_attention(*leaves, H, D, window=window, sinks=sinks, keymask=torch.full((L,), -1e9, device=DEV))
+    dq, dk, dv = torch.autograd.grad(o, leaves, do)
+    i, j = torch.arange(L)[:, None], torch.arange(L)[None, :]
+    left, right = (L if x < 0 else x for x in window)
+    see = (j <= i + right) & ((j >= i - left) | (j < sinks))
+    P = see.double() / see.sum(1, keepdim=True)
+    q, k, v, do = (t.detach().double().cpu().view(L, H, D).transpose(0, 1) for t in (q, k, v, do))
+    dP = do @ v.transpose(1, 2)
+    dS = P * (dP - (P * dP).sum(2, keepdim=True)) / math.sqrt(D)
+    half = torch.finfo(dtype).eps / 2
+    # roundings: P, dS to the operand type, the result, and the row sums under dS (two terms of P |dP|); f32 sums of up to L terms
+    sums = L * O.U32
+    room_S = P * (dP.abs() + 2 * (P * dP.abs()).sum(2, keepdim=True)) / math.sqrt(D)
+    for got, want, room in ((o, P @ v, P @ v.abs()), (dv, P.t() @ do, P.t() @ do.abs()), (dq, dS @ k, room_S @ k.abs()), (dk, dS.transpose(1, 2) @ q, room_S.transpose(1, 2) @ q.abs())):
+        got = got.detach().double().cpu().view(L, H, D).transpose(0, 1)
+        assert ((got - want).abs() <= half * want.abs() + (half + 4 * sums) * room).all()
+
+
+@pytest.mark.parametrize("dtype,pitch", [(BF16, 5 * 2 ** 20), (F32, 3 * 2 ** 20 + 64)])
+def test_rows_far_apart(dtype, pitch):
+    """The [CLS] rows of long sequences inside their projection: more than 8 MB between two rows of q, and between the rows of its gradient."""
+    H, D, Lk, n = 2, 64, 300, 3
+    buf = torch.zeros((n, pitch), dtype=dtype, device=DEV)
+    buf[:, :H * D] = rnd((n, H * D), dtype, 1)
+    q = buf[:, :H * D].detach().requires_grad_(True)
+    k, v, do = rnd((n * Lk, H * D), dtype, 2).requires_grad_(True), rnd((n * Lk, H * D), dtype, 3).requires_grad_(True), rnd((n, H * D), dtype, 4)
+    assert q.stride(0) == pitch
+    wide = torch.zeros_like(buf)
+    wide[:, :H * D] = do
+    o = Fn.window_attention(q, k, v, H, D, nseq=n, window=(50, 50), sinks=1)
+    want = O.batch64(q.detach(), k.detach(), v.detach(), H, H, D, [(b, 1, b * Lk, Lk) for b in range(n)], 50, 50, 1, 0, None, D ** -0.5, do, None, dtype)
+    O.check(o.detach(), want["o"], "o")
+    for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, (q, k, v), wide[:, :H * D])):
+        O.check(g, want[name], name)
+
+
+def test_positions_changed_before_the_backward_pass_are_refused():
+    x = rnd((40, 64), F32, 1).requires_grad_(True)
+    positions = torch.arange(40, device=DEV)
+    y = Fn.rotary(x, None, Fn.RotaryPositions(64), 64, positions=positions)
+    positions.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+
+
 def test_training_captured_and_replayed():
     """Forward and backward of both operators in one graph, with sinks' and split keys' partial sums: each replay equals the eager result."""
     H, D, L = 2, 64, 1500

@@ -130,6 +130,11 @@ __device__ __forceinline__ void p_frag(PFrag<float>& f, const float (&p)[16]) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) f.v[r] = p[r];
 }
+// what that rounding left over (bf16), for a second product with the same other operand
+__device__ __forceinline__ void p_rest(float (&p)[16]) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) p[r] -= bf2f(f2bf(p[r]));
+}
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 // A lane's byte offsets inside a 32-row block, computed once: `row` for the products along D (row c = lane & 31), `col` for the transposing reads of the second
 // product (32-column block i, rows + 8 u).  Blocks are multiples of 32 rows apart, which the chunk permutation does not see, so everything else is an immediate.
@@ -473,6 +478,18 @@ inline void fill(Params& p, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, in
   p.offsets = offsets; p.tiles = tiles; p.ntiles = ntiles; p.keymask = keymask;
 }
 
+// FINE (bf16, training): P and dS are rounded to the operand type for the second products; FINE passes take what that left over as well, in a second instruction each.
+//   Forward, up to 64 visible keys: Delta = rowsum(dO o O) has the probabilities' rounding over the root of the keys that count, which would be seen beside the one rounding that
+//   dS = P o (dP - Delta) has of its own (300 tokens, window 8 + 2: dq 2.60e-3 from 64 bits, then 2.36e-3; at 81 keys 2.39e-3 without it).  8 x 512 tokens, 12 heads, window
+//   16 + 16: 15.8 -> 17.2 us.
+//   Both passes, up to 2^20 pairs of a query and a visible key: few probabilities leave no average of their roundings (4 tokens, 4 heads: 2.6e-3), and a call of that size is
+//   launches and latency: forward and
+//   backward of 8 x 4 tokens 4.8 + 13.1 -> 4.9 + 13.9 us, of 500 tokens, 12 heads, window 80 + 80 (0.97 * 2^20 pairs) 15.5 + 34.9 -> 16.7 + 37.5; errors 2.35e-3 -> 1.66e-3,
+//   which is the results' own rounding.
+inline bool fine_pass(const Params& p, int dtype, bool backward) {
+  const int64_t window = (int64_t)p.left + p.right + 1 + p.sinks, keys = window < p.Lk ? window : p.Lk;
+  return dtype == DT_BF16 && ((!backward && keys <= 64) || keys * p.Mq * p.H <= (1 << 20));
+}
 template <auto KERNEL> int raise_lds(int bytes) {       // more than 64 KB of LDS is opted into, once per kernel and device
   static bool done[64] = {};
   int dev = 0;

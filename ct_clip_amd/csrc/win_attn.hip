@@ -6,7 +6,7 @@
 //                waves take different key tiles and the axis is split over workgroups until the chip is full.  Bound by reading k and v once.
 //   join_kernel  folds the split passes of either.
 // One pass over the keys with the running maximum and sum of the softmax in f32, log2 domain.  P is rounded to the operand type (bf16: half a step is 2^-8 of the value,
-// one rounding per probability) because the matrix cores read it; sums are taken of the unrounded values.  FINE adds what that rounding left over (launch_fwd_d).
+// one rounding per probability) because the matrix cores read it; sums are taken of the unrounded values.  FINE adds what that rounding left over (win_attn.h, fine_pass).
 //
 // Bounds, MI355X.  One token of 4 sequences over 32768 keys, 32 heads of 128 on 8: 113 + 4 us (rows + join), 537 MB at 4.7 TB/s; a large copy runs at 5.1.  4 x 8192 tokens,
 // 12 heads of 64, window 256 + 256: 97 us, 0.53 PFLOP/s of 1.2 that a large product reaches: matrix instructions 0.27 of the time, vector instructions (exponentials, masks,
@@ -90,8 +90,7 @@ __device__ __forceinline__ void key_block(SoftRow<D>& st, f32x16 s, const char* 
   col_frag_lds<D>(vf, vt, at);
   mma_cols<D>(st.acc, vf, pf, lane);
   if constexpr (FINE) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) pr[r] -= bf2f(f2bf(pr[r]));
+    p_rest(pr);
     p_frag(pf, pr);
     mma_cols<D>(st.acc, vf, pf, lane);
   }
@@ -401,12 +400,8 @@ template <typename T, int D, bool DROP, bool FINE> int launch_fwd(Params& p, con
   return ctclip_check_launch("win_attn_fwd join");
 }
 template <typename T, int D> int launch_fwd_d(Params& p, const Plan& pl, hipStream_t s) {
-  // FINE: the second product takes what the rounding of the probabilities left over, too.  Delta = rowsum(dO o O) has an error of the probabilities' rounding over the root of the keys that count; dS
-  // = P o (dP - Delta) has one rounding of its own, and up to 64 visible keys this one would be seen beside it (300 tokens, window 8 + 2:
-  // dq 2.60e-3 from 64 bits, here 2.36e-3; at 81 keys 2.39e-3 without it).  8 x 512 tokens, 12 heads, window 16 + 16: 15.8 -> 17.2 us.
   if constexpr (sizeof(T) == 2) {
-    const int64_t keys = (int64_t)p.left + p.right + 1 + p.sinks < p.Lk ? (int64_t)p.left + p.right + 1 + p.sinks : p.Lk;
-    if (p.out_lo && keys <= 64) return p.drop_p > 0.f ? launch_fwd<T, D, true, true>(p, pl, s) : launch_fwd<T, D, false, true>(p, pl, s);
+    if (p.out_lo && fine_pass(p, DT_BF16, false)) return p.drop_p > 0.f ? launch_fwd<T, D, true, true>(p, pl, s) : launch_fwd<T, D, false, true>(p, pl, s);
   }
   return p.drop_p > 0.f ? launch_fwd<T, D, true, false>(p, pl, s) : launch_fwd<T, D, false, false>(p, pl, s);
 }

@@ -16,7 +16,7 @@
 
 namespace win {
 
-template <typename T, int D, bool DROP>
+template <typename T, int D, bool DROP, bool FINE>
 __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nqt) {
   typedef Geo<T, D> G;
   constexpr int KT = G::KT, TILE = KT * G::ROWB;
@@ -125,6 +125,11 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
         PFrag<T> pf;
         p_frag(pf, pr);
         mma_cols<T, D>(acc, kt, at, pf, lane);
+        if constexpr (FINE) {
+          p_rest(pr);
+          p_frag(pf, pr);
+          mma_cols<T, D>(acc, kt, at, pf, lane);
+        }
       }
     }
     if (more) state = kp.settle(next, next + TILE, kb + (buf ^ 1) * KT, tid);
@@ -180,7 +185,7 @@ __device__ __forceinline__ void drop_of_key(float (&m)[16], const Params& p, int
   }
 }
 // FAR: the sink pass (keys seen because they are sinks, j < i - left); otherwise the window (i - left <= j <= i + right).
-template <typename T, int D, bool DROP, bool FAR>
+template <typename T, int D, bool DROP, bool FAR, bool FINE>
 __device__ __forceinline__ void query_block(KeyState<T, D>& st, const char* qt, const char* dt, const float* stat, int rows, const LaneAt<T, D>& at, const Params& p,
                                             int row, int j, float kbias, bool partial, int lane, int64_t sh) {
   const int half = lane >> 5;
@@ -243,11 +248,21 @@ __device__ __forceinline__ void query_block(KeyState<T, D>& st, const char* qt, 
   if constexpr (IN_LDS) col_frag_lds<D>(dc, dt, at);
   else col_frag_lds<D>(qc, qt, at);
   mma_cols<D>(st.dv, dc, pf, lane);
+  if constexpr (FINE) {
+    p_rest(pd);
+    p_frag(pf, pd);
+    mma_cols<D>(st.dv, dc, pf, lane);
+  }
 #pragma unroll
   for (int r = 0; r < 16; ++r) pr[r] *= (DROP ? dp[r] * dm[r] : dp[r]) - de[r];
   p_frag(df, pr);
   if constexpr (IN_LDS) col_frag_lds<D>(qc, qt, at);
   mma_cols<D>(st.dk, qc, df, lane);
+  if constexpr (FINE) {
+    p_rest(pr);
+    p_frag(df, pr);
+    mma_cols<D>(st.dk, qc, df, lane);
+  }
 }
 
 // A wave's keys j, 32 of the ROWS that its workgroup has (the first is `first`): into its registers, or all of them into LDS, which every wave takes part in.  Hidden keys
@@ -351,7 +366,7 @@ __device__ __forceinline__ int64_t part_row(const Params& p, const Rows& rw, int
 __host__ __device__ inline int64_t part_rows(const Params& p) { return p.nsplit > 1 ? (int64_t)p.Hk * p.Mk : (int64_t)p.nseq * p.Hk * p.s32; }
 __host__ __device__ inline int64_t sink_rows(const Params& p) { return (int64_t)p.nseq * p.Hk * p.s32; }
 
-template <typename T, int D, bool DROP>
+template <typename T, int D, bool DROP, bool FINE>
 __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, int split, int nunits, int nkt) {
   typedef Geo<T, D> G;
   typedef Dkv<T, D> X;
@@ -399,7 +414,7 @@ __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, 
       const int see = any ? Sight(lo, lo + 31 < last ? lo + 31 : last, p.left, p.right, 0, rw.lk).of(jw) : 0;
       if (see) {
         const char* qt = ring + buf * 2 * TILE + 32 * b * G::ROWB;
-        query_block<T, D, DROP, false>(st, qt, qt + TILE, stat + buf * 3 * QT + 32 * b, QT, at, p, r0 + 32 * b, j, kbias, see == 1, lane, sh);
+        query_block<T, D, DROP, false, FINE>(st, qt, qt + TILE, stat + buf * 3 * QT + 32 * b, QT, at, p, r0 + 32 * b, j, kbias, see == 1, lane, sh);
       }
     }
     if (more) rp.settle(stat + (buf ^ 1) * 3 * QT, p.keymask != nullptr, tid);
@@ -439,7 +454,7 @@ __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, 
   store_rows<T, D, false>(turn, st.dv, 1.f, reinterpret_cast<T*>(p.dv) + (rw.k0 + jw) * p.lddv + (int64_t)u.hk * D, p.lddv, rw.lk - jw, lane);
 }
 
-template <typename T, int D, bool DROP>
+template <typename T, int D, bool DROP, bool FINE>
 __device__ __forceinline__ void sink_pass(const Params& p, char* lds, int id, int nblk) {
   typedef Geo<T, D> G;
   typedef Dkv<T, D> X;
@@ -466,7 +481,7 @@ __device__ __forceinline__ void sink_pass(const Params& p, char* lds, int id, in
     rp.issue(p, qtile, dtile, g, r0, lane);
     rp.settle(stat, p.keymask != nullptr, lane);
     wave_sync();
-    query_block<T, D, DROP, true>(st, qtile, dtile, stat, 32, at, p, r0, j, kbias, true, lane, (int64_t)b * p.H + hk * p.G + g);
+    query_block<T, D, DROP, true, FINE>(st, qtile, dtile, stat, 32, at, p, r0, j, kbias, true, lane, (int64_t)b * p.H + hk * p.G + g);
     wave_sync();
   }
   // fold the waves, dK then dV, in their order
@@ -500,13 +515,13 @@ __device__ __forceinline__ void sink_pass(const Params& p, char* lds, int id, in
   }
 }
 // The first nsink workgroups take the sink pass, so that it runs beside the window pass instead of in front of it.
-template <typename T, int D, bool DROP>
+template <typename T, int D, bool DROP, bool FINE>
 __global__ __launch_bounds__((Dkv<T, D>::NT), (D == 128 && sizeof(T) == 4 ? 1 : 2)) void dkv_kernel(Params p, int nunits, int nkt, int nsink) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int id = (int)blockIdx.x - nsink;
-  if (id < 0) { sink_pass<T, D, DROP>(p, lds, blockIdx.x, p.s32 / 32); return; }
+  if (id < 0) { sink_pass<T, D, DROP, FINE>(p, lds, blockIdx.x, p.s32 / 32); return; }
   const int per = (nunits + 7) / 8 * 8;
-  window_pass<T, D, DROP>(p, lds, id % per, id / per, nunits, nkt);
+  window_pass<T, D, DROP, FINE>(p, lds, id % per, id / per, nunits, nkt);
 }
 
 // Keys whose sums came in parts, added in a fixed order: D / 4 threads across the columns of a key, the others across keys (a workgroup of the key range behind `deep`) or,
@@ -593,7 +608,7 @@ inline int64_t bwd_floats(const BwdPlan& b, int nseq, int64_t Mk, int Hk, int D)
   return 2 * (win + (int64_t)b.nchunk * nseq * Hk * b.s32) * D;
 }
 
-template <typename T, int D, bool DROP> int launch_bwd(Params& p, hipStream_t s) {
+template <typename T, int D, bool DROP, bool FINE> int launch_bwd(Params& p, hipStream_t s) {
   typedef Geo<T, D> G;
   int rc;
   {
@@ -601,8 +616,8 @@ template <typename T, int D, bool DROP> int launch_bwd(Params& p, hipStream_t s)
     const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.H : (int64_t)p.nseq * p.H * nqt;
     if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
     const int lds = 4 * G::KT * G::ROWB + 2 * G::KT * 4;
-    if ((rc = raise_lds<dq_kernel<T, D, DROP>>(lds))) return rc;
-    if (nu) hipLaunchKernelGGL((dq_kernel<T, D, DROP>), dim3((unsigned)(8 * cdiv(nu, 8))), dim3(256), lds, s, p, (int)nu, nqt);
+    if ((rc = raise_lds<dq_kernel<T, D, DROP, FINE>>(lds))) return rc;
+    if (nu) hipLaunchKernelGGL((dq_kernel<T, D, DROP, FINE>), dim3((unsigned)(8 * cdiv(nu, 8))), dim3(256), lds, s, p, (int)nu, nqt);
     if ((rc = ctclip_check_launch("win_attn_bwd dq"))) return rc;
   }
   {
@@ -611,8 +626,8 @@ template <typename T, int D, bool DROP> int launch_bwd(Params& p, hipStream_t s)
     const int64_t grid = nsink + 8 * cdiv(nu, 8) * p.nsplit;
     if (grid > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
     constexpr int lds = Dkv<T, D>::LDS;
-    if ((rc = raise_lds<dkv_kernel<T, D, DROP>>(lds))) return rc;
-    if (nu) hipLaunchKernelGGL((dkv_kernel<T, D, DROP>), dim3((unsigned)grid), dim3(Dkv<T, D>::NT), lds, s, p, (int)nu, nkt, (int)nsink);
+    if ((rc = raise_lds<dkv_kernel<T, D, DROP, FINE>>(lds))) return rc;
+    if (nu) hipLaunchKernelGGL((dkv_kernel<T, D, DROP, FINE>), dim3((unsigned)grid), dim3(Dkv<T, D>::NT), lds, s, p, (int)nu, nkt, (int)nsink);
     if ((rc = ctclip_check_launch("win_attn_bwd dkv"))) return rc;
   }
   const int keys = p.nsplit > 1 ? p.Lk : p.s32;
@@ -623,7 +638,12 @@ template <typename T, int D, bool DROP> int launch_bwd(Params& p, hipStream_t s)
   hipLaunchKernelGGL((dkv_reduce_kernel<T, D>), dim3((unsigned)(cdiv(deep, DK) + cdiv(keys - deep, PER)), p.Hk, nz), dim3(256), 0, s, p, keys, deep);
   return ctclip_check_launch("win_attn_bwd reduce");
 }
-template <typename T, int D> int launch_bwd_d(Params& p, hipStream_t s) { return p.drop_p > 0.f ? launch_bwd<T, D, true>(p, s) : launch_bwd<T, D, false>(p, s); }
+template <typename T, int D> int launch_bwd_d(Params& p, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (fine_pass(p, DT_BF16, true)) return p.drop_p > 0.f ? launch_bwd<T, D, true, true>(p, s) : launch_bwd<T, D, false, true>(p, s);
+  }
+  return p.drop_p > 0.f ? launch_bwd<T, D, true, false>(p, s) : launch_bwd<T, D, false, false>(p, s);
+}
 template <typename T> int launch_bwd_t(Params& p, int D, hipStream_t s) {
   return D == 32 ? launch_bwd_d<T, 32>(p, s) : (D == 64 ? launch_bwd_d<T, 64>(p, s) : launch_bwd_d<T, 128>(p, s));
 }

@@ -472,6 +472,26 @@ def test_positions_changed_before_the_backward_pass_are_refused():
         y.sum().backward()
 
 
+@pytest.mark.parametrize("L,H,D,window,sinks", [(4, 4, 64, (10, 0), 0), (100, 2, 64, (20, 5), 3), (70, 2, 32, (-1, -1), 0), (90, 2, 128, (30, 0), 2)])
+def test_small_gradients_cost_one_rounding(L, H, D, window, sinks):
+    """Where few pairs are visible P and dS enter the products to 2^-17: half a step of each gradient, and next to it of the sums of absolute terms what f32 scores (2^-14, see above),
+    the remainders (2^-17 each) and f32 sums (D, L and the row sums: 3 * 128 * 2^-24 < 2^-15) leave: less than 2^-13."""
+    q, k, v, do = (rnd((L, H * D), BF16, 80 + i) for i in range(4))
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(Fn.window_attention(*leaves, H, D, window=window, sinks=sinks), leaves, do)
+    i, j = torch.arange(L)[:, None], torch.arange(L)[None, :]
+    left, right = (L if x < 0 else x for x in window)
+    see = (j <= i + right) & ((j >= i - left) | (j < sinks))
+    q, k, v, do = (t.detach().double().cpu().view(L, H, D).transpose(0, 1) for t in (q, k, v, do))
+    P = ((q @ k.transpose(1, 2)) / math.sqrt(D)).masked_fill(~see, -math.inf).softmax(2)
+    dP, dP_abs = do @ v.transpose(1, 2), do.abs() @ v.abs().transpose(1, 2)
+    dS = P * (dP - (P * dP).sum(2, keepdim=True)) / math.sqrt(D)
+    room = P * (dP_abs + (P * dP_abs).sum(2, keepdim=True)) / math.sqrt(D)
+    for g, want, r in zip(got, (dS @ k, dS.transpose(1, 2) @ q, P.transpose(1, 2) @ do), (room @ k.abs(), room.transpose(1, 2) @ q.abs(), P.transpose(1, 2) @ do.abs())):
+        g = g.double().cpu().view(L, H, D).transpose(0, 1)
+        assert ((g - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -13 * r).all()
+
+
 def test_training_captured_and_replayed():
     """Forward and backward of both operators in one graph, with sinks' and split keys' partial sums: each replay equals the eager result."""
     H, D, L = 2, 64, 1500

@@ -551,3 +551,22 @@ def test_text_tower_with_long_report_options_mixed_precision(options):
             continue
         scale = grads[n.replace("self.key", "self.query")][1].norm() if "key.bias" in n else b.norm()
         assert (a.double() - b).norm() <= 28 * 2.0 ** -8 * scale, n
+
+
+def test_text_tower_cls_rows_of_a_long_batch():
+    """BERT-base's width at 2000 tokens: the [CLS] rows lie 9 MB apart inside the projection.  The same rows as from the pass over every token, up to bf16 (two roundings of the
+    layer's attention output, each half a step, through layers of norm about 1)."""
+    from transformers import BertConfig, BertModel
+    from ct_clip_amd.bert import bert_last_hidden_state
+    torch.manual_seed(0)
+    cfg = BertConfig(vocab_size=50, hidden_size=768, num_hidden_layers=1, num_attention_heads=12, intermediate_size=768, position_embedding_type="rotary", attention_window=64,
+                     attention_sinks=1, hidden_dropout_prob=0.0, attention_probs_dropout_prob=0.0)
+    bert = BertModel(cfg, add_pooling_layer=False).to(DEV)
+    ids = torch.randint(0, 50, (2, 2000), device=DEV)
+    mask = (torch.arange(2000, device=DEV)[None, :] < torch.tensor([[2000], [1500]], device=DEV)).long()
+    every = bert_last_hidden_state(bert, ids, mask, BF16).view(2, 2000, 768)[:, 0]
+    rows = bert_last_hidden_state(bert, ids, mask, BF16, cls_only=True)
+    assert rows.shape == (2, 768) and torch.isfinite(rows).all()
+    assert (rows.float() - every.float()).abs().max() <= 4 * 2.0 ** -8 * every.abs().max().float()
+    rows.float().square().sum().backward()
+    assert all(torch.isfinite(p.grad).all() for p in bert.parameters() if p.grad is not None)

@@ -2,7 +2,7 @@
 //
 // With P from the forward pass's log-sum-exp and Delta = rowsum(dO o O):  dV = P^T dO,  dS = P o (dO V^T - Delta),  dQ = scale dS K,  dK = scale dS^T Q.
 //   dq_kernel     query rows as in the forward kernel: S^T, dP^T with a query per lane, dQ^T += K^T dS^T.  Also writes Delta.
-//   dkv_kernel, window_pass   128 keys of one (sequence, k|v head), 32 per wave: k, v and both gradients stay in registers while the query rows whose windows hold the keys pass
+//   dkv_kernel, window_pass   128 keys of one (sequence, k|v head), 32 per wave: k, v (heads of 128: in LDS) and both gradients stay in registers while the query rows whose windows hold the keys pass
 //                 through a double-buffered LDS ring, for every query head that shares the keys: their gradients are summed here, no atomics.
 //   dkv_kernel, sink_pass     the sinks meet EVERY later row: one key block would walk the whole sequence while all others walk a window.  The pairs (sink, row beyond its
 //                 window) are a pass of their own, split over the rows, a wave per 32-row tile; f32 partial sums.
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
 
 // The shape of the dK / dV kernel.  Four waves with k, v and both gradients of 32 keys each in registers, or (bf16 heads of 128, where that is 192 registers and would leave
 // a SIMD one wave) k and v in LDS and eight waves, two to a 32-key block: 1105 against 1150 us for the backward pass of 2 x 8191 tokens, 32 heads on 8; k in registers
-// beside v in LDS spills (1558).
+// beside v in LDS spills (1558).  Heads of 64 that way: 549 instead of 467 us for 32768 tokens of 12 heads, with four waves per SIMD (spills) 1057.
 template <typename T, int D> struct Dkv {
   static constexpr bool IN_LDS = sizeof(T) == 2 && D == 128;
   static constexpr int PAIR = IN_LDS ? 2 : 1, WAVES = 4 * PAIR, NT = 64 * WAVES;

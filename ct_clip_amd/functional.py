@@ -1200,7 +1200,7 @@ class SdpaFn(Function):
     @staticmethod
     def backward(ctx, do):
         be = B()
-        q, k, v, o, lse, lo, keymask = ctx.saved_tensors
+        q, k, v, o, lse, keymask = ctx.saved_tensors
         nseq, L, H, D, scale, has_mask, dropout = ctx.dims
         do = do.contiguous()
         qt = be.head_transpose(q, nseq, H, L, D)

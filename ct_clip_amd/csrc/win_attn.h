@@ -207,6 +207,8 @@ __device__ __forceinline__ float mask_value(float km) { return km > HIDDEN ? km 
 // chunk permutation is applied to the address that a lane READS.  Rows past the valid ones are outside the buffer descriptor, and the load writes zeros for them.
 // Inline asm on purpose: next to the builtin the compiler waits for all loads in front of every LDS read, since it cannot tell the buffer being filled from the one
 // being read.  There is no output register; dma_arrive() waits for everything in flight.
+// A load writes LDS when its data comes back, past the queue that a wave's own LDS instructions keep their order in: issue() first waits for the wave's reads (of
+// wave-private tiles: what it still reads of the tile that is refilled; shared tiles have a barrier in between, and nothing is left to wait for).
 template <typename T, int D, int ROWS, int NT> struct Dma {
   static constexpr int N = ROWS * Geo<T, D>::NCH / NT;
   static_assert(N >= 1 && ROWS * Geo<T, D>::NCH % NT == 0 && NT % 64 == 0, "whole chunks per thread");
@@ -222,6 +224,7 @@ template <typename T, int D, int ROWS, int NT> struct Dma {
   }
   // tile, ldb (bytes between rows), valid (rows from the tile's first on that may be read, >= 1) are uniform; valid rows lie within 2^31 bytes (check_rows)
   __device__ __forceinline__ void issue(char* lds_tile, const char* tile, int ldb, int valid, int tid) const {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const uint64_t base = reinterpret_cast<uint64_t>(tile);
     const uint32_t bytes = valid >= ROWS ? 0x7fffffffu : (uint32_t)((valid - 1) * ldb) + (uint32_t)Geo<T, D>::ROWB;
     const u32x4 rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)base), (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(base >> 32) & 0xffffu)),
@@ -445,7 +448,7 @@ __device__ __forceinline__ void store_lse(const Params& p, int64_t i, float m, f
   p.lse[i] = l == 0.f ? 0.f : m;
   p.lse[(int64_t)p.H * p.Mq + i] = l == 0.f ? INFINITY : __builtin_amdgcn_logf(l);
 }
-// lanes of a wave exchange through LDS: its operations retire in order, so only the compiler has to keep them in place
+// lanes of a wave exchange through LDS: its LDS instructions retire in order, so only the compiler has to keep them in place (loads into LDS are no such instructions: Dma::issue)
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();

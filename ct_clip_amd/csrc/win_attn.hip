@@ -222,7 +222,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void row
   int it = i0 + wave, buf = 0;
   if (it < i1) fetch(tile_at(tl, it) * 32, 0);
   row_frag_arrive<T, D>(qf);
-  for (; it < i1; it += 4, buf ^= 1) {                             // (no barrier: a wave's tiles are its own, and its LDS operations keep their order)
+  for (; it < i1; it += 4, buf ^= 1) {                             // (no barrier: a wave's tiles are its own, and a refill waits for its reads)
     const int j0 = tile_at(tl, it) * 32;
     dma_arrive();
     int state = 0;

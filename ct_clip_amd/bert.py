@@ -9,7 +9,9 @@ The pooler is skipped: CT-CLIP discards it (ct_clip.py:686,762).
 
 Reports longer than the position table (512 rows), all as attributes of the HF config (``BertConfig(..., position_embedding_type="rotary", attention_window=256)``):
   position_embedding_type = "rotary"   rotary positions on q and k instead of the absolute table (which is then neither read nor trained); rotary_dim (default: the whole
-                                       head), rope_theta (10000), rotary_layout ("half" | "interleaved"), rope_scaling (dict, ``functional.RotaryPositions``);
+                                       head), rope_theta (10000), rotary_layout ("half" | "interleaved"), rope_scaling (dict; by HF's names, as transformers 5 keeps them in
+                                       config.rope_parameters too: "rope_type" "default" | "linear" | "ntk" | "yarn", "factor", for yarn
+                                       "original_max_position_embeddings", or by those of ``functional.RotaryPositions``);
   attention_window = n or (l, r)       every token attends within its window, cost linear in the length; attention_sinks first tokens (default 1: [CLS]) stay visible.
 """
 import math
@@ -23,6 +25,30 @@ def is_hf_bert(module):
         and hasattr(module.embeddings, "word_embeddings")
 
 
+def _rope_options(cfg, dh):
+    """-> (rotated columns, base, layout, scaling of ``functional.RotaryPositions`` or None) from the config, whose constructor rewrites the dict: transformers 5 adds "rope_type" to it,
+    the base and, for yarn, the length of the original context, and reads and writes it as rope_parameters too."""
+    given = {name: value for name, value in dict(getattr(cfg, "rope_scaling", None) or getattr(cfg, "rope_parameters", None) or {}).items() if value is not None}
+    kinds = {given.pop(name) for name in ("rope_type", "type") if name in given}
+    if len(kinds) > 1:
+        raise ValueError(f"rope_scaling: two types, {sorted(kinds)}")
+    kind = kinds.pop() if kinds else "default"
+    bases = {float(b) for b in (given.pop("rope_theta", None), getattr(cfg, "rope_theta", None)) if b}
+    if len(bases) > 1:
+        raise ValueError(f"rope_theta: two values, {sorted(bases)}, beside rope_scaling and in it")
+    part = given.pop("partial_rotary_factor", None)
+    dim = getattr(cfg, "rotary_dim", None) or (int(dh * part) if part is not None else dh)
+    if kind in ("default", "none"):
+        given.pop("factor", None)
+    if kind == "yarn":
+        original = given.pop("original_max_position_embeddings", None)          # (transformers' own: the position table's rows unless the caller said so)
+        given.setdefault("original_length", original)
+        if given.pop("truncate", True) is not True:
+            raise ValueError("rope_scaling yarn: truncate = False is not implemented")
+    scaling = None if kind in ("default", "none") and not given else dict(given, type=kind)
+    return dim, bases.pop() if bases else 10000.0, getattr(cfg, "rotary_layout", None) or "half", scaling
+
+
 def _long_report_options(bert, dh):
     """-> (RotaryPositions or None, (left, right) or None, sinks) from the config."""
     cfg = bert.config
@@ -31,12 +57,10 @@ def _long_report_options(bert, dh):
         raise NotImplementedError("only absolute and rotary position embeddings are implemented")
     rope = None
     if kind == "rotary":
-        scaling = getattr(cfg, "rope_scaling", None)
-        key = (getattr(cfg, "rotary_dim", None) or dh, float(getattr(cfg, "rope_theta", None) or 10000.0), getattr(cfg, "rotary_layout", None) or "half",
-               tuple(sorted(scaling.items())) if scaling else None)
+        key = _rope_options(cfg, dh)
         held = bert.__dict__.get("_ctclip_rope")
         if held is None or held[0] != key:
-            held = bert.__dict__["_ctclip_rope"] = (key, Fn.RotaryPositions(key[0], base=key[1], layout=key[2], scaling=scaling))
+            held = bert.__dict__["_ctclip_rope"] = (key, Fn.RotaryPositions(key[0], base=key[1], layout=key[2], scaling=key[3]))
         rope = held[1]
     window = getattr(cfg, "attention_window", None)
     if window is not None:

@@ -1,12 +1,18 @@
 """Rotary positions and windowed attention where a call can go wrong, without a device: the built code's waits, sizes of workspaces and grids, what a plan holds, options of the
 text tower."""
+import copy
 import os
 import re
 import subprocess
 
 import pytest
+import torch
 
 from ct_clip_amd import build
+from ct_clip_amd import functional as Fn
+from ct_clip_amd.bert import bert_last_hidden_state
+from tests import long_report_oracle as O
+from tests.test_long_reports_cpu import ref  # noqa: F401
 
 OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
 
@@ -50,3 +56,58 @@ def test_a_tile_is_refilled_behind_the_reads_of_it(windowed_kernels):
                 back -= 1
             assert code[back] and "lgkmcnt(0)" in code[back], f"{name}: {code[back]} ... {ins}"
     assert seen == {"fwd_kernel", "rows_kernel", "dq_kernel", "dkv_kernel"}
+
+
+# ------------------------------------------------------------------------------------------------------------- options of the text tower
+
+YARN = dict(type="yarn", factor=8.0, original_length=512)
+CONFIGS = [  # what BertConfig is given, what RotaryPositions of a head of 32 columns must be
+    (dict(), dict()),
+    (dict(rope_theta=500.0), dict(base=500.0)),
+    (dict(rope_scaling=dict(type="linear", factor=4.0)), dict(scaling=dict(type="linear", factor=4.0))),
+    (dict(rope_scaling=dict(rope_type="linear", factor=4.0), rope_theta=500.0, rotary_layout="interleaved"), dict(scaling=dict(type="linear", factor=4.0), base=500.0, layout="interleaved")),
+    (dict(rope_scaling=dict(type="ntk", factor=4.0), rotary_dim=16), dict(scaling=dict(type="ntk", factor=4.0), dim=16)),
+    (dict(rope_scaling=dict(rope_type="yarn", factor=8.0, original_max_position_embeddings=512)), dict(scaling=YARN)),
+    (dict(rope_scaling=dict(type="yarn", factor=8.0, original_length=256), rope_theta=500.0), dict(scaling=dict(YARN, original_length=256), base=500.0)),
+    (dict(rope_scaling=dict(rope_type="yarn", factor=8.0, original_max_position_embeddings=512, beta_fast=16.0, attention_factor=1.5, truncate=True)),
+     dict(scaling=dict(YARN, beta_fast=16.0, attention_factor=1.5))),
+    (dict(rope_parameters=dict(rope_type="default", rope_theta=500.0)), dict(base=500.0)),
+    (dict(rope_parameters=dict(rope_type="linear", rope_theta=500.0, factor=2.0, partial_rotary_factor=0.5)), dict(scaling=dict(type="linear", factor=2.0), base=500.0, dim=16)),
+]
+
+
+def long_bert(**options):
+    from transformers import BertConfig, BertModel
+    torch.manual_seed(1)
+    return BertModel(BertConfig(vocab_size=97, hidden_size=64, num_hidden_layers=1, num_attention_heads=2, intermediate_size=64, hidden_dropout_prob=0.0,
+                                attention_probs_dropout_prob=0.0, position_embedding_type="rotary", **options))
+
+
+@pytest.mark.parametrize("stored", ["constructed", "dict", "saved"])
+@pytest.mark.parametrize("given,want", CONFIGS)
+def test_options_as_the_config_s_constructor_keeps_them(ref, given, want, stored, tmp_path):
+    """... and after a round trip through a dict or a file: the tower's output is that of the 64-bit form with the plan's frequencies."""
+    from transformers import BertConfig
+    model = long_bert(attention_window=(9, 4), attention_sinks=2, **given)
+    if stored == "dict":
+        model.config = BertConfig.from_dict(model.config.to_dict())
+    elif stored == "saved":
+        model.config.save_pretrained(tmp_path)
+        model.config = BertConfig.from_pretrained(tmp_path)
+    kw = dict(want)
+    rope = Fn.RotaryPositions(kw.pop("dim", 32), **kw)
+    ids = torch.randint(0, 97, (2, 50), generator=torch.Generator().manual_seed(2))
+    got = bert_last_hidden_state(model, ids, None, torch.float32)
+    plan = (torch.from_numpy(rope.frequencies), rope.magnitude, rope.dim, rope.interleaved)
+    exact = O.bert64(copy.deepcopy(model).double(), ids, torch.ones_like(ids), plan, (9, 4), 2)
+    torch.testing.assert_close(got.double(), exact, rtol=1e-5, atol=1e-5)          # one layer in f32: some 15 roundings of values of order 1
+
+
+@pytest.mark.parametrize("scaling", [dict(rope_type="dynamic", factor=2.0), dict(rope_type="longrope", factor=2.0), dict(type="linear", rope_type="ntk", factor=2.0),
+                                     dict(type="linear", factor=2.0, mscale=1.0), dict(rope_type="yarn", factor=2.0), dict(rope_type="default", mscale=1.0),
+                                     dict(rope_type="yarn", factor=2.0, original_max_position_embeddings=512, truncate=False), dict(rope_type="linear", factor=2.0, rope_theta=7.0)])
+def test_options_that_the_tower_does_not_have_are_refused(ref, scaling):
+    model = long_bert(rope_theta=500.0)
+    model.config.rope_scaling = scaling
+    with pytest.raises(ValueError):
+        bert_last_hidden_state(model, torch.zeros((1, 4), dtype=torch.long), None, torch.float32)

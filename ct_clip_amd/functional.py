@@ -16,6 +16,7 @@ import os
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.autograd import Function
 
 from . import backend as _be
@@ -1284,6 +1285,12 @@ def _not_twice():
         raise RuntimeError("rotary / window_attention: no derivative of the gradient (create_graph=True)")
 
 
+def _no_tangents(*tensors):
+    """(Calls that pass the autograd functions by would drop a tangent, which counts as a derivative of zero.)"""
+    if fwAD._current_level >= 0 and any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("rotary / window_attention: no forward-mode derivative (torch.autograd.forward_ad)")
+
+
 class RotaryFn(Function):
     @staticmethod
     def forward(ctx, q, k, rope, D, L, positions, start):
@@ -1327,6 +1334,7 @@ def rotary(q, k, rope, D, L=None, positions=None, start=0):
     L, start = max(M, 1) if L is None else int(L), int(start)
     if L < 1 or not -2 ** 62 < start < 2 ** 62:
         raise ValueError("rotary: L >= 1 and a start within 62 bits")
+    _no_tangents(q, k)
     if q.stride(1) != 1:
         q = q.contiguous()
     if k is not None and k.stride(1) != 1:
@@ -1465,6 +1473,7 @@ def window_attention(q, k, v, H, D, nseq=1, kv_heads=None, window=(-1, -1), sink
             raise ValueError(f"window_attention: keymask must be one additive value per key row ({geo.Mk}) on {q.device}")
         if keymask.dtype != torch.float32 or keymask.requires_grad or not keymask.is_contiguous():
             keymask = keymask.detach().to(torch.float32).contiguous()
+    _no_tangents(q, k, v, keymask)
     q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return WindowAttnFn.apply(q, k, v, keymask, geo, scale, dropout)

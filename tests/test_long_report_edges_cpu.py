@@ -111,3 +111,28 @@ def test_options_that_the_tower_does_not_have_are_refused(ref, scaling):
     model.config.rope_scaling = scaling
     with pytest.raises(ValueError):
         bert_last_hidden_state(model, torch.zeros((1, 4), dtype=torch.long), None, torch.float32)
+
+
+# ------------------------------------------------------------------------------------------------------------------ the operators' calls
+
+def test_a_dual_tensor_is_refused(ref):
+    """Forward-mode derivatives: an error whether or not an input requires a gradient, never an output without a tangent; plain tensors pass at a dual level."""
+    import torch.autograd.forward_ad as fwAD
+    rope, x, m = Fn.RotaryPositions(32), torch.randn(6, 64), torch.zeros(6)
+    calls = [lambda a, b: Fn.rotary(a, None, rope, 32), lambda a, b: Fn.rotary(b, a, rope, 32), lambda a, b: Fn.window_attention(a, b, b, 2, 32, window=2),
+             lambda a, b: Fn.window_attention(b, a, b, 2, 32, window=2), lambda a, b: Fn.window_attention(b, b, a, 2, 32, window=2),
+             lambda a, b: Fn.window_attention(a[:0], b, b, 2, 32, window=2)]
+    for grad in (False, True):
+        other = x.clone().requires_grad_(grad)
+        for call in calls:
+            want = call(x, other)
+            with fwAD.dual_level():
+                dual = fwAD.make_dual(x, torch.ones_like(x))
+                with pytest.raises(NotImplementedError):
+                    call(dual, other)
+                with torch.no_grad(), pytest.raises(NotImplementedError):
+                    call(dual, other)
+                for a, b in zip(*(t if isinstance(t, tuple) else (t,) for t in (call(x, other), want))):
+                    assert torch.equal(a, b)
+        with fwAD.dual_level(), pytest.raises(NotImplementedError):
+            Fn.window_attention(x, x, other, 2, 32, keymask=fwAD.make_dual(m, torch.ones_like(m)))

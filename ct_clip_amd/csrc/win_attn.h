@@ -35,7 +35,8 @@ struct Params {
   float scale, scale2;                    // scale2 = scale * log2 e
   uint64_t seed; const unsigned long long* seed_state; float drop_p, inv_keep;
   int nsplit;
-  int s32, nchunk;                        // backward: keys of sink blocks (multiple of 32), chunks of the rows beyond their window
+  int s32, nchunk;                        // backward: keys of sink blocks (multiple of 32; of the longest sequence), chunks of the rows beyond their window
+  int64_t sink_rows, sink_step;           // backward: rows of a k|v head that the sinks' partial sums take, and how they are shared out (win_attn_bwd.hip: sink_row)
 };
 
 template <typename T, int D> struct Geo {

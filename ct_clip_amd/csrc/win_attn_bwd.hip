@@ -359,12 +359,28 @@ template <typename T, int D, int ROWS, int NT> struct RowPipe {    // through LD
     src.put_stat<ROWS>(stat, masked, tid);
   }
 };
+// keys of a sequence's sink blocks: whole blocks of 32 that hold a sink with rows beyond its window (0: the sequence is too short for any)
+__device__ __forceinline__ int sink_keys(const Params& p, const Rows& rw) {
+  const int far = p.q_start + rw.lq - 1 - p.left, n = p.sinks < far ? p.sinks : far;
+  return n > 0 ? (n + 31) & ~31 : 0;
+}
+// Where the partial sums of sink j of a sequence lie.  One behind the other (sequence b at b * s32) or, among packed sequences, of which most may be too short to have any, by
+// the place of the sequence's rows, at floor(k0 * s32 / step).  A sequence of `len` rows has 32 ceil((len - 1 - left) / 32) of these keys, s32 at most; step (sink_steps) is such that
+// floor(len * s32 / step) is never less, so no two sequences meet and the last one ends within floor(Mk * s32 / step).  (8192 tokens beside 999 reports of 30, 12 heads of
+// 64, window 256: 58 MB with 4 sinks, 325 MB with 512; with s32 rows for every sequence it was 393 MB and 6.3 GB.)
+__device__ __forceinline__ int64_t sink_row(const Params& p, const Rows& rw, int b, int hk, int j) {
+  return hk * p.sink_rows + (p.sink_step ? rw.k0 * p.s32 / p.sink_step : (int64_t)b * p.s32) + j;
+}
+// len = left + 2 + 32 i rows are the fewest that have i + 1 blocks: step <= (s32 / 32) (left + 2 + 32 i) / (i + 1) for i = 0 ... s32 / 32 - 1, a monotone function of i
+inline int64_t sink_steps(int s32, int left) {
+  const int64_t last = (int64_t)s32 + left - 30, first = (int64_t)(s32 / 32) * (left + 2);
+  return last < first ? last : first;
+}
 // where the partial sums of key j lie: split passes hold every key, unsplit ones the keys of the sink blocks
 __device__ __forceinline__ int64_t part_row(const Params& p, const Rows& rw, int b, int hk, int j) {
-  return p.nsplit > 1 ? (int64_t)hk * p.Mk + rw.k0 + j : ((int64_t)b * p.Hk + hk) * p.s32 + j;
+  return p.nsplit > 1 ? (int64_t)hk * p.Mk + rw.k0 + j : sink_row(p, rw, b, hk, j);
 }
-__host__ __device__ inline int64_t part_rows(const Params& p) { return p.nsplit > 1 ? (int64_t)p.Hk * p.Mk : (int64_t)p.nseq * p.Hk * p.s32; }
-__host__ __device__ inline int64_t sink_rows(const Params& p) { return (int64_t)p.nseq * p.Hk * p.s32; }
+__host__ __device__ inline int64_t part_rows(const Params& p) { return p.Hk * (p.nsplit > 1 ? p.Mk : p.sink_rows); }
 
 template <typename T, int D, bool DROP, bool FINE>
 __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, int split, int nunits, int nkt) {
@@ -442,7 +458,7 @@ __device__ __forceinline__ void window_pass(const Params& p, char* lds, int id, 
     }
     if (par) return;
   }
-  if (p.nsplit > 1 || jw < p.s32) {
+  if (p.nsplit > 1 || jw < sink_keys(p, rw)) {
     if (j >= rw.lk) return;
     const int64_t N = part_rows(p), r = (int64_t)split * N + part_row(p, rw, u.b, u.hk, j);
     store_part<D>(p.part + r * D, st.dk, half);
@@ -464,7 +480,7 @@ __device__ __forceinline__ void sink_pass(const Params& p, char* lds, int id, in
   const int chunk = id % p.nchunk, blk = id / p.nchunk % nblk, hk = id / (p.nchunk * nblk) % p.Hk, b = id / (p.nchunk * nblk * p.Hk);
   const Rows rw = rows_of(p, b);
   const int jw = 32 * blk, j = jw + c;
-  if (jw >= rw.lk) return;
+  if (jw >= sink_keys(p, rw)) return;
   int rlo = jw + p.left + 1 - p.q_start;                           // first row that has a key of this block beyond its window
   rlo = rlo < 0 ? 0 : rlo;
   const int t0 = rlo / 32, nt = rw.lq > rlo ? (rw.lq - 1) / 32 - t0 + 1 : 0, steps = nt * p.G;
@@ -486,7 +502,7 @@ __device__ __forceinline__ void sink_pass(const Params& p, char* lds, int id, in
   }
   // fold the waves, dK then dV, in their order
   float* fa = reinterpret_cast<float*>(lds);                       // [WAVES][32][D + 4]
-  const int64_t r = ((int64_t)b * p.Hk + hk) * p.s32 + jw, S = sink_rows(p);
+  const int64_t r = sink_row(p, rw, b, hk, jw), S = p.Hk * p.sink_rows;
   float* base = p.part + (int64_t)2 * p.nsplit * part_rows(p) * D;
   constexpr int TPR = X::NT / 32, PER = D / TPR;                   // threads of a row, columns of a thread
   const int fr = tid / TPR, fc = tid % TPR * PER;
@@ -539,17 +555,19 @@ __global__ __launch_bounds__(256) void dkv_reduce_kernel(Params p, int keys, int
   const int end = split ? deep : keys;
   for (int b = blockIdx.z; b < p.nseq; b += gridDim.z) {
     const Rows rw = rows_of(p, b);
-    const bool on = j < end && j < rw.lk;
-    const int64_t N = part_rows(p), S = sink_rows(p), r = part_row(p, rw, b, hk, j);
+    const int sk = sink_keys(p, rw);
+    if (p.nsplit == 1 && !sk) continue;    // (its keys have been stored by the window's pass)
+    const bool on = j < end && j < rw.lk && (p.nsplit > 1 || j < sk);
+    const int64_t N = part_rows(p), S = p.Hk * p.sink_rows, r = part_row(p, rw, b, hk, j), rs = sink_row(p, rw, b, hk, j);
     const float* sink = p.part + 2 * p.nsplit * N * D;
-    const int parts = p.nsplit + (j < p.s32 ? p.nchunk : 0);
+    const int parts = p.nsplit + (j < sk ? p.nchunk : 0);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       float o[4] = {0.f, 0.f, 0.f, 0.f};
       if (on)
         for (int s = pg; s < parts; s += step) {
           const float* src = s < p.nsplit ? p.part + (((int64_t)which * p.nsplit + s) * N + r) * D
-                                          : sink + (((int64_t)which * p.nchunk + s - p.nsplit) * S + ((int64_t)b * p.Hk + hk) * p.s32 + j) * D;
+                                          : sink + (((int64_t)which * p.nchunk + s - p.nsplit) * S + rs) * D;
           float a[4];
           load4(src + col, a);
 #pragma unroll
@@ -579,9 +597,9 @@ __global__ __launch_bounds__(256) void dkv_reduce_kernel(Params p, int keys, int
   }
 }
 
-struct BwdPlan { int nsplit, s32, nchunk; };
-inline BwdPlan bwd_plan(int nseq, int Lq, int Lk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int ntiles, int dtype) {
-  BwdPlan b{1, 0, 0};
+struct BwdPlan { int nsplit, s32, nchunk; int64_t sink_rows, sink_step; };
+inline BwdPlan bwd_plan(int nseq, int Lq, int Lk, int64_t Mk, int H, int Hk, int D, int left, int right, int sinks, int q_start, int ntiles, int dtype) {
+  BwdPlan b{1, 0, 0, 0, 0};
   const int G = H / Hk;
   const int64_t units = ntiles ? (int64_t)ntiles * Hk : (int64_t)nseq * Hk * cdiv(Lk, QB);
   const int64_t span = (int64_t)QB + left + right < Lq ? (int64_t)QB + left + right : Lq;
@@ -596,16 +614,19 @@ inline BwdPlan bwd_plan(int nseq, int Lq, int Lk, int H, int Hk, int D, int left
   if (sinks > 0 && far > 0) {
     const int64_t n = sinks < far ? sinks : far;
     b.s32 = (int)(cdiv(n, 32) * 32);
-    const int64_t blocks = (int64_t)nseq * Hk * (b.s32 / 32), tiles = cdiv(far, 32) * G;
+    b.sink_rows = (int64_t)nseq * b.s32;
+    const int64_t step = sink_steps(b.s32, left), packed = Mk * b.s32 / step;
+    if (ntiles && packed < b.sink_rows) { b.sink_rows = packed; b.sink_step = step; }
+    const int64_t blocks = Hk * cdiv(b.sink_rows, 32), tiles = cdiv(far, 32) * G;
     int64_t ch = cdiv(512, blocks);
     if (ch > tiles / 8) ch = tiles / 8;    // two tiles per wave at least; unsplit, the backward pass of 32768 tokens, 12 heads, takes 549 instead of 490 us
     b.nchunk = (int)(ch < 1 ? 1 : ch);
   }
   return b;
 }
-inline int64_t bwd_floats(const BwdPlan& b, int nseq, int64_t Mk, int Hk, int D) {
-  const int64_t win = b.nsplit > 1 ? (int64_t)b.nsplit * Hk * Mk : (int64_t)nseq * Hk * b.s32;
-  return 2 * (win + (int64_t)b.nchunk * nseq * Hk * b.s32) * D;
+inline int64_t bwd_floats(const BwdPlan& b, int64_t Mk, int Hk, int D) {
+  const int64_t win = b.nsplit > 1 ? b.nsplit * Mk : b.sink_rows;
+  return 2 * (win + b.nchunk * b.sink_rows) * Hk * D;
 }
 
 template <typename T, int D, bool DROP, bool FINE> int launch_bwd(Params& p, hipStream_t s) {
@@ -655,7 +676,7 @@ extern "C" int64_t ctclip_win_attn_bwd_workspace(int nseq, int Lq, int Lk, int64
   const int l = left < 0 || left > Lk ? Lk : left, r = right < 0 || right > Lk ? Lk : right, s = sinks < Lk ? sinks : Lk;
   int64_t need = 0;                        // (of either type: the larger)
   for (int dtype : {DT_F32, DT_BF16}) {
-    const int64_t n = win::bwd_floats(win::bwd_plan(nseq, Lq, Lk, H, Hk, D, l, r, s, q_start, ntiles, dtype), nseq, Mk, Hk, D) * 4;
+    const int64_t n = win::bwd_floats(win::bwd_plan(nseq, Lq, Lk, Mk, H, Hk, D, l, r, s, q_start, ntiles, dtype), Mk, Hk, D) * 4;
     need = n > need ? n : need;
   }
   return need;
@@ -683,9 +704,9 @@ extern "C" int ctclip_win_attn_bwd(const void* q, const void* k, const void* v, 
   fill(p, nseq, Lq, Lk, Mq, Mk, H, Hk, left, right, sinks, q_start, scale, dropout_p, dropout_seed, offsets, tiles, ntiles, keymask);
   p.q = q; p.k = k; p.v = v; p.o = o; p.out_lo = dtype == DT_BF16 ? const_cast<void*>(o_lo) : nullptr; p.dout = dout; p.lse = const_cast<float*>(lse); p.delta = delta; p.dq = dq; p.dk = dk; p.dv = dv;
   p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo; p.lddo = lddo; p.lddq = lddq; p.lddk = lddk; p.lddv = lddv;
-  const BwdPlan b = bwd_plan(nseq, Lq, Lk, H, Hk, D, p.left, p.right, p.sinks, q_start, offsets ? ntiles : 0, dtype);
-  p.nsplit = b.nsplit; p.s32 = b.s32; p.nchunk = b.nchunk;
-  const int64_t need = bwd_floats(b, nseq, Mk, Hk, D) * 4;
+  const BwdPlan b = bwd_plan(nseq, Lq, Lk, Mk, H, Hk, D, p.left, p.right, p.sinks, q_start, offsets ? ntiles : 0, dtype);
+  p.nsplit = b.nsplit; p.s32 = b.s32; p.nchunk = b.nchunk; p.sink_rows = b.sink_rows; p.sink_step = b.sink_step;
+  const int64_t need = bwd_floats(b, Mk, Hk, D) * 4;
   if (need) {
     if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16) { ctclip_set_error("win_attn_bwd: workspace"); return CTCLIP_EWORKSPACE; }
     p.part = (float*)workspace;

@@ -136,3 +136,48 @@ def test_a_dual_tensor_is_refused(ref):
                     assert torch.equal(a, b)
         with fwAD.dual_level(), pytest.raises(NotImplementedError):
             Fn.window_attention(x, x, other, 2, 32, keymask=fwAD.make_dual(m, torch.ones_like(m)))
+
+
+def test_workspace_of_one_long_sequence_among_many_short_ones():
+    """Sequences without a row beyond their window take no room for the sinks: the partial sums are bounded by what the rows can hold, not by sequences times sinks."""
+    from ct_clip_amd import _lib
+    lib, H, D, left = _lib.load(), 12, 64, 256
+    lengths = [8192] + [30] * 999
+    seqs = Fn.PackedSequences(lengths)
+    Mk = seqs.end
+
+    def need(nseq, longest, M, sinks, ntiles):
+        return lib.ctclip_win_attn_bwd_workspace(nseq, longest, longest, M, H, H, D, left, left, sinks, 0, ntiles)
+    for sinks in (1, 4, 32, 512):
+        s32 = (sinks + 31) // 32 * 32
+        rows = Mk * s32 // (s32 + left - 30)
+        one = 2 * rows * H * D * 4                      # a part of dK and dV in f32
+        got = need(len(lengths), 8192, Mk, sinks, seqs.ntiles)
+        assert one < got <= 2 * one, sinks              # the window's part and that of one chunk of rows
+    # few sequences, or all of them long: as many rows as they have sinks
+    assert need(12, 3001, 9688, 2, 84) == need(12, 3001, 9688, 2, 90)
+    assert need(4, 2000, 8000, 4, 64) <= 2 * (1 + 11) * 4 * 32 * H * D * 4
+
+
+def test_packed_sinks_partial_rows_do_not_meet():
+    """The rule by which sequences take their rows: floor(first row * s32 / step), for any window, number of sinks and lengths."""
+    import random
+    rng = random.Random(5)
+    for _ in range(300):
+        left, sinks = rng.choice((0, 1, 7, 29, 30, 31, 64, 300)), rng.choice((1, 31, 32, 33, 100, 700))
+        lengths = [rng.choice((0, 1, left, left + 1, left + 2, left + 3, left + 33, left + 34, left + 35, left + 66, rng.randint(1, 3000))) for _ in range(rng.randint(1, 60))]
+
+        def keys(n):
+            k = min(sinks, n - 1 - left)
+            return (k + 31) // 32 * 32 if k > 0 else 0
+        s32, M, first = max(map(keys, lengths)), sum(lengths), 0
+        if not s32:
+            continue
+        step, end = min(s32 + left - 30, s32 // 32 * (left + 2)), 0
+        for n in lengths:
+            if keys(n):
+                at = first * s32 // step
+                assert at >= end
+                end = at + keys(n)
+            first += n
+        assert end <= M * s32 // step

@@ -127,7 +127,7 @@ def bert_last_hidden_state(bert, input_ids, attention_mask, dtype, operand_dtype
         if rope is None and window is None:
             c, x_res = Fn.QkvSdpaFn.apply(*qkv_args, od, True)
         else:
-            c, x_res = Fn.QkvWindowFn.apply(*qkv_args, rope, window or (-1, -1), sinks if window else 0, last_cls, od, True)
+            c, x_res = Fn.QkvWindowFn.apply(*qkv_args, rope, window or (-1, -1), sinks if window else 0, last_cls, od, True, torch.is_grad_enabled())
         if last_cls:
             # rows b * T of the attention output and of the layer input: everything behind them in this layer is row-wise
             if c.shape[0] != Bsz:

@@ -1587,8 +1587,10 @@ class QkvWindowFn(Function):
     buffer; backward turns dq | dk back in place in front of the grad-input GEMM."""
 
     @staticmethod
-    def forward(ctx, x, wq, wk, wv, bq, bk, bv, keymask, nseq, L, H, D, scale, dropout, rope, window, sinks, first_only, operand_dtype=None, passthrough=False):
-        """rope: ``RotaryPositions`` or None.  first_only: only the first row of every sequence is attended FROM ([CLS] in the last layer) -> o (nseq, H * D)."""
+    def forward(ctx, x, wq, wk, wv, bq, bk, bv, keymask, nseq, L, H, D, scale, dropout, rope, window, sinks, first_only, operand_dtype=None, passthrough=False,
+                keep=True):
+        """rope: ``RotaryPositions`` or None.  first_only: only the first row of every sequence is attended FROM ([CLS] in the last layer) -> o (nseq, H * D).
+        keep: whether a backward pass may follow (torch.is_grad_enabled() of the caller: in here it is off, and the inputs' requires_grad alone does not tell)."""
         be = B()
         N, K = wq.shape
         ctx.x_dtype = x.dtype
@@ -1603,9 +1605,10 @@ class QkvWindowFn(Function):
             be.rotary(q, k, rope.turns(x.device), D, rope.dim, L, None, 0, rope.interleaved, rope.magnitude, out=(q, k))
         q, k, v = QkvWindowFn._views(qkv, N, nseq, L, first_only)
         geo = window_geometry(q.shape[0], k.shape[0], H, H, D, nseq, window, sinks, 0)
-        o, lse, lo = be.win_attn_fwd(q, k, v, keymask, geo, scale, want_lse=any(ctx.needs_input_grad[:7]), dropout=dropout)
-        ctx.wt = _qkv_transposed_shadow(x, wq, wk, wv) if ctx.needs_input_grad[0] else None
-        if lse is not None:
+        keep = keep and any(ctx.needs_input_grad[:7])
+        o, lse, lo = be.win_attn_fwd(q, k, v, keymask, geo, scale, want_lse=keep, dropout=dropout)
+        ctx.wt = _qkv_transposed_shadow(x, wq, wk, wv) if keep and ctx.needs_input_grad[0] else None
+        if keep:
             ctx.save_for_backward(x, wsh, qkv, o, lse, lo, keymask)
         ctx.params = (wq, wk, wv, bq, bk, bv)
         ctx.args = (geo, scale, dropout, rope, nseq, L, N, D, first_only)
@@ -1634,7 +1637,7 @@ class QkvWindowFn(Function):
             dq, dk = dqkv[:, :N], dqkv[:, N:2 * N]
             be.rotary(dq, dk, rope.turns(x.device), D, rope.dim, L, None, 0, rope.interleaved, rope.magnitude, inverse=True, out=(dq, dk))
         dx, gw, gb = _qkv_backward(ctx, dqkv, x, wsh, d_pass)
-        return (dx, *gw, *gb, *([None] * 13))
+        return (dx, *gw, *gb, *([None] * 14))
 
 
 class DropoutAddFn(Function):

@@ -181,3 +181,26 @@ def test_packed_sinks_partial_rows_do_not_meet():
                 end = at + keys(n)
             first += n
         assert end <= M * s32 // step
+
+
+@pytest.mark.parametrize("cls_only", [False, True])
+def test_statistics_are_kept_only_where_a_backward_pass_can_follow(ref, monkeypatch, cls_only):
+    from tests.test_long_reports_cpu import RefOps
+    asked, run = [], RefOps.win_attn_fwd
+    monkeypatch.setattr(RefOps, "win_attn_fwd", lambda self, *a, want_lse=True, **kw: asked.append(want_lse) or run(self, *a, want_lse=want_lse, **kw))
+    model, ids = long_bert(attention_window=3), torch.arange(16).view(2, 8)
+
+    def tower():
+        del asked[:]
+        return bert_last_hidden_state(model, ids, None, torch.float32, cls_only=cls_only)
+    out = tower()
+    assert asked == [True] and out.requires_grad
+    with torch.no_grad():
+        assert torch.equal(tower(), out) and asked == [False]
+    with torch.inference_mode():
+        assert torch.equal(tower(), out) and asked == [False]
+    model.requires_grad_(False)
+    assert torch.equal(tower(), out) and asked == [False]
+    model.requires_grad_(True)
+    tower().square().sum().backward()
+    assert all(p.grad is not None for n, p in model.named_parameters() if "pooler" not in n and "position" not in n)

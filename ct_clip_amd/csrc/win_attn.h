@@ -482,7 +482,7 @@ inline void fill(Params& p, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, in
   p.offsets = offsets; p.tiles = tiles; p.ntiles = ntiles; p.keymask = keymask;
 }
 
-// FINE (bf16, training): P and dS are rounded to the operand type for the second products; FINE passes take what that left over as well, in a second instruction each.
+// FINE (bf16): P and dS are rounded to the operand type for the second products; FINE passes take what that left over as well, in a second instruction each.
 //   Forward, up to 64 visible keys: Delta = rowsum(dO o O) has the probabilities' rounding over the root of the keys that count, which would be seen beside the one rounding that
 //   dS = P o (dP - Delta) has of its own (300 tokens, window 8 + 2: dq 2.60e-3 from 64 bits, then 2.36e-3; at 81 keys 2.39e-3 without it).  8 x 512 tokens, 12 heads, window
 //   16 + 16: 15.8 -> 17.2 us.
@@ -490,6 +490,8 @@ inline void fill(Params& p, int nseq, int Lq, int Lk, int64_t Mq, int64_t Mk, in
 //   launches and latency: forward and
 //   backward of 8 x 4 tokens 4.8 + 13.1 -> 4.9 + 13.9 us, of 500 tokens, 12 heads, window 80 + 80 (0.97 * 2^20 pairs) 15.5 + 34.9 -> 16.7 + 37.5; errors 2.35e-3 -> 1.66e-3,
 //   which is the results' own rounding.
+//   A forward pass without a backward one takes them by the same rule, so that an output's bits do not depend on the mode of autograd: 8 x 512 tokens, 12 heads, window 16 + 16,
+//   13.8 -> 15.4 us, 4 x 8192 tokens, window 30 + 30, 48.9 -> 59.2, the [CLS] rows of 8 x 512 5.7 -> 5.9 (error 2.1e-3 -> 1.7e-3).
 inline bool fine_pass(const Params& p, int dtype, bool backward) {
   const int64_t window = (int64_t)p.left + p.right + 1 + p.sinks, keys = window < p.Lk ? window : p.Lk;
   return dtype == DT_BF16 && ((!backward && keys <= 64) || keys * p.Mq * p.H <= (1 << 20));

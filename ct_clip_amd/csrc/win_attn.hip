@@ -401,7 +401,7 @@ template <typename T, int D, bool DROP, bool FINE> int launch_fwd(Params& p, con
 }
 template <typename T, int D> int launch_fwd_d(Params& p, const Plan& pl, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    if (p.out_lo && fine_pass(p, DT_BF16, false)) return p.drop_p > 0.f ? launch_fwd<T, D, true, true>(p, pl, s) : launch_fwd<T, D, false, true>(p, pl, s);
+    if (fine_pass(p, DT_BF16, false)) return p.drop_p > 0.f ? launch_fwd<T, D, true, true>(p, pl, s) : launch_fwd<T, D, false, true>(p, pl, s);
   }
   return p.drop_p > 0.f ? launch_fwd<T, D, true, false>(p, pl, s) : launch_fwd<T, D, false, false>(p, pl, s);
 }

@@ -1,8 +1,9 @@
-"""Rotary positions and windowed attention on the device where a call can go wrong: one long sequence among many short ones."""
+"""Rotary positions and windowed attention on the device where a call can go wrong: one long sequence among many short ones, modes of autograd."""
 import pytest
 import torch
 
-from tests.test_long_reports_gpu import run_case
+from ct_clip_amd import functional as Fn
+from tests.test_long_reports_gpu import rnd, run_case
 
 pytestmark = pytest.mark.gpu
 
@@ -18,3 +19,20 @@ BF16, F32 = torch.bfloat16, torch.float32
 ])
 def test_sinks_of_packed_sequences_most_of_which_are_short(lengths, first, H, Hk, D, window, sinks, dtype):
     run_case(dtype, None, None, None, H, Hk, D, window, sinks, lengths=lengths, first=first, tail=2, seed=len(lengths))
+
+
+@pytest.mark.parametrize("nseq,Lq,Lk,H,D,window,sinks,mask", [(8, 512, 512, 12, 64, (16, 16), 1, False), (8, 1, 512, 12, 64, (128, 128), 1, True), (2, 40, 40, 4, 32, (-1, -1), 0, False),
+                                                              (4, 300, 300, 2, 128, (20, 3), 2, True), (2, 900, 900, 4, 64, (100, 100), 3, True), (1, 1, 9000, 8, 64, (-1, 0), 0, False)])
+def test_the_output_s_bits_do_not_depend_on_the_mode(nseq, Lq, Lk, H, D, window, sinks, mask):
+    """Forward for training, with frozen inputs and under no_grad: the same numbers."""
+    q, k, v = rnd((nseq * Lq, H * D), BF16, 1), rnd((nseq * Lk, H * D), BF16, 2), rnd((nseq * Lk, H * D), BF16, 3)
+    keymask = torch.where(torch.arange(nseq * Lk, device="cuda") % 7 == 3, torch.finfo(F32).min, 0.0) if mask else None
+
+    def call():
+        return Fn.window_attention(q, k, v, H, D, nseq=nseq, window=window, sinks=sinks, keymask=keymask, q_start=Lk - Lq)
+    frozen = call()
+    q.requires_grad_(True)
+    trained = call()
+    with torch.no_grad():
+        assert torch.equal(call(), trained.detach())
+    assert trained.requires_grad and torch.equal(frozen, trained.detach())

@@ -496,6 +496,12 @@ inline bool fine_pass(const Params& p, int dtype, bool backward) {
   const int64_t window = (int64_t)p.left + p.right + 1 + p.sinks, keys = window < p.Lk ? window : p.Lk;
   return dtype == DT_BF16 && ((!backward && keys <= 64) || keys * p.Mq * p.H <= (1 << 20));
 }
+// a launch holds fewer than 2^32 threads along its grid's first axis
+inline int check_grid(int64_t workgroups, int threads) {
+  if (workgroups < ((int64_t)1 << 32) / threads) return CTCLIP_OK;
+  ctclip_set_error("win_attn: too many sequences, heads or tiles for a launch (2^32 threads)");
+  return CTCLIP_EUNSUPPORTED;
+}
 template <auto KERNEL> int raise_lds(int bytes) {       // more than 64 KB of LDS is opted into, once per kernel and device
   static bool done[64] = {};
   int dev = 0;

@@ -375,19 +375,19 @@ template <typename T, int D, bool DROP, bool FINE> int launch_fwd(Params& p, con
   typedef Geo<T, D> G;
   if (pl.rows) {
     const int64_t nu = (int64_t)p.nseq * p.Hk;
-    if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many sequences"); return CTCLIP_EUNSUPPORTED; }
     int lds = 4 * (2 * 32 * G::ROWB + 256);
     const int fold = 1024 + 4 * 32 * (D + 4) * 4;
     if (fold > lds) lds = fold;
-    const int rc = raise_lds<rows_kernel<T, D, DROP, FINE>>(lds);
+    int rc = check_grid(8 * cdiv(nu, 8), 256);
+    if (!rc) rc = raise_lds<rows_kernel<T, D, DROP, FINE>>(lds);
     if (rc) return rc;
     hipLaunchKernelGGL((rows_kernel<T, D, DROP, FINE>), dim3((unsigned)(8 * cdiv(nu, 8)), p.nsplit), dim3(256), lds, s, p, (int)nu);
   } else {
     const int nqt = (int)cdiv(p.Lq, QB);
     const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.H : (int64_t)p.nseq * p.H * nqt;
-    if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
     const int lds = 4 * G::KT * G::ROWB + 2 * G::KT * 4;
-    const int rc = raise_lds<fwd_kernel<T, D, DROP, FINE>>(lds);
+    int rc = check_grid(8 * cdiv(nu, 8), 256);
+    if (!rc) rc = raise_lds<fwd_kernel<T, D, DROP, FINE>>(lds);
     if (rc) return rc;
     hipLaunchKernelGGL((fwd_kernel<T, D, DROP, FINE>), dim3((unsigned)(8 * cdiv(nu, 8)), p.nsplit), dim3(256), lds, s, p, (int)nu, nqt);
   }

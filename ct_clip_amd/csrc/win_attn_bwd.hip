@@ -631,32 +631,24 @@ inline int64_t bwd_floats(const BwdPlan& b, int64_t Mk, int Hk, int D) {
 
 template <typename T, int D, bool DROP, bool FINE> int launch_bwd(Params& p, hipStream_t s) {
   typedef Geo<T, D> G;
-  int rc;
-  {
-    const int nqt = (int)cdiv(p.Lq, QB);
-    const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.H : (int64_t)p.nseq * p.H * nqt;
-    if (nu > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
-    const int lds = 4 * G::KT * G::ROWB + 2 * G::KT * 4;
-    if ((rc = raise_lds<dq_kernel<T, D, DROP, FINE>>(lds))) return rc;
-    if (nu) hipLaunchKernelGGL((dq_kernel<T, D, DROP, FINE>), dim3((unsigned)(8 * cdiv(nu, 8))), dim3(256), lds, s, p, (int)nu, nqt);
-    if ((rc = ctclip_check_launch("win_attn_bwd dq"))) return rc;
-  }
-  {
-    const int nkt = (int)cdiv(p.Lk, QB);
-    const int64_t nu = p.offsets ? (int64_t)p.ntiles * p.Hk : (int64_t)p.nseq * p.Hk * nkt, nsink = (int64_t)(p.s32 / 32) * p.Hk * p.nseq * p.nchunk;
-    const int64_t grid = nsink + 8 * cdiv(nu, 8) * p.nsplit;
-    if (grid > (1 << 30)) { ctclip_set_error("win_attn: too many tiles"); return CTCLIP_EUNSUPPORTED; }
-    constexpr int lds = Dkv<T, D>::LDS;
-    if ((rc = raise_lds<dkv_kernel<T, D, DROP, FINE>>(lds))) return rc;
-    if (nu) hipLaunchKernelGGL((dkv_kernel<T, D, DROP, FINE>), dim3((unsigned)grid), dim3(Dkv<T, D>::NT), lds, s, p, (int)nu, nkt, (int)nsink);
-    if ((rc = ctclip_check_launch("win_attn_bwd dkv"))) return rc;
-  }
+  constexpr int lds_q = 4 * G::KT * G::ROWB + 2 * G::KT * 4, lds_kv = Dkv<T, D>::LDS;
+  const int nqt = (int)cdiv(p.Lq, QB), nkt = (int)cdiv(p.Lk, QB);
+  const int64_t nq = p.offsets ? (int64_t)p.ntiles * p.H : (int64_t)p.nseq * p.H * nqt, nk = p.offsets ? (int64_t)p.ntiles * p.Hk : (int64_t)p.nseq * p.Hk * nkt;
+  const int64_t nsink = (int64_t)(p.s32 / 32) * p.Hk * p.nseq * p.nchunk, grid = nsink + 8 * cdiv(nk, 8) * p.nsplit;
   const int keys = p.nsplit > 1 ? p.Lk : p.s32;
+  constexpr int PER = 256 / (D / 4), DK = PER < 16 ? 1 : PER / 16;           // (as in dkv_reduce_kernel)
+  const int deep = p.nsplit > 8 ? keys : (p.nsplit + p.nchunk > 8 ? (p.s32 < keys ? p.s32 : keys) : 0);
+  const int64_t nred = cdiv(deep, DK) + cdiv(keys - deep, PER);
+  int rc;                                  // everything that can be refused, before the first launch writes
+  if ((rc = check_grid(8 * cdiv(nq, 8), 256)) || (rc = check_grid(grid, Dkv<T, D>::NT)) || (rc = check_grid(nred, 256)) ||
+      (rc = raise_lds<dq_kernel<T, D, DROP, FINE>>(lds_q)) || (rc = raise_lds<dkv_kernel<T, D, DROP, FINE>>(lds_kv))) return rc;
+  if (nq) hipLaunchKernelGGL((dq_kernel<T, D, DROP, FINE>), dim3((unsigned)(8 * cdiv(nq, 8))), dim3(256), lds_q, s, p, (int)nq, nqt);
+  if ((rc = ctclip_check_launch("win_attn_bwd dq"))) return rc;
+  if (nk) hipLaunchKernelGGL((dkv_kernel<T, D, DROP, FINE>), dim3((unsigned)grid), dim3(Dkv<T, D>::NT), lds_kv, s, p, (int)nk, nkt, (int)nsink);
+  if ((rc = ctclip_check_launch("win_attn_bwd dkv"))) return rc;
   if (!keys) return CTCLIP_OK;
   const unsigned nz = p.nseq < 32768 ? p.nseq : 32768;
-  constexpr int PER = 256 / (D / 4), DK = PER < 16 ? 1 : PER / 16;           // (as in the kernel)
-  const int deep = p.nsplit > 8 ? keys : (p.nsplit + p.nchunk > 8 ? (p.s32 < keys ? p.s32 : keys) : 0);
-  hipLaunchKernelGGL((dkv_reduce_kernel<T, D>), dim3((unsigned)(cdiv(deep, DK) + cdiv(keys - deep, PER)), p.Hk, nz), dim3(256), 0, s, p, keys, deep);
+  hipLaunchKernelGGL((dkv_reduce_kernel<T, D>), dim3((unsigned)nred, p.Hk, nz), dim3(256), 0, s, p, keys, deep);
   return ctclip_check_launch("win_attn_bwd reduce");
 }
 template <typename T, int D> int launch_bwd_d(Params& p, hipStream_t s) {

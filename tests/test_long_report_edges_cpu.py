@@ -204,3 +204,26 @@ def test_statistics_are_kept_only_where_a_backward_pass_can_follow(ref, monkeypa
     model.requires_grad_(True)
     tower().square().sum().backward()
     assert all(p.grad is not None for n, p in model.named_parameters() if "pooler" not in n and "position" not in n)
+
+
+def test_c_entries_refuse_a_grid_that_no_launch_holds():
+    """2^32 threads along the first axis: every launch of a call is refused before the first one writes."""
+    import ctypes
+    from ct_clip_amd import _lib
+    lib = _lib.load()
+    buf = (ctypes.c_char * 512)()
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+
+    def fwd(nseq, L, H, D, dt=1, off=None, nt=0):
+        M = nseq * L
+        return lib.ctclip_win_attn_fwd(p, p, p, None, off, off, nt, p, None, None, nseq, L, L, M, M, H, H, D, 4, 4, 0, 0, H * D, H * D, H * D, H * D, 1.0, 0.0, 0, dt, None, 0, None)
+
+    def bwd(nseq, L, H, Hk, D, dt=1, off=None, nt=0, sinks=0, ws=0):
+        M = nseq * L
+        return lib.ctclip_win_attn_bwd(p, p, p, None, off, off, nt, p, None, p, p, p, p, p, p, nseq, L, L, M, M, H, Hk, D, 4, 4, sinks, 0, H * D, Hk * D, Hk * D, H * D, H * D, H * D, Hk * D,
+                                       Hk * D, 1.0, 0.0, 0, dt, p, ws, None)
+    assert fwd(2 ** 21, 1, 8, 64) == -2 and b"2^32 threads" in lib.ctclip_last_error()           # few rows: a workgroup for a sequence and key head
+    assert fwd(2 ** 20, 33, 16, 64, dt=0) == fwd(2 ** 21, 1, 8, 64, off=p, nt=2 ** 21) == -2     # tiles of rows
+    assert bwd(2 ** 20, 3, 16, 2, 64) == bwd(2 ** 21, 1, 8, 1, 64, off=p, nt=2 ** 21) == -2      # dQ
+    assert bwd(2 ** 20, 3, 8, 8, 128) == -2 and b"2^32 threads" in lib.ctclip_last_error()       # dK / dV, 512 threads
+    assert bwd(2 ** 18, 40, 32, 32, 64, sinks=40, ws=2 ** 60) == -2                              # 2^23 workgroups of keys, and 2^24 of two sink blocks in front

@@ -15,6 +15,10 @@
 
 namespace win {
 
+// Workspace of split passes, `rows` = splits x heads x query rows: maxima and sums of the rows, then (16-byte aligned) their accumulators.
+__host__ __device__ inline int64_t part_acc(int64_t rows) { return (2 * rows + 3) & ~(int64_t)3; }
+inline int64_t part_bytes(int64_t rows, int D) { return (part_acc(rows) + rows * D) * 4; }
+
 template <int D> struct SoftRow {          // the running softmax of a lane's query
   f32x16 acc[D / 32];
   float m, l;
@@ -166,7 +170,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 && !FINE ? 4 : 2)) 
     if (!real) return;
     const int64_t r = ((int64_t)blockIdx.y * p.H + h) * p.Mq + rw.q0 + row;
     const int64_t rows = (int64_t)p.nsplit * p.H * p.Mq;
-    store_part<D>(p.part + 2 * rows + r * D, st.acc, half);
+    store_part<D>(p.part + part_acc(rows) + r * D, st.acc, half);
     if (half == 0) { p.part[r] = st.m; p.part[rows + r] = l; }
     return;
   }
@@ -278,7 +282,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D == 128 ? 1 : 2)) void row
   if (p.nsplit > 1) {
     const int64_t r = ((int64_t)blockIdx.y * p.H + oh) * p.Mq + rw.q0 + orow, rows = (int64_t)p.nsplit * p.H * p.Mq;
 #pragma unroll
-    for (int e = 0; e < PER; e += 4) { const float t[4] = {o[e], o[e + 1], o[e + 2], o[e + 3]}; store4(p.part + 2 * rows + r * D + fc + e, t); }
+    for (int e = 0; e < PER; e += 4) { const float t[4] = {o[e], o[e + 1], o[e + 2], o[e + 3]}; store4(p.part + part_acc(rows) + r * D + fc + e, t); }
     if ((tid & 7) == 0) { p.part[r] = m; p.part[rows + r] = lsum; }
     return;
   }
@@ -311,7 +315,7 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
     const float f = __builtin_amdgcn_exp2f(p.part[s * n + i] - ms);
     l = fmaf(p.part[rows + s * n + i], f, l);
     float a[4];
-    load4(p.part + 2 * rows + (s * n + i) * D + col, a);
+    load4(p.part + part_acc(rows) + (s * n + i) * D + col, a);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(a[e], f, o[e]);
   }
@@ -416,7 +420,7 @@ extern "C" int64_t ctclip_win_attn_fwd_workspace(int nseq, int Lq, int Lk, int H
   const int l = left < 0 || left > Lk ? Lk : left, r = right < 0 || right > Lk ? Lk : right, s = sinks < Lk ? sinks : Lk;
   const int a = win::plan(nseq, Lq, Lk, H, Hk, l, r, s, q_start, false, DT_F32).nsplit, b = win::plan(nseq, Lq, Lk, H, Hk, l, r, s, q_start, false, DT_BF16).nsplit;
   const int n = a > b ? a : b;             // (of either type: the larger)
-  return n > 1 ? (int64_t)n * H * nseq * Lq * (D + 2) * 4 : 0;
+  return n > 1 ? win::part_bytes((int64_t)n * H * nseq * Lq, D) : 0;
 }
 
 // q (Mq, H D), k | v (Mk, Hk D) -> out (Mq, H D), lse [2][H][Mq] f32 (row maximum and log2 of the row's sum, log2 domain; optional: backward needs it).  Sequence b = rows b Lq ... of q and b Lk ... of
@@ -441,7 +445,7 @@ extern "C" int ctclip_win_attn_fwd(const void* q, const void* k, const void* v, 
   const Plan pl = plan(nseq, Lq, Lk, H, Hk, p.left, p.right, p.sinks, q_start, offsets != nullptr, dtype);
   p.nsplit = pl.nsplit;
   if (p.nsplit > 1) {
-    if (!workspace || workspace_bytes < (int64_t)p.nsplit * H * Mq * (D + 2) * 4 || reinterpret_cast<uintptr_t>(workspace) % 16) { ctclip_set_error("win_attn_fwd: workspace"); return CTCLIP_EWORKSPACE; }
+    if (!workspace || workspace_bytes < part_bytes((int64_t)p.nsplit * H * Mq, D) || reinterpret_cast<uintptr_t>(workspace) % 16) { ctclip_set_error("win_attn_fwd: workspace"); return CTCLIP_EWORKSPACE; }
     p.part = (float*)workspace;
   }
   return dtype == DT_F32 ? launch_fwd_t<float>(p, pl, D, stream) : launch_fwd_t<bf16_t>(p, pl, D, stream);

@@ -227,3 +227,16 @@ def test_c_entries_refuse_a_grid_that_no_launch_holds():
     assert bwd(2 ** 20, 3, 16, 2, 64) == bwd(2 ** 21, 1, 8, 1, 64, off=p, nt=2 ** 21) == -2      # dQ
     assert bwd(2 ** 20, 3, 8, 8, 128) == -2 and b"2^32 threads" in lib.ctclip_last_error()       # dK / dV, 512 threads
     assert bwd(2 ** 18, 40, 32, 32, 64, sinks=40, ws=2 ** 60) == -2                              # 2^23 workgroups of keys, and 2^24 of two sink blocks in front
+
+
+def test_accumulators_of_split_passes_start_at_16_bytes():
+    """They are written and read 16 bytes at a time; an odd number of rows stands in front of them twice."""
+    from ct_clip_amd import _lib
+    lib, odd = _lib.load(), 0
+    for Lk in (768, 800, 2400, 5000, 32 * 37):
+        for H, Lq, D in ((1, 1, 64), (3, 1, 32), (1, 33, 64), (5, 7, 128)):
+            n = lib.ctclip_win_attn_fwd_workspace(1, Lq, Lk, H, H, D, -1, -1, 0, 0, 0) // 4
+            rows = n // (D + 2)
+            odd += rows % 2 and n > 0
+            assert n % 4 == 0 and (n == 0 or n - rows * D >= 2 * rows)
+    assert odd

@@ -36,3 +36,9 @@ def test_the_output_s_bits_do_not_depend_on_the_mode(nseq, Lq, Lk, H, D, window,
     with torch.no_grad():
         assert torch.equal(call(), trained.detach())
     assert trained.requires_grad and torch.equal(frozen, trained.detach())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Lq,Lk,H,Hk,D", [(1, 768, 1, 1, 64), (1, 800, 3, 1, 32), (33, 768, 1, 1, 64), (7, 1184, 5, 5, 128)])
+def test_split_passes_of_an_odd_number_of_rows(Lq, Lk, H, Hk, D, dtype):
+    run_case(dtype, 1, Lq, Lk, H, Hk, D, (-1, -1), 0, q_start=Lk - Lq, seed=Lk)

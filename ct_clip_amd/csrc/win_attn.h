@@ -9,6 +9,8 @@
 // LDS tiles are row-major without padding; the 16-byte chunks of row r are XOR-permuted with swz(r) so that the 16 rows of a ds_read_b128 group and the four
 // rows x 64 bytes of a transposing read fall into distinct 16-byte slots of the 256-byte bank row.
 #pragma once
+#include <atomic>
+
 #include "common.h"
 
 namespace win {
@@ -502,14 +504,14 @@ inline int check_grid(int64_t workgroups, int threads) {
   ctclip_set_error("win_attn: too many sequences, heads or tiles for a launch (2^32 threads)");
   return CTCLIP_EUNSUPPORTED;
 }
-template <auto KERNEL> int raise_lds(int bytes) {       // more than 64 KB of LDS is opted into, once per kernel and device
-  static bool done[64] = {};
+template <auto KERNEL> int raise_lds(int bytes) {       // more than 64 KB of LDS is opted into, once per kernel and device (or, by several threads at once, a few times)
+  static std::atomic<bool> done[64] = {};
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) { ctclip_set_error("win_attn: no device"); return CTCLIP_EBADARG; }
-  if (!done[dev]) {
+  if (!done[dev].load(std::memory_order_acquire)) {
     const hipError_t e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) { ctclip_set_error("win_attn: LDS size refused"); return -(1000 + (int)e); }
-    done[dev] = true;
+    done[dev].store(true, std::memory_order_release);
   }
   return CTCLIP_OK;
 }

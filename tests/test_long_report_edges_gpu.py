@@ -42,3 +42,30 @@ def test_the_output_s_bits_do_not_depend_on_the_mode(nseq, Lq, Lk, H, D, window,
 @pytest.mark.parametrize("Lq,Lk,H,Hk,D", [(1, 768, 1, 1, 64), (1, 800, 3, 1, 32), (33, 768, 1, 1, 64), (7, 1184, 5, 5, 128)])
 def test_split_passes_of_an_odd_number_of_rows(Lq, Lk, H, Hk, D, dtype):
     run_case(dtype, 1, Lq, Lk, H, Hk, D, (-1, -1), 0, q_start=Lk - Lq, seed=Lk)
+
+
+def test_calls_from_several_threads():
+    """First calls of kernels that need more than 64 KB of LDS, forward and backward, from eight threads at once, a stream each."""
+    import threading
+    q, k, v, do = (rnd((300, 2 * 128), F32, 3 + i) for i in range(4))
+    out, start = [None] * 8, threading.Barrier(8)
+    torch.cuda.synchronize()
+
+    def call():
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        o = Fn.window_attention(*leaves, 2, 128, window=50, sinks=2, dropout=(0.1, 9))
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            start.wait()
+            out[i] = call()
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    want = call()
+    for got in out:
+        assert got is not None and all(torch.equal(a, b) for a, b in zip(got, want))

@@ -1215,6 +1215,32 @@ class SdpaFn(Function):
 
 # ------------------------------------------------------------------------------------------ long reports: rotary positions, windowed attention
 
+class _Tables:
+    """Small host tables of a plan, copied to a device at its first use there and kept with the plan.  They are read on whatever stream a call runs on, so every other stream than the
+    one they were made on is recorded: the allocator then waits for it before it hands their memory out, whenever the plan goes."""
+
+    def __init__(self, *host):
+        self.host, self.device = host, {}
+
+    def _make(self, device):
+        if device.type != "cuda":
+            held = tuple(t.to(device) for t in self.host), None
+        elif torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("rotary / window_attention: the first call with a plan copies its tables to the device, make it before the capture")
+        else:
+            held = tuple(t.to(device) for t in self.host), torch._C._cuda_getCurrentRawStream(device.index)
+        self.device[device] = held
+        return held
+
+    def on(self, device):
+        tables, stream = self.device.get(device) or self._make(device)
+        if stream is not None and stream != torch._C._cuda_getCurrentRawStream(device.index):
+            here = torch.cuda.current_stream(device)
+            for t in tables:
+                t.record_stream(here)
+        return tables
+
+
 class RotaryPositions:
     """Frequencies of rotary positions (the plan that ``rotary`` takes): pair i of the first `dim` columns of a head turns by base^(-2i/dim) radians per position.
 
@@ -1263,14 +1289,11 @@ class RotaryPositions:
         turn = np.mod(f / (2.0 * math.pi), 1.0) * 2.0 ** 32          # (exact from here on: a 64-bit float has 53 bits, in two halves of 32)
         high = np.floor(turn)
         self.bits = (high.astype(np.uint64) << np.uint64(32)) | ((turn - high) * 2.0 ** 32).astype(np.uint64)
-        self._turns = {}
+        self._turns = _Tables(torch.from_numpy(self.bits.view(np.int64)))
 
     def turns(self, device):
         """(dim / 2) int64 tensor with the bits of the unsigned fractions, on the device (made once)."""
-        t = self._turns.get(device)
-        if t is None:
-            t = self._turns[device] = torch.from_numpy(self.bits.view(np.int64)).to(device)
-        return t
+        return self._turns.on(device)[0]
 
 
 def _aligned_rows(t):
@@ -1362,14 +1385,11 @@ class PackedSequences:
         self.longest = max(self.lengths, default=0)
         tiles = [(b, t) for b, n in enumerate(self.lengths) for t in range((n + 127) // 128)]
         self.ntiles = len(tiles)
-        self._host = (torch.from_numpy(ends.astype(np.int32)), torch.tensor(tiles, dtype=torch.int32).reshape(-1))
-        self._dev, self._geometry = {}, {}
+        self._tables, self._geometry = _Tables(torch.from_numpy(ends.astype(np.int32)), torch.tensor(tiles, dtype=torch.int32).reshape(-1)), {}
 
     def on(self, device):
-        t = self._dev.get(device)
-        if t is None:
-            t = self._dev[device] = tuple(x.to(device) for x in self._host)
-        return t
+        """(first rows and end, (sequence, 128-row tile) pairs) on the device."""
+        return self._tables.on(device)
 
 
 class WindowGeometry:

@@ -240,3 +240,39 @@ def test_accumulators_of_split_passes_start_at_16_bytes():
             odd += rows % 2 and n > 0
             assert n % 4 == 0 and (n == 0 or n - rows * D >= 2 * rows)
     assert odd
+
+
+def test_tables_of_a_plan_are_recorded_on_the_streams_that_read_them(monkeypatch):
+    """... and made before a capture, never inside one."""
+    class Device:
+        type, index = "cuda", 0
+
+    class Table:
+        def __init__(self):
+            self.read_on = []
+
+        def to(self, device):
+            return self
+
+        def record_stream(self, stream):
+            self.read_on.append(stream)
+    now = dict(stream=7, capturing=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: now["stream"], raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: f"stream {now['stream']}")
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+    rope, seqs, device = Fn.RotaryPositions(32), Fn.PackedSequences([3, 200]), Device()
+    rope._turns.host, seqs._tables.host = (Table(),), (Table(), Table())
+    now["capturing"] = True
+    for first in (rope.turns, seqs.on):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            first(device)
+    now["capturing"] = False
+    tables = [rope.turns(device), *seqs.on(device)]
+    rope.turns(device)
+    assert [t.read_on for t in tables] == [[], [], []]
+    now["stream"] = 9
+    assert [rope.turns(device), *seqs.on(device)] == tables
+    assert [t.read_on for t in tables] == [["stream 9"]] * 3
+    now["capturing"] = True
+    rope.turns(device)
+    assert tables[0].read_on == ["stream 9"] * 2

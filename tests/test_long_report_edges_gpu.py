@@ -69,3 +69,45 @@ def test_calls_from_several_threads():
     want = call()
     for got in out:
         assert got is not None and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_plan_dropped_while_another_stream_still_reads_it():
+    """What is allocated next on the stream that the plan was made on must not get the memory of its tables."""
+    from ct_clip_amd import _lib
+    x, lengths = rnd((700, 256), BF16, 1), [300, 1, 399]
+    torch.cuda.synchronize()
+
+    def calls(rope, seqs):
+        return Fn.rotary(x, None, rope, 64, start=11), Fn.window_attention(x, x, x, 4, 64, nseq=seqs, window=9, sinks=2)
+    want = calls(Fn.RotaryPositions(64), Fn.PackedSequences(lengths))
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        rope, seqs = Fn.RotaryPositions(64), Fn.PackedSequences(lengths)
+        rope.turns(x.device), seqs.on(x.device)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            _lib.check(_lib.load().ctclip_spin(20000, side.cuda_stream), "ctclip_spin")          # 20 ms, under which the host runs ahead
+            got = calls(rope, seqs)
+        del rope, seqs
+        import gc
+        gc.collect()                     # (a plan of sequences and the geometries kept with it refer to each other)
+        junk = [torch.full((n,), -1, dtype=torch.int32, device="cuda") for n in (64, 4, 14) * 20]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del junk
+
+
+def test_tables_are_not_made_inside_a_capture():
+    x = rnd((40, 64), BF16, 1)
+    rope, seqs = Fn.RotaryPositions(64), Fn.PackedSequences([40])
+    Fn.rotary(x, None, Fn.RotaryPositions(64), 64)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        with pytest.raises(RuntimeError, match="before the capture"):
+            Fn.rotary(x, None, rope, 64)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            Fn.window_attention(x, x, x, 1, 64, nseq=seqs)
+    graph.replay()
+    assert torch.equal(y, x + 1)
+    assert torch.isfinite(Fn.rotary(x, None, rope, 64)).all()

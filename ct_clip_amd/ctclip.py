@@ -27,7 +27,7 @@ class CTCLIP(nn.Module):
                  text_ssl_loss_weight=0.05, use_visual_ssl=False, visual_ssl=None, visual_ssl_type="simsiam",
                  visual_ssl_hidden_layer=-1, simclr_temperature=0.1, image_ssl_loss_weight=0.05,
                  multiview_loss_weight=0.1, checkpoint_during_training=False, tokenizer=None, compute_dtype=None,
-                 gather_negatives=True, **kwargs):
+                 gather_negatives=True, max_text_len=512, **kwargs):
         super().__init__()
         self.dtype = torch.float32
         self.dim_text, self.dim_image, self.dim_latent = dim_text, dim_image, dim_latent
@@ -63,6 +63,7 @@ class CTCLIP(nn.Module):
 
         # ct_clip.py:585 downloads a tokenizer; offline-safe here: only fetched on demand by tokenize()
         self.tokenizer = tokenizer
+        self.max_text_len = max_text_len       # what tokenize() pads and truncates to (the trainer's keyword of this name): 512 as ct_clip.py, more for a tower of long reports (bert.py)
         self.compute_dtype = compute_dtype or getattr(image_encoder, "compute_dtype", None) or default_compute_dtype()
         if hasattr(image_encoder, "compute_dtype"):
             image_encoder.compute_dtype = self.compute_dtype
@@ -119,7 +120,7 @@ class CTCLIP(nn.Module):
             from transformers import BertTokenizer
             self.tokenizer = BertTokenizer.from_pretrained("microsoft/BiomedVLP-CXR-BERT-specialized", do_lower_case=True)
         dev = self.temperature.device
-        return self.tokenizer(prompt, return_tensors="pt", padding="max_length", truncation=True, max_length=512).to(dev)
+        return self.tokenizer(prompt, return_tensors="pt", padding="max_length", truncation=True, max_length=self.max_text_len).to(dev)
 
     # ---- the two towers on their own (additive API: zero-shot scoring, latent export -- the reference re-runs the whole forward)
     def encode_text(self, text):

@@ -276,3 +276,22 @@ def test_tables_of_a_plan_are_recorded_on_the_streams_that_read_them(monkeypatch
     now["capturing"] = True
     rope.turns(device)
     assert tables[0].read_on == ["stream 9"] * 2
+
+
+def test_raw_strings_are_cut_at_the_model_s_text_length():
+    import ct_clip_amd
+    asked = []
+
+    class Batch(dict):
+        def to(self, device):
+            return self
+
+    def tokenizer(prompt, **kw):
+        asked.append(kw)
+        return Batch()
+
+    def clip(**kw):
+        return ct_clip_amd.CTCLIP(image_encoder=torch.nn.Identity(), text_encoder=long_bert(attention_window=3), dim_text=64, dim_image=32, dim_latent=32, tokenizer=tokenizer, **kw)
+    for kw, n in ((dict(), 512), (dict(max_text_len=4096), 4096)):
+        clip(**kw).tokenize("a report")
+        assert asked.pop() == dict(return_tensors="pt", padding="max_length", truncation=True, max_length=n)

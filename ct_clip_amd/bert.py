@@ -13,6 +13,8 @@ Reports longer than the position table (512 rows), all as attributes of the HF c
                                        config.rope_parameters too: "rope_type" "default" | "linear" | "ntk" | "yarn", "factor", for yarn
                                        "original_max_position_embeddings", or by those of ``functional.RotaryPositions``);
   attention_window = n or (l, r)       every token attends within its window, cost linear in the length; attention_sinks first tokens (default 1: [CLS]) stay visible.
+What reaches the latent: CT-CLIP reads the [CLS] row alone.  A sink is seen by every token but sees no more than they do: [CLS] itself sees the r tokens behind it, and through n
+layers the first n * r; the words after those have no part in the latent.  Choose the window by the longest report.
 """
 import math
 

@@ -295,3 +295,21 @@ def test_raw_strings_are_cut_at_the_model_s_text_length():
     for kw, n in ((dict(), 512), (dict(max_text_len=4096), 4096)):
         clip(**kw).tokenize("a report")
         assert asked.pop() == dict(return_tensors="pt", padding="max_length", truncation=True, max_length=n)
+
+
+def test_reach_of_the_cls_row(ref):
+    """Two layers of a window of 3 to the right: the [CLS] row depends on tokens 1 ... 6 and on none behind them."""
+    from transformers import BertConfig, BertModel
+    torch.manual_seed(3)
+    model = BertModel(BertConfig(vocab_size=97, hidden_size=64, num_hidden_layers=2, num_attention_heads=2, intermediate_size=64, hidden_dropout_prob=0.0,
+                                 attention_probs_dropout_prob=0.0, position_embedding_type="rotary", attention_window=(5, 3), initializer_range=0.3))
+    ids = torch.arange(1, 13)[None]
+
+    def cls(ids):
+        with torch.no_grad():
+            return bert_last_hidden_state(model, ids, None, torch.float32, cls_only=True)
+    base = cls(ids)
+    for j in range(1, 12):
+        other = ids.clone()
+        other[0, j] = 90
+        assert torch.equal(cls(other), base) == (j > 6), j

@@ -111,3 +111,70 @@ def test_tables_are_not_made_inside_a_capture():
     graph.replay()
     assert torch.equal(y, x + 1)
     assert torch.isfinite(Fn.rotary(x, None, rope, 64)).all()
+
+
+def test_cls_rows_with_attention_dropout():
+    """A tower in training mode: the last layer's [CLS] rows attended from alone draw the masks that they draw among all rows, forward and backward."""
+    from transformers import BertConfig, BertModel
+    from ct_clip_amd.bert import bert_last_hidden_state
+    torch.manual_seed(0)
+    bert = BertModel(BertConfig(vocab_size=50, hidden_size=128, num_hidden_layers=2, num_attention_heads=2, intermediate_size=128, position_embedding_type="rotary", attention_window=(20, 9),
+                                attention_sinks=2, hidden_dropout_prob=0.0, attention_probs_dropout_prob=0.3), add_pooling_layer=False).to("cuda").train()
+    ids = torch.randint(0, 50, (3, 70), device="cuda")
+    mask = (torch.arange(70, device="cuda")[None, :] < torch.tensor([[70], [41], [5]], device="cuda")).long()
+    do = rnd((3, 128), F32, 4)
+    runs = []
+    for cls_only in (False, True, True):
+        torch.manual_seed(5 if len(runs) < 2 else 6)
+        x = bert_last_hidden_state(bert, ids, mask, F32, cls_only=cls_only)
+        x = x if cls_only else x.view(3, 70, 128)[:, 0]
+        names = [n for n, p in bert.named_parameters() if "position" not in n]
+        grads = torch.autograd.grad(x, [p for n, p in bert.named_parameters() if "position" not in n], do)
+        runs.append((x.detach(), dict(zip(names, grads))))
+    tol = 2.0 ** -14                                                         # sums of up to 210 terms in another order (210 * 2^-24 < 2^-16), through two layers
+    (a, ga), (b, gb), (c, _) = runs
+    assert (a - b).abs().max() <= tol * a.abs().max()
+    assert (b - c).abs().max() > 16 * tol * a.abs().max()                    # another seed, other masks: the comparison above would notice
+    for n in ga:
+        if "key.bias" not in n:                                              # (its true gradient is zero)
+            assert (ga[n] - gb[n]).norm() <= 4 * tol * ga[n].norm() + 1e-6, n
+
+
+@pytest.mark.parametrize("options", [dict(attention_window=6), dict(attention_window=(3, -1), attention_sinks=2, rope_scaling=dict(type="linear", factor=2.0), rotary_layout="interleaved")])
+def test_training_step_of_a_tower_of_long_reports_replayed(golden, tmp_path, options):
+    """The trainer's step captured into a graph with the tower's options on: replays continue three eager steps bit for bit, with dropout they draw fresh masks."""
+    import ct_clip_amd
+    from ct_clip_amd.trainer import GraphedStep
+    from tests.helpers import TextBatch, build_model
+    g = golden("tiny")
+    text, video = TextBatch(g["input_ids"].to("cuda"), g["attention_mask"].to("cuda")), g["video"].to("cuda")
+
+    def run(n_eager, n_graph, dropout):
+        clip = build_model(g["config"], g["state_dict"], "cuda", BF16)
+        cfg = clip.text_transformer.config
+        for name, value in dict(options, position_embedding_type="rotary", hidden_dropout_prob=dropout, attention_probs_dropout_prob=dropout).items():
+            setattr(cfg, name, value)
+        clip.train()
+        tr = ct_clip_amd.CTClipTrainer(clip, num_train_steps=10, batch_size=2, tokenizer=object(), lr=1e-3, train_dataset=[0], evaluate=False, checkpoint=False,
+                                       results_folder=str(tmp_path / f"res{n_graph}{dropout}"), num_workers=0)
+        table = clip.text_transformer.embeddings.position_embeddings.weight.detach().clone()
+        torch.manual_seed(11)
+        losses = []
+        for _ in range(n_eager):
+            losses.append(tr.forward_backward(video, text).detach().clone())
+            tr.optim.step(tr.max_grad_norm)
+            tr.optim.zero_grad()
+        if n_graph:
+            gs = GraphedStep(tr).capture(video, text)
+            try:
+                for _ in range(n_graph):
+                    losses.append(gs.run().detach().clone())
+            finally:
+                gs.close()
+        torch.cuda.synchronize()
+        assert torch.equal(table, clip.text_transformer.embeddings.position_embeddings.weight)
+        return torch.stack(losses).flatten().tolist(), tr.optim.flat_param.clone(), tr.optim.exp_avg.clone()
+    la, pa, ma = run(6, 0, 0.0)
+    lb, pb, mb = run(3, 3, 0.0)
+    assert la == lb and torch.equal(pa, pb) and torch.equal(ma, mb) and torch.isfinite(pa).all()
+    assert len(set(run(3, 3, 0.1)[0][3:])) == 3

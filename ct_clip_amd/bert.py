@@ -114,6 +114,8 @@ def bert_last_hidden_state(bert, input_ids, attention_mask, dtype, operand_dtype
     x = drop(x, None, 0)
     keymask = None
     if attention_mask is not None:
+        if attention_mask.shape != ids.shape:
+            raise ValueError(f"attention_mask {tuple(attention_mask.shape)} for input_ids {tuple(ids.shape)}")
         # additive key mask, as HF builds it: (1 - mask) * finfo.min
         keymask = ((1.0 - attention_mask.to(device=dev, dtype=torch.float32)) * torch.finfo(torch.float32).min).contiguous()
     scale = 1.0 / math.sqrt(dh)

@@ -313,3 +313,13 @@ def test_reach_of_the_cls_row(ref):
         other = ids.clone()
         other[0, j] = 90
         assert torch.equal(cls(other), base) == (j > 6), j
+
+
+@pytest.mark.parametrize("options", [dict(), dict(position_embedding_type="rotary", attention_window=3)])
+def test_an_attention_mask_of_another_shape_is_refused(ref, options):
+    """The kernels read one value for every token."""
+    model, ids = O.small_bert(**options), torch.zeros((2, 9), dtype=torch.long)
+    bert_last_hidden_state(model, ids, torch.ones(2, 9), torch.float32)
+    for shape in ((2, 8), (1, 9), (9,), (2, 9, 1), (2, 10)):
+        with pytest.raises(ValueError, match="attention_mask"):
+            bert_last_hidden_state(model, ids, torch.ones(shape), torch.float32)

@@ -1355,8 +1355,8 @@ def rotary(q, k, rope, D, L=None, positions=None, start=0):
             raise ValueError(f"rotary: positions must be {M} int32 / int64 values on {q.device}")
         positions = positions.contiguous()
     L, start = max(M, 1) if L is None else int(L), int(start)
-    if L < 1 or not -2 ** 62 < start < 2 ** 62:
-        raise ValueError("rotary: L >= 1 and a start within 62 bits")
+    if not 0 < L < 2 ** 62 or not -2 ** 62 < start < 2 ** 62:
+        raise ValueError("rotary: L >= 1 and a start, each within 62 bits")
     _no_tangents(q, k)
     if q.stride(1) != 1:
         q = q.contiguous()

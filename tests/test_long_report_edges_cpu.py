@@ -323,3 +323,11 @@ def test_an_attention_mask_of_another_shape_is_refused(ref, options):
     for shape in ((2, 8), (1, 9), (9,), (2, 9, 1), (2, 10)):
         with pytest.raises(ValueError, match="attention_mask"):
             bert_last_hidden_state(model, ids, torch.ones(shape), torch.float32)
+
+
+def test_lengths_that_the_c_entry_cannot_take_are_refused(ref):
+    x, rope = torch.zeros(6, 64), Fn.RotaryPositions(32)
+    for L in (2 ** 62, 2 ** 64 + 5):            # (the second one would arrive as 5)
+        with pytest.raises(ValueError):
+            Fn.rotary(x, None, rope, 32, L=L)
+    Fn.rotary(x, None, rope, 32, L=2 ** 40)

@@ -9,8 +9,8 @@
 // one rounding per probability) because the matrix cores read it; sums are taken of the unrounded values.  FINE adds what that rounding left over (win_attn.h, fine_pass).
 //
 // Bounds, MI355X.  One token of 4 sequences over 32768 keys, 32 heads of 128 on 8: 113 + 4 us (rows + join), 537 MB at 4.7 TB/s; a large copy runs at 5.1.  4 x 8192 tokens,
-// 12 heads of 64, window 256 + 256: 97 us, 0.53 PFLOP/s of 1.2 that a large product reaches: matrix instructions 0.27 of the time, vector instructions (exponentials, masks,
-// maxima, conversions) 0.58, LDS 0.20, which add up: a wave's step is a chain through all three, and four waves per SIMD overlap little of it.
+// 12 heads of 64, window 256 + 256: 95 us, 0.54 PFLOP/s of 1.2 that a large product reaches: matrix instructions 0.26 of the time, vector instructions (exponentials, masks,
+// maxima, conversions) 0.58, LDS 0.16, which add up: a wave's step is a chain through all three, and four waves per SIMD overlap little of it.
 #include "win_attn.h"
 
 namespace win {
@@ -106,7 +106,8 @@ template <typename T, int D> __device__ __forceinline__ f32x16 scores(const RowF
   return mma_rows<D>(kf, qf, s);
 }
 
-// Four waves per SIMD where 128 registers hold a wave (bf16, heads up to 64): 98 and 165 us for 4 x 8192 and 1 x 32768 tokens of 12 heads of 64, with two 103 and 172.
+// Four waves per SIMD (bf16, heads up to 64): 98 and 165 us for 4 x 8192 and 1 x 32768 tokens of 12 heads of 64, with two 103 and 172.  128 registers hold such a wave, but for the
+// dropout form of heads of 64, which keeps 6 in scratch and is the faster for it all the same: 4 x 8192 tokens 177 us, with two waves and none in scratch 187.
 template <typename T, int D, bool DROP, bool FINE>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 && D <= 64 && !FINE ? 4 : 2)) void fwd_kernel(Params p, int nunits, int nqt) {
   typedef Geo<T, D> G;
@@ -352,7 +353,7 @@ inline Plan plan(int nseq, int Lq, int Lk, int H, int Hk, int left, int right, i
   const int G = H / Hk;
   if (packed) return pl;
   // rows_kernel where the rows of a group fit its 32: one token of 4 sequences of 32768 keys, 32 heads of 128 on 8, takes 115 us (fwd_kernel, where the heads that share k and v
-  // are rows of different workgroups: 197), the [CLS] rows of 8 x 512 5.6 (6.1).  Split for two workgroups per CU, eight blocks (two per wave) each at least: unsplit 468 us.
+  // are rows of different workgroups: 197), the [CLS] rows of 8 x 512 5.9 (6.9).  Split for two workgroups per CU, eight blocks (two per wave) each at least: unsplit 468 us.
   if ((int64_t)Lq * G <= 32) {
     pl.rows = true;
     const TileList tl = tile_list<32>(q_start, q_start + Lq - 1, left, right, sinks, Lk);

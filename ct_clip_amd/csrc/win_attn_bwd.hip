@@ -9,8 +9,9 @@
 //   dkv_reduce_kernel  adds the partial sums of split keys in a fixed order.  Every result is bit-reproducible.
 // Seven products per visible block (five are needed at least; the other two are S and dP again, because dQ across key tiles would need float atomics).
 //
-// Bounds, MI355X.  32768 tokens, 12 heads of 64, window 512 + 512: dQ 219, dK / dV 311, reduction 7 us (0.70 and 0.66 PFLOP/s of the seven products; a large one reaches 1.2): matrix
-// instructions a third of the time, the rest LDS reads and ~90 vector instructions per 32 x 32 block, one after the other in a wave's step.  2 x 8191 tokens, 32 heads of
+// Bounds, MI355X.  32768 tokens, 12 heads of 64, window 512 + 512: dQ 219, dK / dV 311, reduction 7 us (0.70 and 0.66 PFLOP/s of the seven products; a large one reaches 1.2): dQ has
+// the matrix cores busy 0.36 of the time, the vector units 0.49, the LDS 0.19, dK / dV 0.33, 0.41, 0.27: no unit is at its limit, but the shares add up to the whole, for a wave's step
+// goes from one to the next and the two waves of a SIMD overlap little of it.  2 x 8191 tokens, 32 heads of
 // 128 on 8, causal window 1023: dQ 452-484, dK / dV 640-750 us (cards differ), 0.83 and 0.75 PFLOP/s.
 #include "win_attn.h"
 
@@ -142,6 +143,9 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Params p, int nunits, int nq
 // The shape of the dK / dV kernel.  Four waves with k, v and both gradients of 32 keys each in registers, or (bf16 heads of 128, where that is 192 registers and would leave
 // a SIMD one wave) k and v in LDS and eight waves, two to a 32-key block: 1105 against 1150 us for the backward pass of 2 x 8191 tokens, 32 heads on 8; k in registers
 // beside v in LDS spills (1558).  Heads of 64 that way: 549 instead of 467 us for 32768 tokens of 12 heads, with four waves per SIMD (spills) 1057.
+// Not everything that is shipped fits its registers either: of heads of 128 the bf16 form keeps 21 of them in scratch with dropout and 7 with remainders (65 with both), and in
+// dQ with remainders 18 (24 with dropout too); f32 dQ of heads of 128 keeps 115 (150 with dropout), f32 dK / dV of heads of 64 32 (39).  2 x 4095 tokens, 16 heads of 128, window 511, causal: backward 211 us,
+// 315 with dropout; 4 x 8192 tokens, 12 heads of 64: 301 and 496, most of it the generator's vector work.
 template <typename T, int D> struct Dkv {
   static constexpr bool IN_LDS = sizeof(T) == 2 && D == 128;
   static constexpr int PAIR = IN_LDS ? 2 : 1, WAVES = 4 * PAIR, NT = 64 * WAVES;

@@ -1223,19 +1223,17 @@ class _Tables:
         self.host, self.device = host, {}
 
     def _make(self, device):
-        if device.type != "cuda":
-            held = tuple(t.to(device) for t in self.host), None
-        elif torch.cuda.is_current_stream_capturing():
+        on = torch.device(device)
+        if on.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("rotary / window_attention: the first call with a plan copies its tables to the device, make it before the capture")
-        else:
-            held = tuple(t.to(device) for t in self.host), torch._C._cuda_getCurrentRawStream(device.index)
-        self.device[device] = held
+        tables = tuple(t.to(on) for t in self.host)
+        held = self.device[device] = tables, torch._C._cuda_getCurrentRawStream(tables[0].get_device()) if on.type == "cuda" else None
         return held
 
     def on(self, device):
         tables, stream = self.device.get(device) or self._make(device)
-        if stream is not None and stream != torch._C._cuda_getCurrentRawStream(device.index):
-            here = torch.cuda.current_stream(device)
+        if stream is not None and stream != torch._C._cuda_getCurrentRawStream(tables[0].get_device()):
+            here = torch.cuda.current_stream(tables[0].device)
             for t in tables:
                 t.record_stream(here)
         return tables

@@ -242,17 +242,20 @@ def test_accumulators_of_split_passes_start_at_16_bytes():
     assert odd
 
 
-def test_tables_of_a_plan_are_recorded_on_the_streams_that_read_them(monkeypatch):
+@pytest.mark.parametrize("device", [torch.device("cuda", 0), torch.device("cuda"), "cuda"])
+def test_tables_of_a_plan_are_recorded_on_the_streams_that_read_them(monkeypatch, device):
     """... and made before a capture, never inside one."""
-    class Device:
-        type, index = "cuda", 0
-
     class Table:
+        device = torch.device("cuda", 0)
+
         def __init__(self):
             self.read_on = []
 
         def to(self, device):
             return self
+
+        def get_device(self):
+            return 0
 
         def record_stream(self, stream):
             self.read_on.append(stream)
@@ -260,7 +263,7 @@ def test_tables_of_a_plan_are_recorded_on_the_streams_that_read_them(monkeypatch
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: now["stream"], raising=False)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device: f"stream {now['stream']}")
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
-    rope, seqs, device = Fn.RotaryPositions(32), Fn.PackedSequences([3, 200]), Device()
+    rope, seqs = Fn.RotaryPositions(32), Fn.PackedSequences([3, 200])
     rope._turns.host, seqs._tables.host = (Table(),), (Table(), Table())
     now["capturing"] = True
     for first in (rope.turns, seqs.on):

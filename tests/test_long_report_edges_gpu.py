@@ -178,3 +178,41 @@ def test_training_step_of_a_tower_of_long_reports_replayed(golden, tmp_path, opt
     lb, pb, mb = run(3, 3, 0.0)
     assert la == lb and torch.equal(pa, pb) and torch.equal(ma, mb) and torch.isfinite(pa).all()
     assert len(set(run(3, 3, 0.1)[0][3:])) == 3
+
+
+def test_tables_on_a_device_named_without_an_index():
+    """Made ahead of a capture by whoever holds the plan."""
+    x, rope, seqs = rnd((40, 64), BF16, 1), Fn.RotaryPositions(64), Fn.PackedSequences([40])
+    for device in ("cuda", torch.device("cuda"), x.device):
+        for _ in range(2):
+            assert rope.turns(device).device == x.device and seqs.on(device)[0].device == x.device
+    assert torch.isfinite(Fn.rotary(x, None, rope, 64)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_forms_of_arguments(dtype):
+    """Key masks of other types and shapes, misaligned and expanded tensors, a gradient that is one number expanded, dropout of probability 0: the same as their plain forms."""
+    n, L, H, D = 2, 70, 2, 32
+    q, k, v = (rnd((n * L, H * D), dtype, i) for i in (1, 2, 3))
+    mask = torch.zeros((n, L), device="cuda")
+    mask[0, 40:] = torch.finfo(F32).min
+    mask[1, ::3] = -2.5
+
+    def call(q=q, k=k, v=v, keymask=mask, **kw):
+        return Fn.window_attention(q, k, v, H, D, nseq=n, window=(9, 5), sinks=2, keymask=keymask, **kw)
+    want = call()
+    for m in (mask.double(), mask.bfloat16(), mask[:, None, None, :], mask.reshape(-1), mask.t().contiguous().t(), mask.clone().requires_grad_(True)):
+        assert torch.equal(call(keymask=m), want)
+    assert torch.equal(call(dropout=(0.0, 3)), want)
+
+    def odd(t):          # one element off a 16-byte row
+        wide = torch.zeros((t.shape[0], t.shape[1] + 3), dtype=t.dtype, device="cuda")
+        wide[:, 1:-2] = t
+        return wide[:, 1:-2]
+    assert torch.equal(call(odd(q), odd(k), odd(v)), want)
+    one = [t[:1].clone().requires_grad_(True) for t in (k, v)]
+    full = [t.detach().expand(n * L, -1).contiguous().requires_grad_(True) for t in one]
+    a, b = call(k=one[0].expand(n * L, -1), v=one[1].expand(n * L, -1)), call(k=full[0], v=full[1])
+    assert torch.equal(a, b)
+    ga, gb = torch.autograd.grad(a.sum(), one), torch.autograd.grad(b, full, torch.ones_like(b))
+    assert all(torch.equal(x, y.sum(0, keepdim=True)) for x, y in zip(ga, gb))

@@ -1300,6 +1300,11 @@ def _aligned_rows(t):
     return t if one == 1 and not (t.data_ptr() | ld * t.element_size()) & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
+def _dense_rows(t):
+    """t itself when a row's columns lie side by side (or t is None), else a dense copy (of no rows too: contiguous() leaves those as they are)."""
+    return t if t is None or t.stride(1) == 1 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _not_twice():
     """(Backward functions made of kernels: a graph of them would hold no further derivative.)"""
     if torch.is_grad_enabled():
@@ -1325,10 +1330,7 @@ class RotaryFn(Function):
     @staticmethod
     def backward(ctx, dq, dk=None):
         _not_twice()
-        if dq.stride(1) != 1:
-            dq = dq.contiguous()
-        if dk is not None and dk.stride(1) != 1:
-            dk = dk.contiguous()
+        dq, dk = _dense_rows(dq), _dense_rows(dk)
         positions, = ctx.saved_tensors or (None,)
         gq, gk = B().rotary(dq, dk, *ctx.args[0], positions, *ctx.args[1], True)
         return gq, gk, None, None, None, None, None
@@ -1356,10 +1358,7 @@ def rotary(q, k, rope, D, L=None, positions=None, start=0):
     if not 0 < L < 2 ** 62 or not -2 ** 62 < start < 2 ** 62:
         raise ValueError("rotary: L >= 1 and a start, each within 62 bits")
     _no_tangents(q, k)
-    if q.stride(1) != 1:
-        q = q.contiguous()
-    if k is not None and k.stride(1) != 1:
-        k = k.contiguous()
+    q, k = _dense_rows(q), _dense_rows(k)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return RotaryFn.apply(q, k, rope, D, L, positions, start)
     qo, ko = B().rotary(q, k, rope.turns(q.device), D, rope.dim, L, positions, start, rope.interleaved, rope.magnitude)

@@ -334,3 +334,17 @@ def test_lengths_that_the_c_entry_cannot_take_are_refused(ref):
         with pytest.raises(ValueError):
             Fn.rotary(x, None, rope, 32, L=L)
     Fn.rotary(x, None, rope, 32, L=2 ** 40)
+
+
+def test_gradients_of_no_rows_reach_the_backend_row_by_row(ref, monkeypatch):
+    """A sum's gradient is one number with strides of 0, which contiguous() keeps where there are no rows."""
+    from tests.test_long_reports_cpu import RefOps
+    strides = []
+    monkeypatch.setattr(RefOps, "rotary", lambda self, q, k, *a, **kw: strides.append((q.stride(1), k.stride(1))) or (torch.zeros(q.shape), torch.zeros(k.shape)))
+    x = torch.zeros((0, 64), requires_grad=True)
+    q, k = Fn.rotary(x, x.detach().expand(0, 64), Fn.RotaryPositions(32), 32)
+    torch.autograd.grad(q.sum() + k.sum(), x)
+    y = torch.zeros((5, 64), requires_grad=True)
+    q, k = Fn.rotary(y, y[:1, :1].expand(5, 64), Fn.RotaryPositions(32), 32)
+    torch.autograd.grad(q.sum() + k.sum(), y)
+    assert strides == [(1, 1)] * 4

@@ -216,3 +216,20 @@ def test_forms_of_arguments(dtype):
     assert torch.equal(a, b)
     ga, gb = torch.autograd.grad(a.sum(), one), torch.autograd.grad(b, full, torch.ones_like(b))
     assert all(torch.equal(x, y.sum(0, keepdim=True)) for x, y in zip(ga, gb))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_calls_without_rows(dtype):
+    rope, none, keys = Fn.RotaryPositions(32), torch.zeros((0, 64), dtype=dtype, device="cuda", requires_grad=True), rnd((12, 64), dtype, 1).requires_grad_(True)
+    q, k = Fn.rotary(none, none, rope, 32, L=4, start=9)
+    assert q.shape == k.shape == (0, 64)
+    (g,) = torch.autograd.grad(q.sum() + k.sum(), none)
+    assert g.shape == (0, 64)
+    o = Fn.window_attention(none, keys, keys, 2, 32, nseq=3, window=2)
+    g0, g1 = torch.autograd.grad(o.sum(), (none, keys))
+    assert o.shape == g0.shape == (0, 64) and not g1.any()
+    assert Fn.window_attention(none, none, none, 2, 32, nseq=0).shape == (0, 64)
+    assert Fn.window_attention(none, none, none, 2, 32, nseq=Fn.PackedSequences([])).shape == (0, 64)
+    o = Fn.window_attention(keys, keys, keys, 2, 32, nseq=Fn.PackedSequences([0, 0], first=3))
+    (g,) = torch.autograd.grad(o.sum(), keys)
+    assert not o.any() and not g.any()

@@ -233,3 +233,42 @@ def test_calls_without_rows(dtype):
     o = Fn.window_attention(keys, keys, keys, 2, 32, nseq=Fn.PackedSequences([0, 0], first=3))
     (g,) = torch.autograd.grad(o.sum(), keys)
     assert not o.any() and not g.any()
+
+
+def test_packed_training_captured_and_replayed_and_a_second_backward_pass():
+    """Rows outside the sequences, sinks of one long sequence among short ones, a key mask: each replay equals the eager result; so does the same graph's second backward pass."""
+    H, D, lengths = 2, 64, [30] * 20 + [700] + [1, 0, 45]
+    seqs = Fn.PackedSequences(lengths, first=4)
+    M = seqs.end + 9
+    q, k, v, do = (rnd((M, H * D), BF16, i) for i in range(4))
+    mask = torch.zeros(M, device="cuda")
+    rope = Fn.RotaryPositions(32, layout="interleaved")
+    positions = torch.cat([torch.zeros(4, dtype=torch.int64)] + [torch.arange(n) for n in lengths] + [torch.zeros(9, dtype=torch.int64)]).to("cuda")
+
+    def step(again=False):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        a, b = Fn.rotary(leaves[0], leaves[1], rope, D, positions=positions)
+        o = Fn.window_attention(a, b, leaves[2], H, D, nseq=seqs, window=(60, 20), sinks=3, keymask=mask)
+        grads = torch.autograd.grad(o, leaves, do, retain_graph=again)
+        if again:
+            assert all(torch.equal(x, y) for x, y in zip(grads, torch.autograd.grad(o, leaves, do)))
+        return [o.detach(), *grads]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for rep in range(3):
+        for i, t in enumerate((q, k, v, do)):
+            t.copy_(rnd(tuple(t.shape), BF16, 80 + 4 * rep + i))
+        mask[rep::5] = torch.finfo(F32).min
+        want = step(again=True)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert not any(t[:4].any() or t[seqs.end:].any() for t in out)
